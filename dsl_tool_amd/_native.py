@@ -40,7 +40,9 @@ FMT_MXFP4, FMT_NVFP4 = 0, 1
 OP_FP8, OP_FP4, OP_GROUPED_FP8, OP_BF16 = 0, 1, 2, 3
 QFMT_FP8_G128, QFMT_MXFP4 = 0, 1
 W_BF16, W_F32 = 0, 1
-IN_BF16, IN_F32 = 0, 1
+IN_BF16, IN_F32, IN_F16 = 0, 1, 2
+ROWQ_INT8, ROWQ_FP8, ROWQ_FP8_G128 = 0, 1, 2
+KV_INT8, KV_FP8 = 0, 1
 ABI_VERSION = 10
 
 
@@ -57,6 +59,9 @@ class DslError(RuntimeError):
 
 
 _vp, _i64, _i32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
+
+# pages, heads, page, dim, fmt, table, table_ld, width, seq_lens, starts, seqs
+_CACHE = [_i64, _i64, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _vp, _i64]
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -95,6 +100,14 @@ SIGNATURES = {
     "dsl_moe_grouped_fp8_gemm": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
                                         _i64, _i32, _vp, _vp, _vp]),
     "dsl_moe_combine": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i32, _vp]),
+    "dsl_quant_int8_rows": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "dsl_add_rmsnorm_quant": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i32, ctypes.c_float, _i32, _i32,
+                                     _vp, _vp, _vp, _vp]),
+    "dsl_kv8_write": (_i32, [_vp] * 4 + _CACHE + [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp]),
+    "dsl_kv8_read": (_i32, [_vp] * 4 + _CACHE + [_vp, _vp, _i64, _i32, _vp]),
+    "dsl_kv8_attention": (_i32, [_vp, _i64, _i64, _i64] + [_vp] * 4 + _CACHE +
+                          [_vp, _i64, _i64, _i64, _i64, ctypes.c_float, _i32, _i32, _vp, _sz, _vp]),
+    "dsl_kv8_attention_workspace_bytes": (_sz, [_i64] * 8),
 }
 
 _lib = None

@@ -13,6 +13,8 @@
 // A call costs about 1.5 us beside its launches (ctypes path: about 9).
 #include <Python.h>
 
+#include <cmath>
+
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -491,12 +493,208 @@ PyObject *lora_gemm(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------- 8-bit attention layer --
+int src_code(ScalarType t) {
+  return t == ScalarType::BFloat16 ? DSL_IN_BF16 : (t == ScalarType::Half ? DSL_IN_F16 : -1);
+}
+
+// rows with unit column stride and a row stride of whole 16-byte chunks
+bool row_major(const Tensor &t) {
+  return t.dim() == 2 && t.numel() > 0 && t.stride(1) == 1 && t.stride(0) >= t.size(1) && t.stride(0) % 8 == 0 &&
+         aligned16(t);
+}
+
+// quant_int8_rows(x)
+PyObject *quant_int8_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *x = n == 1 ? gpu_tensor(a[0]) : nullptr;
+  if (!x || !row_major(*x)) return none();
+  const int dt = x->scalar_type() == ScalarType::Float ? DSL_IN_F32 : src_code(x->scalar_type());
+  if (dt < 0) return none();
+  Tensor q, s;
+  const bool ok = on_device(*x, [&] {
+    const int64_t r = x->size(0), c = x->size(1);
+    q = empty({r, c}, ScalarType::Char, *x);
+    s = empty({r}, ScalarType::Float, *x);
+    return dsl_quant_int8_rows(ptr(*x), r, c, x->stride(0), dt, ptr<int8_t>(q), ptr<float>(s), stream_of(*x)) == DSL_OK;
+  });
+  return ok ? pack({q, s}) : none();
+  END_HANDLE_TH_ERRORS
+}
+
+// add_rmsnorm_quant(x, residual or None, weight, eps, qfmt)
+PyObject *add_rmsnorm_quant(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || !PyFloat_CheckExact(a[3]) || !PyLong_CheckExact(a[4])) return none();
+  const Tensor *x = gpu_tensor(a[0]), *r = a[1] == Py_None ? nullptr : gpu_tensor(a[1]), *w = gpu_tensor(a[2]);
+  if (!x || !w || (a[1] != Py_None && !r) || !row_major(*x) || !plain(*w, 1) || w->size(0) != x->size(1) ||
+      w->device() != x->device())
+    return none();
+  const int dt = src_code(x->scalar_type()), fmt = (int)PyLong_AsLong(a[4]);
+  if (dt < 0 || (r && (!row_major(*r) || r->sizes() != x->sizes() || r->scalar_type() != x->scalar_type() ||
+                       r->device() != x->device())))
+    return none();
+  const int wd = w->scalar_type() == ScalarType::BFloat16 ? DSL_W_BF16
+                                                           : (w->scalar_type() == ScalarType::Float ? DSL_W_F32 : -1);
+  if (wd < 0) return none();
+  const float eps = (float)PyFloat_AS_DOUBLE(a[3]);
+  Tensor q, s, h = *x;
+  const bool ok = on_device(*x, [&] {
+    const int64_t rows = x->size(0), c = x->size(1);
+    q = empty({rows, c}, fmt == DSL_ROWQ_INT8 ? ScalarType::Char : ScalarType::Byte, *x);
+    s = fmt == DSL_ROWQ_FP8_G128 ? empty({rows, (c + 127) / 128}, ScalarType::Float, *x)
+                                 : empty({rows}, ScalarType::Float, *x);
+    if (r) h = empty({rows, c}, x->scalar_type(), *x);
+    return dsl_add_rmsnorm_quant(ptr(*x), rows, c, x->stride(0), r ? ptr(*r) : nullptr, r ? r->stride(0) : 0, ptr(*w),
+                                 wd, eps, dt, fmt, r ? ptr(h) : nullptr, ptr(q), ptr<float>(s), stream_of(*x)) == DSL_OK;
+  });
+  if (!ok) return none();
+  if (r) return pack({q, s, h});
+  PyObject *t = pack({q, s, *x});
+  if (t) {                                       // h is x itself
+    Py_INCREF(a[0]);
+    PyObject *old = PyTuple_GET_ITEM(t, 2);
+    PyTuple_SET_ITEM(t, 2, a[0]);
+    Py_DECREF(old);
+  }
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
+// The cache and the sequences of a call, as the C ABI takes them in place.
+struct CacheView {
+  const Tensor *k, *v, *ks, *vs, *lens, *table, *starts;
+  int fmt;
+  int64_t pages, heads, page, dim, ld, width, seqs;
+};
+// a: k, v, k_scale, v_scale; then b: seq_lens, page_table, starts or None
+bool cache_view(PyObject *const *a, PyObject *const *b, CacheView *c) {
+  c->k = gpu_tensor(a[0]);
+  c->v = gpu_tensor(a[1]);
+  c->ks = gpu_tensor(a[2]);
+  c->vs = gpu_tensor(a[3]);
+  c->lens = gpu_tensor(b[0]);
+  c->table = gpu_tensor(b[1]);
+  c->starts = b[2] == Py_None ? nullptr : gpu_tensor(b[2]);
+  if (!c->k || !c->v || !c->ks || !c->vs || !c->lens || !c->table || (b[2] != Py_None && !c->starts)) return false;
+  if (!plain(*c->k, 4) || !plain(*c->v, 4) || !is_scales(*c->ks, ScalarType::Float) ||
+      !is_scales(*c->vs, ScalarType::Float) || !is_scales(*c->lens, ScalarType::Int) || c->lens->dim() != 1 ||
+      c->table->scalar_type() != ScalarType::Int || c->table->dim() != 2 || c->table->numel() == 0 ||
+      c->table->stride(1) != 1)
+    return false;
+  const ScalarType t = c->k->scalar_type();
+  if (t != c->v->scalar_type() || (t != ScalarType::Char && t != ScalarType::Float8_e4m3fn)) return false;
+  c->fmt = t == ScalarType::Char ? DSL_KV_INT8 : DSL_KV_FP8;
+  c->pages = c->k->size(0);
+  c->heads = c->k->size(1);
+  c->page = c->k->size(2);
+  c->dim = c->k->size(3);
+  c->seqs = c->lens->size(0);
+  c->width = c->table->size(1);
+  c->ld = c->seqs > 1 ? c->table->stride(0) : c->width;
+  const at::Device d = c->k->device();
+  if (c->v->size(0) != c->pages || c->v->size(1) != c->heads || c->v->size(2) != c->dim || c->v->size(3) != c->page ||
+      c->ks->dim() != 2 || c->ks->size(0) != c->pages || c->ks->size(1) != c->heads || c->vs->sizes() != c->ks->sizes() ||
+      c->table->size(0) != c->seqs || c->ld < c->width || c->v->device() != d || c->ks->device() != d ||
+      c->vs->device() != d || c->lens->device() != d || c->table->device() != d)
+    return false;
+  return !c->starts || (is_scales(*c->starts, ScalarType::Int) && c->starts->dim() == 1 &&
+                        c->starts->size(0) == c->seqs + 1 && c->starts->device() == d);
+}
+#define DSL_CACHE(c)                                                                                              \
+  ptr((*(c).k)), ptr((*(c).v)), ptr<float>(*(c).ks), ptr<float>(*(c).vs), (c).pages, (c).heads, (c).page, (c).dim, \
+      (c).fmt, ptr<int32_t>(*(c).table), (c).ld, (c).width, ptr<int32_t>(*(c).lens),                              \
+      (c).starts ? ptr<int32_t>(*(c).starts) : nullptr, (c).seqs
+
+// [rows][heads][dim] read in place: unit stride in dim, 16-byte aligned rows
+bool head_rows(const Tensor *t, const CacheView &c) {
+  return t && t->dim() == 3 && t->numel() > 0 && t->size(2) == c.dim && t->stride(2) == 1 && t->stride(1) % 8 == 0 &&
+         t->stride(0) % 8 == 0 && t->stride(1) >= c.dim && aligned16(*t) && t->device() == c.k->device();
+}
+
+// most new tokens of a sequence: a number, or None (one, or all rows); -1: leave the call
+int64_t most_new(PyObject *o, const CacheView &c, int64_t rows) {
+  if (o == Py_None) return c.starts ? rows : 1;
+  if (!PyLong_CheckExact(o)) return -1;
+  int over = 0;
+  const long long n = PyLong_AsLongLongAndOverflow(o, &over);
+  return over || n < 0 ? -1 : n;
+}
+
+// kv8_write(k_cache, v_cache, k_scale, v_scale, k, v, seq_lens, page_table, starts, max_q)
+PyObject *kv8_write(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  CacheView c;
+  if (n != 10 || !cache_view(a, a + 6, &c)) return none();
+  const Tensor *k = gpu_tensor(a[4]), *v = gpu_tensor(a[5]);
+  if (!head_rows(k, c) || !head_rows(v, c) || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() ||
+      k->size(1) != c.heads)
+    return none();
+  const int dt = src_code(k->scalar_type());
+  const int64_t rows = k->size(0), most = most_new(a[9], c, rows);
+  if (dt < 0 || most < 0 || (!c.starts && rows != c.seqs)) return none();
+  const bool ok = on_device(*k, [&] {
+    return dsl_kv8_write(DSL_CACHE(c), ptr(*k), k->stride(0), k->stride(1), ptr(*v), v->stride(0), v->stride(1), rows,
+                         most, dt, stream_of(*k)) == DSL_OK;
+  });
+  if (!ok) return none();
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// kv8_read(k_cache, v_cache, k_scale, v_scale, seq_lens, page_table, starts, total, dtype)
+PyObject *kv8_read(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  CacheView c;
+  if (n != 9 || !THPDtype_Check(a[8]) || !PyLong_CheckExact(a[7]) || !cache_view(a, a + 4, &c) || !c.starts) return none();
+  const ScalarType t = reinterpret_cast<THPDtype *>(a[8])->scalar_type;
+  const int dt = src_code(t);
+  int over = 0;
+  const long long rows = PyLong_AsLongLongAndOverflow(a[7], &over);
+  if (dt < 0 || over || rows <= 0) return none();
+  Tensor k, v;
+  const bool ok = on_device(*c.k, [&] {
+    k = empty({rows, c.heads, c.dim}, t, *c.k);
+    v = empty({rows, c.heads, c.dim}, t, *c.k);
+    return dsl_kv8_read(DSL_CACHE(c), ptr(k), ptr(v), rows, dt, stream_of(*c.k)) == DSL_OK;
+  });
+  return ok ? pack({k, v}) : none();
+  END_HANDLE_TH_ERRORS
+}
+
+// kv8_attention(q, k_cache, v_cache, k_scale, v_scale, seq_lens, page_table, starts, max_q, scale, causal)
+PyObject *kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  CacheView c;
+  if (n != 11 || !PyBool_Check(a[10]) || (a[9] != Py_None && !PyFloat_CheckExact(a[9])) || !cache_view(a + 1, a + 5, &c))
+    return none();
+  const Tensor *q = gpu_tensor(a[0]);
+  if (!head_rows(q, c) || q->size(1) % c.heads != 0) return none();
+  const int dt = src_code(q->scalar_type());
+  const int64_t rows = q->size(0), hq = q->size(1), most = most_new(a[8], c, rows);
+  if (dt < 0 || most < 0 || (!c.starts && rows != c.seqs)) return none();
+  const double sc = a[9] == Py_None ? 1.0 / std::sqrt((double)c.dim) : PyFloat_AS_DOUBLE(a[9]);
+  const bool causal = a[10] == Py_True;
+  Tensor o;
+  const bool ok = on_device(*q, [&] {
+    o = empty({rows, hq, c.dim}, q->scalar_type(), *q);
+    const size_t nb = dsl_kv8_attention_workspace_bytes(c.heads, c.page, c.dim, c.width, c.seqs, rows, hq, most);
+    Tensor ws;
+    if (nb) ws = bytes((int64_t)nb, *q);
+    return dsl_kv8_attention(ptr(*q), q->stride(0), q->stride(1), hq, DSL_CACHE(c), ptr(o), hq * c.dim, c.dim, rows,
+                             most, (float)sc, causal, dt, nb ? ptr(ws) : nullptr, nb, stream_of(*q)) == DSL_OK;
+  });
+  return ok ? THPVariable_Wrap(o) : none();
+  END_HANDLE_TH_ERRORS
+}
+
 #define DSL_FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {DSL_FN(quant_fp8_tensor), DSL_FN(quant_fp8_blocks), DSL_FN(quant_mxfp4),
                          DSL_FN(quant_nvfp4),      DSL_FN(fp8_gemm),         DSL_FN(fp4_gemm),
                          DSL_FN(bf16_gemm),        DSL_FN(grouped_fp8_gemm), DSL_FN(rmsnorm_quant),
                          DSL_FN(swiglu_quant),     DSL_FN(moe_projection),   DSL_FN(lora_gemm),
-                         DSL_FN(quant_fp8_rows_batched),
+                         DSL_FN(quant_fp8_rows_batched), DSL_FN(quant_int8_rows), DSL_FN(add_rmsnorm_quant),
+                         DSL_FN(kv8_write),        DSL_FN(kv8_read),         DSL_FN(kv8_attention),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "dsl_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

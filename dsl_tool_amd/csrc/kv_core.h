@@ -1,0 +1,106 @@
+// Codes of the paged 8-bit cache and its sequences, shared by the kernels that
+// write, read and attend over it (kvcache.hip, attn.hip, attn_prefill.hip).
+//
+// Page p, head h: keys k[p][h][token][dim] and values v[p][h][dim][token], so
+// that both lie along the dimension that attention's products sum over (dim
+// for the scores, tokens for the output) and both feed matrix instructions
+// without a transpose.  A code c stands for c * scale[p][h].
+#pragma once
+
+#include "common.h"
+#include "serve_args.h"
+
+namespace dsl {
+
+// One element of a 16-bit row, widened.
+template <int SRC>
+DSL_DEV float widen(uint16_t b) {
+  if constexpr (SRC == SRC_BF16) return bf16_to_f32(b);
+  else return (float)__builtin_bit_cast(_Float16, b);
+}
+template <int SRC>
+DSL_DEV uint32_t narrow2(float a, float b) {
+  if constexpr (SRC == SRC_BF16) return pack_bf16x2(a, b);
+  else return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
+}
+template <int SRC>
+DSL_DEV void widen8s(const uint4 &v, float *f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = widen<SRC>((uint16_t)w[i]);
+    f[2 * i + 1] = widen<SRC>((uint16_t)(w[i] >> 16));
+  }
+}
+
+// The values of four codes.
+template <bool FP8>
+DSL_DEV void code_values(uint32_t w, float *f) {
+  if constexpr (FP8) {
+    f[0] = __builtin_amdgcn_cvt_f32_fp8((int)w, 0);
+    f[1] = __builtin_amdgcn_cvt_f32_fp8((int)w, 1);
+    f[2] = __builtin_amdgcn_cvt_f32_fp8((int)w, 2);
+    f[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
+  } else {
+    f[0] = (float)(int8_t)w;
+    f[1] = (float)(int8_t)(w >> 8);
+    f[2] = (float)(int8_t)(w >> 16);
+    f[3] = (float)(int8_t)(w >> 24);
+  }
+}
+
+// The codes of x[i] / s (the IEEE quotient), byte i = element i.
+template <bool FP8>
+DSL_DEV uint32_t codes_of(float a, float b, float c, float d, float s) {
+  a = __fdiv_rn(a, s);
+  b = __fdiv_rn(b, s);
+  c = __fdiv_rn(c, s);
+  d = __fdiv_rn(d, s);
+  if constexpr (FP8) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
+  } else {
+    const uint32_t ia = (uint32_t)(int)__builtin_rintf(a), ib = (uint32_t)(int)__builtin_rintf(b);
+    const uint32_t ic = (uint32_t)(int)__builtin_rintf(c), id = (uint32_t)(int)__builtin_rintf(d);
+    return __builtin_amdgcn_perm(ib, ia, 0x0c0c0400u) | __builtin_amdgcn_perm(id, ic, 0x04000c0cu);
+  }
+}
+
+constexpr float kInt8Top = 127.0f;
+template <bool FP8>
+DSL_DEV float kv_scale_of(float amax) {
+  return fmaxf(__fdiv_rn(amax, FP8 ? kE4M3Max : kInt8Top), kScaleFloor);
+}
+
+// A sequence's new tokens: n rows from row0 of the token tensors, at positions
+// first .. first + n - 1 = len - 1.  Starts are held to the tensors' rows
+// whatever the table says; first < 0 where there are more rows than tokens.
+struct SeqView {
+  int len, first, n, row0;
+};
+DSL_DEV SeqView seq_view(const KvCacheArgs &c, int b) {
+  SeqView s;
+  const int len = c.lens[b];
+  s.len = len > 0 ? len : 0;
+  if (c.starts) {
+    const int lo = c.starts[b], hi = c.starts[b + 1];
+    s.row0 = lo < 0 ? 0 : (lo > c.rows ? c.rows : lo);
+    const int end = hi > c.rows ? c.rows : hi;
+    s.n = end > s.row0 ? end - s.row0 : 0;
+  } else {
+    s.row0 = b;
+    s.n = b < c.rows ? 1 : 0;
+  }
+  s.first = s.len - s.n;
+  return s;
+}
+
+// The page that holds the tokens [page * pg, ..) of sequence b, or -1: pages
+// past the table's row and numbers out of range hold none.
+DSL_DEV int64_t page_of(const KvCacheArgs &c, int b, int pg) {
+  if (pg >= c.width) return -1;
+  const int64_t pid = c.table[(int64_t)b * c.table_ld + pg];
+  return pid >= 0 && pid < c.pages ? pid : -1;
+}
+
+}  // namespace dsl

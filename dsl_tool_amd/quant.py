@@ -144,3 +144,29 @@ def quant_nvfp4(x: torch.Tensor):
         N.call("dsl_quant_nvfp4", N.ptr(x), R, C, x.stride(0), x.stride(1), xd, N.ptr(q), N.ptr(sb),
                N.ptr(sg), N.ptr(ws), ws.numel() * 4, N.stream_of(x.device))
     return q, sb, sg
+
+
+def quant_int8_rows(x: torch.Tensor):
+    """int8 codes of ``x [R, C]`` (bf16, fp16 or fp32) with one scale per row:
+    ``(q int8 [R, C], scales float32 [R])``, ``s = max(amax/127, 1e-12)``,
+    ``q = round(x / s)`` (ties to even): activations per token, weights per
+    output channel, as :func:`gemm.int8_gemm_packed` takes them.  C % 8 == 0,
+    C <= 32768."""
+    r = N.fast().quant_int8_rows(x)
+    if r is not None:
+        return r
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("quant_int8_rows: expected a 2-D tensor")
+    if x.device.type != "cuda":
+        raise ValueError(f"quant_int8_rows: tensor must be on a GPU device (got {x.device})")
+    codes = {torch.bfloat16: N.IN_BF16, torch.float16: N.IN_F16, torch.float32: N.IN_F32}
+    if x.dtype not in codes:
+        raise TypeError(f"quant_int8_rows: unsupported dtype {x.dtype} (bfloat16, float16 or float32)")
+    x = N.vec_rows(x, 8)
+    R, C = x.shape
+    q = torch.empty((R, C), dtype=torch.int8, device=x.device)
+    scales = torch.empty(R, dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        N.call("dsl_quant_int8_rows", N.ptr(x), R, C, x.stride(0), codes[x.dtype], N.ptr(q), N.ptr(scales),
+               N.stream_of(x.device))
+    return q, scales

@@ -44,7 +44,9 @@ enum { DSL_FMT_MXFP4 = 0, DSL_FMT_NVFP4 = 1 };
 enum { DSL_OP_FP8 = 0, DSL_OP_FP4 = 1, DSL_OP_GROUPED_FP8 = 2, DSL_OP_BF16 = 3 };
 enum { DSL_QFMT_FP8_G128 = 0, DSL_QFMT_MXFP4 = 1 };
 enum { DSL_W_BF16 = 0, DSL_W_F32 = 1 };
-enum { DSL_IN_BF16 = 0, DSL_IN_F32 = 1 };
+enum { DSL_IN_BF16 = 0, DSL_IN_F32 = 1, DSL_IN_F16 = 2 };   /* F16: the serving entry points only */
+enum { DSL_ROWQ_INT8 = 0, DSL_ROWQ_FP8 = 1, DSL_ROWQ_FP8_G128 = 2 };
+enum { DSL_KV_INT8 = 0, DSL_KV_FP8 = 1 };
 
 /* Last error message of the calling thread ("" when none). */
 const char *dsl_last_error(void);
@@ -354,6 +356,79 @@ int dsl_moe_combine(const void *y, int64_t rows, int64_t n, int64_t ldy, const i
  * scale arrays at a padded pitch (16-byte aligned workspace); a launch given
  * less takes a kernel that does without the copy. */
 size_t dsl_gemm_workspace_bytes(int op, int64_t m, int64_t n, int64_t k);
+
+/* ------------------------------------------------- 8-bit attention layer --
+ * The operators of a decoder layer's attention block served in 8 bits.  The
+ * reference has none of them.
+ */
+
+/* int8 codes with one scale per row: s = max(amax/127, 1e-12), q =
+ * round(x / s) (the IEEE quotient, ties to even).  x bf16, fp16 or fp32 with
+ * unit column stride; cols % 8 == 0, cols <= 32768, ldx % 8 == 0.  q [rows][cols]. */
+int dsl_quant_int8_rows(const void *x, int64_t rows, int64_t cols, int64_t ldx, int x_dtype,
+                        int8_t *q, float *scales, void *stream);
+
+/* h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight; codes and scales of
+ * y.  x, residual and h bf16 or fp16 (x_dtype); the sums, y and its scales are
+ * fp32, and h is rounded only where it is stored.  residual NULL: h = x; h NULL:
+ * not stored.  qfmt DSL_ROWQ_INT8 / DSL_ROWQ_FP8: int8 / E4M3 with scales
+ * [rows]; DSL_ROWQ_FP8_G128: E4M3 with scales [rows][ceil(cols/128)].  h and q
+ * [rows][cols]; limits as above.  Codes of infinities and NaN are not specified. */
+int dsl_add_rmsnorm_quant(const void *x, int64_t rows, int64_t cols, int64_t ldx,
+                          const void *residual, int64_t ldr, const void *weight, int weight_dtype,
+                          float eps, int x_dtype, int qfmt, void *h, void *q, float *scales,
+                          void *stream);
+
+/* The paged 8-bit cache.  Pages of `page` tokens (16, 32, 64, 128 or 256) of
+ * one sequence: k_cache [pages][heads][page][dim], v_cache
+ * [pages][heads][dim][page] (int8, or E4M3 with fmt DSL_KV_FP8), k_scale and
+ * v_scale [pages][heads]; dim 64, 128 or 256.  Sequence b's token t is in page
+ * table[b * table_ld + t / page], at t % page; `width` pages per table row.
+ * seq_lens[b] counts its tokens, new ones included.  Its new tokens are rows
+ * starts[b] .. starts[b+1]-1 of the token tensors (`rows` in all), at the
+ * sequence's end; starts NULL: one new token per sequence, row b.  Page numbers
+ * outside [0, pages), tokens past the table's row and rows outside [0, rows)
+ * are skipped, wherever the device tables hold them.  max_q sizes the launch
+ * (most new tokens of a sequence; a smaller number costs time only). */
+
+/* Writes the new tokens' keys and values (k, v [rows][heads][dim], bf16 or
+ * fp16, strides in elements, unit stride in dim).  A page's scale becomes
+ * max(the one it has, amax(new)/top, 1e-12), the one it has only where older
+ * tokens stay in the page, whose codes are then moved to the new scale,
+ * round(c * old / new).  No page may be written for two sequences in one call. */
+int dsl_kv8_write(void *k_cache, void *v_cache, float *k_scale, float *v_scale, int64_t pages,
+                  int64_t heads, int64_t page, int64_t dim, int fmt, const int32_t *table,
+                  int64_t table_ld, int64_t width, const int32_t *seq_lens, const int32_t *starts,
+                  int64_t seqs, const void *k, int64_t k_row, int64_t k_head, const void *v,
+                  int64_t v_row, int64_t v_head, int64_t rows, int64_t max_q, int x_dtype,
+                  void *stream);
+
+/* Rows starts[b] .. starts[b+1]-1 of k and v [rows][heads][dim] (out_dtype bf16
+ * or fp16) become sequence b's tokens from its first on, code * scale.  Rows
+ * past its length, and of pages that are none, are zeros. */
+int dsl_kv8_read(const void *k_cache, const void *v_cache, const float *k_scale,
+                 const float *v_scale, int64_t pages, int64_t heads, int64_t page, int64_t dim,
+                 int fmt, const int32_t *table, int64_t table_ld, int64_t width,
+                 const int32_t *seq_lens, const int32_t *starts, int64_t seqs, void *k, void *v,
+                 int64_t rows, int out_dtype, void *stream);
+
+/* out = softmax(scale q k^T) v over each sequence's cached tokens; causal: new
+ * token i of n sees the tokens up to its own position len - n + i, else all of
+ * them.  q and out [rows][q_heads][dim], bf16 or fp16; query head h reads cache
+ * head h / (q_heads / heads).  A row that sees no token is zeros; rows of no
+ * sequence are not specified.  Workspace: the partial results of a context
+ * that is split over workgroups; it depends on the sizes only. */
+int dsl_kv8_attention(const void *q, int64_t q_row, int64_t q_head, int64_t q_heads,
+                      const void *k_cache, const void *v_cache, const float *k_scale,
+                      const float *v_scale, int64_t pages, int64_t heads, int64_t page, int64_t dim,
+                      int fmt, const int32_t *table, int64_t table_ld, int64_t width,
+                      const int32_t *seq_lens, const int32_t *starts, int64_t seqs, void *out,
+                      int64_t o_row, int64_t o_head, int64_t rows, int64_t max_q, float scale,
+                      int causal, int x_dtype, void *workspace, size_t workspace_bytes,
+                      void *stream);
+size_t dsl_kv8_attention_workspace_bytes(int64_t heads, int64_t page, int64_t dim, int64_t width,
+                                         int64_t seqs, int64_t rows, int64_t q_heads,
+                                         int64_t max_q);
 
 #ifdef __cplusplus
 }
