@@ -100,6 +100,7 @@ SIGNATURES = {
     "dsl_moe_grouped_fp8_gemm": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
                                         _i64, _i32, _vp, _vp, _vp]),
     "dsl_moe_combine": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i32, _vp]),
+    "dsl_int8_gemm": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp]),
     "dsl_quant_int8_rows": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp]),
     "dsl_add_rmsnorm_quant": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i32, ctypes.c_float, _i32, _i32,
                                      _vp, _vp, _vp, _vp]),

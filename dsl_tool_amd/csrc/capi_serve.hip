@@ -1,5 +1,5 @@
 // extern "C" entry points of the 8-bit attention layer, declared in
-// include/dsl_gemm.h: the residual norm, int8 row codes, the paged 8-bit cache
+// include/dsl_gemm.h: the int8 product, the residual norm, int8 row codes, the paged 8-bit cache
 // and attention over it.  As in capi.hip, everything is validated on the host
 // before anything is enqueued, and nothing is allocated.
 #include "capi_util.h"
@@ -92,6 +92,32 @@ int check_heads(const char *fn, const char *name, const void *x, int64_t row, in
 }  // namespace
 
 extern "C" {
+
+int dsl_int8_gemm(const int8_t *a, const int8_t *b, void *c, int64_t m, int64_t n, int64_t k, int64_t ldc,
+                  int out_dtype, const float *scale_a, const float *scale_b, void *stream) {
+  const char *fn = "dsl_int8_gemm";
+  int rc = check_gemm_dims(fn, m, n, k, ldc, 16, out_dtype);
+  if (rc) return rc;
+  if (k >= 1 << 17) return fail(DSL_ERR_UNSUPPORTED, "%s: k=%lld: int32 sums hold k < 131072", fn, (long long)k);
+  if (m == 0 || n == 0) return ok();
+  if ((rc = check_out(fn, a, "a")) || (rc = check_out(fn, b, "b"))) return rc;
+  if (!c || !aligned(c, out_dtype == DSL_OUT_F32 ? 4 : 2)) return fail(DSL_ERR_ARG, "%s: c is NULL or misaligned", fn);
+  if (!scale_a || !scale_b || !aligned(scale_a, 4) || !aligned(scale_b, 4))
+    return fail(DSL_ERR_ARG, "%s: scales are NULL or misaligned", fn);
+  dsl::GemmArgs p{};
+  p.a = reinterpret_cast<const uint8_t *>(a);
+  p.b = reinterpret_cast<const uint8_t *>(b);
+  p.c = c;
+  p.M = (int)m;
+  p.N = (int)n;
+  p.K = p.Kb = (int)k;
+  p.ldc = ldc;
+  p.sa = scale_a;
+  p.sb = scale_b;
+  p.ksplit = 1;
+  p.out_f32 = out_dtype == DSL_OUT_F32;
+  return hip_status(dsl::launch_gemm(dsl::MODE_INT8, p, static_cast<hipStream_t>(stream)), fn);
+}
 
 int dsl_quant_int8_rows(const void *x, int64_t rows, int64_t cols, int64_t ldx, int x_dtype, int8_t *q,
                         float *scales, void *stream) {

@@ -34,6 +34,7 @@ typedef int      v4i  __attribute__((ext_vector_type(4)));
 typedef int      v2i  __attribute__((ext_vector_type(2)));
 typedef float    v4f  __attribute__((ext_vector_type(4)));
 typedef float    v16f __attribute__((ext_vector_type(16)));
+typedef int      v16i __attribute__((ext_vector_type(16)));
 typedef __bf16   v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16   v2bf __attribute__((ext_vector_type(2)));
 

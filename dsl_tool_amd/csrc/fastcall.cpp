@@ -504,6 +504,29 @@ bool row_major(const Tensor &t) {
          aligned16(t);
 }
 
+// int8_gemm(qa, qw, scale_a, scale_b, out_dtype)
+PyObject *int8_gemm(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5) return none();
+  const Tensor *qa = gpu_tensor(a[0]), *qw = gpu_tensor(a[1]), *sa = gpu_tensor(a[2]), *sb = gpu_tensor(a[3]);
+  const int code = out_code(a[4]);
+  if (!qa || !qw || !sa || !sb || code < 0 || qa->scalar_type() != ScalarType::Char ||
+      qw->scalar_type() != ScalarType::Char || !plain(*qa, 2) || !plain(*qw, 2) || qa->size(1) != qw->size(1) ||
+      !is_scales(*sa, ScalarType::Float) || !is_scales(*sb, ScalarType::Float) || sa->numel() != qa->size(0) ||
+      sb->numel() != qw->size(0) || qw->device() != qa->device() || sa->device() != qa->device() ||
+      sb->device() != qa->device())
+    return none();
+  const int64_t m = qa->size(0), nn = qw->size(0), k = qa->size(1);
+  Tensor c;
+  const bool ok = on_device(*qa, [&] {
+    c = out_matrix(m, nn, code, *qa);
+    return dsl_int8_gemm(ptr<int8_t>(*qa), ptr<int8_t>(*qw), ptr(c), m, nn, k, nn, code, ptr<float>(*sa),
+                         ptr<float>(*sb), stream_of(*qa)) == DSL_OK;
+  });
+  return ok ? THPVariable_Wrap(c) : none();
+  END_HANDLE_TH_ERRORS
+}
+
 // quant_int8_rows(x)
 PyObject *quant_int8_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -693,7 +716,7 @@ PyMethodDef methods[] = {DSL_FN(quant_fp8_tensor), DSL_FN(quant_fp8_blocks), DSL
                          DSL_FN(quant_nvfp4),      DSL_FN(fp8_gemm),         DSL_FN(fp4_gemm),
                          DSL_FN(bf16_gemm),        DSL_FN(grouped_fp8_gemm), DSL_FN(rmsnorm_quant),
                          DSL_FN(swiglu_quant),     DSL_FN(moe_projection),   DSL_FN(lora_gemm),
-                         DSL_FN(quant_fp8_rows_batched), DSL_FN(quant_int8_rows), DSL_FN(add_rmsnorm_quant),
+                         DSL_FN(quant_fp8_rows_batched), DSL_FN(int8_gemm),        DSL_FN(quant_int8_rows), DSL_FN(add_rmsnorm_quant),
                          DSL_FN(kv8_write),        DSL_FN(kv8_read),         DSL_FN(kv8_attention),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "dsl_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -188,6 +188,23 @@ DSL_DEV void stage_store(uint8_t *smem, int buf, const StageRegs<Cfg> &r) {
 }
 
 // ----------------------------------------------------------- MFMA helpers --
+// int8: the lane's 32 bytes in two 16x16x64 steps, summed exactly in int32
+// (below 2^31 for K < 2^17); the sum stays in its registers as it is.
+DSL_DEV v4f mfma_int8(const v8i &a, const v8i &b, const v4f &c) {
+  v4i s = __builtin_bit_cast(v4i, c);
+  s = __builtin_amdgcn_mfma_i32_16x16x64_i8((v4i){a[0], a[1], a[2], a[3]}, (v4i){b[0], b[1], b[2], b[3]}, s, 0, 0, 0);
+  s = __builtin_amdgcn_mfma_i32_16x16x64_i8((v4i){a[4], a[5], a[6], a[7]}, (v4i){b[4], b[5], b[6], b[7]}, s, 0, 0, 0);
+  return __builtin_bit_cast(v4f, s);
+}
+// The same for 32x32 tiles (32x32x32 steps).
+DSL_DEV v16f mfma_int8_32(const v8i &a, const v8i &b, const v16f &c) {
+  v16i s = __builtin_bit_cast(v16i, c);
+  s = __builtin_amdgcn_mfma_i32_32x32x32_i8((v4i){a[0], a[1], a[2], a[3]}, (v4i){b[0], b[1], b[2], b[3]}, s, 0, 0, 0);
+  s = __builtin_amdgcn_mfma_i32_32x32x32_i8((v4i){a[4], a[5], a[6], a[7]}, (v4i){b[4], b[5], b[6], b[7]}, s, 0, 0, 0);
+  return __builtin_bit_cast(v16f, s);
+}
+DSL_DEV float int_value(float bits) { return (float)__builtin_bit_cast(int, bits); }
+
 DSL_DEV v4f mfma_fp8(const v8i &a, const v8i &b, const v4f &c) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
 }

@@ -88,6 +88,7 @@ struct PersCfg {
   static constexpr bool MX = MODE == MODE_MXFP4;
   static constexpr bool NV = MODE == MODE_NVFP4;
   static constexpr bool BF16 = MODE == MODE_BF16;
+  static constexpr bool INT8 = MODE == MODE_INT8;
   static constexpr bool SCALED = BLOCK || MX || NV;
   static constexpr int PKB = 128;                      // K bytes per pair (per row)
   static constexpr int CH = PKB / 16, RPI = 1024 / PKB;  // chunks per row, rows per DMA
@@ -98,10 +99,11 @@ struct PersCfg {
   static constexpr int SQA = SCALED ? BM * 16 : 0;                  // [row][16 B]
   static constexpr int SQB = BLOCK ? 1024 : (SCALED ? BN * 16 : 0); // block: [2 blocks][16 B] (+copies)
   static constexpr int SQ = SQA + SQB;
-  // grouped: per-tile epilogue scales sx[256] and sw[256] (fp32) in a ring
+  // grouped, INT8: per-tile epilogue scales sx[256] and sw[256] (fp32) in a ring
   // of three slots (the slot of tile t is refilled with tile t+3's first
   // pair, after tile t's epilogue even when a tile is a single pair)
-  static constexpr int ES = GROUPED ? 2 * 256 * 4 : 0, NES = 3;
+  static constexpr bool EPI = GROUPED || INT8;
+  static constexpr int ES = EPI ? 2 * 256 * 4 : 0, NES = 3;
   // gather: the A-row tables (256 int32) of two tiles
   static constexpr int TAB = GATHER ? 256 * 4 : 0;
   static constexpr int TAB_OFF = 2 * PAIR + 2 * SQ + NES * ES;
@@ -122,7 +124,7 @@ struct PersCfg {
   static_assert(!BLOCK || (WN <= 128 && 128 % WN == 0), "one weight-scale block per wave");
   static_assert(!GROUPED || BN == 256, "grouped: 256x256 tiles");
   static_assert(!GROUPED || MODE == MODE_FP8_TENSOR, "grouped: FP8 with row x channel scales");
-  static_assert(!GROUPED || NW == 8, "grouped: one epilogue-scale DMA per wave");
+  static_assert(!EPI || NW == 8, "one epilogue-scale DMA per wave");
   static_assert(!GATHER || (GROUPED && A_DMA == 4 * DD), "gather: A copied by waves 0-3");
 };
 
@@ -564,6 +566,9 @@ DSL_DEV void mma_row(const Frag<Cfg> &fa, const Frag<Cfg> &fb, int i, v16f (&acc
       acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w0, a0, FRESH ? zero : acc[i][j], 0, 0, 0);
       acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w1, a1, acc[i][j], 0, 0, 0);
     }
+  } else if constexpr (Cfg::INT8) {
+#pragma unroll
+    for (int j = 0; j < Cfg::TN; ++j) acc[i][j] = mfma_int8_32(fb.b[j], fa.a[i], FRESH ? zero : acc[i][j]);
   } else {
 #pragma unroll
     for (int j = 0; j < Cfg::TN; ++j)
@@ -794,16 +799,18 @@ void gemm_persist_kernel(const Args p) {
         ring.issue_scales(__builtin_amdgcn_readfirstlane((int)(quad && ring.full)), qq / Cfg::QP,
                           pipe::lds_addr(squad) + (uint32_t)((iqc & 1) * Cfg::SQ));
     }
-    if constexpr (GR) {
+    if constexpr (Cfg::EPI) {
       // a tile's first pair also brings its epilogue scales: waves 0-3 the
-      // 256 row scales sx, waves 4-7 the 256 channel scales sw of its group
+      // 256 row scales sx, waves 4-7 the 256 channel scales sw (of its group)
       if (i < 0 || i == TM - 1) {
         const bool rows = wave < 4;
         const int w4 = rows ? wave : wave - 4;
         const int last = (rows ? itr.mend - itr.m0 : p.N - itr.n0) - 1;
         int k = w4 * 64 + pers::lane_id();
         k = k < last ? k : last;
-        const float *src = rows ? p.sx + itr.m0 : p.sw + (int64_t)itr.e * p.N + itr.n0;
+        const float *src;
+        if constexpr (GR) src = rows ? p.sx + itr.m0 : p.sw + (int64_t)itr.e * p.N + itr.n0;
+        else src = rows ? static_cast<const float *>(p.sa) + itr.m0 : static_cast<const float *>(p.sb) + itr.n0;
         pers::dma4_if(__builtin_amdgcn_readfirstlane((int)(qq == 0 && iq < nkp)),
                       reinterpret_cast<const uint8_t *>(src), (uint32_t)k * 4u,
                       lds0 + (uint32_t)(2 * Cfg::PAIR + 2 * Cfg::SQ + ies * Cfg::ES + wave * 256));
@@ -838,7 +845,7 @@ void gemm_persist_kernel(const Args p) {
   // (all but a ragged last column of tiles) take the wide-store path, where
   // rows past the end (a group's or the matrix's last partial tile) are
   // masked per lane; the rest check every element.
-  int ces = 0;                     // grouped: epilogue-scale slot of the tile being finished
+  int ces = 0;                     // grouped, INT8: epilogue-scale slot of the tile being finished
   auto epilogue = [&](int t) __attribute__((always_inline)) {
     // the lane's coordinates are formed afresh (opaque to CSE): values kept
     // from the prologue would be live across the whole loop and spill
@@ -862,7 +869,8 @@ void gemm_persist_kernel(const Args p) {
     const float *esw = esx + 256;
     auto val = [&](int i, int j, int r) __attribute__((always_inline)) {
       float x = acc[i][j][r];
-      if constexpr (GR) {
+      if constexpr (Cfg::INT8) x = int_value(x);
+      if constexpr (Cfg::EPI) {
         // (acc * sx[row]) * sw[g, col], the grouped epilogue
         x = (x * esx[wm * Cfg::WM + i * 32 + r32]) *
             esw[wn * Cfg::WN + j * 32 + 8 * (r >> 2) + 4 * h + (r & 3)];
@@ -1178,7 +1186,7 @@ bool persist_supported(int mode, int M, int N, int K, int Kb, bool scales4) {
   (void)N;
   if (Kb % 16 != 0 || Kb < 128) return false;            // whole chunks
   if (Kb >= (1 << 24)) return false;                     // 24-bit row offsets
-  if (mode == MODE_FP8_TENSOR || mode == MODE_BF16) return true;
+  if (mode == MODE_FP8_TENSOR || mode == MODE_BF16 || mode == MODE_INT8) return true;
   if (mode == MODE_FP8_BLOCK) return scales4 && K > 384;  // a scale row holds a quad
   return mode == MODE_MXFP4 || mode == MODE_NVFP4;
 }
@@ -1191,6 +1199,7 @@ static hipError_t launch_persist_bn(int mode, const GemmArgs &p, hipStream_t st)
     case MODE_MXFP4: return launch_persist_mode<MODE_MXFP4, BN>(p, st);
     case MODE_NVFP4: return launch_persist_mode<MODE_NVFP4, BN>(p, st);
     case MODE_BF16: return launch_persist_mode<MODE_BF16, BN>(p, st);
+    case MODE_INT8: return launch_persist_mode<MODE_INT8, BN>(p, st);
     default: return hipErrorInvalidValue;
   }
 }

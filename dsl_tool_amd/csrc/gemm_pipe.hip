@@ -35,6 +35,26 @@ void gemm_pipe_kernel(const GemmArgs p) {
     s1 = *p.ga;
     s2 = *p.gb;
   }
+  // INT8: the scales of the lane's rows and columns (rows and columns past
+  // the edge repeat the last one's)
+  static_assert(!Cfg::INT8 || TR, "INT8 tiles are staged");
+  float srow[Cfg::INT8 ? Cfg::TM : 1];
+  v4f scol[Cfg::INT8 ? Cfg::TN : 1][4];
+  if constexpr (Cfg::INT8) {
+    const float *sa = static_cast<const float *>(p.sa), *sb = static_cast<const float *>(p.sb);
+#pragma unroll
+    for (int i = 0; i < Cfg::TM; ++i) {
+      const int row = m0 + wm * Cfg::WM + i * 32 + r32;
+      srow[i] = sa[row < p.M ? row : p.M - 1];
+    }
+#pragma unroll
+    for (int j = 0; j < Cfg::TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int col = n0 + wn * Cfg::WN + j * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
+        scol[j][r >> 2][r & 3] = sb[col < p.N ? col : p.N - 1];
+      }
+  }
   using Out = pipe::OutStage<Cfg::BM, Cfg::BN>;
   if constexpr (TR) {
     static_assert(Cfg::BM * Cfg::BN * 2 <= Cfg::LDS, "TR stages the bf16 tile in LDS");
@@ -42,6 +62,7 @@ void gemm_pipe_kernel(const GemmArgs p) {
     // 32j + 8q + 4h .. +3
     auto val = [&](int i, int j, int r) __attribute__((always_inline)) {
       float v = acc[i][j][r];
+      if constexpr (Cfg::INT8) v = (int_value(v) * srow[i]) * scol[j][r >> 2][r & 3];
       if constexpr (GLOBAL) v = (v * s1) * s2;
       return v;
     };
@@ -581,8 +602,13 @@ static hipError_t launch_pipe_cfg(const GemmArgs &p, hipStream_t st) {
   else if constexpr (Cfg::BLOCK) gemm_pipe_block_kernel<Cfg><<<tiles, Cfg::NT, 0, st>>>(p);
   else if constexpr (Cfg::BM * Cfg::BN * 2 <= Cfg::LDS) {
     const bool staged = !p.out_f32 || Cfg::BM * Cfg::BN * 4 <= Cfg::LDS;
-    if (staged) gemm_pipe_kernel<Cfg, true><<<tiles, Cfg::NT, 0, st>>>(p);
-    else gemm_pipe_kernel<Cfg, false><<<tiles, Cfg::NT, 0, st>>>(p);
+    if constexpr (Cfg::INT8) {
+      static_assert(!Cfg::INT8 || Cfg::BM * Cfg::BN * 4 <= Cfg::LDS, "either output type is staged");
+      gemm_pipe_kernel<Cfg, true><<<tiles, Cfg::NT, 0, st>>>(p);
+    } else {
+      if (staged) gemm_pipe_kernel<Cfg, true><<<tiles, Cfg::NT, 0, st>>>(p);
+      else gemm_pipe_kernel<Cfg, false><<<tiles, Cfg::NT, 0, st>>>(p);
+    }
   } else {
     gemm_pipe_kernel<Cfg, false><<<tiles, Cfg::NT, 0, st>>>(p);
   }
@@ -604,6 +630,7 @@ static hipError_t launch_pipe_small(int mode, const GemmArgs &p, hipStream_t st)
     case MODE_BF16: return launch_pipe_cfg<PipeCfg<MODE_BF16, 64, 128, 1, 4, 4, 128, 1, 1, RAG>>(p, st);
     case MODE_FP8_TENSOR: return launch_pipe_cfg<PipeCfg<MODE_FP8_TENSOR, 64, 128, 1, 4, 4, 128, 1, 1, RAG>>(p, st);
     case MODE_MXFP4: return launch_pipe_cfg<PipeCfg<MODE_MXFP4, 64, 128, 2, 4, 4, 128, 2, 0, RAG>>(p, st);
+    case MODE_INT8: return launch_pipe_cfg<PipeCfg<MODE_INT8, 64, 128, 1, 4, 4, 128, 1, 1, RAG>>(p, st);
     default: return hipErrorInvalidValue;
   }
 }
@@ -621,6 +648,7 @@ static hipError_t launch_pipe_deep(int mode, const GemmArgs &p, hipStream_t st) 
     case MODE_BF16: return launch_pipe_cfg<PipeCfg<MODE_BF16, 128, 128, 2, 2, 4, 128, 1, 1, RAG>>(p, st);
     case MODE_FP8_TENSOR: return launch_pipe_cfg<PipeCfg<MODE_FP8_TENSOR, 128, 128, 2, 2, 4, 128, 1, 1, RAG>>(p, st);
     case MODE_MXFP4: return launch_pipe_cfg<PipeCfg<MODE_MXFP4, 128, 128, 2, 4, 4, 128, 2, 0, RAG>>(p, st);
+    case MODE_INT8: return launch_pipe_cfg<PipeCfg<MODE_INT8, 128, 128, 2, 2, 4, 128, 1, 1, RAG>>(p, st);
     default: return hipErrorInvalidValue;
   }
 }
@@ -637,7 +665,7 @@ hipError_t launch_gemm_pipe(int mode, const GemmArgs &p, int variant, hipStream_
   // C += result: fp32 output through the plain epilogue only
   if (p.accumulate && (!p.out_f32 || mode_grouped_k(mode))) return hipErrorInvalidValue;
   // whole stages, an even number of them on the prefetch schedule
-  const bool pf = mode == MODE_FP8_TENSOR || mode == MODE_BF16;
+  const bool pf = mode == MODE_FP8_TENSOR || mode == MODE_BF16 || mode == MODE_INT8;
   const bool rag = p.Kb % 128 != 0, rag_deep = p.Kb % (pf ? 256 : 128) != 0;
   // the deep rings keep a tile's weight-block scales in LDS: longer K takes
   // the two-stage 128x128 tiles, which read them from memory
@@ -654,6 +682,7 @@ hipError_t launch_gemm_pipe(int mode, const GemmArgs &p, int variant, hipStream_
       case MODE_FP8_TENSOR:
         return launch_pipe_cfg<PipeCfg<MODE_FP8_TENSOR, 128, 128, 2, 2, 4, 64, 0, 1, true>>(p, st);
       case MODE_NVFP4: return launch_pipe_cfg<PipeCfg<MODE_NVFP4, 128, 128, 2, 4, 4, 64, 0, 0, true>>(p, st);
+      case MODE_INT8: return launch_pipe_cfg<PipeCfg<MODE_INT8, 128, 128, 2, 2, 4, 64, 0, 1, true>>(p, st);
       default: return launch_pipe_cfg<PipeCfg<MODE_MXFP4, 128, 128, 2, 4, 4, 64, 0, 0, true>>(p, st);
     }
   }
@@ -671,6 +700,8 @@ hipError_t launch_gemm_pipe(int mode, const GemmArgs &p, int variant, hipStream_
   // 1536x2048x4096 38.5 -> 33.5, fp32 out 1024x4096x4096 43.5 -> 40.0);
   // MXFP4 takes eight waves of 64x32 instead, two per SIMD (768x4096x2048
   // 10.5 -> 9.3 us; with the prefetch schedule it gained less).
+  if (mode == MODE_INT8)                           // variant 1
+    return launch_pipe_cfg<PipeCfg<MODE_INT8, 128, 128, 2, 2, 4, 64, 0, 1>>(p, st);
   if (mode == MODE_BF16)
     return launch_pipe_cfg<PipeCfg<MODE_BF16, 128, 128, 2, 2, 4, 64, 0, 1>>(p, st);
   if (mode == MODE_FP8_BLOCK) {

@@ -75,6 +75,7 @@ struct StreamCfg {
   static constexpr bool BLOCK = mode_grouped_k(MODE);   // fp32 scales per 128-K group
   static constexpr bool GCOL = MODE == MODE_FP8_GCOL;   // ... per W row (output column)
   static constexpr bool NV = MODE == MODE_NVFP4;
+  static constexpr bool INT8 = MODE == MODE_INT8;
   static constexpr int CHUNK = CHUNK_;               // bytes of one row per item
   static constexpr int STEPS = CHUNK / 128;          // 128-byte MFMA steps (FP8 block: groups)
   static constexpr int SBK = CHUNK / 256;            // MXFP4 512-element superblocks
@@ -121,7 +122,7 @@ struct StreamRegs {
 };
 
 // One workgroup's tile: C rows [m0, m0 + BM) x columns [n0, n0 + BN) of the
-// problem p over all of K.  gsx / gsw (grouped FP8): the output is (acc *
+// problem p over all of K.  gsx / gsw (grouped FP8, INT8): the output is (acc *
 // gsx[row]) * gsw[col] instead of the per-tensor scaling.  GATHER: row m of
 // the problem reads activation row arow[m] (clamped to [0, xrows)) of p.a;
 // each lane's row offsets are loaded once, before the first copy.
@@ -382,6 +383,8 @@ DSL_DEV void stream_tile(const GemmArgs &p, const int m0, const int n0, const fl
               const v4f sc = (v4f){sa[0][s], sa[1][s], sa[2][s], sa[3][s]} *
                              st.sb[Cfg::GCOL ? t : 0][s];
               st.acc[t][A] = part * sc + st.acc[t][A];
+            } else if constexpr (Cfg::INT8) {
+              st.acc[t][A] = mfma_int8(af, st.wf[t][s], st.acc[t][A]);
             } else if constexpr (Cfg::MODE == MODE_BF16) {
               st.acc[t][A] = mfma_bf16(af, st.wf[t][s], st.acc[t][A]);
             } else {
@@ -441,8 +444,15 @@ DSL_DEV void stream_tile(const GemmArgs &p, const int m0, const int n0, const fl
     const int combo = sl >> 6, ln = sl & 63;   // combo = t * TMA + a
     v4f v = *reinterpret_cast<const v4f *>(red + (combo * 64 + ln) * 4);
 #pragma unroll
-    for (int w = 1; w < NW; ++w)
-      v += *reinterpret_cast<const v4f *>(red + ((w * TN * TMA + combo) * 64 + ln) * 4);
+    for (int w = 1; w < NW; ++w) {
+      const v4f o = *reinterpret_cast<const v4f *>(red + ((w * TN * TMA + combo) * 64 + ln) * 4);
+      if constexpr (Cfg::INT8) v = __builtin_bit_cast(v4f, __builtin_bit_cast(v4i, v) + __builtin_bit_cast(v4i, o));
+      else v += o;
+    }
+    if constexpr (Cfg::INT8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = int_value(v[i]);
+    }
     const int t = combo / TMA, a = combo % TMA;
     const int col = t * 16 + (ln & 15), row0 = a * 16 + 4 * (ln >> 4);
 #pragma unroll
@@ -481,7 +491,7 @@ DSL_DEV void stream_tile(const GemmArgs &p, const int m0, const int n0, const fl
 
   const int row = m0 + lrow, col0 = n0 + lcol;
   if (row >= p.M) return;
-  if (gsx) {                                 // grouped: (acc * sx[row]) * sw[col]
+  if (gsx) {                                 // grouped, INT8: (acc * sx[row]) * sw[col]
     const float sxr = gsx[row];
 #pragma unroll
     for (int c = 0; c < CPT; ++c) v[c] = (v[c] * sxr) * gsw[col0 + c < p.N ? col0 + c : p.N - 1];
@@ -526,7 +536,8 @@ __global__ __launch_bounds__(Cfg::NT) void gemm_stream_kernel(const GemmArgs p) 
   const int local = blockIdx.x >> 3;
   const int mblk = local % nmb, nblk = (local / nmb) * 8 + (blockIdx.x & 7);
   if (nblk >= nnb) return;                   // whole workgroup: no barrier reached
-  stream_tile<Cfg>(p, mblk * Cfg::BM, nblk * Cfg::BN, nullptr, nullptr);
+  stream_tile<Cfg>(p, mblk * Cfg::BM, nblk * Cfg::BN, Cfg::INT8 ? static_cast<const float *>(p.sa) : nullptr,
+                   Cfg::INT8 ? static_cast<const float *>(p.sb) : nullptr);
 }
 
 // Grouped FP8 (MoE) on the streaming tiles: workgroup -> (BM-row block of one
@@ -679,7 +690,7 @@ StreamPlan plan_for(int mode, int M, int N, int Kb, bool tail) {
   // block, when that grid is one round of 192 or more workgroups (M=64
   // N=4096 K=4096: 7.4 against 8.1 us per-tensor, 11.3 against 12.2 bf16;
   // past one round, and in the block / MXFP4 forms, it measured slower)
-  if (!force_tma && (mode == MODE_FP8_TENSOR || mode == MODE_BF16) && M > 32 && M <= 64 &&
+  if (!force_tma && (mode == MODE_FP8_TENSOR || mode == MODE_BF16 || mode == MODE_INT8) && M > 32 && M <= 64 &&
       pl.tma == 4) {
     const int64_t g = (int64_t)((M + 31) / 32) * ((N + 31) / 32);
     if (g >= 192 && g <= device_cu_count()) pl.tma = pl.tn = 2;
@@ -817,6 +828,7 @@ hipError_t launch_gemm_stream(int mode, const GemmArgs &p, hipStream_t st) {
     case MODE_MXFP4: return launch_mode<MODE_MXFP4>(p, pl, st);
     case MODE_BF16: return launch_mode<MODE_BF16>(p, pl, st);
     case MODE_NVFP4: return launch_mode<MODE_NVFP4>(p, pl, st);
+    case MODE_INT8: return launch_mode<MODE_INT8>(p, pl, st);
     default: return hipErrorInvalidValue;
   }
 }

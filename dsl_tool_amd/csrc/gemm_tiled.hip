@@ -606,8 +606,9 @@ static GemmArgs columns_from(int mode, GemmArgs p, int n1) {
   p.b += (int64_t)n1 * p.Kb;
   p.c = static_cast<uint8_t *>(p.c) + (int64_t)n1 * (p.out_f32 ? 4 : 2);
   if (p.sb) {
-    const int64_t off = mode == MODE_FP8_BLOCK ? (int64_t)(n1 / 128) * ((p.K + 127) / 128) * 4
-                                               : (int64_t)n1 * scale_row_len(mode, p.K);
+    const int64_t off = mode == MODE_INT8        ? (int64_t)n1 * 4
+                        : mode == MODE_FP8_BLOCK ? (int64_t)(n1 / 128) * ((p.K + 127) / 128) * 4
+                                                 : (int64_t)n1 * scale_row_len(mode, p.K);
     p.sb = static_cast<const uint8_t *>(p.sb) + off;
   }
   p.N -= n1;
@@ -645,6 +646,31 @@ static int pipe_variant(int mode, int M, int N, int Kb) {
   return (int64_t)((M + 127) / 128) * ((N + 127) / 128) <= cu && deep_pays(mode, Kb) ? 7 : 1;
 }
 
+// INT8 codes move, and feed the matrix units, at the rate of E4M3 ones, so the
+// kernel is the one that the per-tensor form takes; there is no skinny-M kernel
+// and no split over K of its own: those shapes stream (more than 1024 rows too),
+// as does a problem of few pipelined tiles that is predicted faster streamed.
+static Route int8_route(int M, int N, int K, int Kb, bool f32) {
+  Route r = pick_route(MODE_FP8_TENSOR, M, N, K, Kb, true, true, false, f32, true);
+  if (r.path == PATH_DECODE || r.path == PATH_TILED) r.path = PATH_STREAM;
+  if (r.path != PATH_PIPE) return r;
+  if (r.variant != 6 && r.variant != 7) r.variant = 1;
+  if (stream_estimate(MODE_FP8_TENSOR, M, N, K, Kb, true) < pipe_estimate(MODE_FP8_TENSOR, r, M, N, Kb))
+    r.path = PATH_STREAM;
+  return r;
+}
+
+// The columns a persistent launch leaves over (strip_columns), streamed or on
+// pipelined tiles.
+static Route strip_route(int mode, int M, int N, int K, int Kb, bool sc4, bool sc16, bool f32) {
+  Route r = mode == MODE_INT8 ? int8_route(M, N, K, Kb, f32) : route_for(mode, M, N, K, Kb, sc4, sc16, false, f32, 0);
+  if (r.path != PATH_STREAM) {
+    r.path = PATH_PIPE;
+    r.variant = pipe_variant(mode == MODE_INT8 ? MODE_FP8_TENSOR : mode, M, N, Kb);
+  }
+  return r;
+}
+
 void describe_gemm(int mode, int64_t M, int64_t N, int64_t K, bool f32, bool accumulate, char *buf,
                    size_t len) {
   const int Kb = (mode == MODE_MXFP4 || mode == MODE_NVFP4) ? (int)(K / 2)
@@ -665,7 +691,8 @@ void describe_gemm(int mode, int64_t M, int64_t N, int64_t K, bool f32, bool acc
       snprintf(to, room, "decode");
     }
   };
-  Route r = route_for(mode, (int)M, (int)N, (int)K, Kb, true, true, true, f32, SIZE_MAX);
+  Route r = mode == MODE_INT8 ? int8_route((int)M, (int)N, (int)K, Kb, f32)
+                              : route_for(mode, (int)M, (int)N, (int)K, Kb, true, true, true, f32, SIZE_MAX);
   if (accumulate && f32) accumulate_route(mode, &r, (int)M, (int)N, (int)K, Kb, true, true);
   name(r, (int)M, (int)N, buf, len);
   GemmArgs p{};
@@ -674,11 +701,7 @@ void describe_gemm(int mode, int64_t M, int64_t N, int64_t K, bool f32, bool acc
   p.accumulate = accumulate;
   const int strip = r.path != PATH_PERSIST || r.narrow || r.pad_scales ? 0 : strip_columns(p);
   if (strip == 0) return;
-  Route rest = route_for(mode, (int)M, strip, (int)K, Kb, true, true, false, f32, 0);
-  if (rest.path != PATH_STREAM) {
-    rest.path = PATH_PIPE;
-    rest.variant = pipe_variant(mode, (int)M, strip, Kb);
-  }
+  const Route rest = strip_route(mode, (int)M, strip, (int)K, Kb, true, true, f32);
   const size_t used = strlen(buf);
   snprintf(buf + used, len - used, " + ");
   name(rest, (int)M, strip, buf + strlen(buf), len - strlen(buf));
@@ -702,8 +725,9 @@ hipError_t launch_gemm(int mode, GemmArgs p, hipStream_t st) {
   const bool padded = (mode == MODE_MXFP4 || mode == MODE_NVFP4) && p.ws &&
                       (reinterpret_cast<uintptr_t>(p.ws) & 15) == 0 &&
                       p.ws_bytes >= (size_t)((int64_t)p.M + p.N) * (size_t)padded_pitch(mode, p.K);
-  Route r = route_for(mode, p.M, p.N, p.K, p.Kb, (sc & 3) == 0, (sc & 15) == 0, padded, p.out_f32 != 0,
-                      p.ws ? p.ws_bytes : 0);
+  Route r = mode == MODE_INT8 ? int8_route(p.M, p.N, p.K, p.Kb, p.out_f32 != 0)
+                              : route_for(mode, p.M, p.N, p.K, p.Kb, (sc & 3) == 0, (sc & 15) == 0, padded,
+                                          p.out_f32 != 0, p.ws ? p.ws_bytes : 0);
   if (p.lora_scales) {   // the LoRA epilogue: the streaming kernel only
     if (mode != MODE_BF16 || !stream_supported(mode, p.M, p.N, p.K, p.Kb, true) || p.accumulate)
       return hipErrorInvalidValue;
@@ -741,10 +765,8 @@ hipError_t launch_gemm(int mode, GemmArgs p, hipStream_t st) {
       const hipError_t e = launch_gemm_persist(mode, main, st, false);
       if (e != hipSuccess) return e;
       const GemmArgs rest = columns_from(mode, p, main.N);
-      return route_for(mode, rest.M, rest.N, rest.K, rest.Kb, (sc & 3) == 0, (sc & 15) == 0, false, p.out_f32 != 0, 0).path ==
-                     PATH_STREAM
-                 ? launch_gemm_stream(mode, rest, st)
-                 : launch_gemm_pipe(mode, rest, pipe_variant(mode, rest.M, rest.N, rest.Kb), st);
+      const Route rr = strip_route(mode, rest.M, rest.N, rest.K, rest.Kb, (sc & 3) == 0, (sc & 15) == 0, p.out_f32 != 0);
+      return rr.path == PATH_STREAM ? launch_gemm_stream(mode, rest, st) : launch_gemm_pipe(mode, rest, rr.variant, st);
     }
     return launch_gemm_persist(mode, p, st, r.narrow);
   }

@@ -38,10 +38,12 @@ size_t quant_scratch_bytes();
 // ---------------------------------------------------------------- GEMMs --
 // FP8_BLOCK: 1x128 activation groups and 128x128 weight blocks; FP8_GCOL:
 // 1x128 activation groups and one weight scale per output column per
-// 128-K group (the reference's groupwise layout sb[K/128][N]).
+// 128-K group (the reference's groupwise layout sb[K/128][N]).  INT8: int8
+// codes with one scale per activation row and per output column; its
+// accumulators are int32, held in the fp32 modes' registers bit for bit.
 enum GemmMode {
   MODE_FP8_TENSOR = 0, MODE_FP8_BLOCK = 1, MODE_MXFP4 = 2, MODE_NVFP4 = 3, MODE_BF16 = 4,
-  MODE_FP8_GCOL = 5
+  MODE_FP8_GCOL = 5, MODE_INT8 = 6
 };
 // Both FP8 modes whose scales change with every 128-K group.
 constexpr bool mode_grouped_k(int mode) { return mode == MODE_FP8_BLOCK || mode == MODE_FP8_GCOL; }
@@ -55,11 +57,11 @@ struct GemmArgs {
   const uint8_t *b;      // [N][Kb] packed, K-major
   void *c;               // [M][ldc] bf16 or fp32
   int M, N, K;           // K in elements
-  int Kb;                // bytes per packed row (FP8: K, FP4: K/2, BF16: 2K)
+  int Kb;                // bytes per packed row (FP8, INT8: K, FP4: K/2, BF16: 2K)
   int64_t ldc;
   const void *sa;        // FP8_BLOCK / GCOL: float [M][nkg]; MX: uint8 [M][K/32]; NV: uint8 [M][K/16]
   const void *sb;        // FP8_BLOCK: float [ceil(N/128)][nkg]; FP8_GCOL: float [nkg][N];
-                         // MX/NV as sa for N
+                         // MX/NV as sa for N; INT8: float sa [M], sb [N]
   const float *ga;       // FP8_TENSOR: scale_a; NV: global_a
   const float *gb;       // FP8_TENSOR: scale_b; NV: global_b
   float *ws;             // split-K: one fp32 [M][N] partial slice per K split

@@ -112,6 +112,7 @@ struct PipeCfg {
   static constexpr bool NV = MODE == MODE_NVFP4;
   static constexpr bool FP4 = MX || NV;
   static constexpr bool BF16 = MODE == MODE_BF16;           // 64-byte k-step = 32 bf16 of K
+  static constexpr bool INT8 = MODE == MODE_INT8;           // int32 sums in acc's registers
   static constexpr bool BLOCK = mode_grouped_k(MODE);       // one 128-K scale group per stage
   static constexpr bool GCOL = MODE == MODE_FP8_GCOL;       // ... with a weight scale per column
   static constexpr int CH = SKB / 16, RPI = 1024 / SKB;     // chunks per row, rows per DMA
@@ -425,6 +426,8 @@ struct KFrag<Cfg, false> {
     for (int j = 0; j < Cfg::TN; ++j) {
       if constexpr (Cfg::BF16)
         acc[i][j] = mma_bf16(a[i], b[j], acc[i][j]);
+      else if constexpr (Cfg::INT8)
+        acc[i][j] = mfma_int8_32(a[i], b[j], acc[i][j]);
       else
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b[j], acc[i][j], 0, 0,
                                                                     0, 0, 0, 0);
@@ -438,6 +441,8 @@ struct KFrag<Cfg, false> {
     for (int j = 0; j < Cfg::TN; ++j) {
       if constexpr (Cfg::BF16)
         acc[i][j] = mma_bf16(b[j], a[i], acc[i][j]);
+      else if constexpr (Cfg::INT8)
+        acc[i][j] = mfma_int8_32(b[j], a[i], acc[i][j]);
       else
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a[i], acc[i][j], 0, 0,
                                                                     0, 0, 0, 0);

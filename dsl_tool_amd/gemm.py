@@ -278,6 +278,38 @@ def fp4_gemm_packed(qa, sa, qw, sw, *, fmt: str = "mxfp4", global_a=None, global
     return c
 
 
+def int8_gemm_packed(qa, qw, scale_a, scale_b, *, out_dtype=torch.bfloat16, out=None):
+    """GEMM on int8 codes: ``C[m, n] = scale_a[m] * scale_b[n] * sum_k qa[m, k]
+    qw[n, k]``, the sum exact in int32.
+
+    qa [M, K] and qw [N, K] int8 (K % 16 == 0, K < 131072), scale_a [M] (one per
+    token, :func:`quant.quant_int8_rows` or :func:`fused.add_rmsnorm_quant`) and
+    scale_b [N] (one per output channel) float32.
+    """
+    if out is None:
+        c = N.fast().int8_gemm(qa, qw, scale_a, scale_b, out_dtype)
+        if c is not None:
+            return c
+    dev = _require_gpu(qa, qw, scale_a, scale_b)
+    if qa.dtype != torch.int8 or qw.dtype != torch.int8:
+        raise TypeError(f"int8_gemm_packed: codes must be int8 (got {qa.dtype}, {qw.dtype})")
+    if qa.dim() != 2 or qw.dim() != 2:
+        raise ValueError("int8_gemm_packed: codes must be 2-D")
+    qa, qw = N.vec_rows(qa), N.vec_rows(qw)
+    M, K = qa.shape
+    Nn, K2 = qw.shape
+    if K != K2:
+        raise ValueError(f"K mismatch: A has {K}, W has {K2}")
+    scale_a, scale_b = scale_a.contiguous().float(), scale_b.contiguous().float()
+    if scale_a.numel() != M or scale_b.numel() != Nn:
+        raise ValueError("int8_gemm_packed: scales must be [M] and [N]")
+    c = _out_tensor(out, M, Nn, out_dtype, dev)
+    with torch.cuda.device(dev):
+        N.call("dsl_int8_gemm", N.ptr(qa), N.ptr(qw), N.ptr(c), M, Nn, K, c.stride(0), _out_code(c.dtype),
+               N.ptr(scale_a), N.ptr(scale_b), N.stream_of(dev))
+    return c
+
+
 def grouped_fp8_gemm_packed(qx, sx, qw, sw, offsets, *, out_dtype=torch.bfloat16, out=None):
     """Variable-size grouped GEMM on E4M3 codes.
 

@@ -362,6 +362,14 @@ size_t dsl_gemm_workspace_bytes(int op, int64_t m, int64_t n, int64_t k);
  * reference has none of them.
  */
 
+/* C[M,N] = scale_a[m] * scale_b[n] * sum_k A[m,k] W[n,k] on int8 codes, A
+ * [M][K] and W [N][K] (`b`) K-major, one scale per row of each (token, output
+ * channel); C bf16 or fp32, ldc >= n.  The sums are exact (int32), then scaled
+ * in fp32.  k % 16 == 0, k < 131072; no workspace. */
+int dsl_int8_gemm(const int8_t *a, const int8_t *b, void *c, int64_t m, int64_t n, int64_t k,
+                  int64_t ldc, int out_dtype, const float *scale_a, const float *scale_b,
+                  void *stream);
+
 /* int8 codes with one scale per row: s = max(amax/127, 1e-12), q =
  * round(x / s) (the IEEE quotient, ties to even).  x bf16, fp16 or fp32 with
  * unit column stride; cols % 8 == 0, cols <= 32768, ldx % 8 == 0.  q [rows][cols]. */
