@@ -16,6 +16,7 @@
 namespace dsl {
 
 constexpr int kTile = 64;      // tokens per step of a wave
+constexpr int kPromptRows = 64;   // query rows of a sequence and cache head from which attn_prompt.hip serves
 
 // RB blocks of 16 query rows share every load.  blockIdx: x split, y head +
 // heads * row block, z sequence.
@@ -277,11 +278,27 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const 
 }
 
 struct AttnPlan {
+  bool prompt;
   int rb, nblk, nsplit;
 };
 static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
   AttnPlan a;
   const int64_t rows = (int64_t)max_q * (q_heads / c.heads);
+  a.prompt = rows > kPromptRows;
+  if (a.prompt) {
+    const int per = attn_prompt_rows(c.dim);
+    const int64_t pairs = (int64_t)c.heads * c.seqs, blocks = (rows + per - 1) / per;
+    const int64_t room = ((int64_t)1 << 30) / pairs;
+    a.rb = 0;
+    a.nblk = (int)(blocks < room ? blocks : room);
+    // one workgroup per CU; a split has four tiles at least
+    const int64_t tiles = ((int64_t)c.width * c.page + kTile - 1) / kTile;
+    int64_t ns = device_cu_count() / (pairs * a.nblk);
+    if (ns > tiles / 4) ns = tiles / 4;
+    if (ns > 64) ns = 64;
+    a.nsplit = ns < 1 ? 1 : (int)ns;
+    return a;
+  }
   // (dim 256: two blocks of rows spill)
   a.rb = rows <= 16 || c.dim > 128 ? 1 : 2;
   const int64_t blocks = (rows + 16 * a.rb - 1) / (16 * a.rb), room = 65535 / c.heads;
@@ -311,7 +328,10 @@ static void launch_rows(const KvCacheArgs &c, const AttnArgs &p, const AttnPlan 
 template <int SRC>
 static hipError_t launch_src(const KvCacheArgs &c, const AttnArgs &p, hipStream_t st) {
   const AttnPlan a = attn_plan(c, p.q_heads, p.max_q);
-  if (c.fp8) {
+  if (a.prompt) {
+    const hipError_t e = launch_attn_prompt(SRC, c, p, a.nblk, a.nsplit, st);
+    if (e != hipSuccess) return e;
+  } else if (c.fp8) {
     if (c.dim == 64) launch_rows<SRC, true, 64>(c, p, a, st);
     else if (c.dim == 128) launch_rows<SRC, true, 128>(c, p, a, st);
     else launch_rows<SRC, true, 256>(c, p, a, st);
