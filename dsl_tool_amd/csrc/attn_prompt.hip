@@ -45,6 +45,32 @@ DSL_DEV float halves_sum(float v) {
   return u2f(a[0]) + u2f(a[1]);
 }
 
+// v *= f when the wave-uniform `on` is non-zero.  The branch is inside the asm:
+// one in the source made the compiler keep a second copy of the output and move
+// all of it there and back in every tile.  (The products that wrote v are done:
+// the caller has read later ones' results; f comes from v_exp_f32, hence the
+// s_nop.)
+DSL_DEV void scale_if(int on, v16f &v, float f) {
+  float e[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) e[i] = v[i];
+  asm volatile(
+      "s_cmp_eq_u32 %17, 0\n\t"
+      "s_cbranch_scc1 .Lscale_skip_%=\n\t"
+      "s_nop 1\n\t"
+      "v_mul_f32 %0, %0, %16\n\tv_mul_f32 %1, %1, %16\n\tv_mul_f32 %2, %2, %16\n\tv_mul_f32 %3, %3, %16\n\t"
+      "v_mul_f32 %4, %4, %16\n\tv_mul_f32 %5, %5, %16\n\tv_mul_f32 %6, %6, %16\n\tv_mul_f32 %7, %7, %16\n\t"
+      "v_mul_f32 %8, %8, %16\n\tv_mul_f32 %9, %9, %16\n\tv_mul_f32 %10, %10, %16\n\tv_mul_f32 %11, %11, %16\n\t"
+      "v_mul_f32 %12, %12, %16\n\tv_mul_f32 %13, %13, %16\n\tv_mul_f32 %14, %14, %16\n\tv_mul_f32 %15, %15, %16\n"
+      ".Lscale_skip_%=:"
+      : "+v"(e[0]), "+v"(e[1]), "+v"(e[2]), "+v"(e[3]), "+v"(e[4]), "+v"(e[5]), "+v"(e[6]), "+v"(e[7]), "+v"(e[8]),
+        "+v"(e[9]), "+v"(e[10]), "+v"(e[11]), "+v"(e[12]), "+v"(e[13]), "+v"(e[14]), "+v"(e[15])
+      : "v"(f), "s"(on)
+      : "scc");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = e[i];
+}
+
 // LDS slot of 16-byte chunk c of row r: rows of D bytes * 2 (K) and 128 bytes
 // (V); both readers (32 rows, chunks c and c + 1 by lane half) meet no bank twice.
 template <int CHUNKS>
@@ -74,19 +100,32 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
   constexpr bool F16 = SRC == SRC_F16;
   constexpr int KK = D / 16, DT = D / 32, U = Cfg::UNITS, KU = kPTile * D / 16;
   __shared__ __align__(16) uint8_t lds[2 * Cfg::STAGE];
-  __shared__ float s_scale[2][8];                // of a tile's four 16-token groups: ks, vs
-  __shared__ int s_flag[2][2];                   // groups in no page (bits), NaN codes among V
+  __shared__ __align__(16) float s_scale[2][8];  // of a tile's four 16-token groups: ks, vs
+  __shared__ float2 s_log[2][4];                 // log2 vs, 1 / vs
+  __shared__ __align__(16) int s_page[4][4];     // the groups' pages, -1: none
+  __shared__ int s_odd[2], s_bad[4];             // scales off the common path; NaN codes among V
   // tokens (bits) whose V code is NaN, by column: staged as 0, since 0 * NaN
   // would carry one to rows that do not see it
   __shared__ uint64_t s_nan[2][FP8 ? D : 1];
+  __shared__ uint32_t s_row[FP8 ? Cfg::ROWS : 1][DT];   // ... and the columns (bits) that a row gets one in
   const int pairs = c.heads * c.seqs;
-  const int blk = nblk - 1 - blockIdx.x / pairs, pair = blockIdx.x % pairs;   // the longest first
+  // Row blocks from the last, the longest, on.  Workgroups go to the eight XCDs,
+  // and there to four shader engines, in turn: the pairs of an XCD (whose rows
+  // share its L2) are rotated from row to row, or every other engine could get
+  // one sequence's and run idle where that is the shorter one (two prompts of
+  // 3600 and 2000 tokens: CUs busy 54% of the time).
+  int blk = blockIdx.x / pairs, pair = blockIdx.x % pairs;
+  if (pairs % 8 == 0) {
+    const int n = pairs / 8, j = (blockIdx.x >> 3) % n;
+    pair = (j + (n == 2 ? blk / 2 : blk)) % n * 8 + (blockIdx.x & 7);
+  }
+  blk = nblk - 1 - blk;
   const int head = pair % c.heads, b = pair / c.heads, split = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, h = lane >> 5;
   const SeqView s = seq_view(c, b);
   const int rows = s.n * p.group;
-  const int P = c.page, room = c.width * P;
+  const int P = c.page, pshift = 31 - __builtin_clz(P), room = c.width * P;
   const int len = s.len < room ? s.len : room;
   const int64_t hstride = (int64_t)P * D;
 
@@ -110,6 +149,10 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
 #pragma unroll
       for (int k = 0; k < KK; ++k) qf[k] = *reinterpret_cast<const v4i *>(qp + 16 * k + 8 * h);
     }
+    // they have arrived before the loop: a wait for them there would be one for
+    // the tiles' loads too
+#pragma unroll
+    for (int k = 0; k < KK; ++k) asm volatile("" : "+v"(qf[k]));
     const int seen = s.first + qi + 1;
     const int limit = p.causal ? (seen > 0 ? (seen < len ? seen : len) : 0) : len;
     int low = len;                               // tokens that every row of the wave sees
@@ -124,60 +167,71 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = (v16f){};
 
-    // this thread's loads of a tile: units tid + NT j, K's first
-    int pid[U], spid = -1;                       // pages of its units, of its scale
+    // Pages go to LDS three tiles ahead (four threads look them up a tile before
+    // that), codes and scales to registers two tiles ahead.
     uint4 raw[U];
     float sraw = 0.f;
+    int page = -1;
     auto find = [&](int tile) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int u = tid + Cfg::NT * j;
-        const int tok = tile * kPTile + (u < KU ? u / (D / 16) : (u & 3) * 16);
-        pid[j] = tok < len ? (int)page_of(c, b, tok / P) : -1;
-      }
-      const int tok = tile * kPTile + (tid & 3) * 16;
-      spid = tid < 8 && tok < len ? (int)page_of(c, b, tok / P) : -1;
+      const int tok = tile * kPTile + tid * 16;
+      if (tid < 4) page = tile < t1 && tok < len ? (int)page_of(c, b, tok >> pshift) : -1;
     };
+    auto keep = [&](int tile) __attribute__((always_inline)) {
+      if (tid < 4) s_page[tile & 3][tid] = page;
+    };
+    // this thread's unit j: 16 codes of K (D <= 64: by wave) or of V
+    auto is_k = [&](int j) __attribute__((always_inline)) { return U > 1 ? j < U / 2 : wave < Cfg::NW / 2; };
     auto load = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         const int u = tid + Cfg::NT * j;
-        const int64_t base = ((int64_t)(pid[j] < 0 ? 0 : pid[j]) * c.heads + head) * hstride;
-        const uint8_t *at = u < KU ? c.k + base + (int64_t)((tile * kPTile + u / (D / 16)) & (P - 1)) * D + (u % (D / 16)) * 16
-                                   : c.v + base + (int64_t)((u - KU) >> 2) * P + ((tile * kPTile + (u & 3) * 16) & (P - 1));
-        raw[j] = *reinterpret_cast<const uint4 *>(at);
-        if (u >= KU && pid[j] < 0) raw[j] = make_uint4(0, 0, 0, 0);
+        if (is_k(j)) {
+          const int r = u / (D / 16), pg = s_page[tile & 3][r >> 4];
+          const uint8_t *at = c.k + ((int64_t)(pg < 0 ? 0 : pg) * c.heads + head) * hstride +
+                              (((tile * kPTile + r) & (P - 1)) * D + (u % (D / 16)) * 16);
+          raw[j] = *reinterpret_cast<const uint4 *>(at);
+        } else {
+          const int g = u & 3, pg = s_page[tile & 3][g];
+          const uint8_t *at = c.v + ((int64_t)(pg < 0 ? 0 : pg) * c.heads + head) * hstride +
+                              ((((u - KU) >> 2) << pshift) + ((tile * kPTile + g * 16) & (P - 1)));
+          raw[j] = *reinterpret_cast<const uint4 *>(at);
+          if (FP8 && pg < 0) raw[j] = make_uint4(0, 0, 0, 0);
+        }
       }
-      if (tid < 8) sraw = spid < 0 ? 0.f : (tid < 4 ? c.k_scale : c.v_scale)[(int64_t)spid * c.heads + head];
+      if (tid < 8) {
+        const int pg = s_page[tile & 3][tid & 3];
+        sraw = pg < 0 ? 0.f : (tid < 4 ? c.k_scale : c.v_scale)[(int64_t)pg * c.heads + head];
+      }
     };
     // the loaded tile as 16-bit operands
-    auto stage = [&](int tile, int buf, bool absent) __attribute__((always_inline)) {
+    auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
       uint8_t *kb = lds + buf * Cfg::STAGE, *vb = kb + Cfg::TILE;
       uint32_t bad = 0;
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         const int u = tid + Cfg::NT * j;
         uint4 w = raw[j];
-        if (u < KU) {
+        if (is_k(j)) {
           const int r = u / (D / 16), ch = (u % (D / 16)) * 2;
-          *reinterpret_cast<v4i *>(kb + r * (2 * D) + pslot<Cfg::KC>(r, ch) * 16) = codes8<FP8, F16>(w.x, w.y);
-          *reinterpret_cast<v4i *>(kb + r * (2 * D) + pslot<Cfg::KC>(r, ch + 1) * 16) = codes8<FP8, F16>(w.z, w.w);
+          uint8_t *to = kb + r * (2 * D);
+          const int at = pslot<Cfg::KC>(r, ch) * 16;
+          *reinterpret_cast<v4i *>(to + at) = codes8<FP8, F16>(w.x, w.y);
+          *reinterpret_cast<v4i *>(to + (at ^ 16)) = codes8<FP8, F16>(w.z, w.w);
         } else {
           const int d = (u - KU) >> 2, g = u & 3;
-          if constexpr (FP8) {                   // codes past the end can be NaN
-            const int nv = len - (tile * kPTile + g * 16);
-            if (nv < 16) {
-              uint32_t *x = &w.x;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int n = nv - 4 * i;
-                x[i] &= n >= 4 ? 0xffffffffu : (n <= 0 ? 0u : (1u << (8 * n)) - 1);
-              }
+          if constexpr (FP8) {
+            if (tile * kPTile + kPTile > len) {  // codes past the end can be NaN
+              const int nv = len - (tile * kPTile + g * 16);
+              auto first = [&](int n) { return n >= 4 ? 0xffffffffu : (n <= 0 ? 0u : (1u << (8 * n)) - 1); };
+              w.x &= first(nv);
+              w.y &= first(nv - 4);
+              w.z &= first(nv - 8);
+              w.w &= first(nv - 12);
             }
             const uint32_t bx = nan_bytes(w.x), by = nan_bytes(w.y), bz = nan_bytes(w.z), bw = nan_bytes(w.w);
             uint32_t at = 0;
             if (bx | by | bz | bw) {
-              auto nibble = [](uint32_t m) { return ((m >> 7) * 0x01020408u) >> 24 & 15; };
+              auto nibble = [](uint32_t x) { return ((x >> 7) * 0x01020408u) >> 24 & 15; };
               at = nibble(bx) | nibble(by) << 4 | nibble(bz) << 8 | nibble(bw) << 12;
               w.x &= ~((bx >> 7) * 255u);
               w.y &= ~((by >> 7) * 255u);
@@ -187,134 +241,157 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
             reinterpret_cast<uint16_t *>(&s_nan[buf][d])[g] = (uint16_t)at;
             bad |= at;
           }
-          *reinterpret_cast<v4i *>(vb + d * 128 + pslot<8>(d, 2 * g) * 16) = codes8<FP8, false>(w.x, w.z);
-          *reinterpret_cast<v4i *>(vb + d * 128 + pslot<8>(d, 2 * g + 1) * 16) = codes8<FP8, false>(w.y, w.w);
+          uint8_t *to = vb + d * 128;
+          const int at = pslot<8>(d, 2 * g) * 16;
+          *reinterpret_cast<v4i *>(to + at) = codes8<FP8, false>(w.x, w.z);
+          *reinterpret_cast<v4i *>(to + (at ^ 16)) = codes8<FP8, false>(w.y, w.w);
         }
       }
-      if (tid < 8) s_scale[buf][tid] = sraw * (tid < 4 ? p.scale * kLog2e : 1.f);
-      if (tid < 64) {
-        const uint64_t none = __ballot(absent && tid < 4);
-        if (tid == 0) s_flag[buf][0] = (int)none;
+      if (tid < 8) {
+        const float x = tid < 4 ? sraw * (p.scale * kLog2e) : sraw;
+        s_scale[buf][tid] = x;
+        // scales that the common path takes: its scores' maximum follows the
+        // codes', and probabilities take theirs as a logarithm
+        const bool odd = tid < 4 ? !(x >= 0.f) : !(x >= 0x1p-60f && x <= 0x1p60f);
+        const uint64_t some = __ballot(odd);
+        if (tid == 0) s_odd[buf] = some != 0;
+        if (tid >= 4) s_log[buf][tid & 3] = make_float2(__builtin_amdgcn_logf(x), 1.0f / x);
       }
       if constexpr (FP8) {
-        if (__any(bad) && lane == 0) s_flag[buf][1] = 1;
+        if (__any(bad) && lane == 0) s_bad[tile & 3] = 1;
       }
     };
 
-    if (tid < 2) s_flag[tid][1] = 0;
-    __syncthreads();                             // also: the last block's readers
-    bool absent = false;                         // of the loaded tile: this thread's scale has no page
-    if (t0 < t1) {
-      find(t0);
-      load(t0);
-      absent = spid < 0;
-      if (t0 + 1 < t1) find(t0 + 1);
-      stage(t0, t0 & 1, absent);
-      if (t0 + 1 < t1) {
-        load(t0 + 1);
-        absent = spid < 0;
-      }
-      if (t0 + 2 < t1) find(t0 + 2);
+    __syncthreads();                             // the last block's readers
+    if (tid < 4) s_bad[tid] = 0;
+    if constexpr (FP8) {
+      for (int i = tid; i < Cfg::ROWS * DT; i += Cfg::NT) s_row[i / DT][i % DT] = 0;
     }
-    for (int tile = t0; tile < t1; ++tile) {
-      __syncthreads();                           // the tile is staged, the other stage is read
+    if (t0 < t1) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        find(t0 + i);
+        keep(t0 + i);
+      }
+      find(t0 + 3);
+      __syncthreads();
+      load(t0);
+      stage(t0, t0 & 1);
+      if (t0 + 1 < t1) load(t0 + 1);
+    }
+    // what follows a tile, behind its scores: the next one's operands, the loads of
+    // the one after, the pages of the third
+    auto advance = [&](int tile) __attribute__((always_inline)) {
+      if (tile + 1 < t1) {
+        if (FP8 && tid == 0) s_bad[(tile + 2) & 3] = 0;   // set a tile later at the earliest
+        stage(tile + 1, (tile + 1) & 1);
+        if (tile + 2 < t1) load(tile + 2);
+        keep(tile + 3);
+        find(tile + 4);
+      }
+    };
+    // a tile whose tokens all rows of the wave see, in pages that there are, of
+    // common scales
+    auto common = [&](int tile) __attribute__((always_inline)) {
+      const v4i pg = *reinterpret_cast<const v4i *>(s_page[tile & 3]);
+      const bool none = min(min(pg[0], pg[1]), min(pg[2], pg[3])) < 0;
+      return __builtin_amdgcn_readfirstlane((int)(tile * kPTile + kPTile <= low && !none && !s_odd[tile & 1])) != 0;
+    };
+    // fragment addresses: the rows' swizzles do not depend on t and d, and flip no
+    // bit of 32 k, so one register each; formed afresh in every tile (kept for all
+    // k they spill)
+    const int kat0 = r32 * (2 * D) + pslot<Cfg::KC>(r32, h) * 16, vat0 = r32 * 128 + pslot<8>(r32, h) * 16;
+    auto step = [&](auto slow_tag, int tile) __attribute__((always_inline)) {
+      constexpr bool SLOW = decltype(slow_tag)::value;
       const int buf = tile & 1;
       const uint8_t *kb = lds + buf * Cfg::STAGE, *vb = kb + Cfg::TILE;
-      // the fragments' addresses: the rows' swizzles do not depend on t and d, and
-      // flip no bit of 32 k, so one register each; formed afresh in every tile
-      // (kept for all k they spill)
-      int kat = r32 * (2 * D) + pslot<Cfg::KC>(r32, h) * 16, vat = r32 * 128 + pslot<8>(r32, h) * 16;
+      int kat = kat0, vat = vat0;
       asm volatile("" : "+v"(kat), "+v"(vat));
-      const bool work = tile * kPTile < limit;
-      const bool any = __any(work);
-
-      v16f sc[2];
-      float ks[4], vs[4];
-      bool masked = false;
-      int none = 0, nans = 0;
-      if (any) {
-        const v4f k4 = *reinterpret_cast<const v4f *>(&s_scale[buf][0]), v4 = *reinterpret_cast<const v4f *>(&s_scale[buf][4]);
+      // four fragments ahead of the products that take them
+      v16f sc[2] = {};
+      {
+        v4i a[2][4];
+        auto read = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          ks[g] = k4[g];
-          vs[g] = v4[g];
-        }
-        none = s_flag[buf][0];
-        nans = FP8 ? s_flag[buf][1] : 0;
-        masked = __builtin_amdgcn_readfirstlane(
-            (int)(tile * kPTile + kPTile > low || none || !(fminf(fminf(ks[0], ks[1]), fminf(ks[2], ks[3])) >= 0.f)));
+          for (int i = 0; i < 4; ++i)
+            a[n & 1][i] = *reinterpret_cast<const v4i *>(kb + (kat ^ (32 * (2 * n + (i >> 1)))) + (i & 1) * 32 * 2 * D);
+        };
+        read(0);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          sc[t] = (v16f){};
+        for (int n = 0; n < KK / 2; ++n) {
+          if (n + 1 < KK / 2) read(n + 1);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int k = 0; k < KK; ++k) {
-            const v4i a = *reinterpret_cast<const v4i *>(kb + (kat ^ (32 * k)) + t * 32 * 2 * D);
-            sc[t] = mfma32<F16>(a, qf[k], sc[t]);
-          }
+          for (int i = 0; i < 4; ++i) sc[i & 1] = mfma32<F16>(a[n & 1][i], qf[2 * n + (i >> 1)], sc[i & 1]);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if (tile + 1 < t1) {
-        if (tid == 0 && FP8) s_flag[buf ^ 1][1] = 0;
-        stage(tile + 1, buf ^ 1, absent);
-        if (tile + 2 < t1) {
-          load(tile + 2);
-          absent = spid < 0;
-        }
-        if (tile + 3 < t1) find(tile + 3);
-      }
-      if (!any) continue;
+      advance(tile);
       __builtin_amdgcn_sched_barrier(0);
 
-      float top;
-      if (!masked) {
-        top = -INFINITY;
+      const v4f ks = *reinterpret_cast<const v4f *>(&s_scale[buf][0]);
+      float top = -INFINITY;
+      if constexpr (!SLOW) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          float x = sc[g >> 1][8 * (g & 1)];
+          float x = -INFINITY;
 #pragma unroll
-          for (int i = 1; i < 8; ++i) x = fmaxf(x, sc[g >> 1][8 * (g & 1) + i]);
+          for (int i = 0; i < 8; i += 2) x = fmaxf(fmaxf(x, sc[g >> 1][8 * (g & 1) + i]), sc[g >> 1][8 * (g & 1) + i + 1]);
           top = fmaxf(top, x * ks[g]);
         }
       } else {
-        top = -INFINITY;
+        const v4i pg = *reinterpret_cast<const v4i *>(s_page[tile & 3]);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int tok = tile * kPTile + 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * h + (i & 3);
-          float v = sc[i >> 4][i & 15] * ks[i >> 3];
-          v = tok < limit && !(none >> (i >> 3) & 1) ? v : -INFINITY;
-          sc[i >> 4][i & 15] = v;
-          top = fmaxf(top, v);
-        }
+        for (int g = 0; g < 4; ++g)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) ks[g] = 1.f;
+          for (int i = 0; i < 8; ++i) {
+            const int tok = tile * kPTile + 16 * g + 8 * (i >> 2) + 4 * h + (i & 3);
+            const float v = tok < limit && pg[g] >= 0 ? sc[g >> 1][8 * (g & 1) + i] * ks[g] : -INFINITY;
+            sc[g >> 1][8 * (g & 1) + i] = v;
+            top = fmaxf(top, v);
+          }
       }
       top = halves_max(top);
-      if (__any(top > m + 8.f || m == -INFINITY)) {
-        const float now = fmaxf(m, top), ref = now == -INFINITY ? 0.f : now;
-        const float alpha = __builtin_amdgcn_exp2f(m - ref);
-        m = now;
-        l *= alpha;
+      const int grow = __builtin_amdgcn_readfirstlane((int)__any(top > m + 8.f || m == -INFINITY));
+      const float now = grow ? fmaxf(m, top) : m, ref = now == -INFINITY ? 0.f : now;
+      const float alpha = __builtin_amdgcn_exp2f(m - ref);   // 1 unless it grew
+      m = now;
+      l *= alpha;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] *= alpha;
-      }
-      const float ref = m == -INFINITY ? 0.f : m;
+      for (int d = 0; d < DT; ++d) scale_if(grow, o[d], alpha);
+      v4i va[2][4];
+      auto read_v = [&](int n) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int g = (4 * n + i) / DT, d = (4 * n + i) % DT;
+          va[n & 1][i] = *reinterpret_cast<const v4i *>(vb + (vat ^ (32 * g)) + d * 32 * 128);
+        }
+      };
+      read_v(0);
       v4i pf[4], pl[F16 ? 4 : 1];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         float e[8];
+        if constexpr (!SLOW) {
+          // exp(s - m) vs from one exponential; the sum takes 1 / vs per group
+          const float2 lg = s_log[buf][g];
+          const float off = lg.x - ref;
+          float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float x = sc[g >> 1][8 * (g & 1) + i];
-          e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, ks[g], -ref));
-          l += e[i];
-          sc[g >> 1][8 * (g & 1) + i] = x;
-        }
-        if (masked) {                            // 0 stays 0 whatever the scale
-#pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = sc[g >> 1][8 * (g & 1) + i] == -INFINITY ? 0.f : e[i] * vs[g];
+          for (int i = 0; i < 8; ++i) {
+            e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + i], ks[g], off));
+            sum = i ? sum + e[i] : e[i];
+          }
+          l = __builtin_fmaf(sum, lg.y, l);
         } else {
+          const float vs = s_scale[buf][4 + g];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] *= vs[g];
+          for (int i = 0; i < 8; ++i) {
+            const float x = sc[g >> 1][8 * (g & 1) + i];
+            e[i] = __builtin_amdgcn_exp2f(x - ref);
+            l += e[i];
+            e[i] = x == -INFINITY ? 0.f : e[i] * vs;       // whatever the scale
+          }
         }
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -325,21 +402,57 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int n = 0; n < DT; ++n) {
+        if (n + 1 < DT) read_v(n + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const v4i a = *reinterpret_cast<const v4i *>(vb + (vat ^ (32 * g)) + d * 32 * 128);
-          o[d] = mfma32<false>(a, pf[g], o[d]);
-          if constexpr (F16) o[d] = mfma32<false>(a, pl[g], o[d]);
+        for (int i = 0; i < 4; ++i) {
+          const int g = (4 * n + i) / DT, d = (4 * n + i) % DT;
+          o[d] = mfma32<false>(va[n & 1][i], pf[g], o[d]);
+          if constexpr (F16) o[d] = mfma32<false>(va[n & 1][i], pl[g], o[d]);
         }
-      if (FP8 && nans) {                         // NaN where the row sees a NaN code
-        const int n = limit - tile * kPTile;
-        const uint64_t sees = n >= 64 ? ~0ull : (n > 0 ? (1ull << n) - 1 : 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (FP8) {
+        if (__builtin_amdgcn_readfirstlane(s_bad[tile & 3])) {   // columns that get a NaN
+          const int n = limit - tile * kPTile;
+          const uint64_t sees = n >= 64 ? ~0ull : (n > 0 ? (1ull << n) - 1 : 0);
+          for (int d = h; d < D; d += 2)
+            if (s_nan[buf][d] & sees) atomicOr(&s_row[wave * 32 + r32][d >> 5], 1u << (d & 31));
+        }
+      }
+    };
+
+    int tile = t0;
+    while (tile < t1) {
+      __syncthreads();                           // the tile is staged, the other stage is read
+      if (!__any(tile * kPTile < limit)) break;
+      if (common(tile)) {
+        for (;;) {
+          step(std::false_type{}, tile);
+          if (++tile >= t1) break;
+          __syncthreads();
+          if (!common(tile)) break;
+        }
+        if (tile >= t1 || !__any(tile * kPTile < limit)) break;
+      }
+      step(std::true_type{}, tile++);
+    }
+    // rows that see no more: the workgroup's others do (the tile's barrier is passed)
+    for (; tile < t1; ++tile) {
+      advance(tile);
+      if (tile + 1 < t1) __syncthreads();
+    }
+    if constexpr (FP8) {
+      __syncthreads();
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d) {
+        const uint32_t bad = s_row[wave * 32 + r32][d];
+        if (__any(bad)) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (s_nan[buf][32 * d + 8 * (i >> 2) + 4 * h + (i & 3)] & sees) o[d][i] = __builtin_nanf("");
+            if (bad >> (8 * (i >> 2) + 4 * h + (i & 3)) & 1) o[d][i] = __builtin_nanf("");
+        }
       }
     }
 
