@@ -26,7 +26,6 @@
 
 namespace dsl {
 
-constexpr int kPTile = 64;     // tokens per tile
 
 template <bool F16>
 DSL_DEV v16f mfma32(const v4i &a, const v4i &b, const v16f &c) {
@@ -47,9 +46,9 @@ DSL_DEV float halves_sum(float v) {
 
 // v *= f when the wave-uniform `on` is non-zero.  The branch is inside the asm:
 // one in the source made the compiler keep a second copy of the output and move
-// all of it there and back in every tile.  (The products that wrote v are done:
-// the caller has read later ones' results; f comes from v_exp_f32, hence the
-// s_nop.)
+// all of it there and back in every tile.  The compiler adds no wait states to
+// inline asm: the 20 here cover a product that may still be writing v (19 at most)
+// and the v_exp_f32 that gave f.
 DSL_DEV void scale_if(int on, v16f &v, float f) {
   float e[16];
 #pragma unroll
@@ -57,7 +56,7 @@ DSL_DEV void scale_if(int on, v16f &v, float f) {
   asm volatile(
       "s_cmp_eq_u32 %17, 0\n\t"
       "s_cbranch_scc1 .Lscale_skip_%=\n\t"
-      "s_nop 1\n\t"
+      "s_nop 15\n\ts_nop 3\n\t"
       "v_mul_f32 %0, %0, %16\n\tv_mul_f32 %1, %1, %16\n\tv_mul_f32 %2, %2, %16\n\tv_mul_f32 %3, %3, %16\n\t"
       "v_mul_f32 %4, %4, %16\n\tv_mul_f32 %5, %5, %16\n\tv_mul_f32 %6, %6, %16\n\tv_mul_f32 %7, %7, %16\n\t"
       "v_mul_f32 %8, %8, %16\n\tv_mul_f32 %9, %9, %16\n\tv_mul_f32 %10, %10, %16\n\tv_mul_f32 %11, %11, %16\n\t"
@@ -75,39 +74,83 @@ DSL_DEV void scale_if(int on, v16f &v, float f) {
 // (V); both readers (32 rows, chunks c and c + 1 by lane half) meet no bank twice.
 template <int CHUNKS>
 DSL_DEV int pslot(int row, int c) {
-  if constexpr (CHUNKS == 8) return c ^ pipe::swz<128>(row);
+  if constexpr (CHUNKS == 4) return c ^ pipe::swz<64>(row);
+  else if constexpr (CHUNKS == 8) return c ^ pipe::swz<128>(row);
   else return c ^ (row & 15);
 }
 
-// Bit 7 of each byte that is an E4M3 NaN code.
-DSL_DEV uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// Scores of a tile's 16-token group to powers of two, -infinity where hidden: token
+// offsets T .. T + 3, T + 8 .. T + 11 of the lane against lim, the tokens that its
+// row sees (T without the lane half's part).  In place, under a branch of its own,
+// like scale_if.
+template <int T>
+DSL_DEV void mask_if(int on, v16f &v, int at, float ks, int lim) {
+  float e[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = v[at + i];
+  asm volatile(
+      "s_cmp_eq_u32 %11, 0\n\t"
+      "s_cbranch_scc1 .Lmask_skip_%=\n\t"
+      "s_nop 15\n\ts_nop 3\n\t"
+      "v_mul_f32 %0, %0, %8\n\tv_mul_f32 %1, %1, %8\n\tv_mul_f32 %2, %2, %8\n\tv_mul_f32 %3, %3, %8\n\t"
+      "v_mul_f32 %4, %4, %8\n\tv_mul_f32 %5, %5, %8\n\tv_mul_f32 %6, %6, %8\n\tv_mul_f32 %7, %7, %8\n\t"
+      "v_cmp_lt_i32 vcc, %12, %9\n\ts_nop 1\n\tv_cndmask_b32 %0, %10, %0, vcc\n\t"
+      "v_cmp_lt_i32 vcc, %13, %9\n\ts_nop 1\n\tv_cndmask_b32 %1, %10, %1, vcc\n\t"
+      "v_cmp_lt_i32 vcc, %14, %9\n\ts_nop 1\n\tv_cndmask_b32 %2, %10, %2, vcc\n\t"
+      "v_cmp_lt_i32 vcc, %15, %9\n\ts_nop 1\n\tv_cndmask_b32 %3, %10, %3, vcc\n\t"
+      "v_cmp_lt_i32 vcc, %16, %9\n\ts_nop 1\n\tv_cndmask_b32 %4, %10, %4, vcc\n\t"
+      "v_cmp_lt_i32 vcc, %17, %9\n\ts_nop 1\n\tv_cndmask_b32 %5, %10, %5, vcc\n\t"
+      "v_cmp_lt_i32 vcc, %18, %9\n\ts_nop 1\n\tv_cndmask_b32 %6, %10, %6, vcc\n\t"
+      "v_cmp_lt_i32 vcc, %19, %9\n\ts_nop 1\n\tv_cndmask_b32 %7, %10, %7, vcc\n"
+      ".Lmask_skip_%=:"
+      : "+v"(e[0]), "+v"(e[1]), "+v"(e[2]), "+v"(e[3]), "+v"(e[4]), "+v"(e[5]), "+v"(e[6]), "+v"(e[7])
+      : "v"(ks), "v"(lim), "v"(-INFINITY), "s"(on), "n"(T), "n"(T + 1), "n"(T + 2), "n"(T + 3), "n"(T + 8), "n"(T + 9),
+        "n"(T + 10), "n"(T + 11)
+      : "scc", "vcc");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[at + i] = e[i];
+}
+
+// LDS writes of this wave have landed; then the workgroup's barrier.  Loads from
+// memory stay in flight (__syncthreads would wait for them).
+DSL_DEV void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int D>
 struct PromptCfg {
-  static constexpr int NW = D > 128 ? 4 : 8, NT = NW * 64, ROWS = NW * 32;
-  static constexpr int WPS = NW / 4;                         // waves per SIMD
-  static constexpr int KC = D / 8;                           // 16-byte chunks of a K row
-  static constexpr int TILE = kPTile * D * 2;                // bytes of K or V
-  static constexpr int UNITS = 2 * kPTile * D / 16 / NT;     // 16-code loads per thread
-  static constexpr int STAGE = 2 * TILE;
+  static constexpr int NW = 8, NT = NW * 64;                 // two waves per SIMD
+  // dim 256: tiles of 32 tokens, and two waves compute the same scores, each half
+  // of the output's columns (all of them would take 128 of its 256 registers)
+  static constexpr int HALVES = D > 128 ? 2 : 1, T = D > 128 ? 32 : 64;
+  static constexpr int ROWS = NW / HALVES * 32;              // query rows
+  static constexpr int G = T / 16, TS = T / 32;              // 16-token groups, 32-token score tiles
+  static constexpr int DH = D / HALVES, DT = DH / 32;        // the wave's output columns
+  static constexpr int KC = D / 8, VC = T / 8;               // 16-byte chunks of K's and V's rows
+  static constexpr int TILE = T * D * 2;                     // bytes of K or V
+  static constexpr int UNITS = 2 * T * D / 16 / NT;          // 16-code loads per thread
+  // dim 128: the queries stay in LDS (kept in registers, others spill)
+  static constexpr bool QLDS = D == 128;
+  static constexpr int QBYTES = QLDS ? NW * (D / 16) * 1024 : 0;
 };
 
 // blockIdx: x (row block from the last on) * heads * sequences + ..., y split.
 template <int SRC, bool FP8, int D>
-__global__ __launch_bounds__(PromptCfg<D>::NT) __attribute__((amdgpu_waves_per_eu(PromptCfg<D>::WPS, PromptCfg<D>::WPS)))
+__global__ __launch_bounds__(PromptCfg<D>::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, const int nsplit) {
   using Cfg = PromptCfg<D>;
   constexpr bool F16 = SRC == SRC_F16;
-  constexpr int KK = D / 16, DT = D / 32, U = Cfg::UNITS, KU = kPTile * D / 16;
-  __shared__ __align__(16) uint8_t lds[2 * Cfg::STAGE];
-  __shared__ __align__(16) float s_scale[2][8];  // of a tile's four 16-token groups: ks, vs
-  __shared__ float2 s_log[2][4];                 // log2 vs, 1 / vs
-  __shared__ __align__(16) int s_page[4][4];     // the groups' pages, -1: none
-  __shared__ int s_odd[2], s_bad[4];             // scales off the common path; NaN codes among V
+  constexpr int T = Cfg::T, G = Cfg::G, TS = Cfg::TS, DT = Cfg::DT;
+  constexpr int KK = D / 16, U = Cfg::UNITS, KU = T * D / 16;
+  constexpr int VBASE = 2 * Cfg::TILE, QBASE = 4 * Cfg::TILE;
+  __shared__ __align__(16) uint8_t lds[4 * Cfg::TILE + Cfg::QBYTES];   // two tiles of K, two of V, queries
+  __shared__ __align__(16) float s_ks[4][4], s_vs[4][4];     // scales of a tile's 16-token groups
+  __shared__ __align__(16) float s_log[4][4], s_inv[4][4];   // log2 vs, 1 / vs
+  __shared__ __align__(16) int s_page[4][4];                 // the groups' pages, -1: none
+  __shared__ int s_none[4], s_oddk[4], s_oddv[4];            // a group in no page; scales off the common path
+  __shared__ int s_bad[4];                                   // NaN codes among V
   // tokens (bits) whose V code is NaN, by column: staged as 0, since 0 * NaN
   // would carry one to rows that do not see it
   __shared__ uint64_t s_nan[2][FP8 ? D : 1];
-  __shared__ uint32_t s_row[FP8 ? Cfg::ROWS : 1][DT];   // ... and the columns (bits) that a row gets one in
+  __shared__ uint32_t s_row[FP8 ? Cfg::ROWS : 1][D / 32];   // ... and the columns (bits) that a row gets one in
   const int pairs = c.heads * c.seqs;
   // Row blocks from the last, the longest, on.  Workgroups go to the eight XCDs,
   // and there to four shader engines, in turn: the pairs of an XCD (whose rows
@@ -123,94 +166,84 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
   const int head = pair % c.heads, b = pair / c.heads, split = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, h = lane >> 5;
+  const int wrow = wave / Cfg::HALVES * 32, half = wave % Cfg::HALVES;
   const SeqView s = seq_view(c, b);
   const int rows = s.n * p.group;
   const int P = c.page, pshift = 31 - __builtin_clz(P), room = c.width * P;
   const int len = s.len < room ? s.len : room;
-  const int64_t hstride = (int64_t)P * D;
+  const uint32_t hstride = (uint32_t)P * D, pstride = hstride * (uint32_t)c.heads;   // < 2^31
+  const uint8_t *const kbase = c.k + (int64_t)head * hstride, *const vbase = c.v + (int64_t)head * hstride;
 
   for (int rb = blk; rb * Cfg::ROWS < rows; rb += nblk) {
-    // tokens that the block's last row sees
-    int end = len;
-    if (p.causal) {
-      int last = rb * Cfg::ROWS + Cfg::ROWS - 1;
-      last = last < rows ? last : rows - 1;
-      const int lim = s.first + last / p.group + 1;
-      end = lim < end ? (lim > 0 ? lim : 0) : end;
-    }
-    const int ntiles = (end + kPTile - 1) / kPTile;
+    // tokens that the block's first and last rows see
+    auto sees = [&](int r) {
+      const int n = s.first + (r < rows ? r : rows - 1) / p.group + 1;
+      return p.causal ? (n > 0 ? (n < len ? n : len) : 0) : len;
+    };
+    const int every = sees(rb * Cfg::ROWS), end = sees(rb * Cfg::ROWS + Cfg::ROWS - 1);
+    const int ntiles = (end + T - 1) / T;
     const int t0 = (int)((int64_t)ntiles * split / nsplit), t1 = (int)((int64_t)ntiles * (split + 1) / nsplit);
 
-    const int row = rb * Cfg::ROWS + wave * 32 + r32, rr = row < rows ? row : rows - 1;
-    const int qi = rr / p.group, hq = head * p.group + rr % p.group;
     v4i qf[KK];
+    const int qrow = rb * Cfg::ROWS + wrow + r32;
     {
+      const int rr = qrow < rows ? qrow : rows - 1, qi = rr / p.group, hq = head * p.group + rr % p.group;
       const uint16_t *qp = static_cast<const uint16_t *>(p.q) + (int64_t)(s.row0 + qi) * p.q_row + (int64_t)hq * p.q_head;
 #pragma unroll
       for (int k = 0; k < KK; ++k) qf[k] = *reinterpret_cast<const v4i *>(qp + 16 * k + 8 * h);
     }
-    // they have arrived before the loop: a wait for them there would be one for
-    // the tiles' loads too
-#pragma unroll
-    for (int k = 0; k < KK; ++k) asm volatile("" : "+v"(qf[k]));
-    const int seen = s.first + qi + 1;
-    const int limit = p.causal ? (seen > 0 ? (seen < len ? seen : len) : 0) : len;
-    int low = len;                               // tokens that every row of the wave sees
-    if (p.causal) {
-      const int r0 = rb * Cfg::ROWS + wave * 32;
-      const int f = s.first + (r0 < rows ? r0 : rows - 1) / p.group + 1;
-      low = f > 0 ? (f < len ? f : len) : 0;
-    }
+    const int limit = sees(qrow);
+    // tokens that every row of the wave sees, and that one of them sees
+    const int low = __builtin_amdgcn_readfirstlane(limit);
+    const int high = __builtin_amdgcn_readlane(limit, 31);
+    int w1 = (high + T - 1) / T;                 // the wave's tiles: t0 .. w1 - 1
+    w1 = w1 < t1 ? w1 : t1;
 
     v16f o[DT];
     float m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = (v16f){};
 
-    // Pages go to LDS three tiles ahead (four threads look them up a tile before
-    // that), codes and scales to registers two tiles ahead.
+    // Pages go to LDS four tiles ahead (four threads look them up a tile before
+    // that), codes and scales to registers a tile before they are staged.  Past the
+    // last tile the pages are none, which read page 0 and stage it where nobody
+    // looks.
     uint4 raw[U];
-    float sraw = 0.f;
+    float kraw = 0.f, vraw = 0.f;
     int page = -1;
     auto find = [&](int tile) __attribute__((always_inline)) {
-      const int tok = tile * kPTile + tid * 16;
-      if (tid < 4) page = tile < t1 && tok < len ? (int)page_of(c, b, tok >> pshift) : -1;
+      const int tok = tile * T + tid * 16;
+      if (tid < G) page = tile < t1 && tok < len ? (int)page_of(c, b, tok >> pshift) : -1;
     };
     auto keep = [&](int tile) __attribute__((always_inline)) {
-      if (tid < 4) s_page[tile & 3][tid] = page;
+      if (tid < G) {
+        s_page[tile & 3][tid] = page;
+        const uint64_t none = __ballot(page < 0);
+        if (tid == 0) s_none[tile & 3] = none != 0;
+      }
     };
-    // this thread's unit j: 16 codes of K (D <= 64: by wave) or of V
+    // this thread's unit j: 16 codes of K (dim 64: by wave) or of V
     auto is_k = [&](int j) __attribute__((always_inline)) { return U > 1 ? j < U / 2 : wave < Cfg::NW / 2; };
-    auto load = [&](int tile) __attribute__((always_inline)) {
+    // (K of `tile`, V of the one before)
+    auto load = [&](int tk) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         const int u = tid + Cfg::NT * j;
-        if (is_k(j)) {
-          const int r = u / (D / 16), pg = s_page[tile & 3][r >> 4];
-          const uint8_t *at = c.k + ((int64_t)(pg < 0 ? 0 : pg) * c.heads + head) * hstride +
-                              (((tile * kPTile + r) & (P - 1)) * D + (u % (D / 16)) * 16);
-          raw[j] = *reinterpret_cast<const uint4 *>(at);
-        } else {
-          const int g = u & 3, pg = s_page[tile & 3][g];
-          const uint8_t *at = c.v + ((int64_t)(pg < 0 ? 0 : pg) * c.heads + head) * hstride +
-                              ((((u - KU) >> 2) << pshift) + ((tile * kPTile + g * 16) & (P - 1)));
-          raw[j] = *reinterpret_cast<const uint4 *>(at);
-          if (FP8 && pg < 0) raw[j] = make_uint4(0, 0, 0, 0);
-        }
-      }
-      if (tid < 8) {
-        const int pg = s_page[tile & 3][tid & 3];
-        sraw = pg < 0 ? 0.f : (tid < 4 ? c.k_scale : c.v_scale)[(int64_t)pg * c.heads + head];
+        const bool isk = is_k(j);
+        const int tile = isk ? tk : tk - 1;
+        const int g = isk ? u / (D / 16) >> 4 : u & (G - 1), pg = s_page[tile & 3][g];
+        const uint32_t off = isk ? (uint32_t)(((tile * T + u / (D / 16)) & (P - 1)) * D + (u % (D / 16)) * 16)
+                                 : (uint32_t)((((u - KU) / G) << pshift) + ((tile * T + g * 16) & (P - 1)));
+        raw[j] = *reinterpret_cast<const uint4 *>((isk ? kbase : vbase) + (uint64_t)(uint32_t)(pg < 0 ? 0 : pg) * pstride + off);
       }
     };
-    // the loaded tile as 16-bit operands
-    auto stage = [&](int tile, int buf) __attribute__((always_inline)) {
-      uint8_t *kb = lds + buf * Cfg::STAGE, *vb = kb + Cfg::TILE;
-      uint32_t bad = 0;
+    // this thread's part of K of a tile and of V of the one before as 16-bit operands
+    auto stage = [&](int tk) __attribute__((always_inline)) {
+      uint8_t *kb = lds + (tk & 1) * Cfg::TILE, *vb = lds + VBASE + ((tk - 1) & 1) * Cfg::TILE;
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         const int u = tid + Cfg::NT * j;
-        uint4 w = raw[j];
+        const uint4 w = raw[j];
         if (is_k(j)) {
           const int r = u / (D / 16), ch = (u % (D / 16)) * 2;
           uint8_t *to = kb + r * (2 * D);
@@ -218,138 +251,160 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
           *reinterpret_cast<v4i *>(to + at) = codes8<FP8, F16>(w.x, w.y);
           *reinterpret_cast<v4i *>(to + (at ^ 16)) = codes8<FP8, F16>(w.z, w.w);
         } else {
-          const int d = (u - KU) >> 2, g = u & 3;
-          if constexpr (FP8) {
-            if (tile * kPTile + kPTile > len) {  // codes past the end can be NaN
-              const int nv = len - (tile * kPTile + g * 16);
-              auto first = [&](int n) { return n >= 4 ? 0xffffffffu : (n <= 0 ? 0u : (1u << (8 * n)) - 1); };
-              w.x &= first(nv);
-              w.y &= first(nv - 4);
-              w.z &= first(nv - 8);
-              w.w &= first(nv - 12);
-            }
-            const uint32_t bx = nan_bytes(w.x), by = nan_bytes(w.y), bz = nan_bytes(w.z), bw = nan_bytes(w.w);
-            uint32_t at = 0;
-            if (bx | by | bz | bw) {
-              auto nibble = [](uint32_t x) { return ((x >> 7) * 0x01020408u) >> 24 & 15; };
-              at = nibble(bx) | nibble(by) << 4 | nibble(bz) << 8 | nibble(bw) << 12;
-              w.x &= ~((bx >> 7) * 255u);
-              w.y &= ~((by >> 7) * 255u);
-              w.z &= ~((bz >> 7) * 255u);
-              w.w &= ~((bw >> 7) * 255u);
-            }
-            reinterpret_cast<uint16_t *>(&s_nan[buf][d])[g] = (uint16_t)at;
-            bad |= at;
-          }
-          uint8_t *to = vb + d * 128;
-          const int at = pslot<8>(d, 2 * g) * 16;
+          const int d = (u - KU) / G, g = u & (G - 1);
+          uint8_t *to = vb + d * (2 * T);
+          const int at = pslot<Cfg::VC>(d, 2 * g) * 16;
           *reinterpret_cast<v4i *>(to + at) = codes8<FP8, false>(w.x, w.z);
           *reinterpret_cast<v4i *>(to + (at ^ 16)) = codes8<FP8, false>(w.y, w.w);
         }
       }
-      if (tid < 8) {
-        const float x = tid < 4 ? sraw * (p.scale * kLog2e) : sraw;
-        s_scale[buf][tid] = x;
-        // scales that the common path takes: its scores' maximum follows the
-        // codes', and probabilities take theirs as a logarithm
-        const bool odd = tid < 4 ? !(x >= 0.f) : !(x >= 0x1p-60f && x <= 0x1p60f);
-        const uint64_t some = __ballot(odd);
-        if (tid == 0) s_odd[buf] = some != 0;
-        if (tid >= 4) s_log[buf][tid & 3] = make_float2(__builtin_amdgcn_logf(x), 1.0f / x);
-      }
+    };
+    // V of `tile` that some row must not meet, in the thread's own staged units: codes
+    // past the end or of no page, which can be NaN, become 0; NaN ones that a row
+    // may not see move to s_nan.  (Here, not in registers before: that spilled.)
+    auto clean = [&](int tile) __attribute__((always_inline)) {
       if constexpr (FP8) {
+        if (!__builtin_amdgcn_readfirstlane((int)(tile * T + T > every || s_none[tile & 3]))) return;
+        int t = tid;
+        asm volatile("" : "+v"(t));
+        uint32_t bad = 0;
+#pragma unroll 1
+        for (int j = U > 1 ? U / 2 : 0; j < U; ++j) {
+          const int u = t + Cfg::NT * j, d = (u - KU) / G, g = u & (G - 1);
+          if (u < KU) continue;
+          const int nv = s_page[tile & 3][g] < 0 ? 0 : len - (tile * T + g * 16);
+          uint8_t *row = lds + VBASE + (tile & 1) * Cfg::TILE + d * (2 * T);
+          uint32_t at = 0;
+#pragma unroll 1
+          for (int x = 0; x < 8; ++x) {          // two tokens of a chunk: half x / 4, word x % 4
+            uint32_t *w = reinterpret_cast<uint32_t *>(row + pslot<Cfg::VC>(d, 2 * g + (x >> 2)) * 16) + (x & 3);
+            const int tok = 4 * (x >> 2) + 8 * ((x & 3) >> 1) + 2 * (x & 1);
+            uint32_t v = *w;
+            if (tok >= nv) v &= 0xffff0000u;
+            if (tok + 1 >= nv) v &= 0xffffu;
+            if ((v & 0x7fffu) > 0x7f80u) {
+              at |= 1u << tok;
+              v &= 0xffff0000u;
+            }
+            if ((v & 0x7fffffffu) > 0x7f80ffffu) {
+              at |= 2u << tok;
+              v &= 0xffffu;
+            }
+            *w = v;
+          }
+          reinterpret_cast<uint16_t *>(&s_nan[tile & 1][d])[g] = (uint16_t)at;
+          bad |= at;
+        }
         if (__any(bad) && lane == 0) s_bad[tile & 3] = 1;
+      }
+    };
+    // the scales: four threads of wave 1
+    const int sg = tid - 64;
+    auto load_scales = [&](int tile) __attribute__((always_inline)) {
+      if (sg >= 0 && sg < G) {
+        const int pg = s_page[tile & 3][sg];
+        const int64_t at = (int64_t)(pg < 0 ? 0 : pg) * c.heads + head;
+        kraw = c.k_scale[at];
+        vraw = c.v_scale[at];
+      }
+    };
+    auto stage_scales = [&](int tile) __attribute__((always_inline)) {
+      if (sg >= 0 && sg < G) {
+        const bool none = s_page[tile & 3][sg] < 0;
+        const float ks = none ? 0.f : kraw * (p.scale * kLog2e), vs = none ? 1.f : vraw;
+        const bool odd = !(vs >= 0x1p-60f && vs <= 0x1p60f);
+        s_ks[tile & 3][sg] = ks;
+        s_vs[tile & 3][sg] = odd ? vs : 1.f;
+        s_log[tile & 3][sg] = odd ? 0.f : __builtin_amdgcn_logf(vs);
+        s_inv[tile & 3][sg] = odd ? 1.f : __builtin_amdgcn_rcpf(vs);
+        const uint64_t ok = __ballot(!(ks >= 0.f)), ov = __ballot(odd);
+        if (sg == 0) {
+          s_oddk[tile & 3] = ok != 0;
+          s_oddv[tile & 3] = ov != 0;
+        }
+      }
+    };
+
+    // in step `tile`, once stage(tile + 2) has taken the codes
+    auto fetch = [&](int tile) __attribute__((always_inline)) {
+      load(tile + 3);
+      if (wave == 0) {
+        if (FP8 && tid == 0) s_bad[(tile + 2) & 3] = 0;      // set in the next step at the earliest
+        keep(tile + 4);
+        find(tile + 5);
+      }
+      if (wave == 1) {
+        stage_scales(tile + 2);
+        load_scales(tile + 3);
       }
     };
 
     __syncthreads();                             // the last block's readers
     if (tid < 4) s_bad[tid] = 0;
     if constexpr (FP8) {
-      for (int i = tid; i < Cfg::ROWS * DT; i += Cfg::NT) s_row[i / DT][i % DT] = 0;
+      for (int i = tid; i < Cfg::ROWS * (D / 32); i += Cfg::NT) s_row[i / (D / 32)][i % (D / 32)] = 0;
     }
     if (t0 < t1) {
 #pragma unroll
-      for (int i = 0; i < 3; ++i) {
+      for (int i = 0; i < 4; ++i) {
         find(t0 + i);
         keep(t0 + i);
       }
-      find(t0 + 3);
       __syncthreads();
-      load(t0);
-      stage(t0, t0 & 1);
-      if (t0 + 1 < t1) load(t0 + 1);
+      load(t0);                                  // (V of no tile: overwritten below)
+      load_scales(t0);
+      stage(t0);
+      stage_scales(t0);
+      __syncthreads();
+      load(t0 + 1);
+      load_scales(t0 + 1);
+      stage(t0 + 1);
+      clean(t0);
+      stage_scales(t0 + 1);
+      load(t0 + 2);
+      load_scales(t0 + 2);
+      find(t0 + 4);
     }
-    // what follows a tile, behind its scores: the next one's operands, the loads of
-    // the one after, the pages of the third
-    auto advance = [&](int tile) __attribute__((always_inline)) {
-      if (tile + 1 < t1) {
-        if (FP8 && tid == 0) s_bad[(tile + 2) & 3] = 0;   // set a tile later at the earliest
-        stage(tile + 1, (tile + 1) & 1);
-        if (tile + 2 < t1) load(tile + 2);
-        keep(tile + 3);
-        find(tile + 4);
-      }
+    // the queries have arrived before the loop: a wait for them there would be one
+    // for the tiles' loads too
+#pragma unroll
+    for (int k = 0; k < KK; ++k) {
+      if constexpr (Cfg::QLDS) *reinterpret_cast<v4i *>(lds + QBASE + (wave * KK + k) * 1024 + lane * 16) = qf[k];
+      else asm volatile("" : "+v"(qf[k]));
+    }
+    auto query = [&](int k) __attribute__((always_inline)) {
+      if constexpr (Cfg::QLDS) return *reinterpret_cast<const v4i *>(lds + QBASE + (wave * KK + k) * 1024 + lane * 16);
+      else return qf[k];
     };
-    // a tile whose tokens all rows of the wave see, in pages that there are, of
-    // common scales
-    auto common = [&](int tile) __attribute__((always_inline)) {
-      const v4i pg = *reinterpret_cast<const v4i *>(s_page[tile & 3]);
-      const bool none = min(min(pg[0], pg[1]), min(pg[2], pg[3])) < 0;
-      return __builtin_amdgcn_readfirstlane((int)(tile * kPTile + kPTile <= low && !none && !s_odd[tile & 1])) != 0;
-    };
+
     // fragment addresses: the rows' swizzles do not depend on t and d, and flip no
     // bit of 32 k, so one register each; formed afresh in every tile (kept for all
     // k they spill)
-    const int kat0 = r32 * (2 * D) + pslot<Cfg::KC>(r32, h) * 16, vat0 = r32 * 128 + pslot<8>(r32, h) * 16;
-    auto step = [&](auto slow_tag, int tile) __attribute__((always_inline)) {
-      constexpr bool SLOW = decltype(slow_tag)::value;
-      const int buf = tile & 1;
-      const uint8_t *kb = lds + buf * Cfg::STAGE, *vb = kb + Cfg::TILE;
-      int kat = kat0, vat = vat0;
-      asm volatile("" : "+v"(kat), "+v"(vat));
-      // four fragments ahead of the products that take them
-      v16f sc[2] = {};
-      {
-        v4i a[2][4];
-        auto read = [&](int n) __attribute__((always_inline)) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            a[n & 1][i] = *reinterpret_cast<const v4i *>(kb + (kat ^ (32 * (2 * n + (i >> 1)))) + (i & 1) * 32 * 2 * D);
-        };
-        read(0);
-#pragma unroll
-        for (int n = 0; n < KK / 2; ++n) {
-          if (n + 1 < KK / 2) read(n + 1);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sc[i & 1] = mfma32<F16>(a[n & 1][i], qf[2 * n + (i >> 1)], sc[i & 1]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+    const int kat0 = r32 * (2 * D) + pslot<Cfg::KC>(r32, h) * 16;
+    const int vat0 = (half * Cfg::DH + r32) * (2 * T) + pslot<Cfg::VC>(r32, h) * 16;
+    float kq[G], off[G];                         // the current scores' factors; log2 vs - m
+    // Scores of `tile` are there: hide what is hidden, take their maximum, and bring
+    // sum and output to it where it grew.
+    auto prepare = [&](int tile, v16f (&sc)[TS]) __attribute__((always_inline)) {
+      const v4f ks = *reinterpret_cast<const v4f *>(s_ks[tile & 3]), lg = *reinterpret_cast<const v4f *>(s_log[tile & 3]);
+      const int slow = __builtin_amdgcn_readfirstlane(
+          (int)(tile * T + T > low || tile >= w1 || s_none[tile & 3] || s_oddk[tile & 3]));
+      const v4i pg = *reinterpret_cast<const v4i *>(s_page[tile & 3]);
+      const int lim = tile < w1 ? limit - tile * T - 4 * h : 0;
+      mask_if<0>(slow, sc[0], 0, ks[0], pg[0] < 0 ? 0 : lim);
+      mask_if<16>(slow, sc[0], 8, ks[1], pg[1] < 0 ? 0 : lim);
+      if constexpr (TS > 1) {
+        mask_if<32>(slow, sc[TS - 1], 0, ks[2], pg[2] < 0 ? 0 : lim);
+        mask_if<48>(slow, sc[TS - 1], 8, ks[3], pg[3] < 0 ? 0 : lim);
       }
-      advance(tile);
-      __builtin_amdgcn_sched_barrier(0);
-
-      const v4f ks = *reinterpret_cast<const v4f *>(&s_scale[buf][0]);
       float top = -INFINITY;
-      if constexpr (!SLOW) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float x = -INFINITY;
+      for (int g = 0; g < G; ++g) {
+        kq[g] = slow ? 1.f : ks[g];
+        float x = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) x = fmaxf(fmaxf(x, sc[g >> 1][8 * (g & 1) + i]), sc[g >> 1][8 * (g & 1) + i + 1]);
-          top = fmaxf(top, x * ks[g]);
-        }
-      } else {
-        const v4i pg = *reinterpret_cast<const v4i *>(s_page[tile & 3]);
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int tok = tile * kPTile + 16 * g + 8 * (i >> 2) + 4 * h + (i & 3);
-            const float v = tok < limit && pg[g] >= 0 ? sc[g >> 1][8 * (g & 1) + i] * ks[g] : -INFINITY;
-            sc[g >> 1][8 * (g & 1) + i] = v;
-            top = fmaxf(top, v);
-          }
+        for (int i = 0; i < 8; i += 2) x = fmaxf(fmaxf(x, sc[g >> 1][8 * (g & 1) + i]), sc[g >> 1][8 * (g & 1) + i + 1]);
+        top = fmaxf(top, x * kq[g]);
       }
       top = halves_max(top);
       const int grow = __builtin_amdgcn_readfirstlane((int)__any(top > m + 8.f || m == -INFINITY));
@@ -359,95 +414,141 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
       l *= alpha;
 #pragma unroll
       for (int d = 0; d < DT; ++d) scale_if(grow, o[d], alpha);
-      v4i va[2][4];
-      auto read_v = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int g = (4 * n + i) / DT, d = (4 * n + i) % DT;
-          va[n & 1][i] = *reinterpret_cast<const v4i *>(vb + (vat ^ (32 * g)) + d * 32 * 128);
-        }
+      for (int g = 0; g < G; ++g) off[g] = lg[g] - ref;
+    };
+    // One tile: the exponentials of its scores `sc` between the products of the next
+    // tile's scores `nx`; its output's products between the staging of the tile after
+    // that; then the next scores' maximum.
+    auto step = [&](int tile, v16f (&sc)[TS], v16f (&nx)[TS]) __attribute__((always_inline)) {
+      const uint8_t *kb = lds + ((tile + 1) & 1) * Cfg::TILE, *vb = lds + VBASE + (tile & 1) * Cfg::TILE;
+      int kat = kat0, vat = vat0;
+      asm volatile("" : "+v"(kat), "+v"(vat));
+      const v4f inv = *reinterpret_cast<const v4f *>(s_inv[tile & 3]);
+      const int oddv = __builtin_amdgcn_readfirstlane(s_oddv[tile & 3]);
+      const int nans = FP8 ? __builtin_amdgcn_readfirstlane(s_bad[tile & 3]) : 0;
+      v4i pf[G], pl[F16 ? G : 1];
+      // fragment f of K: step f / TS, part f % TS of the tokens; three are on their way
+      constexpr int NF = KK * TS, PER = NF / G;
+      v4i a[4], q[2];
+      auto read = [&](int f) __attribute__((always_inline)) {
+        if (f < NF) a[f & 3] = *reinterpret_cast<const v4i *>(kb + (kat ^ (32 * (f / TS))) + (f % TS) * 32 * 2 * D);
       };
-      read_v(0);
-      v4i pf[4], pl[F16 ? 4 : 1];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float e[8];
-        if constexpr (!SLOW) {
-          // exp(s - m) vs from one exponential; the sum takes 1 / vs per group
-          const float2 lg = s_log[buf][g];
-          const float off = lg.x - ref;
-          float sum = 0.f;
+      for (int f = 0; f < 3; ++f) read(f);
+      q[0] = query(0);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + i], ks[g], off));
-            sum = i ? sum + e[i] : e[i];
-          }
-          l = __builtin_fmaf(sum, lg.y, l);
-        } else {
-          const float vs = s_scale[buf][4 + g];
+      for (int g = 0; g < G; ++g) {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float x = sc[g >> 1][8 * (g & 1) + i];
-            e[i] = __builtin_amdgcn_exp2f(x - ref);
-            l += e[i];
-            e[i] = x == -INFINITY ? 0.f : e[i] * vs;       // whatever the scale
-          }
+        for (int i = 0; i < PER; ++i) {
+          const int f = g * PER + i;
+          read(f + 3);
+          if (f % TS == 0 && f / TS + 1 < KK) q[(f / TS + 1) & 1] = query(f / TS + 1);
+          nx[f % TS] = mfma32<F16>(a[f & 3], q[f / TS & 1], f >= TS ? nx[f % TS] : (v16f){});
         }
+        float e[8], sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          // exp(s - m) vs from one exponential; the sum takes 1 / vs
+          e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + i], kq[g], off[g]));
+          sum = i ? sum + e[i] : e[i];
+        }
+        l = __builtin_fmaf(sum, inv[g], l);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const uint32_t hi = pack_bf16x2(e[2 * w], e[2 * w + 1]);
           pf[g][w] = (int)hi;
           if constexpr (F16) pl[g][w] = (int)pack_bf16x2(e[2 * w] - u2f(hi << 16), e[2 * w + 1] - u2f(hi & 0xffff0000u));
         }
+        // a product, then the vector operations that run beside it
+#pragma unroll
+        for (int i = 0; i < PER / TS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x100, TS + Cfg::QLDS, 0);
+#pragma unroll
+          for (int t = 0; t < TS; ++t) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x402, (F16 ? 48 : 32) / PER, 0);
+          }
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
+      if (oddv) {                                // scales no logarithm is taken of
+        const v4f vs = *reinterpret_cast<const v4f *>(s_vs[tile & 3]);
 #pragma unroll
-      for (int n = 0; n < DT; ++n) {
-        if (n + 1 < DT) read_v(n + 1);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int g = (4 * n + i) / DT, d = (4 * n + i) % DT;
-          o[d] = mfma32<false>(va[n & 1][i], pf[g], o[d]);
-          if constexpr (F16) o[d] = mfma32<false>(va[n & 1][i], pl[g], o[d]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+          for (int w = 0; w < 4; ++w) {
+            auto scaled = [&](int x) {
+              const float lo = u2f((uint32_t)x << 16), hi = u2f((uint32_t)x & 0xffff0000u);
+              return (int)pack_bf16x2(lo == 0.f ? 0.f : lo * vs[g], hi == 0.f ? 0.f : hi * vs[g]);
+            };
+            pf[g][w] = scaled(pf[g][w]);
+            if constexpr (F16) pl[g][w] = scaled(pl[g][w]);
+          }
       }
-      if constexpr (FP8) {
-        if (__builtin_amdgcn_readfirstlane(s_bad[tile & 3])) {   // columns that get a NaN
-          const int n = limit - tile * kPTile;
-          const uint64_t sees = n >= 64 ? ~0ull : (n > 0 ? (1ull << n) - 1 : 0);
-          for (int d = h; d < D; d += 2)
-            if (s_nan[buf][d] & sees) atomicOr(&s_row[wave * 32 + r32][d >> 5], 1u << (d & 31));
-        }
+      auto read_v = [&](int f) __attribute__((always_inline)) {
+        if (f < G * DT) a[f & 3] = *reinterpret_cast<const v4i *>(vb + (vat ^ (32 * (f / DT))) + (f % DT) * 32 * 2 * T);
+      };
+#pragma unroll
+      for (int f = 0; f < 3; ++f) read_v(f);
+#pragma unroll
+      for (int f = 0; f < G * DT; ++f) {
+        if (f % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+        read_v(f + 3);
+        o[f % DT] = mfma32<false>(a[f & 3], pf[f / DT], o[f % DT]);
+        if constexpr (F16) o[f % DT] = mfma32<false>(a[f & 3], pl[f / DT], o[f % DT]);
+        if (f == 3) stage(tile + 2);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      clean(tile + 1);
+      fetch(tile);
+      if (FP8 && nans) {                         // columns that get a NaN
+        const int n = limit - tile * T;
+        const uint64_t seen = n >= 64 ? ~0ull : (n > 0 ? (1ull << n) - 1 : 0);
+#pragma unroll 1
+        for (int d = half * Cfg::DH + h; d < (half + 1) * Cfg::DH; d += 2)
+          if (s_nan[tile & 1][d] & seen) atomicOr(&s_row[wrow + r32][d >> 5], 1u << (d & 31));
+      }
+      prepare(tile + 1, nx);
+      lds_barrier();
     };
 
-    int tile = t0;
-    while (tile < t1) {
-      __syncthreads();                           // the tile is staged, the other stage is read
-      if (!__any(tile * kPTile < limit)) break;
-      if (common(tile)) {
-        for (;;) {
-          step(std::false_type{}, tile);
-          if (++tile >= t1) break;
-          __syncthreads();
-          if (!common(tile)) break;
+    if (t0 < t1) {
+      lds_barrier();
+      int tile = t0;
+      if (t0 < w1) {
+        v16f sa[TS] = {}, sb[TS];
+        {
+          const uint8_t *kb = lds + (t0 & 1) * Cfg::TILE;
+#pragma unroll
+          for (int k = 0; k < KK; ++k)
+#pragma unroll
+            for (int t = 0; t < TS; ++t)
+              sa[t] = mfma32<F16>(*reinterpret_cast<const v4i *>(kb + (kat0 ^ (32 * k)) + t * 32 * 2 * D), query(k), sa[t]);
         }
-        if (tile >= t1 || !__any(tile * kPTile < limit)) break;
+        prepare(t0, sa);
+        lds_barrier();                           // step t0 stages over these K
+        for (;;) {
+          step(tile, sa, sb);
+          if (++tile >= w1) break;
+          step(tile, sb, sa);
+          if (++tile >= w1) break;
+        }
+      } else {
+        lds_barrier();
       }
-      step(std::true_type{}, tile++);
-    }
-    // rows that see no more: the workgroup's others do (the tile's barrier is passed)
-    for (; tile < t1; ++tile) {
-      advance(tile);
-      if (tile + 1 < t1) __syncthreads();
+      for (; tile < t1; ++tile) {                // no row of this wave sees more
+        stage(tile + 2);
+        clean(tile + 1);
+        fetch(tile);
+        lds_barrier();
+      }
     }
     if constexpr (FP8) {
-      __syncthreads();
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        const uint32_t bad = s_row[wave * 32 + r32][d];
+        const uint32_t bad = s_row[wrow + r32][half * DT + d];
         if (__any(bad)) {
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -456,18 +557,23 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
       }
     }
 
-    // lane: row r32, columns 32 d + 8 q + 4 h .. + 3 of register quad q
+    // lane: row r32, columns 32 d + 8 q + 4 h .. + 3 of register quad q (of the half)
     l = halves_sum(l);
+    // (the row's place is formed afresh: kept through the loop it spills)
+    int ln = tid & 63;
+    asm volatile("" : "+v"(ln));
+    const int row = rb * Cfg::ROWS + wrow + (ln & 31), h = ln >> 5, col = half * Cfg::DH + 4 * h;
     if (row < rows) {
+      const int qi = row / p.group, hq = head * p.group + row % p.group;
       if (nsplit > 1) {
         const int64_t n = (int64_t)c.rows * p.q_heads, at = (int64_t)split * n + (int64_t)(s.row0 + qi) * p.q_heads + hq;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<v4f *>(p.ws + at * D + 32 * d + 8 * q + 4 * h) =
+            *reinterpret_cast<v4f *>(p.ws + at * D + col + 32 * d + 8 * q) =
                 (v4f){o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
-        if (h == 0) {
+        if (h == 0 && half == 0) {
           float *ml = p.ws + (int64_t)nsplit * n * D + at * 2;
           ml[0] = m;
           ml[1] = l;
@@ -479,7 +585,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint2 *>(op + 32 * d + 8 * q + 4 * h) =
+            *reinterpret_cast<uint2 *>(op + col + 32 * d + 8 * q) =
                 make_uint2(narrow2<SRC>(o[d][4 * q] * inv, o[d][4 * q + 1] * inv),
                            narrow2<SRC>(o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv));
       }
