@@ -44,32 +44,6 @@ DSL_DEV float halves_sum(float v) {
   return u2f(a[0]) + u2f(a[1]);
 }
 
-// v *= f when the wave-uniform `on` is non-zero.  The branch is inside the asm:
-// one in the source made the compiler keep a second copy of the output and move
-// all of it there and back in every tile.  The compiler adds no wait states to
-// inline asm: the 20 here cover a product that may still be writing v (19 at most)
-// and the v_exp_f32 that gave f.
-DSL_DEV void scale_if(int on, v16f &v, float f) {
-  float e[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) e[i] = v[i];
-  asm volatile(
-      "s_cmp_eq_u32 %17, 0\n\t"
-      "s_cbranch_scc1 .Lscale_skip_%=\n\t"
-      "s_nop 15\n\ts_nop 3\n\t"
-      "v_mul_f32 %0, %0, %16\n\tv_mul_f32 %1, %1, %16\n\tv_mul_f32 %2, %2, %16\n\tv_mul_f32 %3, %3, %16\n\t"
-      "v_mul_f32 %4, %4, %16\n\tv_mul_f32 %5, %5, %16\n\tv_mul_f32 %6, %6, %16\n\tv_mul_f32 %7, %7, %16\n\t"
-      "v_mul_f32 %8, %8, %16\n\tv_mul_f32 %9, %9, %16\n\tv_mul_f32 %10, %10, %16\n\tv_mul_f32 %11, %11, %16\n\t"
-      "v_mul_f32 %12, %12, %16\n\tv_mul_f32 %13, %13, %16\n\tv_mul_f32 %14, %14, %16\n\tv_mul_f32 %15, %15, %16\n"
-      ".Lscale_skip_%=:"
-      : "+v"(e[0]), "+v"(e[1]), "+v"(e[2]), "+v"(e[3]), "+v"(e[4]), "+v"(e[5]), "+v"(e[6]), "+v"(e[7]), "+v"(e[8]),
-        "+v"(e[9]), "+v"(e[10]), "+v"(e[11]), "+v"(e[12]), "+v"(e[13]), "+v"(e[14]), "+v"(e[15])
-      : "v"(f), "s"(on)
-      : "scc");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = e[i];
-}
-
 // LDS slot of 16-byte chunk c of row r: rows of D bytes * 2 (K) and 128 bytes
 // (V); both readers (32 rows, chunks c and c + 1 by lane half) meet no bank twice.
 template <int CHUNKS>
@@ -77,38 +51,6 @@ DSL_DEV int pslot(int row, int c) {
   if constexpr (CHUNKS == 4) return c ^ pipe::swz<64>(row);
   else if constexpr (CHUNKS == 8) return c ^ pipe::swz<128>(row);
   else return c ^ (row & 15);
-}
-
-// Scores of a tile's 16-token group to powers of two, -infinity where hidden: token
-// offsets T .. T + 3, T + 8 .. T + 11 of the lane against lim, the tokens that its
-// row sees (T without the lane half's part).  In place, under a branch of its own,
-// like scale_if.
-template <int T>
-DSL_DEV void mask_if(int on, v16f &v, int at, float ks, int lim) {
-  float e[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = v[at + i];
-  asm volatile(
-      "s_cmp_eq_u32 %11, 0\n\t"
-      "s_cbranch_scc1 .Lmask_skip_%=\n\t"
-      "s_nop 15\n\ts_nop 3\n\t"
-      "v_mul_f32 %0, %0, %8\n\tv_mul_f32 %1, %1, %8\n\tv_mul_f32 %2, %2, %8\n\tv_mul_f32 %3, %3, %8\n\t"
-      "v_mul_f32 %4, %4, %8\n\tv_mul_f32 %5, %5, %8\n\tv_mul_f32 %6, %6, %8\n\tv_mul_f32 %7, %7, %8\n\t"
-      "v_cmp_lt_i32 vcc, %12, %9\n\ts_nop 1\n\tv_cndmask_b32 %0, %10, %0, vcc\n\t"
-      "v_cmp_lt_i32 vcc, %13, %9\n\ts_nop 1\n\tv_cndmask_b32 %1, %10, %1, vcc\n\t"
-      "v_cmp_lt_i32 vcc, %14, %9\n\ts_nop 1\n\tv_cndmask_b32 %2, %10, %2, vcc\n\t"
-      "v_cmp_lt_i32 vcc, %15, %9\n\ts_nop 1\n\tv_cndmask_b32 %3, %10, %3, vcc\n\t"
-      "v_cmp_lt_i32 vcc, %16, %9\n\ts_nop 1\n\tv_cndmask_b32 %4, %10, %4, vcc\n\t"
-      "v_cmp_lt_i32 vcc, %17, %9\n\ts_nop 1\n\tv_cndmask_b32 %5, %10, %5, vcc\n\t"
-      "v_cmp_lt_i32 vcc, %18, %9\n\ts_nop 1\n\tv_cndmask_b32 %6, %10, %6, vcc\n\t"
-      "v_cmp_lt_i32 vcc, %19, %9\n\ts_nop 1\n\tv_cndmask_b32 %7, %10, %7, vcc\n"
-      ".Lmask_skip_%=:"
-      : "+v"(e[0]), "+v"(e[1]), "+v"(e[2]), "+v"(e[3]), "+v"(e[4]), "+v"(e[5]), "+v"(e[6]), "+v"(e[7])
-      : "v"(ks), "v"(lim), "v"(-INFINITY), "s"(on), "n"(T), "n"(T + 1), "n"(T + 2), "n"(T + 3), "n"(T + 8), "n"(T + 9),
-        "n"(T + 10), "n"(T + 11)
-      : "scc", "vcc");
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[at + i] = e[i];
 }
 
 // LDS writes of this wave have landed; then the workgroup's barrier.  Loads from
@@ -120,7 +62,7 @@ struct PromptCfg {
   static constexpr int NW = 8, NT = NW * 64;                 // two waves per SIMD
   // dim 256: tiles of 32 tokens, and two waves compute the same scores, each half
   // of the output's columns (all of them would take 128 of its 256 registers)
-  static constexpr int HALVES = D > 128 ? 2 : 1, T = D > 128 ? 32 : 64;
+  static constexpr int HALVES = D > 128 ? 2 : 1, T = D >= 128 ? 32 : 64;
   static constexpr int ROWS = NW / HALVES * 32;              // query rows
   static constexpr int G = T / 16, TS = T / 32;              // 16-token groups, 32-token score tiles
   static constexpr int DH = D / HALVES, DT = DH / 32;        // the wave's output columns
@@ -128,7 +70,7 @@ struct PromptCfg {
   static constexpr int TILE = T * D * 2;                     // bytes of K or V
   static constexpr int UNITS = 2 * T * D / 16 / NT;          // 16-code loads per thread
   // dim 128: the queries stay in LDS (kept in registers, others spill)
-  static constexpr bool QLDS = D == 128;
+  static constexpr bool QLDS = false;
   static constexpr int QBYTES = QLDS ? NW * (D / 16) * 1024 : 0;
 };
 
@@ -383,44 +325,62 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
     const int kat0 = r32 * (2 * D) + pslot<Cfg::KC>(r32, h) * 16;
     const int vat0 = (half * Cfg::DH + r32) * (2 * T) + pslot<Cfg::VC>(r32, h) * 16;
     float kq[G], off[G];                         // the current scores' factors; log2 vs - m
-    // Scores of `tile` are there: hide what is hidden, take their maximum, and bring
-    // sum and output to it where it grew.
-    auto prepare = [&](int tile, v16f (&sc)[TS]) __attribute__((always_inline)) {
+    auto group_max = [&](const v16f (&sc)[TS], int g) __attribute__((always_inline)) {
+      float x = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) x = fmaxf(fmaxf(x, sc[g >> 1][8 * (g & 1) + i]), sc[g >> 1][8 * (g & 1) + i + 1]);
+      return x;
+    };
+    // The scores of `tile` are there.  True where they need `settle` first: a token
+    // is hidden from some row, a scale is off the common path, a row's maximum grew
+    // by more than 2^16, or the wave is done.
+    auto common = [&](int tile, const v16f (&sc)[TS]) __attribute__((always_inline)) {
       const v4f ks = *reinterpret_cast<const v4f *>(s_ks[tile & 3]), lg = *reinterpret_cast<const v4f *>(s_log[tile & 3]);
-      const int slow = __builtin_amdgcn_readfirstlane(
-          (int)(tile * T + T > low || tile >= w1 || s_none[tile & 3] || s_oddk[tile & 3]));
-      const v4i pg = *reinterpret_cast<const v4i *>(s_page[tile & 3]);
-      const int lim = tile < w1 ? limit - tile * T - 4 * h : 0;
-      mask_if<0>(slow, sc[0], 0, ks[0], pg[0] < 0 ? 0 : lim);
-      mask_if<16>(slow, sc[0], 8, ks[1], pg[1] < 0 ? 0 : lim);
-      if constexpr (TS > 1) {
-        mask_if<32>(slow, sc[TS - 1], 0, ks[2], pg[2] < 0 ? 0 : lim);
-        mask_if<48>(slow, sc[TS - 1], 8, ks[3], pg[3] < 0 ? 0 : lim);
-      }
+      const int odd = s_none[tile & 3] | s_oddk[tile & 3];
       float top = -INFINITY;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        kq[g] = slow ? 1.f : ks[g];
-        float x = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) x = fmaxf(fmaxf(x, sc[g >> 1][8 * (g & 1) + i]), sc[g >> 1][8 * (g & 1) + i + 1]);
-        top = fmaxf(top, x * kq[g]);
+        kq[g] = ks[g];
+        off[g] = lg[g] - m;
+        top = fmaxf(top, group_max(sc, g) * ks[g]);
       }
       top = halves_max(top);
-      const int grow = __builtin_amdgcn_readfirstlane((int)__any(top > m + 8.f || m == -INFINITY));
-      const float now = grow ? fmaxf(m, top) : m, ref = now == -INFINITY ? 0.f : now;
-      const float alpha = __builtin_amdgcn_exp2f(m - ref);   // 1 unless it grew
-      m = now;
+      return __builtin_amdgcn_readfirstlane((int)(__any(!(top <= m + 16.f)) || odd || tile * T + T > low || tile >= w1)) != 0;
+    };
+    // The same in general: scores to powers of two, -infinity where hidden, and sum
+    // and output to their maximum.  (Outside the loop of the common tiles: there,
+    // the compiler kept a second copy of the output and moved all of it in every
+    // tile.)
+    auto settle = [&](int tile, v16f (&sc)[TS]) __attribute__((always_inline)) {
+      const v4f ks = *reinterpret_cast<const v4f *>(s_ks[tile & 3]), lg = *reinterpret_cast<const v4f *>(s_log[tile & 3]);
+      const v4i pg = *reinterpret_cast<const v4i *>(s_page[tile & 3]);
+      const int lim = limit - tile * T - 4 * h;
+      float top = m;
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float v = sc[g >> 1][8 * (g & 1) + i] * ks[g];
+          const float x = 16 * g + 8 * (i >> 2) + (i & 3) < lim && pg[g] >= 0 ? v : -INFINITY;
+          sc[g >> 1][8 * (g & 1) + i] = x;
+          top = fmaxf(top, x);
+        }
+      top = halves_max(top);
+      const float ref = top == -INFINITY ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - ref);
+      m = top;
       l *= alpha;
 #pragma unroll
-      for (int d = 0; d < DT; ++d) scale_if(grow, o[d], alpha);
+      for (int d = 0; d < DT; ++d) o[d] *= alpha;
 #pragma unroll
-      for (int g = 0; g < G; ++g) off[g] = lg[g] - ref;
+      for (int g = 0; g < G; ++g) {
+        kq[g] = 1.f;
+        off[g] = lg[g] - ref;
+      }
     };
     // One tile: the exponentials of its scores `sc` between the products of the next
     // tile's scores `nx`; its output's products between the staging of the tile after
     // that; then the next scores' maximum.
-    auto step = [&](int tile, v16f (&sc)[TS], v16f (&nx)[TS]) __attribute__((always_inline)) {
+    auto step = [&](int tile, const v16f (&sc)[TS], v16f (&nx)[TS]) __attribute__((always_inline)) {
       const uint8_t *kb = lds + ((tile + 1) & 1) * Cfg::TILE, *vb = lds + VBASE + (tile & 1) * Cfg::TILE;
       int kat = kat0, vat = vat0;
       asm volatile("" : "+v"(kat), "+v"(vat));
@@ -455,6 +415,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
           sum = i ? sum + e[i] : e[i];
         }
         l = __builtin_fmaf(sum, inv[g], l);
+        asm volatile("" : "+v"(l));              // here, not where l is used: the 32 terms would be kept until then
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const uint32_t hi = pack_bf16x2(e[2 * w], e[2 * w + 1]);
@@ -510,8 +471,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
         for (int d = half * Cfg::DH + h; d < (half + 1) * Cfg::DH; d += 2)
           if (s_nan[tile & 1][d] & seen) atomicOr(&s_row[wrow + r32][d >> 5], 1u << (d & 31));
       }
-      prepare(tile + 1, nx);
-      lds_barrier();
+      return common(tile + 1, nx);
     };
 
     if (t0 < t1) {
@@ -527,13 +487,23 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
             for (int t = 0; t < TS; ++t)
               sa[t] = mfma32<F16>(*reinterpret_cast<const v4i *>(kb + (kat0 ^ (32 * k)) + t * 32 * 2 * D), query(k), sa[t]);
         }
-        prepare(t0, sa);
+        // (a barrier behind settle too: the next step takes the tile's page entries)
+        settle(tile, sa);
         lds_barrier();                           // step t0 stages over these K
         for (;;) {
-          step(tile, sa, sb);
-          if (++tile >= w1) break;
-          step(tile, sb, sa);
-          if (++tile >= w1) break;
+          for (;;) {
+            if (step(tile++, sa, sb)) {
+#pragma unroll
+              for (int t = 0; t < TS; ++t) sa[t] = sb[t];
+              break;
+            }
+            lds_barrier();
+            if (step(tile++, sb, sa)) break;
+            lds_barrier();
+          }
+          if (tile < w1) settle(tile, sa);
+          lds_barrier();
+          if (tile >= w1) break;
         }
       } else {
         lds_barrier();
