@@ -57,21 +57,27 @@ DSL_DEV int pslot(int row, int c) {
 // memory stay in flight (__syncthreads would wait for them).
 DSL_DEV void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// A wave's LDS reads but the last N (all: more false) have returned.
+template <int N>
+DSL_DEV void wait_reads(bool more) {
+  if (more) __builtin_amdgcn_s_waitcnt((15 << 0) | (7 << 4) | (N << 8) | (3 << 14));
+  else pipe::wait_lds();
+}
+
 template <int D>
 struct PromptCfg {
   static constexpr int NW = 8, NT = NW * 64;                 // two waves per SIMD
-  // dim 256: tiles of 32 tokens, and two waves compute the same scores, each half
-  // of the output's columns (all of them would take 128 of its 256 registers)
-  static constexpr int HALVES = D > 128 ? 2 : 1, T = D >= 128 ? 32 : 64;
+  // Dim 256: two waves compute the same scores, each half of the output's columns
+  // (all of them would take 128 of its 256 registers).
+  static constexpr int HALVES = D > 128 ? 2 : 1;
+  static constexpr int T = 8192 / D;                         // tokens of a step
   static constexpr int ROWS = NW / HALVES * 32;              // query rows
   static constexpr int G = T / 16, TS = T / 32;              // 16-token groups, 32-token score tiles
   static constexpr int DH = D / HALVES, DT = DH / 32;        // the wave's output columns
-  static constexpr int KC = D / 8, VC = T / 8;               // 16-byte chunks of K's and V's rows
-  static constexpr int TILE = T * D * 2;                     // bytes of K or V
-  static constexpr int UNITS = 2 * T * D / 16 / NT;          // 16-code loads per thread
-  // dim 128: the queries stay in LDS (kept in registers, others spill)
-  static constexpr bool QLDS = false;
-  static constexpr int QBYTES = QLDS ? NW * (D / 16) * 1024 : 0;
+  static constexpr int VT = T < 64 ? T : 64;                 // tokens of a row of V in LDS (128: two matrices)
+  static constexpr int KC = D / 8, VC = VT / 8;              // 16-byte chunks of K's and V's rows
+  static constexpr int STAGE = T * D * 2;                    // bytes of K or V
+  static_assert(T * D / 16 == NT, "a thread stages 16 codes of K and of V");
 };
 
 // blockIdx: x (row block from the last on) * heads * sequences + ..., y split.
@@ -80,18 +86,19 @@ __global__ __launch_bounds__(PromptCfg<D>::NT) __attribute__((amdgpu_waves_per_e
 void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, const int nsplit) {
   using Cfg = PromptCfg<D>;
   constexpr bool F16 = SRC == SRC_F16;
-  constexpr int T = Cfg::T, G = Cfg::G, TS = Cfg::TS, DT = Cfg::DT;
-  constexpr int KK = D / 16, U = Cfg::UNITS, KU = T * D / 16;
-  constexpr int VBASE = 2 * Cfg::TILE, QBASE = 4 * Cfg::TILE;
-  __shared__ __align__(16) uint8_t lds[4 * Cfg::TILE + Cfg::QBYTES];   // two tiles of K, two of V, queries
-  __shared__ __align__(16) float s_ks[4][4], s_vs[4][4];     // scales of a tile's 16-token groups
-  __shared__ __align__(16) float s_log[4][4], s_inv[4][4];   // log2 vs, 1 / vs
-  __shared__ __align__(16) int s_page[4][4];                 // the groups' pages, -1: none
-  __shared__ int s_none[4], s_oddk[4], s_oddv[4];            // a group in no page; scales off the common path
-  __shared__ int s_bad[4];                                   // NaN codes among V
+  constexpr int T = Cfg::T, G = Cfg::G, TS = Cfg::TS, DT = Cfg::DT, VT = Cfg::VT, VG = VT / 16;
+  constexpr int KK = D / 16, VBASE = 2 * Cfg::STAGE;
+  __shared__ __align__(16) uint8_t lds[5 * Cfg::STAGE];      // two stages of K, three of V
+  // per 16-token group of a stage: score and V scales, log2 and 1 / of the latter,
+  // pages (-1: none)
+  __shared__ __align__(16) float s_ks[4][G], s_vs[4][G], s_log[4][G], s_inv[4][G];
+  __shared__ __align__(16) int s_page[8][G];
+  __shared__ int s_odd[4];                       // scales off the common path (bit 1: of V), or a group of no page
+  __shared__ int s_none[8];                      // a group of no page
+  __shared__ int s_bad[4];                       // NaN codes among V
   // tokens (bits) whose V code is NaN, by column: staged as 0, since 0 * NaN
   // would carry one to rows that do not see it
-  __shared__ uint64_t s_nan[2][FP8 ? D : 1];
+  __shared__ uint64_t s_nan[3][T / VT][FP8 ? D : 1];
   __shared__ uint32_t s_row[FP8 ? Cfg::ROWS : 1][D / 32];   // ... and the columns (bits) that a row gets one in
   const int pairs = c.heads * c.seqs;
   // Row blocks from the last, the longest, on.  Workgroups go to the eight XCDs,
@@ -109,6 +116,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, h = lane >> 5;
   const int wrow = wave / Cfg::HALVES * 32, half = wave % Cfg::HALVES;
+  const int late = wave / 4;                     // a SIMD's second wave
   const SeqView s = seq_view(c, b);
   const int rows = s.n * p.group;
   const int P = c.page, pshift = 31 - __builtin_clz(P), room = c.width * P;
@@ -138,7 +146,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
     // tokens that every row of the wave sees, and that one of them sees
     const int low = __builtin_amdgcn_readfirstlane(limit);
     const int high = __builtin_amdgcn_readlane(limit, 31);
-    int w1 = (high + T - 1) / T;                 // the wave's tiles: t0 .. w1 - 1
+    int w1 = (high + T - 1) / T;                 // the wave's steps: t0 .. w1 - 1
     w1 = w1 < t1 ? w1 : t1;
 
     v16f o[DT];
@@ -146,11 +154,10 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = (v16f){};
 
-    // Pages go to LDS four tiles ahead (four threads look them up a tile before
-    // that), codes and scales to registers a tile before they are staged.  Past the
-    // last tile the pages are none, which read page 0 and stage it where nobody
-    // looks.
-    uint4 raw[U];
+    // Pages go to LDS three tiles ahead (looked up a tile before that), codes and
+    // scales to registers a tile before they are staged.  Past the last tile the
+    // pages are none, which read page 0 and stage it where nobody looks.
+    uint4 rawk, rawv;
     float kraw = 0.f, vraw = 0.f;
     int page = -1;
     auto find = [&](int tile) __attribute__((always_inline)) {
@@ -158,93 +165,65 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
       if (tid < G) page = tile < t1 && tok < len ? (int)page_of(c, b, tok >> pshift) : -1;
     };
     auto keep = [&](int tile) __attribute__((always_inline)) {
-      if (tid < G) {
-        s_page[tile & 3][tid] = page;
-        const uint64_t none = __ballot(page < 0);
-        if (tid == 0) s_none[tile & 3] = none != 0;
-      }
+      if (tid < G) s_page[tile & 7][tid] = page;
     };
-    // this thread's unit j: 16 codes of K (dim 64: by wave) or of V
-    auto is_k = [&](int j) __attribute__((always_inline)) { return U > 1 ? j < U / 2 : wave < Cfg::NW / 2; };
-    // (K of `tile`, V of the one before)
-    auto load = [&](int tk) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int u = tid + Cfg::NT * j;
-        const bool isk = is_k(j);
-        const int tile = isk ? tk : tk - 1;
-        const int g = isk ? u / (D / 16) >> 4 : u & (G - 1), pg = s_page[tile & 3][g];
-        const uint32_t off = isk ? (uint32_t)(((tile * T + u / (D / 16)) & (P - 1)) * D + (u % (D / 16)) * 16)
-                                 : (uint32_t)((((u - KU) / G) << pshift) + ((tile * T + g * 16) & (P - 1)));
-        raw[j] = *reinterpret_cast<const uint4 *>((isk ? kbase : vbase) + (uint64_t)(uint32_t)(pg < 0 ? 0 : pg) * pstride + off);
-      }
+    const int krow = tid / (D / 16), kcol = tid % (D / 16);  // the thread's 16 codes of K
+    const int vd = tid / G, vg = tid % G;                    // ... and of V: column, group
+    auto load = [&](int tile) __attribute__((always_inline)) {
+      const int pk = s_page[tile & 7][krow >> 4], pv = s_page[tile & 7][vg];
+      rawk = *reinterpret_cast<const uint4 *>(kbase + (uint64_t)(uint32_t)(pk < 0 ? 0 : pk) * pstride +
+                                              (uint32_t)(((tile * T + krow) & (P - 1)) * D + kcol * 16));
+      rawv = *reinterpret_cast<const uint4 *>(vbase + (uint64_t)(uint32_t)(pv < 0 ? 0 : pv) * pstride +
+                                              (uint32_t)((vd << pshift) + ((tile * T + vg * 16) & (P - 1))));
     };
-    // this thread's part of K of a tile and of V of the one before as 16-bit operands
-    auto stage = [&](int tk) __attribute__((always_inline)) {
-      uint8_t *kb = lds + (tk & 1) * Cfg::TILE, *vb = lds + VBASE + ((tk - 1) & 1) * Cfg::TILE;
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int u = tid + Cfg::NT * j;
-        const uint4 w = raw[j];
-        if (is_k(j)) {
-          const int r = u / (D / 16), ch = (u % (D / 16)) * 2;
-          uint8_t *to = kb + r * (2 * D);
-          const int at = pslot<Cfg::KC>(r, ch) * 16;
-          *reinterpret_cast<v4i *>(to + at) = codes8<FP8, F16>(w.x, w.y);
-          *reinterpret_cast<v4i *>(to + (at ^ 16)) = codes8<FP8, F16>(w.z, w.w);
-        } else {
-          const int d = (u - KU) / G, g = u & (G - 1);
-          uint8_t *to = vb + d * (2 * T);
-          const int at = pslot<Cfg::VC>(d, 2 * g) * 16;
-          *reinterpret_cast<v4i *>(to + at) = codes8<FP8, false>(w.x, w.z);
-          *reinterpret_cast<v4i *>(to + (at ^ 16)) = codes8<FP8, false>(w.y, w.w);
-        }
-      }
+    // as 16-bit operands
+    const int kput = krow * (2 * D) + pslot<Cfg::KC>(krow, 2 * kcol) * 16;
+    const int vput = vg / VG * (VT * D * 2) + vd * (2 * VT) + pslot<Cfg::VC>(vd, 2 * (vg % VG)) * 16;
+    auto stage = [&](int tile) __attribute__((always_inline)) {
+      uint8_t *kb = lds + (tile & 1) * Cfg::STAGE, *vb = lds + VBASE + tile % 3 * Cfg::STAGE;
+      *reinterpret_cast<v4i *>(kb + kput) = codes8<FP8, F16>(rawk.x, rawk.y);
+      *reinterpret_cast<v4i *>(kb + (kput ^ 16)) = codes8<FP8, F16>(rawk.z, rawk.w);
+      *reinterpret_cast<v4i *>(vb + vput) = codes8<FP8, false>(rawv.x, rawv.z);
+      *reinterpret_cast<v4i *>(vb + (vput ^ 16)) = codes8<FP8, false>(rawv.y, rawv.w);
     };
-    // V of `tile` that some row must not meet, in the thread's own staged units: codes
-    // past the end or of no page, which can be NaN, become 0; NaN ones that a row
-    // may not see move to s_nan.  (Here, not in registers before: that spilled.)
+    // V that some row must not meet, in the thread's own staged codes: those past the
+    // end or of no page, which can be NaN, become 0; NaN ones that a row may not see
+    // move to s_nan.  (Here, not in registers before: that spilled.)
     auto clean = [&](int tile) __attribute__((always_inline)) {
       if constexpr (FP8) {
-        if (!__builtin_amdgcn_readfirstlane((int)(tile * T + T > every || s_none[tile & 3]))) return;
+        if (!(tile * T + T > every || __builtin_amdgcn_readfirstlane(s_none[tile & 7]))) return;
         int t = tid;
         asm volatile("" : "+v"(t));
-        uint32_t bad = 0;
+        const int d = t / G, g = t % G;
+        const int nv = s_page[tile & 7][g] < 0 ? 0 : len - (tile * T + g * 16);
+        uint8_t *row = lds + VBASE + tile % 3 * Cfg::STAGE + g / VG * (VT * D * 2) + d * (2 * VT);
+        uint32_t at = 0;
 #pragma unroll 1
-        for (int j = U > 1 ? U / 2 : 0; j < U; ++j) {
-          const int u = t + Cfg::NT * j, d = (u - KU) / G, g = u & (G - 1);
-          if (u < KU) continue;
-          const int nv = s_page[tile & 3][g] < 0 ? 0 : len - (tile * T + g * 16);
-          uint8_t *row = lds + VBASE + (tile & 1) * Cfg::TILE + d * (2 * T);
-          uint32_t at = 0;
-#pragma unroll 1
-          for (int x = 0; x < 8; ++x) {          // two tokens of a chunk: half x / 4, word x % 4
-            uint32_t *w = reinterpret_cast<uint32_t *>(row + pslot<Cfg::VC>(d, 2 * g + (x >> 2)) * 16) + (x & 3);
-            const int tok = 4 * (x >> 2) + 8 * ((x & 3) >> 1) + 2 * (x & 1);
-            uint32_t v = *w;
-            if (tok >= nv) v &= 0xffff0000u;
-            if (tok + 1 >= nv) v &= 0xffffu;
-            if ((v & 0x7fffu) > 0x7f80u) {
-              at |= 1u << tok;
-              v &= 0xffff0000u;
-            }
-            if ((v & 0x7fffffffu) > 0x7f80ffffu) {
-              at |= 2u << tok;
-              v &= 0xffffu;
-            }
-            *w = v;
+        for (int x = 0; x < 8; ++x) {            // two tokens of a chunk: half x / 4, word x % 4
+          uint32_t *w = reinterpret_cast<uint32_t *>(row + pslot<Cfg::VC>(d, 2 * (g % VG) + (x >> 2)) * 16) + (x & 3);
+          const int tok = 4 * (x >> 2) + 8 * ((x & 3) >> 1) + 2 * (x & 1);
+          uint32_t v = *w;
+          if (tok >= nv) v &= 0xffff0000u;
+          if (tok + 1 >= nv) v &= 0xffffu;
+          if ((v & 0x7fffu) > 0x7f80u) {
+            at |= 1u << tok;
+            v &= 0xffff0000u;
           }
-          reinterpret_cast<uint16_t *>(&s_nan[tile & 1][d])[g] = (uint16_t)at;
-          bad |= at;
+          if ((v & 0x7fffffffu) > 0x7f80ffffu) {
+            at |= 2u << tok;
+            v &= 0xffffu;
+          }
+          *w = v;
         }
-        if (__any(bad) && lane == 0) s_bad[tile & 3] = 1;
+        reinterpret_cast<uint16_t *>(&s_nan[tile % 3][g / VG][d])[g % VG] = (uint16_t)at;
+        if (__any(at) && lane == 0) s_bad[tile & 3] = 1;
       }
     };
-    // the scales: four threads of wave 1
+    // the scales: G threads of wave 1
     const int sg = tid - 64;
     auto load_scales = [&](int tile) __attribute__((always_inline)) {
       if (sg >= 0 && sg < G) {
-        const int pg = s_page[tile & 3][sg];
+        const int pg = s_page[tile & 7][sg];
         const int64_t at = (int64_t)(pg < 0 ? 0 : pg) * c.heads + head;
         kraw = c.k_scale[at];
         vraw = c.v_scale[at];
@@ -252,119 +231,140 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
     };
     auto stage_scales = [&](int tile) __attribute__((always_inline)) {
       if (sg >= 0 && sg < G) {
-        const bool none = s_page[tile & 3][sg] < 0;
+        const bool none = s_page[tile & 7][sg] < 0;
         const float ks = none ? 0.f : kraw * (p.scale * kLog2e), vs = none ? 1.f : vraw;
         const bool odd = !(vs >= 0x1p-60f && vs <= 0x1p60f);
         s_ks[tile & 3][sg] = ks;
         s_vs[tile & 3][sg] = odd ? vs : 1.f;
         s_log[tile & 3][sg] = odd ? 0.f : __builtin_amdgcn_logf(vs);
         s_inv[tile & 3][sg] = odd ? 1.f : __builtin_amdgcn_rcpf(vs);
-        const uint64_t ok = __ballot(!(ks >= 0.f)), ov = __ballot(odd);
-        if (sg == 0) {
-          s_oddk[tile & 3] = ok != 0;
-          s_oddv[tile & 3] = ov != 0;
-        }
+        const uint64_t ok = __ballot(none || !(ks >= 0.f)), ov = __ballot(odd);
+        if (sg == 0) s_odd[tile & 3] = (ok != 0) | (ov != 0) << 1;
       }
     };
-
-    // in step `tile`, once stage(tile + 2) has taken the codes
-    auto fetch = [&](int tile) __attribute__((always_inline)) {
-      load(tile + 3);
+    // what a wave does for later tiles beside the output's products of `tile`: the
+    // late waves, which do those a barrier later, stage a tile further on
+    auto advance = [&](int tile) __attribute__((always_inline)) {
+      const int mine = tile + 1 + late;
+      clean(mine);
+      load(mine + 1);
       if (wave == 0) {
-        if (FP8 && tid == 0) s_bad[(tile + 2) & 3] = 0;      // set in the next step at the earliest
-        keep(tile + 4);
-        find(tile + 5);
+        if (FP8 && tid == 0) s_bad[(tile + 2) & 3] = 0;      // set behind the next barrier at the earliest
+        keep(tile + 3);
+        if constexpr (FP8) {
+          const uint64_t none = __ballot(tid < G && page < 0);
+          if (tid == 0) s_none[(tile + 3) & 7] = none != 0;
+        }
+        find(tile + 4);
       }
       if (wave == 1) {
-        stage_scales(tile + 2);
-        load_scales(tile + 3);
+        stage_scales(tile + 1);
+        load_scales(tile + 2);
       }
     };
 
     __syncthreads();                             // the last block's readers
     if (tid < 4) s_bad[tid] = 0;
+    if (tid < 8) s_none[tid] = 1;                // (the first tiles: as if)
     if constexpr (FP8) {
       for (int i = tid; i < Cfg::ROWS * (D / 32); i += Cfg::NT) s_row[i / (D / 32)][i % (D / 32)] = 0;
     }
     if (t0 < t1) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 3; ++i) {
         find(t0 + i);
         keep(t0 + i);
       }
       __syncthreads();
-      load(t0);                                  // (V of no tile: overwritten below)
+      load(t0);
       load_scales(t0);
       stage(t0);
+      clean(t0);
       stage_scales(t0);
-      __syncthreads();
       load(t0 + 1);
       load_scales(t0 + 1);
-      stage(t0 + 1);
-      clean(t0);
-      stage_scales(t0 + 1);
-      load(t0 + 2);
-      load_scales(t0 + 2);
-      find(t0 + 4);
+      if (late) {
+        stage(t0 + 1);
+        clean(t0 + 1);
+        load(t0 + 2);
+      }
+      find(t0 + 3);
     }
     // the queries have arrived before the loop: a wait for them there would be one
     // for the tiles' loads too
 #pragma unroll
-    for (int k = 0; k < KK; ++k) {
-      if constexpr (Cfg::QLDS) *reinterpret_cast<v4i *>(lds + QBASE + (wave * KK + k) * 1024 + lane * 16) = qf[k];
-      else asm volatile("" : "+v"(qf[k]));
-    }
-    auto query = [&](int k) __attribute__((always_inline)) {
-      if constexpr (Cfg::QLDS) return *reinterpret_cast<const v4i *>(lds + QBASE + (wave * KK + k) * 1024 + lane * 16);
-      else return qf[k];
-    };
+    for (int k = 0; k < KK; ++k) asm volatile("" : "+v"(qf[k]));
 
     // fragment addresses: the rows' swizzles do not depend on t and d, and flip no
     // bit of 32 k, so one register each; formed afresh in every tile (kept for all
     // k they spill)
     const int kat0 = r32 * (2 * D) + pslot<Cfg::KC>(r32, h) * 16;
-    const int vat0 = (half * Cfg::DH + r32) * (2 * T) + pslot<Cfg::VC>(r32, h) * 16;
-    float kq[G], off[G];                         // the current scores' factors; log2 vs - m
-    auto group_max = [&](const v16f (&sc)[TS], int g) __attribute__((always_inline)) {
-      float x = -INFINITY;
+    const int vat0 = (half * Cfg::DH + r32) * (2 * VT) + pslot<Cfg::VC>(r32, h) * 16;
+    v16f sc[TS];
+    float kq[G], off[G];                         // the scores' factors; log2 vs - m
+    // S^T, four fragments ahead of the products that take them
+    auto scores = [&](int tile) __attribute__((always_inline)) {
+      const uint8_t *kb = lds + (tile & 1) * Cfg::STAGE;
+      int kat = kat0;
+      asm volatile("" : "+v"(kat));
+      constexpr int NF = KK * TS, PER = 4;       // fragment f: step f / TS, part f % TS of the tokens
+      v4i a[2][PER];
+      auto read = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) x = fmaxf(fmaxf(x, sc[g >> 1][8 * (g & 1) + i]), sc[g >> 1][8 * (g & 1) + i + 1]);
-      return x;
+        for (int i = 0; i < PER; ++i) {
+          const int f = n * PER + i;
+          a[n & 1][i] = *reinterpret_cast<const v4i *>(kb + (kat ^ (32 * (f / TS))) + (f % TS) * 32 * 2 * D);
+        }
+      };
+      read(0);
+#pragma unroll
+      for (int n = 0; n < NF / PER; ++n) {
+        if (n + 1 < NF / PER) read(n + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        wait_reads<PER>(n + 1 < NF / PER);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int f = n * PER + i;
+          sc[f % TS] = mfma32<F16>(a[n & 1][i], qf[f / TS], f >= TS ? sc[f % TS] : (v16f){});
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     };
-    // The scores of `tile` are there.  True where they need `settle` first: a token
-    // is hidden from some row, a scale is off the common path, a row's maximum grew
-    // by more than 2^16, or the wave is done.
-    auto common = [&](int tile, const v16f (&sc)[TS]) __attribute__((always_inline)) {
-      const v4f ks = *reinterpret_cast<const v4f *>(s_ks[tile & 3]), lg = *reinterpret_cast<const v4f *>(s_log[tile & 3]);
-      const int odd = s_none[tile & 3] | s_oddk[tile & 3];
+    // True where the scores need no `settle`: no token hidden from a row, no scale
+    // off the common path, no row's maximum grown by more than 2^16.
+    auto common = [&](int tile) __attribute__((always_inline)) {
+      const int odd = s_odd[tile & 3];
       float top = -INFINITY;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        kq[g] = ks[g];
-        off[g] = lg[g] - m;
-        top = fmaxf(top, group_max(sc, g) * ks[g]);
+        kq[g] = s_ks[tile & 3][g];
+        off[g] = s_log[tile & 3][g] - m;
+        float x = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) x = fmaxf(fmaxf(x, sc[g >> 1][8 * (g & 1) + i]), sc[g >> 1][8 * (g & 1) + i + 1]);
+        top = fmaxf(top, x * kq[g]);
       }
       top = halves_max(top);
-      return __builtin_amdgcn_readfirstlane((int)(__any(!(top <= m + 16.f)) || odd || tile * T + T > low || tile >= w1)) != 0;
+      return !__builtin_amdgcn_readfirstlane((int)(__any(!(top <= m + 16.f)) || odd || tile * T + T > low));
     };
-    // The same in general: scores to powers of two, -infinity where hidden, and sum
-    // and output to their maximum.  (Outside the loop of the common tiles: there,
-    // the compiler kept a second copy of the output and moved all of it in every
-    // tile.)
-    auto settle = [&](int tile, v16f (&sc)[TS]) __attribute__((always_inline)) {
-      const v4f ks = *reinterpret_cast<const v4f *>(s_ks[tile & 3]), lg = *reinterpret_cast<const v4f *>(s_log[tile & 3]);
-      const v4i pg = *reinterpret_cast<const v4i *>(s_page[tile & 3]);
+    // In general: scores to powers of two, -infinity where hidden; sum and output to
+    // their maximum.  (Outside the loop of the common tiles: there, the compiler kept
+    // a second copy of the output and moved all of it in every tile.)
+    auto settle = [&](int tile) __attribute__((always_inline)) {
       const int lim = limit - tile * T - 4 * h;
       float top = m;
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+      for (int g = 0; g < G; ++g) {
+        const float ks = s_ks[tile & 3][g];
+        const bool there = s_page[tile & 7][g] >= 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float v = sc[g >> 1][8 * (g & 1) + i] * ks[g];
-          const float x = 16 * g + 8 * (i >> 2) + (i & 3) < lim && pg[g] >= 0 ? v : -INFINITY;
+          const float v = sc[g >> 1][8 * (g & 1) + i] * ks;
+          const float x = 16 * g + 8 * (i >> 2) + (i & 3) < lim && there ? v : -INFINITY;
           sc[g >> 1][8 * (g & 1) + i] = x;
           top = fmaxf(top, x);
         }
+      }
       top = halves_max(top);
       const float ref = top == -INFINITY ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - ref);
       m = top;
@@ -374,39 +374,13 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         kq[g] = 1.f;
-        off[g] = lg[g] - ref;
+        off[g] = s_log[tile & 3][g] - ref;
       }
     };
-    // One tile: the exponentials of its scores `sc` between the products of the next
-    // tile's scores `nx`; its output's products between the staging of the tile after
-    // that; then the next scores' maximum.
-    auto step = [&](int tile, const v16f (&sc)[TS], v16f (&nx)[TS]) __attribute__((always_inline)) {
-      const uint8_t *kb = lds + ((tile + 1) & 1) * Cfg::TILE, *vb = lds + VBASE + (tile & 1) * Cfg::TILE;
-      int kat = kat0, vat = vat0;
-      asm volatile("" : "+v"(kat), "+v"(vat));
-      const v4f inv = *reinterpret_cast<const v4f *>(s_inv[tile & 3]);
-      const int oddv = __builtin_amdgcn_readfirstlane(s_oddv[tile & 3]);
-      const int nans = FP8 ? __builtin_amdgcn_readfirstlane(s_bad[tile & 3]) : 0;
-      v4i pf[G], pl[F16 ? G : 1];
-      // fragment f of K: step f / TS, part f % TS of the tokens; three are on their way
-      constexpr int NF = KK * TS, PER = NF / G;
-      v4i a[4], q[2];
-      auto read = [&](int f) __attribute__((always_inline)) {
-        if (f < NF) a[f & 3] = *reinterpret_cast<const v4i *>(kb + (kat ^ (32 * (f / TS))) + (f % TS) * 32 * 2 * D);
-      };
-#pragma unroll
-      for (int f = 0; f < 3; ++f) read(f);
-      q[0] = query(0);
+    v4i pf[G], pl[F16 ? G : 1];
+    auto exponentials = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int f = g * PER + i;
-          read(f + 3);
-          if (f % TS == 0 && f / TS + 1 < KK) q[(f / TS + 1) & 1] = query(f / TS + 1);
-          nx[f % TS] = mfma32<F16>(a[f & 3], q[f / TS & 1], f >= TS ? nx[f % TS] : (v16f){});
-        }
         float e[8], sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -414,105 +388,108 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
           e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + i], kq[g], off[g]));
           sum = i ? sum + e[i] : e[i];
         }
-        l = __builtin_fmaf(sum, inv[g], l);
-        asm volatile("" : "+v"(l));              // here, not where l is used: the 32 terms would be kept until then
+        l = __builtin_fmaf(sum, s_inv[tile & 3][g], l);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const uint32_t hi = pack_bf16x2(e[2 * w], e[2 * w + 1]);
           pf[g][w] = (int)hi;
           if constexpr (F16) pl[g][w] = (int)pack_bf16x2(e[2 * w] - u2f(hi << 16), e[2 * w + 1] - u2f(hi & 0xffff0000u));
         }
-        // a product, then the vector operations that run beside it
+      }
+      asm volatile("" : "+v"(l));                // here, not where l is used: the terms would be kept until then
+    };
+    auto output = [&](int tile) __attribute__((always_inline)) {
+      const uint8_t *vb = lds + VBASE + tile % 3 * Cfg::STAGE;
+      int vat = vat0;
+      asm volatile("" : "+v"(vat));
+      constexpr int NF = G * DT, PER = 4;        // fragment f: group f / DT, columns f % DT
+      v4i a[2][PER];
+      auto read = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < PER / TS; ++i) {
-          __builtin_amdgcn_sched_group_barrier(0x100, TS + Cfg::QLDS, 0);
+        for (int i = 0; i < PER; ++i) {
+          const int g = (n * PER + i) / DT, d = (n * PER + i) % DT;
+          a[n & 1][i] = *reinterpret_cast<const v4i *>(vb + g / VG * (VT * D * 2) + (vat ^ (32 * (g % VG))) + d * 32 * 2 * VT);
+        }
+      };
+      read(0);
 #pragma unroll
-          for (int t = 0; t < TS; ++t) {
-            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x402, (F16 ? 48 : 32) / PER, 0);
-          }
+      for (int n = 0; n < NF / PER; ++n) {
+        if (n + 1 < NF / PER) read(n + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        wait_reads<PER>(n + 1 < NF / PER);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int g = (n * PER + i) / DT, d = (n * PER + i) % DT;
+          o[d] = mfma32<false>(a[n & 1][i], pf[g], o[d]);
+          if constexpr (F16) o[d] = mfma32<false>(a[n & 1][i], pl[g], o[d]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (FP8) {
+        if (__builtin_amdgcn_readfirstlane(s_bad[tile & 3])) {   // columns that get a NaN
+          const int n = limit - tile * T;
+#pragma unroll 1
+          for (int d = half * Cfg::DH + h; d < (half + 1) * Cfg::DH; d += 2)
+#pragma unroll 1
+            for (int x = 0; x < T / VT; ++x) {
+              const int k = n - x * VT;
+              const uint64_t seen = k >= 64 ? ~0ull : (k > 0 ? (1ull << k) - 1 : 0);
+              if (s_nan[tile % 3][x][d] & seen) atomicOr(&s_row[wrow + r32][d >> 5], 1u << (d & 31));
+            }
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
-      if (oddv) {                                // scales no logarithm is taken of
-        const v4f vs = *reinterpret_cast<const v4f *>(s_vs[tile & 3]);
+    };
+    auto odd_scales = [&](int tile) __attribute__((always_inline)) {   // those that no logarithm is taken of
+      if (__builtin_amdgcn_readfirstlane(s_odd[tile & 3] & 2)) {
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g) {
+          const float vs = s_vs[tile & 3][g];
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             auto scaled = [&](int x) {
               const float lo = u2f((uint32_t)x << 16), hi = u2f((uint32_t)x & 0xffff0000u);
-              return (int)pack_bf16x2(lo == 0.f ? 0.f : lo * vs[g], hi == 0.f ? 0.f : hi * vs[g]);
+              return (int)pack_bf16x2(lo == 0.f ? 0.f : lo * vs, hi == 0.f ? 0.f : hi * vs);
             };
             pf[g][w] = scaled(pf[g][w]);
             if constexpr (F16) pl[g][w] = scaled(pl[g][w]);
           }
+        }
       }
-      auto read_v = [&](int f) __attribute__((always_inline)) {
-        if (f < G * DT) a[f & 3] = *reinterpret_cast<const v4i *>(vb + (vat ^ (32 * (f / DT))) + (f % DT) * 32 * 2 * T);
-      };
-#pragma unroll
-      for (int f = 0; f < 3; ++f) read_v(f);
-#pragma unroll
-      for (int f = 0; f < G * DT; ++f) {
-        if (f % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-        read_v(f + 3);
-        o[f % DT] = mfma32<false>(a[f & 3], pf[f / DT], o[f % DT]);
-        if constexpr (F16) o[f % DT] = mfma32<false>(a[f & 3], pl[f / DT], o[f % DT]);
-        if (f == 3) stage(tile + 2);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      clean(tile + 1);
-      fetch(tile);
-      if (FP8 && nans) {                         // columns that get a NaN
-        const int n = limit - tile * T;
-        const uint64_t seen = n >= 64 ? ~0ull : (n > 0 ? (1ull << n) - 1 : 0);
-#pragma unroll 1
-        for (int d = half * Cfg::DH + h; d < (half + 1) * Cfg::DH; d += 2)
-          if (s_nan[tile & 1][d] & seen) atomicOr(&s_row[wrow + r32][d >> 5], 1u << (d & 31));
-      }
-      return common(tile + 1, nx);
     };
 
     if (t0 < t1) {
+      // One barrier per tile.  Between two of them the early waves do scores, softmax
+      // and output of a tile, a SIMD's late wave the output of the tile before, then
+      // scores and softmax: one's products run beside the other's exponentials.
       lds_barrier();
       int tile = t0;
       if (t0 < w1) {
-        v16f sa[TS] = {}, sb[TS];
-        {
-          const uint8_t *kb = lds + (t0 & 1) * Cfg::TILE;
-#pragma unroll
-          for (int k = 0; k < KK; ++k)
-#pragma unroll
-            for (int t = 0; t < TS; ++t)
-              sa[t] = mfma32<F16>(*reinterpret_cast<const v4i *>(kb + (kat0 ^ (32 * k)) + t * 32 * 2 * D), query(k), sa[t]);
-        }
-        // (a barrier behind settle too: the next step takes the tile's page entries)
-        settle(tile, sa);
-        lds_barrier();                           // step t0 stages over these K
-        for (;;) {
+        scores(t0);
+        bool more = true;
+        do {
+          settle(tile);
           for (;;) {
-            if (step(tile++, sa, sb)) {
-#pragma unroll
-              for (int t = 0; t < TS; ++t) sa[t] = sb[t];
+            exponentials(tile);
+            odd_scales(tile);
+            if (late) lds_barrier();
+            output(tile);
+            stage(tile + 1 + late);
+            advance(tile);
+            if (!late) lds_barrier();
+            if (++tile >= w1) {
+              more = false;
               break;
             }
-            lds_barrier();
-            if (step(tile++, sb, sa)) break;
-            lds_barrier();
+            scores(tile);
+            if (!common(tile)) break;
           }
-          if (tile < w1) settle(tile, sa);
-          lds_barrier();
-          if (tile >= w1) break;
-        }
-      } else {
-        lds_barrier();
+        } while (more);
       }
       for (; tile < t1; ++tile) {                // no row of this wave sees more
-        stage(tile + 2);
-        clean(tile + 1);
-        fetch(tile);
-        lds_barrier();
+        if (late) lds_barrier();
+        stage(tile + 1 + late);
+        advance(tile);
+        if (!late) lds_barrier();
       }
     }
     if constexpr (FP8) {
