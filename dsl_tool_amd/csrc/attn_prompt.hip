@@ -169,12 +169,14 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
     };
     const int krow = tid / (D / 16), kcol = tid % (D / 16);  // the thread's 16 codes of K
     const int vd = tid / G, vg = tid % G;                    // ... and of V: column, group
-    auto load = [&](int tile) __attribute__((always_inline)) {
-      const int pk = s_page[tile & 7][krow >> 4], pv = s_page[tile & 7][vg];
+    auto load_pages = [&](int tile, int pk, int pv) __attribute__((always_inline)) {
       rawk = *reinterpret_cast<const uint4 *>(kbase + (uint64_t)(uint32_t)(pk < 0 ? 0 : pk) * pstride +
                                               (uint32_t)(((tile * T + krow) & (P - 1)) * D + kcol * 16));
       rawv = *reinterpret_cast<const uint4 *>(vbase + (uint64_t)(uint32_t)(pv < 0 ? 0 : pv) * pstride +
                                               (uint32_t)((vd << pshift) + ((tile * T + vg * 16) & (P - 1))));
+    };
+    auto load = [&](int tile) __attribute__((always_inline)) {
+      load_pages(tile, s_page[tile & 7][krow >> 4], s_page[tile & 7][vg]);
     };
     // as 16-bit operands
     const int kput = krow * (2 * D) + pslot<Cfg::KC>(krow, 2 * kcol) * 16;
@@ -189,9 +191,9 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
     // V that some row must not meet, in the thread's own staged codes: those past the
     // end or of no page, which can be NaN, become 0; NaN ones that a row may not see
     // move to s_nan.  (Here, not in registers before: that spilled.)
-    auto clean = [&](int tile) __attribute__((always_inline)) {
+    auto clean = [&](int tile, int none) __attribute__((always_inline)) {
       if constexpr (FP8) {
-        if (!(tile * T + T > every || __builtin_amdgcn_readfirstlane(s_none[tile & 7]))) return;
+        if (!(tile * T + T > every || __builtin_amdgcn_readfirstlane(none))) return;
         int t = tid;
         asm volatile("" : "+v"(t));
         const int d = t / G, g = t % G;
@@ -244,10 +246,15 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
     };
     // what a wave does for later tiles beside the output's products of `tile`: the
     // late waves, which do those a barrier later, stage a tile further on
-    auto advance = [&](int tile) __attribute__((always_inline)) {
+    auto advance = [&](int tile, auto between) __attribute__((always_inline)) {
+      // (read ahead of the products: each wait would be exposed behind them)
       const int mine = tile + 1 + late;
-      clean(mine);
-      load(mine + 1);
+      const int none = FP8 ? s_none[mine & 7] : 0, bad = FP8 ? s_bad[tile & 3] : 0;
+      const int pk = s_page[(mine + 1) & 7][krow >> 4], pv = s_page[(mine + 1) & 7][vg];
+      between(bad);
+      stage(mine);
+      clean(mine, none);
+      load_pages(mine + 1, pk, pv);
       if (wave == 0) {
         if (FP8 && tid == 0) s_bad[(tile + 2) & 3] = 0;      // set behind the next barrier at the earliest
         keep(tile + 3);
@@ -279,13 +286,13 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
       load(t0);
       load_scales(t0);
       stage(t0);
-      clean(t0);
+      clean(t0, 1);
       stage_scales(t0);
       load(t0 + 1);
       load_scales(t0 + 1);
       if (late) {
         stage(t0 + 1);
-        clean(t0 + 1);
+        clean(t0 + 1, 1);
         load(t0 + 2);
       }
       find(t0 + 3);
@@ -302,6 +309,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
     const int vat0 = (half * Cfg::DH + r32) * (2 * VT) + pslot<Cfg::VC>(r32, h) * 16;
     v16f sc[TS];
     float kq[G], off[G];                         // the scores' factors; log2 vs - m
+    int odd = 0;                                 // s_odd of the scores' tile
     // S^T, four fragments ahead of the products that take them
     auto scores = [&](int tile) __attribute__((always_inline)) {
       const uint8_t *kb = lds + (tile & 1) * Cfg::STAGE;
@@ -333,7 +341,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
     // True where the scores need no `settle`: no token hidden from a row, no scale
     // off the common path, no row's maximum grown by more than 2^16.
     auto common = [&](int tile) __attribute__((always_inline)) {
-      const int odd = s_odd[tile & 3];
+      odd = s_odd[tile & 3];
       float top = -INFINITY;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
@@ -351,6 +359,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
     // their maximum.  (Outside the loop of the common tiles: there, the compiler kept
     // a second copy of the output and moved all of it in every tile.)
     auto settle = [&](int tile) __attribute__((always_inline)) {
+      odd = s_odd[tile & 3];
       const int lim = limit - tile * T - 4 * h;
       float top = m;
 #pragma unroll
@@ -398,7 +407,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
       }
       asm volatile("" : "+v"(l));                // here, not where l is used: the terms would be kept until then
     };
-    auto output = [&](int tile) __attribute__((always_inline)) {
+    auto output = [&](int tile, int bad) __attribute__((always_inline)) {
       const uint8_t *vb = lds + VBASE + tile % 3 * Cfg::STAGE;
       int vat = vat0;
       asm volatile("" : "+v"(vat));
@@ -426,7 +435,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
         __builtin_amdgcn_sched_barrier(0);
       }
       if constexpr (FP8) {
-        if (__builtin_amdgcn_readfirstlane(s_bad[tile & 3])) {   // columns that get a NaN
+        if (__builtin_amdgcn_readfirstlane(bad)) {   // columns that get a NaN
           const int n = limit - tile * T;
 #pragma unroll 1
           for (int d = half * Cfg::DH + h; d < (half + 1) * Cfg::DH; d += 2)
@@ -440,7 +449,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
       }
     };
     auto odd_scales = [&](int tile) __attribute__((always_inline)) {   // those that no logarithm is taken of
-      if (__builtin_amdgcn_readfirstlane(s_odd[tile & 3] & 2)) {
+      if (__builtin_amdgcn_readfirstlane(odd) & 2) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           const float vs = s_vs[tile & 3][g];
@@ -472,9 +481,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
             exponentials(tile);
             odd_scales(tile);
             if (late) lds_barrier();
-            output(tile);
-            stage(tile + 1 + late);
-            advance(tile);
+            advance(tile, [&](int bad) __attribute__((always_inline)) { output(tile, bad); });
             if (!late) lds_barrier();
             if (++tile >= w1) {
               more = false;
@@ -487,8 +494,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
       }
       for (; tile < t1; ++tile) {                // no row of this wave sees more
         if (late) lds_barrier();
-        stage(tile + 1 + late);
-        advance(tile);
+        advance(tile, [](int) {});
         if (!late) lds_barrier();
       }
     }
