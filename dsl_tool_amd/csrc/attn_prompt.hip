@@ -88,7 +88,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
   constexpr bool F16 = SRC == SRC_F16;
   constexpr int T = Cfg::T, G = Cfg::G, TS = Cfg::TS, DT = Cfg::DT, VT = Cfg::VT, VG = VT / 16;
   constexpr int KK = D / 16, VBASE = 2 * Cfg::STAGE;
-  __shared__ __align__(16) uint8_t lds[5 * Cfg::STAGE];      // two stages of K, three of V
+  __shared__ __align__(16) uint8_t lds[4 * Cfg::STAGE];      // two tiles of K, two of V
   // per 16-token group of a stage: score and V scales, log2 and 1 / of the latter,
   // pages (-1: none)
   __shared__ __align__(16) float s_ks[4][G], s_vs[4][G], s_log[4][G], s_inv[4][G];
@@ -98,7 +98,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
   __shared__ int s_bad[4];                       // NaN codes among V
   // tokens (bits) whose V code is NaN, by column: staged as 0, since 0 * NaN
   // would carry one to rows that do not see it
-  __shared__ uint64_t s_nan[3][T / VT][FP8 ? D : 1];
+  __shared__ uint64_t s_nan[2][T / VT][FP8 ? D : 1];
   __shared__ uint32_t s_row[FP8 ? Cfg::ROWS : 1][D / 32];   // ... and the columns (bits) that a row gets one in
   const int pairs = c.heads * c.seqs;
   // Row blocks from the last, the longest, on.  Workgroups go to the eight XCDs,
@@ -116,7 +116,6 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, h = lane >> 5;
   const int wrow = wave / Cfg::HALVES * 32, half = wave % Cfg::HALVES;
-  const int late = wave / 4;                     // a SIMD's second wave
   const SeqView s = seq_view(c, b);
   const int rows = s.n * p.group;
   const int P = c.page, pshift = 31 - __builtin_clz(P), room = c.width * P;
@@ -182,7 +181,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
     const int kput = krow * (2 * D) + pslot<Cfg::KC>(krow, 2 * kcol) * 16;
     const int vput = vg / VG * (VT * D * 2) + vd * (2 * VT) + pslot<Cfg::VC>(vd, 2 * (vg % VG)) * 16;
     auto stage = [&](int tile) __attribute__((always_inline)) {
-      uint8_t *kb = lds + (tile & 1) * Cfg::STAGE, *vb = lds + VBASE + tile % 3 * Cfg::STAGE;
+      uint8_t *kb = lds + (tile & 1) * Cfg::STAGE, *vb = lds + VBASE + (tile & 1) * Cfg::STAGE;
       *reinterpret_cast<v4i *>(kb + kput) = codes8<FP8, F16>(rawk.x, rawk.y);
       *reinterpret_cast<v4i *>(kb + (kput ^ 16)) = codes8<FP8, F16>(rawk.z, rawk.w);
       *reinterpret_cast<v4i *>(vb + vput) = codes8<FP8, false>(rawv.x, rawv.z);
@@ -198,7 +197,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
         asm volatile("" : "+v"(t));
         const int d = t / G, g = t % G;
         const int nv = s_page[tile & 7][g] < 0 ? 0 : len - (tile * T + g * 16);
-        uint8_t *row = lds + VBASE + tile % 3 * Cfg::STAGE + g / VG * (VT * D * 2) + d * (2 * VT);
+        uint8_t *row = lds + VBASE + (tile & 1) * Cfg::STAGE + g / VG * (VT * D * 2) + d * (2 * VT);
         uint32_t at = 0;
 #pragma unroll 1
         for (int x = 0; x < 8; ++x) {            // two tokens of a chunk: half x / 4, word x % 4
@@ -217,7 +216,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
           }
           *w = v;
         }
-        reinterpret_cast<uint16_t *>(&s_nan[tile % 3][g / VG][d])[g % VG] = (uint16_t)at;
+        reinterpret_cast<uint16_t *>(&s_nan[tile & 1][g / VG][d])[g % VG] = (uint16_t)at;
         if (__any(at) && lane == 0) s_bad[tile & 3] = 1;
       }
     };
@@ -244,17 +243,15 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
         if (sg == 0) s_odd[tile & 3] = (ok != 0) | (ov != 0) << 1;
       }
     };
-    // what a wave does for later tiles beside the output's products of `tile`: the
-    // late waves, which do those a barrier later, stage a tile further on
+    // what a wave does for later tiles around the output's products of `tile`
     auto advance = [&](int tile, auto between) __attribute__((always_inline)) {
       // (read ahead of the products: each wait would be exposed behind them)
-      const int mine = tile + 1 + late;
-      const int none = FP8 ? s_none[mine & 7] : 0, bad = FP8 ? s_bad[tile & 3] : 0;
-      const int pk = s_page[(mine + 1) & 7][krow >> 4], pv = s_page[(mine + 1) & 7][vg];
+      const int none = FP8 ? s_none[(tile + 1) & 7] : 0, bad = FP8 ? s_bad[tile & 3] : 0;
+      const int pk = s_page[(tile + 2) & 7][krow >> 4], pv = s_page[(tile + 2) & 7][vg];
       between(bad);
-      stage(mine);
-      clean(mine, none);
-      load_pages(mine + 1, pk, pv);
+      stage(tile + 1);
+      load_pages(tile + 2, pk, pv);
+      clean(tile + 1, none);
       if (wave == 0) {
         if (FP8 && tid == 0) s_bad[(tile + 2) & 3] = 0;      // set behind the next barrier at the earliest
         keep(tile + 3);
@@ -290,11 +287,6 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
       stage_scales(t0);
       load(t0 + 1);
       load_scales(t0 + 1);
-      if (late) {
-        stage(t0 + 1);
-        clean(t0 + 1, 1);
-        load(t0 + 2);
-      }
       find(t0 + 3);
     }
     // the queries have arrived before the loop: a wait for them there would be one
@@ -408,7 +400,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
       asm volatile("" : "+v"(l));                // here, not where l is used: the terms would be kept until then
     };
     auto output = [&](int tile, int bad) __attribute__((always_inline)) {
-      const uint8_t *vb = lds + VBASE + tile % 3 * Cfg::STAGE;
+      const uint8_t *vb = lds + VBASE + (tile & 1) * Cfg::STAGE;
       int vat = vat0;
       asm volatile("" : "+v"(vat));
       constexpr int NF = G * DT, PER = 4;        // fragment f: group f / DT, columns f % DT
@@ -443,7 +435,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
             for (int x = 0; x < T / VT; ++x) {
               const int k = n - x * VT;
               const uint64_t seen = k >= 64 ? ~0ull : (k > 0 ? (1ull << k) - 1 : 0);
-              if (s_nan[tile % 3][x][d] & seen) atomicOr(&s_row[wrow + r32][d >> 5], 1u << (d & 31));
+              if (s_nan[tile & 1][x][d] & seen) atomicOr(&s_row[wrow + r32][d >> 5], 1u << (d & 31));
             }
         }
       }
@@ -467,9 +459,9 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
     };
 
     if (t0 < t1) {
-      // One barrier per tile.  Between two of them the early waves do scores, softmax
-      // and output of a tile, a SIMD's late wave the output of the tile before, then
-      // scores and softmax: one's products run beside the other's exponentials.
+      // One barrier per tile.  (A SIMD's second wave half a tile behind the first, so
+      // that one's products always ran beside the other's exponentials, was slower:
+      // 270 against 255 us.)
       lds_barrier();
       int tile = t0;
       if (t0 < w1) {
@@ -480,9 +472,8 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
           for (;;) {
             exponentials(tile);
             odd_scales(tile);
-            if (late) lds_barrier();
             advance(tile, [&](int bad) __attribute__((always_inline)) { output(tile, bad); });
-            if (!late) lds_barrier();
+            lds_barrier();
             if (++tile >= w1) {
               more = false;
               break;
@@ -493,9 +484,8 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
         } while (more);
       }
       for (; tile < t1; ++tile) {                // no row of this wave sees more
-        if (late) lds_barrier();
         advance(tile, [](int) {});
-        if (!late) lds_barrier();
+        lds_barrier();
       }
     }
     if constexpr (FP8) {
