@@ -16,31 +16,44 @@
 namespace dsl {
 
 constexpr int kTile = 64;      // tokens per step of a wave
+constexpr int SPLIT_WGS = 2;
 constexpr int kPromptRows = 64;   // query rows of a sequence and cache head from which attn_prompt.hip serves
 
-// RB blocks of 16 query rows share every load.  blockIdx: x split, y head +
-// heads * row block, z sequence.
+// RB blocks of 16 query rows share every load.  blockIdx: x split * pairs + pair
+// (sequence and head), y row block.  Workgroups go to the XCDs in turn: with the
+// split running fastest, the late splits, which only long sequences have, all
+// landed on the same ones (64 sequences of 2000 to 8192 tokens: 170 against 12x us).
 template <int SRC, bool FP8, int D, int RB>
 __global__ __launch_bounds__(256) void attn_rows_kernel(const KvCacheArgs c, const AttnArgs p, const int nsplit,
-                                                        const int nblk) {
+                                                        const int chunk, const int nblk) {
   constexpr bool F16 = SRC == SRC_F16;
   constexpr int NW = 4, DT = D / 16, DC = D / 64;
   constexpr int LD = D + 4;                      // floats per row of the joined tile
   __shared__ __align__(16) float so[NW][16 * LD];
   __shared__ float sm[NW][16], sl[NW][16];
-  const int b = blockIdx.z, head = blockIdx.y % c.heads, split = blockIdx.x;
+  const int pairs = c.heads * c.seqs, pair = blockIdx.x % pairs;
+  const int b = pair / c.heads, head = pair % c.heads, split = blockIdx.x / pairs;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const SeqView s = seq_view(c, b);
   const int rows = s.n * p.group;
   const int room = c.width * c.page;             // tokens that the table has pages for
   const int ntiles = ((s.len < room ? s.len : room) + kTile - 1) / kTile;
-  const int t0 = (int)((int64_t)ntiles * split / nsplit), t1 = (int)((int64_t)ntiles * (split + 1) / nsplit);
+  const int t0 = split * chunk, t1 = t0 + chunk < ntiles ? t0 + chunk : ntiles;
   const int ktok = 16 * (r16 >> 2) + (r16 & 3);  // the lane's token of K tile 0 (tile t: + 4 t)
   const int P = c.page;
   const int64_t hstride = (int64_t)P * D;
 
-  for (int rb = blockIdx.y / c.heads; rb * 16 * RB < rows; rb += nblk) {
+  if (nsplit > 1 && t0 >= t1) {                  // behind the sequence's end: no sums
+    for (int r = blockIdx.y * 256 + threadIdx.x; r < rows; r += nblk * 256) {
+      const int i = r / p.group, hq = head * p.group + r % p.group;
+      float *ml = p.ws + (int64_t)nsplit * c.rows * p.q_heads * D + (((int64_t)split * c.rows + s.row0 + i) * p.q_heads + hq) * 2;
+      ml[0] = -INFINITY;
+      ml[1] = 0.f;
+    }
+    return;
+  }
+  for (int rb = blockIdx.y; rb * 16 * RB < rows; rb += nblk) {
     // the rows' queries, as they stand in the products
     v4i qf[RB][2 * DC];
     int limit[RB];
@@ -251,40 +264,64 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const KvCacheArgs c, con
   }
 }
 
-// Joins the splits of one query row and head: four columns per thread.
-template <int SRC>
-__global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const int64_t rows, const int D,
-                                                        const int nsplit) {
-  const int per = D / 4;
-  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x, n = rows * p.q_heads;
-  const int64_t at = x / per;
-  if (at >= n) return;
-  const int col = (int)(x % per) * 4;
+// Joins the splits of one query row and head in a workgroup: a split per thread for
+// the maximum and the sum, then four columns per thread, the splits dealt to 1024 / D
+// threads of each.  (All splits in one thread's loop, a load's latency each, took 14
+// to 27 us.)  An empty split has no sums.
+constexpr int kMaxSplits = 256;
+template <int SRC, int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const int64_t rows, const int nsplit) {
+  constexpr int CG = D / 4, SL = 256 / CG;
+  __shared__ float s_f[kMaxSplits], s_red[8];
+  __shared__ v4f s_v[SL][CG];
+  const int64_t at = blockIdx.x, n = rows * p.q_heads;
+  const int tid = threadIdx.x;
   const float *ml = p.ws + (int64_t)nsplit * n * D;
-  float m = -INFINITY;
-  for (int s = 0; s < nsplit; ++s) m = fmaxf(m, ml[(s * n + at) * 2]);
-  float l = 0.f;
-  v4f v = (v4f){0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < nsplit; ++s) {
-    const float ms = ml[(s * n + at) * 2];
-    if (ms == -INFINITY) continue;               // an empty split wrote no sums
-    const float f = __builtin_amdgcn_exp2f(ms - m);
-    l += ml[(s * n + at) * 2 + 1] * f;
-    v += *reinterpret_cast<const v4f *>(p.ws + (s * n + at) * D + col) * f;
+  float m = -INFINITY, l = 0.f;
+  if (tid < nsplit) {
+    m = ml[(tid * n + at) * 2];
+    l = ml[(tid * n + at) * 2 + 1];
   }
+  float top = m;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if ((tid & 63) == 0) s_red[tid >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+  const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+  s_f[tid] = f;
+  l *= f;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+  if ((tid & 63) == 0) s_red[4 + (tid >> 6)] = l;
+  __syncthreads();
+  const int cg = tid % CG, sl = tid / CG;
+  v4f v = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = sl; s < nsplit; s += SL) {
+    const float fs = s_f[s];
+    if (fs != 0.f) v += *reinterpret_cast<const v4f *>(p.ws + (s * n + at) * D + cg * 4) * fs;
+  }
+  s_v[sl][cg] = v;
+  __syncthreads();
+  if (tid >= CG) return;
+#pragma unroll
+  for (int k = 1; k < SL; ++k) v += s_v[k][cg];
+  l = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
   const float inv = l > 0.f ? 1.0f / l : 0.f;
-  uint16_t *op = static_cast<uint16_t *>(p.o) + (at / p.q_heads) * p.o_row + (at % p.q_heads) * p.o_head + col;
+  uint16_t *op = static_cast<uint16_t *>(p.o) + (at / p.q_heads) * p.o_row + (at % p.q_heads) * p.o_head + cg * 4;
   *reinterpret_cast<uint2 *>(op) = make_uint2(narrow2<SRC>(v[0] * inv, v[1] * inv), narrow2<SRC>(v[2] * inv, v[3] * inv));
 }
 
 struct AttnPlan {
   bool prompt;
-  int rb, nblk, nsplit;
+  int rb, nblk, nsplit, chunk;   // chunk: tiles of a split (few rows)
 };
 static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
   AttnPlan a;
   const int64_t rows = (int64_t)max_q * (q_heads / c.heads);
   a.prompt = rows > kPromptRows;
+  a.chunk = 0;
   if (a.prompt) {
     const int per = attn_prompt_rows(c.dim);
     const int64_t pairs = (int64_t)c.heads * c.seqs, blocks = (rows + per - 1) / per;
@@ -301,15 +338,20 @@ static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
   }
   // (dim 256: two blocks of rows spill)
   a.rb = rows <= 16 || c.dim > 128 ? 1 : 2;
-  const int64_t blocks = (rows + 16 * a.rb - 1) / (16 * a.rb), room = 65535 / c.heads;
+  const int64_t blocks = (rows + 16 * a.rb - 1) / (16 * a.rb), room = 65535;
   a.nblk = (int)(blocks < 1 ? 1 : (blocks < room ? blocks : room));   // each walks every nblk-th
-  // two workgroups per CU, at least one tile for every wave
-  const int64_t units = (int64_t)c.heads * c.seqs * a.nblk, want = 2 * (int64_t)device_cu_count();
+  // Splits of equal length, so that sequences of any lengths load the CUs evenly
+  // (those behind a sequence's end leave at once); at least one tile for every wave.
+  const int64_t units = (int64_t)c.heads * c.seqs * a.nblk, want = SPLIT_WGS * (int64_t)device_cu_count();
   const int64_t tiles = ((int64_t)c.width * c.page + kTile - 1) / kTile, most = (tiles + 3) / 4;
   int64_t ns = units > 0 ? want / units : 1;
   if (ns > most) ns = most;
-  if (ns > 256) ns = 256;
-  a.nsplit = ns < 1 ? 1 : (int)ns;
+  if (ns > kMaxSplits) ns = kMaxSplits;
+  if (ns < 1) ns = 1;
+  a.chunk = (int)((tiles + ns - 1) / ns);
+  a.chunk = (a.chunk + 3) / 4 * 4;               // whole rounds of the four waves
+  a.nsplit = (int)((tiles + a.chunk - 1) / (a.chunk > 0 ? a.chunk : 1));
+  if (a.nsplit < 1) a.nsplit = 1;
   return a;
 }
 
@@ -320,9 +362,9 @@ size_t attn_workspace_bytes(const KvCacheArgs &c, int q_heads, int max_q) {
 
 template <int SRC, bool FP8, int D>
 static void launch_rows(const KvCacheArgs &c, const AttnArgs &p, const AttnPlan &a, hipStream_t st) {
-  const dim3 grid((unsigned)a.nsplit, (unsigned)(c.heads * a.nblk), (unsigned)c.seqs);
-  if (a.rb == 1) attn_rows_kernel<SRC, FP8, D, 1><<<grid, 256, 0, st>>>(c, p, a.nsplit, a.nblk);
-  else if constexpr (D <= 128) attn_rows_kernel<SRC, FP8, D, 2><<<grid, 256, 0, st>>>(c, p, a.nsplit, a.nblk);
+  const dim3 grid((unsigned)((int64_t)a.nsplit * c.heads * c.seqs), (unsigned)a.nblk);
+  if (a.rb == 1) attn_rows_kernel<SRC, FP8, D, 1><<<grid, 256, 0, st>>>(c, p, a.nsplit, a.chunk, a.nblk);
+  else if constexpr (D <= 128) attn_rows_kernel<SRC, FP8, D, 2><<<grid, 256, 0, st>>>(c, p, a.nsplit, a.chunk, a.nblk);
 }
 
 template <int SRC>
@@ -341,8 +383,10 @@ static hipError_t launch_src(const KvCacheArgs &c, const AttnArgs &p, hipStream_
     else launch_rows<SRC, false, 256>(c, p, a, st);
   }
   if (a.nsplit > 1) {
-    const int64_t n = (int64_t)c.rows * p.q_heads * (c.dim / 4);
-    attn_join_kernel<SRC><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p, c.rows, c.dim, a.nsplit);
+    const unsigned n = (unsigned)c.rows * (unsigned)p.q_heads;
+    if (c.dim == 64) attn_join_kernel<SRC, 64><<<n, 256, 0, st>>>(p, c.rows, a.nsplit);
+    else if (c.dim == 128) attn_join_kernel<SRC, 128><<<n, 256, 0, st>>>(p, c.rows, a.nsplit);
+    else attn_join_kernel<SRC, 256><<<n, 256, 0, st>>>(p, c.rows, a.nsplit);
   }
   return hipGetLastError();
 }
