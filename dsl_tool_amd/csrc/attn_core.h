@@ -1,5 +1,5 @@
 // Pieces shared by the attention kernels over the paged 8-bit cache
-// (attn.hip: few query rows; attn_prefill.hip: many).
+// (attn.hip: few query rows; attn_prompt.hip: many).
 //
 // With K codes kc, V codes vc and their page's scales ks, vs:
 //   s = (scale ks) (kc . q),  o = sum_t exp(s_t - m) vs_t vc_t / sum_t exp(s_t - m).

@@ -190,7 +190,7 @@ int dsl_kv8_write(void *k_cache, void *v_cache, float *k_scale, float *v_scale, 
   if ((rc = check_heads(fn, "k", k, k_row, k_head, heads, dim)) ||
       (rc = check_heads(fn, "v", v, v_row, v_head, heads, dim)))
     return rc;
-  const dsl::KvWriteArgs p{k, v, k_row, k_head, v_row, v_head, (int)(max_q < rows ? max_q : rows)};
+  const dsl::KvWriteArgs p{k, v, k_row, k_head, v_row, v_head};
   return hip_status(dsl::launch_kv_write(src_of(x_dtype), c, p, static_cast<hipStream_t>(stream)), fn);
 }
 

@@ -1,5 +1,5 @@
 // Codes of the paged 8-bit cache and its sequences, shared by the kernels that
-// write, read and attend over it (kvcache.hip, attn.hip, attn_prefill.hip).
+// write, read and attend over it (kvcache.hip, attn.hip, attn_prompt.hip).
 //
 // Page p, head h: keys k[p][h][token][dim] and values v[p][h][dim][token], so
 // that both lie along the dimension that attention's products sum over (dim
@@ -49,13 +49,9 @@ DSL_DEV void code_values(uint32_t w, float *f) {
   }
 }
 
-// The codes of x[i] / s (the IEEE quotient), byte i = element i.
+// The codes of four quotients, the first in the low byte.
 template <bool FP8>
-DSL_DEV uint32_t codes_of(float a, float b, float c, float d, float s) {
-  a = __fdiv_rn(a, s);
-  b = __fdiv_rn(b, s);
-  c = __fdiv_rn(c, s);
-  d = __fdiv_rn(d, s);
+DSL_DEV uint32_t codes_pack(float a, float b, float c, float d) {
   if constexpr (FP8) {
     const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);

@@ -50,7 +50,6 @@ struct KvCacheArgs {
 struct KvWriteArgs {
   const void *k, *v;     // [rows][heads][dim], unit stride in dim
   int64_t k_row, k_head, v_row, v_head;
-  int max_q;             // most new tokens of a sequence (sizes the launch)
 };
 hipError_t launch_kv_write(int src, const KvCacheArgs &c, const KvWriteArgs &p, hipStream_t st);
 

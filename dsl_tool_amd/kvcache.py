@@ -128,12 +128,13 @@ def kv8_write(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, seq_lens: torch
     """Quantize the new tokens' keys and values ``[rows, heads, dim]`` (bf16 or
     fp16, views of a fused projection included) into the cache.
 
-    Rows ``q_starts[b] .. q_starts[b+1]`` are the last tokens of sequence b
-    (None: one token each, row b).  The scale of a page and head becomes
+    Rows ``q_starts[b] .. q_starts[b+1]`` (ascending) are the last tokens of
+    sequence b (None: one token each, row b).  The scale of a page and head becomes
     ``max(kept, amax(new)/top, 1e-12)``; ``kept`` is the one it had where older
     tokens stay in the page, and their codes move to a larger scale.  Two
     sequences must not write one page in the same call.  ``max_q_len`` (the most
-    new tokens of a sequence) sizes the launch.
+    new tokens of a sequence) is taken so that one set of arguments serves this
+    call and ``kv8_attention``; the launch is sized by the rows.
     """
     r = N.fast().kv8_write(*cache, k, v, seq_lens, page_table, q_starts, max_q_len)
     if r is not None:
@@ -153,7 +154,7 @@ def kv8_write(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, seq_lens: torch
 def kv8_read(cache: KV8Cache, seq_lens: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor, total: int, *,
              dtype: torch.dtype = torch.bfloat16):
     """The cached tokens back in 16 bits: ``(k, v)``, each ``[total, heads,
-    dim]``; rows ``starts[b] .. starts[b+1]`` are sequence b's tokens from its
+    dim]``; rows ``starts[b] .. starts[b+1]`` (ascending) are sequence b's tokens from its
     first on (rows past its length are zeros)."""
     if dtype not in _SRC:
         raise TypeError(f"kv8_read: dtype must be bfloat16 or float16 (got {dtype})")

@@ -396,8 +396,9 @@ int dsl_add_rmsnorm_quant(const void *x, int64_t rows, int64_t cols, int64_t ldx
  * starts[b] .. starts[b+1]-1 of the token tensors (`rows` in all), at the
  * sequence's end; starts NULL: one new token per sequence, row b.  Page numbers
  * outside [0, pages), tokens past the table's row and rows outside [0, rows)
- * are skipped, wherever the device tables hold them.  max_q sizes the launch
- * (most new tokens of a sequence; a smaller number costs time only). */
+ * are skipped, wherever the device tables hold them.  starts
+ * ascend.  max_q (most new tokens of a sequence) sizes the attention's launch;
+ * a smaller number costs time only. */
 
 /* Writes the new tokens' keys and values (k, v [rows][heads][dim], bf16 or
  * fp16, strides in elements, unit stride in dim).  A page's scale becomes
