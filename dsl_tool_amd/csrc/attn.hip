@@ -6,61 +6,126 @@
 // runs of a key row, whole kilobytes of V^T), converted and fed to the matrix
 // instructions; the next tile's keys are in flight behind the softmax, the
 // tile's values behind its scores.  No LDS and no barrier in the loop.  Four
-// waves of a workgroup take every fourth tile of a split of the context and
-// join in LDS; with too few sequences and heads for the chip the context is
-// split over workgroups, whose partial sums a second kernel joins in split
-// order.
+// waves of a workgroup take every fourth tile of a range of the context and
+// join in LDS.  The ranges: every unit (16 RB query rows of a sequence and
+// cache head) has its context in rounds of `chunk` tiles, all units' rounds
+// stand in one line, and each workgroup takes an equal run of it.  So
+// sequences of any lengths load the CUs alike (64 sequences of 2000 to 8192
+// tokens of 8 heads: 131 us, 5.2 TB/s; 162 with a workgroup per sequence and head, 149 with splits of
+// one length).  A unit that one run holds whole is written at once; the parts
+// of the others a second kernel joins in their order.
 #include "attn_core.h"
 #include "launch.h"
 
 namespace dsl {
 
 constexpr int kTile = 64;      // tokens per step of a wave
-constexpr int SPLIT_WGS = 2;
+constexpr int kRowsWgs = 2;    // workgroups of a CU
 constexpr int kPromptRows = 64;   // query rows of a sequence and cache head from which attn_prompt.hip serves
 
-// RB blocks of 16 query rows share every load.  blockIdx: x split * pairs + pair
-// (sequence and head), y row block.  Workgroups go to the XCDs in turn: with the
-// split running fastest, the late splits, which only long sequences have, all
-// landed on the same ones (64 sequences of 2000 to 8192 tokens: 170 against 12x us).
+// The workspace of a call whose units are split: a run has at most two parts,
+// the end of a unit (slot 2 w) and the beginning of one (2 w + 1).
+template <int D, int ROWS>
+struct Parts {
+  float *v, *ml;                 // [slot][ROWS][D], [slot][ROWS][maximum, sum]
+  int2 *where;                   // [row][query head]: (-1, 0) written, else (first run, last run * 64 + row of the slot)
+  DSL_DEV Parts(float *ws, int runs)
+      : v(ws), ml(ws + (int64_t)2 * runs * ROWS * D), where(reinterpret_cast<int2 *>(ml + (int64_t)4 * runs * ROWS)) {}
+};
+
+// The line of all units' rounds: by sequence, cache head, row block.  A wave
+// looks at 64 sequences at a time.
+struct LineUnit {
+  int b, rounds, blocks;         // sequence; rounds of a unit, row blocks of a head
+  int off;                       // of the position in the sequence's part
+};
+template <int ROWS>
+struct Line {
+  const KvCacheArgs &c;
+  const int group, chunk, lane;
+  int at, rounds, blocks;        // of this lane's sequence
+  int before, upto;              // the line's length before these 64; up to and with this lane's
+  DSL_DEV Line(const KvCacheArgs &c, int group, int chunk)
+      : c(c), group(group), chunk(chunk), lane(threadIdx.x & 63), at(-64), before(0), upto(0) {}
+  DSL_DEV void advance() {
+    if (at >= 0) before += __shfl(upto, 63);
+    at += 64;
+    rounds = blocks = 0;
+    if (at + lane < c.seqs) {
+      const SeqView s = seq_view(c, at + lane);
+      const int room = c.width * c.page, tiles = ((s.len < room ? s.len : room) + kTile - 1) / kTile;
+      rounds = tiles > chunk ? (tiles + chunk - 1) / chunk : 1;      // of no token: one, for its zeros
+      blocks = (int)(((int64_t)s.n * group + ROWS - 1) / ROWS);
+    }
+    upto = rounds * c.heads * blocks;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(upto, o);
+      if (lane >= o) upto += v;
+    }
+  }
+  DSL_DEV int length() {                         // of the whole line; back to its beginning
+    while (at + 64 < c.seqs) advance();
+    const int n = before + __shfl(upto, 63);
+    if (at > 0) {
+      at = -64;
+      before = 0;
+      advance();
+    }
+    return n;
+  }
+  DSL_DEV LineUnit find(int x) {                 // x not before an earlier one
+    while (x >= before + __shfl(upto, 63)) advance();
+    const int k = __builtin_ctzll(__ballot(before + upto > x));
+    LineUnit u;
+    u.b = __builtin_amdgcn_readfirstlane(at + k);
+    u.rounds = __builtin_amdgcn_readfirstlane(__shfl(rounds, k));
+    u.blocks = __builtin_amdgcn_readfirstlane(__shfl(blocks, k));
+    u.off = __builtin_amdgcn_readfirstlane(x - before - __shfl(upto, k)) + u.rounds * c.heads * u.blocks;
+    return u;
+  }
+};
+
+// The NaN codes (E4M3: 0x7f, 0xff) of four, as bytes of ones.
+DSL_DEV uint32_t nan_bytes(uint32_t w) { return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu; }
+constexpr uint32_t kOnes = 0x38383838u;          // 1.0 four times
+
+// RB blocks of 16 query rows share every load.
 template <int SRC, bool FP8, int D, int RB>
-__global__ __launch_bounds__(256) void attn_rows_kernel(const KvCacheArgs c, const AttnArgs p, const int nsplit,
-                                                        const int chunk, const int nblk) {
+__global__ __launch_bounds__(256, D * RB <= 128 ? 2 : 1) void attn_rows_kernel(const KvCacheArgs c, const AttnArgs p, const int chunk, const bool split) {
   constexpr bool F16 = SRC == SRC_F16;
-  constexpr int NW = 4, DT = D / 16, DC = D / 64;
+  constexpr int NW = 4, DT = D / 16, DC = D / 64, ROWS = 16 * RB;
   constexpr int LD = D + 4;                      // floats per row of the joined tile
   __shared__ __align__(16) float so[NW][16 * LD];
   __shared__ float sm[NW][16], sl[NW][16];
-  const int pairs = c.heads * c.seqs, pair = blockIdx.x % pairs;
-  const int b = pair / c.heads, head = pair % c.heads, split = blockIdx.x / pairs;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
-  const SeqView s = seq_view(c, b);
-  const int rows = s.n * p.group;
-  const int room = c.width * c.page;             // tokens that the table has pages for
-  const int ntiles = ((s.len < room ? s.len : room) + kTile - 1) / kTile;
-  const int t0 = split * chunk, t1 = t0 + chunk < ntiles ? t0 + chunk : ntiles;
+  Line<ROWS> line(c, p.group, chunk);
+  const int whole = line.length(), per = (whole + (int)gridDim.x - 1) / (int)gridDim.x;
+  const int end = whole - per > (int)blockIdx.x * per ? ((int)blockIdx.x + 1) * per : whole;
+  const Parts<D, ROWS> part(p.ws, gridDim.x);
   const int ktok = 16 * (r16 >> 2) + (r16 & 3);  // the lane's token of K tile 0 (tile t: + 4 t)
   const int P = c.page;
   const int64_t hstride = (int64_t)P * D;
 
-  if (nsplit > 1 && t0 >= t1) {                  // behind the sequence's end: no sums
-    for (int r = blockIdx.y * 256 + threadIdx.x; r < rows; r += nblk * 256) {
-      const int i = r / p.group, hq = head * p.group + r % p.group;
-      float *ml = p.ws + (int64_t)nsplit * c.rows * p.q_heads * D + (((int64_t)split * c.rows + s.row0 + i) * p.q_heads + hq) * 2;
-      ml[0] = -INFINITY;
-      ml[1] = 0.f;
-    }
-    return;
-  }
-  for (int rb = blockIdx.y; rb * 16 * RB < rows; rb += nblk) {
+  for (int x = (int)blockIdx.x * per; x < end;) {
+    const LineUnit u = line.find(x);
+    const int b = u.b, r0 = u.off % u.rounds, unit = u.off / u.rounds, head = unit / u.blocks, rb = unit % u.blocks;
+    const int left = u.rounds - r0, count = left < end - x ? left : end - x;
+    const bool parted = count < u.rounds;
+    x += count;
+    const SeqView s = seq_view(c, b);
+    const int rows = s.n * p.group;
+    const int room = c.width * c.page;           // tokens that the table has pages for
+    const int seen = s.len < room ? s.len : room, ntiles = (seen + kTile - 1) / kTile;
+    const int t0 = r0 * chunk, t1 = ntiles - t0 > count * chunk ? t0 + count * chunk : ntiles;
     // the rows' queries, as they stand in the products
     v4i qf[RB][2 * DC];
     int limit[RB];
     int lo = s.len;                              // tokens that every row sees
 #pragma unroll
     for (int k = 0; k < RB; ++k) {
-      const int r = rb * 16 * RB + k * 16 + r16, rr = r < rows ? r : rows - 1;
+      const int r = rb * ROWS + k * 16 + r16, rr = r < rows ? r : rows - 1;
       const int i = rr / p.group, hq = head * p.group + rr % p.group;
       const uint16_t *qp = static_cast<const uint16_t *>(p.q) + (int64_t)(s.row0 + i) * p.q_row + (int64_t)hq * p.q_head;
 #pragma unroll
@@ -72,7 +137,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const KvCacheArgs c, con
       limit[k] = p.causal ? (last > 0 ? last : 0) : s.len;
     }
     if (p.causal) {
-      lo = s.first + (rb * 16 * RB) / p.group + 1;
+      lo = s.first + (rb * ROWS) / p.group + 1;
       lo = lo > 0 ? lo : 0;
     }
 
@@ -87,8 +152,10 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const KvCacheArgs c, con
     }
 
     // pages of a tile: the lane's key row, and its 16 tokens (V, scales)
-    auto kpage = [&](int tile) { return page_of(c, b, (tile * kTile + 16 * (r16 >> 2)) / P); };
-    auto vpage = [&](int tile) { return page_of(c, b, (tile * kTile + 16 * g) / P); };
+    // (what the table and the scales hold past the last token's page is not read)
+    auto page = [&](int tok) { return tok < s.len ? page_of(c, b, tok / P) : -1; };
+    auto kpage = [&](int tile) { return page(tile * kTile + 16 * (r16 >> 2)); };
+    auto vpage = [&](int tile) { return page(tile * kTile + 16 * g); };
     uint4 kr[4][DC];
     auto load_k = [&](int tile, int64_t pid) {
       const uint8_t *base = c.k + ((pid < 0 ? 0 : pid) * c.heads + head) * hstride +
@@ -155,6 +222,41 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const KvCacheArgs c, con
           vr[d].w &= keep[3];
         }
       }
+      if (FP8 && masked && p.causal) {
+        // a NaN code among new tokens that only some rows see: it leaves the
+        // products, and the rows that see it get it by the count of such codes
+        bool any = false;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) any |= (nan_bytes(vr[d].x) | nan_bytes(vr[d].y) | nan_bytes(vr[d].z) | nan_bytes(vr[d].w)) != 0;
+        if (__any(any)) {
+          v4i vis[RB][2];
+#pragma unroll
+          for (int k = 0; k < RB; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const int tok = pos + 8 * h + 2 * w;
+                vis[k][h][w] = (tok < limit[k] ? 0x3f80 : 0) | (tok + 1 < limit[k] ? 0x3f800000 : 0);
+              }
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const uint32_t n0 = nan_bytes(vr[d].x), n1 = nan_bytes(vr[d].y), n2 = nan_bytes(vr[d].z), n3 = nan_bytes(vr[d].w);
+            vr[d].x &= ~n0;
+            vr[d].y &= ~n1;
+            vr[d].z &= ~n2;
+            vr[d].w &= ~n3;
+            const v4i a0 = codes8<true, false>(n0 & kOnes, n1 & kOnes), a1 = codes8<true, false>(n2 & kOnes, n3 & kOnes);
+#pragma unroll
+            for (int k = 0; k < RB; ++k) {
+              const v4f nans = mfma16<false>(a1, vis[k][1], mfma16<false>(a0, vis[k][0], (v4f){0.f, 0.f, 0.f, 0.f}));
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (nans[i] != 0.f) o[k][d][i] = __builtin_nanf("");
+            }
+          }
+        }
+      }
       v4i pf[RB][2], pl[RB][2];                  // P, tokens 8h .. 8h+7 of the lane's 16 (pl: fp16's low parts)
 #pragma unroll
       for (int k = 0; k < RB; ++k) {
@@ -181,6 +283,13 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const KvCacheArgs c, con
             sum += e;
             sc[k][t][i] = e * vs;
           }
+        if (masked) {                            // whatever a hidden token's scale is
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!(pos + 4 * t + i < limit[k])) sc[k][t][i] = 0.f;
+        }
         l[k] = l[k] * alpha + sum;
         if (__any(alpha != 1.f)) {
 #pragma unroll
@@ -233,7 +342,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const KvCacheArgs c, con
       // 16 rows x D: thread -> row, 4 columns at a time
       for (int x = threadIdx.x; x < 16 * (D / 4); x += 256) {
         const int row = x / (D / 4), col = (x % (D / 4)) * 4;
-        const int r = rb * 16 * RB + k * 16 + row;
+        const int r = rb * ROWS + k * 16 + row;
         if (r >= rows) continue;
         float mr = sm[0][row];
 #pragma unroll
@@ -246,13 +355,15 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const KvCacheArgs c, con
           v += *reinterpret_cast<const v4f *>(&so[w][row * LD + col]);
         }
         const int i = r / p.group, hq = head * p.group + r % p.group;
-        if (nsplit > 1) {
-          const int64_t at = ((int64_t)split * c.rows + s.row0 + i) * p.q_heads + hq;
-          *reinterpret_cast<v4f *>(p.ws + at * D + col) = v;
+        if (split && r0 == 0 && col == 0)
+          part.where[(int64_t)(s.row0 + i) * p.q_heads + hq] =
+              make_int2(parted ? (int)blockIdx.x : -1, parted ? ((int)blockIdx.x + (left - count + per - 1) / per) * 64 + k * 16 + row : 0);
+        if (parted) {
+          const int64_t at = ((int64_t)2 * blockIdx.x + (r0 == 0)) * ROWS + k * 16 + row;
+          *reinterpret_cast<v4f *>(part.v + at * D + col) = v;
           if (col == 0) {
-            float *ml = p.ws + (int64_t)nsplit * c.rows * p.q_heads * D + at * 2;
-            ml[0] = mr;
-            ml[1] = lr;
+            part.ml[2 * at] = mr;
+            part.ml[2 * at + 1] = lr;
           }
         } else {
           const float inv = lr > 0.f ? 1.0f / lr : 0.f;    // a row that sees nothing is 0
@@ -264,33 +375,51 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const KvCacheArgs c, con
   }
 }
 
-// Joins the splits of one query row and head in a workgroup: a split per thread for
-// the maximum and the sum, then four columns per thread, the splits dealt to 1024 / D
-// threads of each.  (All splits in one thread's loop, a load's latency each, took 14
-// to 27 us.)  An empty split has no sums.
-constexpr int kMaxSplits = 256;
-template <int SRC, int D>
-__global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const int64_t rows, const int nsplit) {
+// Joins the parts of one query row and head in a workgroup: a part per thread for
+// the maximum and the sum, then four columns per thread, the parts dealt to 1024 / D
+// threads of each.  (All parts in one thread's loop, a load's latency each, took 14
+// to 27 us.)  ROWS: the parts of attn_rows_kernel; 0: one per split of a prompt,
+// [split][row][head].  A part that saw no token has no sums.
+constexpr int kMaxParts = 1024;
+template <int SRC, int D, int ROWS>
+__global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const int64_t rows, const int runs) {
   constexpr int CG = D / 4, SL = 256 / CG;
-  __shared__ float s_f[kMaxSplits], s_red[8];
+  __shared__ float s_f[kMaxParts], s_red[8];
   __shared__ v4f s_v[SL][CG];
   const int64_t at = blockIdx.x, n = rows * p.q_heads;
   const int tid = threadIdx.x;
-  const float *ml = p.ws + (int64_t)nsplit * n * D;
-  float m = -INFINITY, l = 0.f;
-  if (tid < nsplit) {
-    m = ml[(tid * n + at) * 2];
-    l = ml[(tid * n + at) * 2 + 1];
+  int parts = runs, first = 0, row = 0;
+  const float *ml = p.ws + (int64_t)runs * n * D;
+  if constexpr (ROWS > 0) {
+    const Parts<D, ROWS> part(p.ws, runs);
+    const int2 w = part.where[at];
+    if (w.x < 0 || w.x >= runs) return;          // written already (or a row of no sequence)
+    ml = part.ml;
+    first = w.x;
+    row = w.y & (ROWS - 1);
+    parts = (w.y >> 6) - first + 1;
+    parts = parts < runs - first ? parts : runs - first;
   }
-  float top = m;
+  auto index = [&](int s) -> int64_t {
+    if constexpr (ROWS > 0) return (int64_t)(s == 0 ? 2 * first + 1 : 2 * (first + s)) * ROWS + row;
+    else return s * n + at;
+  };
+  float top = -INFINITY, l = 0.f;
+  for (int s = tid; s < parts; s += 256) {
+    const float m = ml[index(s) * 2];
+    s_f[s] = m;
+    top = fmaxf(top, m);
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   if ((tid & 63) == 0) s_red[tid >> 6] = top;
   __syncthreads();
   top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-  const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-  s_f[tid] = f;
-  l *= f;
+  for (int s = tid; s < parts; s += 256) {
+    const float m = s_f[s], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    s_f[s] = f;
+    l += f != 0.f ? ml[index(s) * 2 + 1] * f : 0.f;
+  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
   if ((tid & 63) == 0) s_red[4 + (tid >> 6)] = l;
@@ -298,9 +427,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const 
   const int cg = tid % CG, sl = tid / CG;
   v4f v = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = sl; s < nsplit; s += SL) {
+  for (int s = sl; s < parts; s += SL) {
     const float fs = s_f[s];
-    if (fs != 0.f) v += *reinterpret_cast<const v4f *>(p.ws + (s * n + at) * D + cg * 4) * fs;
+    if (fs != 0.f) v += *reinterpret_cast<const v4f *>(p.ws + index(s) * D + cg * 4) * fs;
   }
   s_v[sl][cg] = v;
   __syncthreads();
@@ -315,18 +444,18 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const 
 
 struct AttnPlan {
   bool prompt;
-  int rb, nblk, nsplit, chunk;   // chunk: tiles of a split (few rows)
+  int rb, nblk, nsplit;          // prompts: row blocks, splits
+  int runs, chunk;               // few rows: workgroups, tiles of a round
+  bool split;                    // they are runs of the line, and parts are joined
 };
 static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
-  AttnPlan a;
+  AttnPlan a{};
   const int64_t rows = (int64_t)max_q * (q_heads / c.heads);
   a.prompt = rows > kPromptRows;
-  a.chunk = 0;
   if (a.prompt) {
     const int per = attn_prompt_rows(c.dim);
     const int64_t pairs = (int64_t)c.heads * c.seqs, blocks = (rows + per - 1) / per;
     const int64_t room = ((int64_t)1 << 30) / pairs;
-    a.rb = 0;
     a.nblk = (int)(blocks < room ? blocks : room);
     // one workgroup per CU; a split has four tiles at least
     const int64_t tiles = ((int64_t)c.width * c.page + kTile - 1) / kTile;
@@ -338,57 +467,58 @@ static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
   }
   // (dim 256: two blocks of rows spill)
   a.rb = rows <= 16 || c.dim > 128 ? 1 : 2;
-  const int64_t blocks = (rows + 16 * a.rb - 1) / (16 * a.rb), room = 65535;
-  a.nblk = (int)(blocks < 1 ? 1 : (blocks < room ? blocks : room));   // each walks every nblk-th
-  // Splits of equal length, so that sequences of any lengths load the CUs evenly
-  // (those behind a sequence's end leave at once); at least one tile for every wave.
-  const int64_t units = (int64_t)c.heads * c.seqs * a.nblk, want = SPLIT_WGS * (int64_t)device_cu_count();
-  const int64_t tiles = ((int64_t)c.width * c.page + kTile - 1) / kTile, most = (tiles + 3) / 4;
-  int64_t ns = units > 0 ? want / units : 1;
-  if (ns > most) ns = most;
-  if (ns > kMaxSplits) ns = kMaxSplits;
-  if (ns < 1) ns = 1;
-  a.chunk = (int)((tiles + ns - 1) / ns);
-  a.chunk = (a.chunk + 3) / 4 * 4;               // whole rounds of the four waves
-  a.nsplit = (int)((tiles + a.chunk - 1) / (a.chunk > 0 ? a.chunk : 1));
-  if (a.nsplit < 1) a.nsplit = 1;
+  const int64_t group = q_heads / c.heads, most = c.rows < c.seqs ? c.rows : c.seqs;
+  const int64_t units = c.heads * ((int64_t)c.rows * group / (16 * a.rb) + most);        // at most
+  const int64_t likely = c.heads * most * ((rows + 16 * a.rb - 1) / (16 * a.rb));
+  const int64_t tiles = ((int64_t)c.width * c.page + kTile - 1) / kTile;
+  // rounds of a tile per wave, longer ones where the line's length would pass an int
+  a.chunk = 4;
+  while ((tiles + a.chunk - 1) / a.chunk * units > 1 << 30 && a.chunk < tiles) a.chunk *= 2;
+  a.runs = kRowsWgs * device_cu_count();
+  if (a.runs > kMaxParts) a.runs = kMaxParts;
+  // With many units for every run, or contexts of one round, a workgroup per unit.
+  a.split = tiles > a.chunk && likely < 8 * (int64_t)a.runs;
+  if (!a.split) {
+    a.chunk = tiles > 1 ? (int)tiles : 1;
+    a.runs = (int)units;
+  }
   return a;
 }
 
 size_t attn_workspace_bytes(const KvCacheArgs &c, int q_heads, int max_q) {
   const AttnPlan a = attn_plan(c, q_heads, max_q);
-  return a.nsplit > 1 ? (size_t)a.nsplit * c.rows * q_heads * (c.dim + 2) * sizeof(float) : 0;
+  const size_t n = (size_t)c.rows * q_heads, row = (c.dim + 2) * sizeof(float);
+  if (a.prompt) return a.nsplit > 1 ? a.nsplit * n * row : 0;
+  return a.split ? (size_t)2 * a.runs * 16 * a.rb * row + n * sizeof(int2) : 0;
 }
 
-template <int SRC, bool FP8, int D>
+template <int SRC, int D, int RB>
 static void launch_rows(const KvCacheArgs &c, const AttnArgs &p, const AttnPlan &a, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.nsplit * c.heads * c.seqs), (unsigned)a.nblk);
-  if (a.rb == 1) attn_rows_kernel<SRC, FP8, D, 1><<<grid, 256, 0, st>>>(c, p, a.nsplit, a.chunk, a.nblk);
-  else if constexpr (D <= 128) attn_rows_kernel<SRC, FP8, D, 2><<<grid, 256, 0, st>>>(c, p, a.nsplit, a.chunk, a.nblk);
+  if (c.fp8) attn_rows_kernel<SRC, true, D, RB><<<a.runs, 256, 0, st>>>(c, p, a.chunk, a.split);
+  else attn_rows_kernel<SRC, false, D, RB><<<a.runs, 256, 0, st>>>(c, p, a.chunk, a.split);
+  if (a.split) attn_join_kernel<SRC, D, 16 * RB><<<(unsigned)c.rows * (unsigned)p.q_heads, 256, 0, st>>>(p, c.rows, a.runs);
 }
 
-template <int SRC>
-static hipError_t launch_src(const KvCacheArgs &c, const AttnArgs &p, hipStream_t st) {
+template <int SRC, int D>
+static hipError_t launch_dim(const KvCacheArgs &c, const AttnArgs &p, hipStream_t st) {
   const AttnPlan a = attn_plan(c, p.q_heads, p.max_q);
   if (a.prompt) {
     const hipError_t e = launch_attn_prompt(SRC, c, p, a.nblk, a.nsplit, st);
     if (e != hipSuccess) return e;
-  } else if (c.fp8) {
-    if (c.dim == 64) launch_rows<SRC, true, 64>(c, p, a, st);
-    else if (c.dim == 128) launch_rows<SRC, true, 128>(c, p, a, st);
-    else launch_rows<SRC, true, 256>(c, p, a, st);
-  } else {
-    if (c.dim == 64) launch_rows<SRC, false, 64>(c, p, a, st);
-    else if (c.dim == 128) launch_rows<SRC, false, 128>(c, p, a, st);
-    else launch_rows<SRC, false, 256>(c, p, a, st);
-  }
-  if (a.nsplit > 1) {
-    const unsigned n = (unsigned)c.rows * (unsigned)p.q_heads;
-    if (c.dim == 64) attn_join_kernel<SRC, 64><<<n, 256, 0, st>>>(p, c.rows, a.nsplit);
-    else if (c.dim == 128) attn_join_kernel<SRC, 128><<<n, 256, 0, st>>>(p, c.rows, a.nsplit);
-    else attn_join_kernel<SRC, 256><<<n, 256, 0, st>>>(p, c.rows, a.nsplit);
+    if (a.nsplit > 1) attn_join_kernel<SRC, D, 0><<<(unsigned)c.rows * (unsigned)p.q_heads, 256, 0, st>>>(p, c.rows, a.nsplit);
+  } else if (a.rb == 1) {
+    launch_rows<SRC, D, 1>(c, p, a, st);
+  } else if constexpr (D <= 128) {
+    launch_rows<SRC, D, 2>(c, p, a, st);
   }
   return hipGetLastError();
+}
+
+template <int SRC>
+static hipError_t launch_src(const KvCacheArgs &c, const AttnArgs &p, hipStream_t st) {
+  if (c.dim == 64) return launch_dim<SRC, 64>(c, p, st);
+  if (c.dim == 128) return launch_dim<SRC, 128>(c, p, st);
+  return launch_dim<SRC, 256>(c, p, st);
 }
 
 hipError_t launch_attn(int src, const KvCacheArgs &c, const AttnArgs &p, hipStream_t st) {

@@ -40,7 +40,9 @@ int check_cache(const char *fn, dsl::KvCacheArgs *c, const void *k, const void *
     return fail(DSL_ERR_UNSUPPORTED, "%s: page size %lld must be 16, 32, 64, 128 or 256", fn, (long long)page);
   if (heads > 16384 || seqs > 65535)
     return fail(DSL_ERR_UNSUPPORTED, "%s: at most 16384 heads and 65535 sequences in a call", fn);
-  if (width * page >= (int64_t)1 << 31) return fail(DSL_ERR_ARG, "%s: page table rows span 2^31 tokens or more", fn);
+  // tokens are counted in ints, whole tiles beyond a sequence's last one included
+  if (width > (((int64_t)1 << 31) - 65536) / page)
+    return fail(DSL_ERR_ARG, "%s: page table rows span more than 2^31 - 65536 tokens", fn);
   if (fmt != DSL_KV_INT8 && fmt != DSL_KV_FP8) return fail(DSL_ERR_ARG, "%s: unknown fmt %d", fn, fmt);
   if (x_dtype != DSL_IN_BF16 && x_dtype != DSL_IN_F16)
     return fail(DSL_ERR_ARG, "%s: x_dtype %d must be bf16 or fp16", fn, x_dtype);
@@ -242,8 +244,7 @@ int dsl_kv8_attention(const void *q, int64_t q_row, int64_t q_head, int64_t q_he
   if (max_q < 0) return fail(DSL_ERR_ARG, "%s: max_q must be >= 0", fn);
   if (!(scale - scale == 0.f)) return fail(DSL_ERR_ARG, "%s: scale must be finite", fn);
   if (rows == 0 || seqs == 0) return ok();
-  if (rows * (q_heads / heads) >= (int64_t)1 << 31)
-    return fail(DSL_ERR_ARG, "%s: rows x query heads per cache head must be < 2^31", fn);
+  if (rows > ((int64_t)1 << 30) / q_heads) return fail(DSL_ERR_ARG, "%s: rows x query heads must be at most 2^30", fn);
   if ((rc = check_heads(fn, "q", q, q_row, q_head, q_heads, dim)) ||
       (rc = check_heads(fn, "out", out, o_row, o_head, q_heads, dim)))
     return rc;
