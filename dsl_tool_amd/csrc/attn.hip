@@ -33,6 +33,17 @@ struct Parts {
       : v(ws), ml(ws + (int64_t)2 * runs * ROWS * D), where(reinterpret_cast<int2 *>(ml + (int64_t)4 * runs * ROWS)) {}
 };
 
+// The sum of a wave's values up to and with each lane's.
+DSL_DEV int lanes_sum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
 // The line of all units' rounds: by sequence, cache head, row block.  A wave
 // looks at 64 sequences at a time.
 struct LineUnit {
@@ -44,11 +55,11 @@ struct Line {
   const KvCacheArgs &c;
   const int group, chunk, lane;
   int at, rounds, blocks;        // of this lane's sequence
-  int before, upto;              // the line's length before these 64; up to and with this lane's
+  int before, total, upto;       // the line's length before these 64; theirs; theirs up to and with this lane's
   DSL_DEV Line(const KvCacheArgs &c, int group, int chunk)
-      : c(c), group(group), chunk(chunk), lane(threadIdx.x & 63), at(-64), before(0), upto(0) {}
+      : c(c), group(group), chunk(chunk), lane(threadIdx.x & 63), at(-64), before(0), total(0), upto(0) {}
   DSL_DEV void advance() {
-    if (at >= 0) before += __shfl(upto, 63);
+    before += total;
     at += 64;
     rounds = blocks = 0;
     if (at + lane < c.seqs) {
@@ -57,31 +68,27 @@ struct Line {
       rounds = tiles > chunk ? (tiles + chunk - 1) / chunk : 1;      // of no token: one, for its zeros
       blocks = (int)(((int64_t)s.n * group + ROWS - 1) / ROWS);
     }
-    upto = rounds * c.heads * blocks;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(upto, o);
-      if (lane >= o) upto += v;
-    }
+    upto = lanes_sum(rounds * c.heads * blocks);
+    total = __builtin_amdgcn_readlane(upto, 63);
   }
   DSL_DEV int length() {                         // of the whole line; back to its beginning
     while (at + 64 < c.seqs) advance();
-    const int n = before + __shfl(upto, 63);
+    const int n = before + total;
     if (at > 0) {
       at = -64;
-      before = 0;
+      before = total = 0;
       advance();
     }
     return n;
   }
   DSL_DEV LineUnit find(int x) {                 // x not before an earlier one
-    while (x >= before + __shfl(upto, 63)) advance();
+    while (x >= before + total) advance();
     const int k = __builtin_ctzll(__ballot(before + upto > x));
     LineUnit u;
-    u.b = __builtin_amdgcn_readfirstlane(at + k);
-    u.rounds = __builtin_amdgcn_readfirstlane(__shfl(rounds, k));
-    u.blocks = __builtin_amdgcn_readfirstlane(__shfl(blocks, k));
-    u.off = __builtin_amdgcn_readfirstlane(x - before - __shfl(upto, k)) + u.rounds * c.heads * u.blocks;
+    u.b = at + k;
+    u.rounds = __builtin_amdgcn_readlane(rounds, k);
+    u.blocks = __builtin_amdgcn_readlane(blocks, k);
+    u.off = x - before - __builtin_amdgcn_readlane(upto, k) + u.rounds * c.heads * u.blocks;
     return u;
   }
 };
