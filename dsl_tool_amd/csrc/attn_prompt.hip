@@ -433,7 +433,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
           for (int d = half * Cfg::DH + h; d < (half + 1) * Cfg::DH; d += 2)
 #pragma unroll 1
             for (int x = 0; x < T / VT; ++x) {
-              const int k = n - x * VT;
+              const int k = n - x * VT < VT ? n - x * VT : VT;   // (bits past VT are not written)
               const uint64_t seen = k >= 64 ? ~0ull : (k > 0 ? (1ull << k) - 1 : 0);
               if (s_nan[tile & 1][x][d] & seen) atomicOr(&s_row[wrow + r32][d >> 5], 1u << (d & 31));
             }
@@ -447,12 +447,17 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
           const float vs = s_vs[tile & 3][g];
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            auto scaled = [&](int x) {
-              const float lo = u2f((uint32_t)x << 16), hi = u2f((uint32_t)x & 0xffff0000u);
-              return (int)pack_bf16x2(lo == 0.f ? 0.f : lo * vs, hi == 0.f ? 0.f : hi * vs);
-            };
-            pf[g][w] = scaled(pf[g][w]);
-            if constexpr (F16) pl[g][w] = scaled(pl[g][w]);
+            // (two roundings to bf16 in such a tile; fp16's two parts are joined first)
+            float a = u2f((uint32_t)pf[g][w] << 16), z = u2f((uint32_t)pf[g][w] & 0xffff0000u);
+            if constexpr (F16) {
+              a += u2f((uint32_t)pl[g][w] << 16);
+              z += u2f((uint32_t)pl[g][w] & 0xffff0000u);
+            }
+            a = a == 0.f ? 0.f : a * vs;
+            z = z == 0.f ? 0.f : z * vs;
+            const uint32_t hi = pack_bf16x2(a, z);
+            pf[g][w] = (int)hi;
+            if constexpr (F16) pl[g][w] = (int)pack_bf16x2(a - u2f(hi << 16), z - u2f(hi & 0xffff0000u));
           }
         }
       }
