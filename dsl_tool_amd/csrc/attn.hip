@@ -17,11 +17,19 @@
 #include "attn_core.h"
 #include "launch.h"
 
+#include <cstdlib>
+
 namespace dsl {
 
 constexpr int kTile = 64;      // tokens per step of a wave
-constexpr int kRowsWgs = 2;    // workgroups of a CU
-constexpr int kPromptRows = 64;   // query rows of a sequence and cache head from which attn_prompt.hip serves
+constexpr int kRowsWgs = 2;    // workgroups of a CU: what its registers hold
+// Up to kFewRows query rows of a sequence and cache head, or where the line gives a
+// run kFewRounds rounds at most, the kernel of few rows serves, else
+// attn_prompt.hip's: 32 query heads on 8 of dim 128, 16 sequences of up to 4000
+// tokens, rows 64 / 96 / 128: 67 / 90 / 108 against 81 / 85 / 91 us; one of 8000:
+// 29 / 34 / 35 against 32 / 35 / 37, and rows 256, 4 rounds: 48 against 40; one of
+// 1000, rows 256: 18 against 30.
+constexpr int kFewRows = 96, kFewRounds = 2;
 
 // The workspace of a call whose units are split: a run has at most two parts,
 // the end of a unit (slot 2 w) and the beginning of one (2 w + 1).
@@ -458,31 +466,32 @@ struct AttnPlan {
 static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
   AttnPlan a{};
   const int64_t rows = (int64_t)max_q * (q_heads / c.heads);
-  a.prompt = rows > kPromptRows;
+  // (dim 256: two blocks of rows spill)
+  a.rb = rows <= 16 || c.dim > 128 ? 1 : 2;
+  const int64_t group = q_heads / c.heads, most = c.rows < c.seqs ? c.rows : c.seqs;
+  const int64_t likely = c.heads * most * ((rows + 16 * a.rb - 1) / (16 * a.rb));        // units
+  const int64_t tiles = ((int64_t)c.width * c.page + kTile - 1) / kTile;
+  a.runs = kRowsWgs * device_cu_count();
+  if (a.runs > kMaxParts) a.runs = kMaxParts;
+  const char *few = getenv("DSL_ATTN_FEW_ROWS");       // read per launch (tests switch it)
+  if (few) a.prompt = rows > atoi(few);
+  else a.prompt = rows > kFewRows && (double)likely * (double)((tiles + 3) / 4) > (double)(kFewRounds * a.runs);
   if (a.prompt) {
     const int per = attn_prompt_rows(c.dim);
     const int64_t pairs = (int64_t)c.heads * c.seqs, blocks = (rows + per - 1) / per;
     const int64_t room = ((int64_t)1 << 30) / pairs;
     a.nblk = (int)(blocks < room ? blocks : room);
     // one workgroup per CU; a split has four tiles at least
-    const int64_t tiles = ((int64_t)c.width * c.page + kTile - 1) / kTile;
     int64_t ns = device_cu_count() / (pairs * a.nblk);
     if (ns > tiles / 4) ns = tiles / 4;
     if (ns > 64) ns = 64;
     a.nsplit = ns < 1 ? 1 : (int)ns;
     return a;
   }
-  // (dim 256: two blocks of rows spill)
-  a.rb = rows <= 16 || c.dim > 128 ? 1 : 2;
-  const int64_t group = q_heads / c.heads, most = c.rows < c.seqs ? c.rows : c.seqs;
   const int64_t units = c.heads * ((int64_t)c.rows * group / (16 * a.rb) + most);        // at most
-  const int64_t likely = c.heads * most * ((rows + 16 * a.rb - 1) / (16 * a.rb));
-  const int64_t tiles = ((int64_t)c.width * c.page + kTile - 1) / kTile;
   // rounds of a tile per wave, longer ones where the line's length would pass an int
   a.chunk = 4;
   while ((tiles + a.chunk - 1) / a.chunk * units > 1 << 30 && a.chunk < tiles) a.chunk *= 2;
-  a.runs = kRowsWgs * device_cu_count();
-  if (a.runs > kMaxParts) a.runs = kMaxParts;
   // With many units for every run, or contexts of one round, a workgroup per unit.
   a.split = tiles > a.chunk && likely < 8 * (int64_t)a.runs;
   if (!a.split) {

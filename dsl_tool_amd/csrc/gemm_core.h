@@ -18,7 +18,9 @@
 //   MXFP4       E8M0 bytes go straight into v_mfma_scale_f32_16x16x128_f8f6f4;
 //   NVFP4       E2M1 -> fp16 (hardware convert), times the E4M3 block scale
 //               in fp16 (exact), fp16 MFMA; global scales in the epilogue;
-//   BF16        unscaled bf16 MFMA (a stage is 64 elements of K).
+//   BF16        unscaled bf16 MFMA (a stage is 64 elements of K);
+//   INT8        int8 MFMA into int32 sums over all K, exact; (acc * sa[m]) * sb[n]
+//               in the epilogue.
 #pragma once
 
 #include "common.h"

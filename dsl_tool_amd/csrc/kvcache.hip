@@ -107,8 +107,8 @@ DSL_DEV uint32_t codes_moved(uint32_t w, float kept, const Divisor &v) {
 // the fetch of the code itself, so what every call runs is short: one set of
 // quotients for keys and values, whose codes are turned by byte permutes (64
 // sequences' tokens, 8 heads of 128: 5.6 us; 18 with a copy of the quotients per
-// use).  A long call is bound by the bytes: 8000 tokens of the same heads, 49 MB,
-// in 9.3 us, where a workgroup per value and key tile that read its tokens twice
+// use).  A long call is bound by the bytes: prompts of 8 heads, 34 MB, in
+// 9.3 us, where a workgroup per value and key tile that read its tokens twice
 // and stored values by words took 14.3.
 template <int SRC, bool FP8, int NT, int UN, bool HELD>
 __global__ __launch_bounds__(NT) void kv_write_kernel(const KvCacheArgs c, const KvWriteArgs p) {
@@ -280,8 +280,8 @@ hipError_t launch_kv_write(int src, const KvCacheArgs &c, const KvWriteArgs &p, 
 // Rows [starts[b], starts[b+1]) of the result are the sequence's tokens from
 // its first on; rows past its length, or of pages that are none, are zeros.
 // Grid: x items (64 tokens of a sequence, of one page or several), y head.
-// Bound by the bytes: 8 sequences of 8192 tokens, 8 heads of 128, pages of 16,
-// 403 MB in 58 us; 92 with a workgroup per page and of keys or values, whose
+// Bound by the bytes: 8 sequences of up to 8192 tokens, pages of 16, 275 MB in
+// 58 us; 92 with a workgroup per page and of keys or values, whose
 // threads read a word of each value row.
 template <int SRC, bool FP8, int D>
 __global__ __launch_bounds__(256) void kv_read_kernel(const KvCacheArgs c, const KvReadArgs p) {

@@ -13,9 +13,19 @@ from dsl_tool_amd import kvcache as KV
 from dsl_tool_amd import layer8 as L
 from dsl_tool_amd import quant as Q
 from oracle import serving as O
-from tests.test_gpu_serving import (DEV, check_attention, random_cache, randn, same_cache, spoil, table_of, to, within)
+from tests.test_gpu_serving import (ATTN, DEV, check_attention, random_cache, randn, same_cache, spoil, table_of, to,
+                                    within)
+from tests import test_gpu_serving as S
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["auto", "prompt"])
+def route(request, monkeypatch):
+    """Attention as the sizes have it, and all of it by the kernel of prompts."""
+    if request.param == "prompt":
+        monkeypatch.setenv("DSL_ATTN_FEW_ROWS", "0")
+    return request.param
 
 
 def ints(x):
@@ -91,10 +101,33 @@ def test_write_scales_of_every_kind(fmt):
 
 # --------------------------------------------------------------- attention --
 
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page,dim,heads,group", ATTN)
+@pytest.mark.parametrize("causal", [True, False])
+def test_every_size_by_the_prompts_kernel(page, dim, heads, group, src, fmt, causal, monkeypatch):
+    monkeypatch.setenv("DSL_ATTN_FEW_ROWS", "0")
+    S.test_attention_prompts(page, dim, heads, group, src, fmt, causal)
+    if causal:
+        S.test_attention_single_tokens(page, dim, heads, group, src, fmt)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,group", [(64, 8), (128, 4), (256, 1)])
+def test_prompts_of_many_blocks(dim, group, src, fmt):
+    """Enough rows that the sizes themselves choose the kernel of prompts."""
+    lens, new = [2100, 1300], [1100, 1300]
+    table, pages = table_of(lens, 64, 770)
+    cache = random_cache(pages, 4, dim, 64, fmt, 771)
+    spoil(cache, lens, table)
+    check_attention(randn((2400, 4 * group, dim), 772, src), cache, lens, table, [0, 1100, 2400], max_q_len=1300)
+
+
 @pytest.mark.parametrize("group,new", [(1, 6), (4, 5), (8, 40), (1, 300)])
 @pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("dim", [64, 128, 256])
-def test_hidden_nan_codes(dim, src, group, new):
+def test_hidden_nan_codes(dim, src, group, new, route):
     """An E4M3 NaN in a new token: the rows before it are as without it, the
     rows from it on are NaN (in its column, for a value; wholly, for a key)."""
     length = 70 + new
@@ -128,7 +161,7 @@ def test_hidden_nan_codes(dim, src, group, new):
 
 @pytest.mark.parametrize("fmt", ["int8", "fp8"])
 @pytest.mark.parametrize("new", [1, 7, 100])
-def test_nothing_past_the_end_is_seen(new, fmt):
+def test_nothing_past_the_end_is_seen(new, fmt, route):
     """Table entries behind the last token's page name pages whose scales are
     NaN; so does the last page of another sequence's row."""
     lens = [65 + new, 128 + new]
@@ -147,7 +180,7 @@ def test_nothing_past_the_end_is_seen(new, fmt):
 @pytest.mark.parametrize("fmt", ["int8", "fp8"])
 @pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("page,dim,group", [(16, 64, 4), (64, 128, 4), (32, 128, 1), (128, 256, 2), (256, 64, 16)])
-def test_long_prompts(page, dim, group, src, fmt):
+def test_long_prompts(page, dim, group, src, fmt, route):
     """Prompts over many tiles, whose context is split and joined; a page of none
     in the middle."""
     lens, new = [1500, 333, 64, 0], [150, 333, 1, 2]
@@ -163,7 +196,7 @@ def test_long_prompts(page, dim, group, src, fmt):
 
 @pytest.mark.parametrize("fmt", ["int8", "fp8"])
 @pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
-def test_prompt_scales_of_every_kind(src, fmt):
+def test_prompt_scales_of_every_kind(src, fmt, route):
     """Page scales of zero, negative ones, and ones decades apart, in prompts and
     for few rows."""
     lens = [700]
