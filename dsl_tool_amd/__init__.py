@@ -4,6 +4,8 @@
   (the callables registered as ``gemm.*`` under backend ``hip``) and their
   packed-operand forms;
 * ``dsl_tool_amd.quant``      -- GPU quantize/pack (E4M3, MXFP4, NVFP4);
+* ``dsl_tool_amd.kvcache``, ``attention``, ``layer8`` -- a paged 8-bit key-value cache,
+  attention over it, and a layer of both with the residual norm and int8 products;
 * ``dsl_tool_amd.dispatcher`` -- registry / KernelDispatcher / REST / CLI;
 * ``dsl_tool_amd.build``      -- hipcc build of ``_lib/libdsl_gemm.so``.
 """
