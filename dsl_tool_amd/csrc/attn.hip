@@ -11,8 +11,8 @@
 // cache head) has its context in rounds of `chunk` tiles, all units' rounds
 // stand in one line, and each workgroup takes an equal run of it.  So
 // sequences of any lengths load the CUs alike (64 sequences of 2000 to 8192
-// tokens of 8 heads: 131 us, 5.2 TB/s; 162 with a workgroup per sequence and head, 149 with splits of
-// one length).  A unit that one run holds whole is written at once; the parts
+// tokens, 645 MB: 130 us, 5.0 TB/s; 162 with a workgroup per sequence and head,
+// 149 with splits of one length).  A unit that one run holds whole is written at once; the parts
 // of the others a second kernel joins in their order.
 #include "attn_core.h"
 #include "launch.h"
@@ -30,6 +30,14 @@ constexpr int kRowsWgs = 2;    // workgroups of a CU: what its registers hold
 // 29 / 34 / 35 against 32 / 35 / 37, and rows 256, 4 rounds: 48 against 40; one of
 // 1000, rows 256: 18 against 30.
 constexpr int kFewRows = 96, kFewRounds = 2;
+// Whether units are split into runs (and joined, about 5 us), by the rounds R that
+// the table has room for and the units U per run; else a workgroup takes a unit
+// whole.  32 query heads on 8 of dim 128, ragged contexts up to 256 R, split against
+// whole, us: U 1/8, R 2 / 4 / 8: 11.2 / 11.6 / 14.6 against 9.2 / 15 / 25; U 1/2, R 4
+// / 6 / 8: 22 / 26 / 27 against 17 / 22 / 27; U 1, R 4: 28 against 24, R 32: 134
+// against 169; U 2, R 8: 84 against 89; U 4, R 4 / 16: 98 / 271 against 95 / 315; U 8,
+// R 8: 290 against 283.  Past kLineSeqs sequences the line takes long to walk.
+constexpr int kFewUnits = 8, kLongRounds = 8, kLineSeqs = 512;
 
 // The workspace of a call whose units are split: a run has at most two parts,
 // the end of a unit (slot 2 w) and the beginning of one (2 w + 1).
@@ -115,25 +123,52 @@ __global__ __launch_bounds__(256, D * RB <= 128 ? 2 : 1) void attn_rows_kernel(c
   __shared__ float sm[NW][16], sl[NW][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
-  Line<ROWS> line(c, p.group, chunk);
-  const int whole = line.length(), per = (whole + (int)gridDim.x - 1) / (int)gridDim.x;
-  const int end = whole - per > (int)blockIdx.x * per ? ((int)blockIdx.x + 1) * per : whole;
   const Parts<D, ROWS> part(p.ws, gridDim.x);
+  Line<ROWS> line(c, p.group, chunk);
+  int per = 1, end = 1, x = 0;
+  if (split) {
+    const int whole = line.length();
+    per = (whole + (int)gridDim.x - 1) / (int)gridDim.x;
+    x = (int)blockIdx.x * per;
+    end = whole - per > x ? x + per : whole;
+  }
   const int ktok = 16 * (r16 >> 2) + (r16 & 3);  // the lane's token of K tile 0 (tile t: + 4 t)
   const int P = c.page;
   const int64_t hstride = (int64_t)P * D;
 
-  for (int x = (int)blockIdx.x * per; x < end;) {
-    const LineUnit u = line.find(x);
-    const int b = u.b, r0 = u.off % u.rounds, unit = u.off / u.rounds, head = unit / u.blocks, rb = unit % u.blocks;
-    const int left = u.rounds - r0, count = left < end - x ? left : end - x;
-    const bool parted = count < u.rounds;
+  while (x < end) {
+    int b, head, rb, r0 = 0, left = 1, count = 1;
+    SeqView s;
+    if (split) {
+      const LineUnit u = line.find(x);
+      const int unit = u.off / u.rounds;
+      b = u.b;
+      r0 = u.off % u.rounds;
+      head = unit / u.blocks;
+      rb = unit % u.blocks;
+      left = u.rounds - r0;
+      count = left < end - x ? left : end - x;
+      s = seq_view(c, b);
+    } else if (c.starts) {                       // x row block, y cache head
+      s = item_seq(c, blockIdx.x, [&](int row, int q) { return row * p.group / ROWS + q; }, b, rb);
+      b = __builtin_amdgcn_readfirstlane(b);
+      rb = __builtin_amdgcn_readfirstlane(rb);
+      head = blockIdx.y;
+      if (b < 0 || rb < 0) return;
+    } else {
+      const int blocks = (p.group + ROWS - 1) / ROWS;
+      b = blockIdx.x / blocks;
+      rb = blockIdx.x % blocks;
+      head = blockIdx.y;
+      s = seq_view(c, b);
+    }
+    const bool parted = left > count || r0 > 0;
     x += count;
-    const SeqView s = seq_view(c, b);
     const int rows = s.n * p.group;
+    if (rb * ROWS >= rows) return;               // (a workgroup for every block there may be)
     const int room = c.width * c.page;           // tokens that the table has pages for
     const int seen = s.len < room ? s.len : room, ntiles = (seen + kTile - 1) / kTile;
-    const int t0 = r0 * chunk, t1 = ntiles - t0 > count * chunk ? t0 + count * chunk : ntiles;
+    const int t0 = r0 * chunk, t1 = split && ntiles - t0 > count * chunk ? t0 + count * chunk : ntiles;
     // the rows' queries, as they stand in the products
     v4i qf[RB][2 * DC];
     int limit[RB];
@@ -488,15 +523,16 @@ static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
     a.nsplit = ns < 1 ? 1 : (int)ns;
     return a;
   }
-  const int64_t units = c.heads * ((int64_t)c.rows * group / (16 * a.rb) + most);        // at most
   // rounds of a tile per wave, longer ones where the line's length would pass an int
+  const int64_t units = c.heads * ((int64_t)c.rows * group / (16 * a.rb) + most);        // at most
   a.chunk = 4;
   while ((tiles + a.chunk - 1) / a.chunk * units > 1 << 30 && a.chunk < tiles) a.chunk *= 2;
-  // With many units for every run, or contexts of one round, a workgroup per unit.
-  a.split = tiles > a.chunk && likely < 8 * (int64_t)a.runs;
+  const int64_t rounds = (tiles + a.chunk - 1) / a.chunk;
+  a.split = likely < kFewUnits * (int64_t)a.runs && c.seqs <= kLineSeqs &&
+            (rounds >= kLongRounds || (rounds - 3) * a.runs >= 8 * likely);
   if (!a.split) {
-    a.chunk = tiles > 1 ? (int)tiles : 1;
-    a.runs = (int)units;
+    const int64_t per = 16 * a.rb;
+    a.runs = (int)(c.starts ? c.rows * group / per + c.seqs : c.seqs * ((group + per - 1) / per));
   }
   return a;
 }
@@ -510,8 +546,9 @@ size_t attn_workspace_bytes(const KvCacheArgs &c, int q_heads, int max_q) {
 
 template <int SRC, int D, int RB>
 static void launch_rows(const KvCacheArgs &c, const AttnArgs &p, const AttnPlan &a, hipStream_t st) {
-  if (c.fp8) attn_rows_kernel<SRC, true, D, RB><<<a.runs, 256, 0, st>>>(c, p, a.chunk, a.split);
-  else attn_rows_kernel<SRC, false, D, RB><<<a.runs, 256, 0, st>>>(c, p, a.chunk, a.split);
+  const dim3 grid((unsigned)a.runs, a.split ? 1u : (unsigned)c.heads);
+  if (c.fp8) attn_rows_kernel<SRC, true, D, RB><<<grid, 256, 0, st>>>(c, p, a.chunk, a.split);
+  else attn_rows_kernel<SRC, false, D, RB><<<grid, 256, 0, st>>>(c, p, a.chunk, a.split);
   if (a.split) attn_join_kernel<SRC, D, 16 * RB><<<(unsigned)c.rows * (unsigned)p.q_heads, 256, 0, st>>>(p, c.rows, a.runs);
 }
 

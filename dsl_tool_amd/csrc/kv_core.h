@@ -91,6 +91,50 @@ DSL_DEV SeqView seq_view(const KvCacheArgs &c, int b) {
   return s;
 }
 
+// The sequence b that item `id` of a flat launch belongs to (-1: none), and the
+// item's number in it.  Sequence b's items begin at first(row, b), row its first
+// row: floor(row / span) + extra * b.  As floor((s + n) / span) >= floor(s / span)
+// + floor(n / span), a sequence of n rows has at least floor(n / span) + extra
+// items of its own, and rows / span + extra * seqs suffice for all: few workgroups
+// of a ragged batch find nothing to do, whatever its longest sequence.  All lanes
+// search, 64 sequences a step, and the last step has the sequence's other numbers
+// with its start.  Without starts an item is a sequence.
+template <class F>
+DSL_DEV SeqView item_seq(const KvCacheArgs &c, int id, const F &first, int &b, int &item) {
+  SeqView s{0, 0, 0, 0};
+  if (!c.starts) {
+    b = id < c.seqs ? id : -1;
+    item = 0;
+    return b < 0 ? s : seq_view(c, b);
+  }
+  const int lane = threadIdx.x & 63;
+  auto row = [&](int i) {
+    const int v = c.starts[i];
+    return v < 0 ? 0 : v > c.rows ? c.rows : v;
+  };
+  int lo = 0, n = c.seqs;
+  while (n > 64) {
+    const int step = (n + 63) >> 6, off = lane * step;
+    const int f = off < n ? first(row(lo + off), lo + off) : 0;
+    const int cnt = __popcll(__ballot(off < n && f <= id)), skip = (cnt > 0 ? cnt - 1 : 0) * step;
+    lo += skip;
+    n = n - skip < step ? n - skip : step;
+  }
+  const int at = lo + (lane < n ? lane : n - 1);
+  const int from = row(at), to = row(at + 1), len = c.lens[at];
+  const int f = first(from, at);
+  const int cnt = __popcll(__ballot(lane < n && f <= id)), pick = cnt > 0 ? cnt - 1 : 0;
+  b = cnt > 0 ? lo + pick : -1;
+  item = id - __shfl(f, pick);
+  s.len = __shfl(len, pick);
+  s.len = s.len > 0 ? s.len : 0;
+  s.row0 = __shfl(from, pick);
+  s.n = __shfl(to, pick) - s.row0;
+  s.n = s.n > 0 ? s.n : 0;
+  s.first = s.len - s.n;
+  return s;
+}
+
 // The page that holds the tokens [page * pg, ..) of sequence b, or -1: pages
 // past the table's row and numbers out of range hold none.
 DSL_DEV int64_t page_of(const KvCacheArgs &c, int b, int pg) {

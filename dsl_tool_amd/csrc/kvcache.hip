@@ -17,48 +17,6 @@
 
 namespace dsl {
 
-// The sequence that item `id` of a flat launch belongs to, -1 if none, and the
-// item's number in it.  Sequence b's items begin at starts[b] / span + extra * b:
-// floor((s + n) / span) >= floor(s / span) + floor(n / span), so a sequence of n
-// rows has at least floor(n / span) + extra of its own, and rows / span +
-// extra * seqs suffice for all: few workgroups of a ragged batch find nothing
-// to do, whatever its longest sequence.  All lanes search, 64 sequences a step,
-// and the last step has the sequence's other numbers with its start.
-DSL_DEV SeqView item_seq(const KvCacheArgs &c, int id, int span_log, int extra, int &b, int &item) {
-  SeqView s{0, 0, 0, 0};
-  if (!c.starts) {                               // a row each
-    b = id < c.seqs ? id : -1;
-    item = 0;
-    return b < 0 ? s : seq_view(c, b);
-  }
-  const int lane = threadIdx.x & 63;
-  auto row = [&](int i) {
-    const int v = c.starts[i];
-    return v < 0 ? 0 : v > c.rows ? c.rows : v;
-  };
-  int lo = 0, n = c.seqs;
-  while (n > 64) {
-    const int step = (n + 63) >> 6, off = lane * step;
-    const int f = off < n ? (row(lo + off) >> span_log) + extra * (lo + off) : 0;
-    const int cnt = __popcll(__ballot(off < n && f <= id)), skip = (cnt > 0 ? cnt - 1 : 0) * step;
-    lo += skip;
-    n = n - skip < step ? n - skip : step;
-  }
-  const int at = lo + (lane < n ? lane : n - 1);
-  const int from = row(at), to = row(at + 1), len = c.lens[at];
-  const int f = (from >> span_log) + extra * at;
-  const int cnt = __popcll(__ballot(lane < n && f <= id)), pick = cnt > 0 ? cnt - 1 : 0;
-  b = cnt > 0 ? lo + pick : -1;
-  item = id - __shfl(f, pick);
-  s.len = __shfl(len, pick);
-  s.len = s.len > 0 ? s.len : 0;
-  s.row0 = __shfl(from, pick);
-  s.n = __shfl(to, pick) - s.row0;
-  s.n = s.n > 0 ? s.n : 0;
-  s.first = s.len - s.n;
-  return s;
-}
-
 // Word of a value tile in shared memory: row d, 4 tokens from 4 * t4.  Rows of
 // `words` words, four more after each eighth row, so that the 64 lanes of a
 // wave (16 chunks of dimensions x 4 groups of tokens) write to 64 banks.
@@ -118,7 +76,7 @@ __global__ __launch_bounds__(NT) void kv_write_kernel(const KvCacheArgs c, const
   const bool vals = blockIdx.y & 1;
   const int P = c.page, plog = __builtin_ctz(P), dlog = __builtin_ctz(c.dim) - 3, D = c.dim;
   int b, item;
-  const SeqView s = item_seq(c, blockIdx.x, plog, 2, b, item);
+  const SeqView s = item_seq(c, blockIdx.x, [&](int row, int q) { return (row >> plog) + 2 * q; }, b, item);
   if (b < 0 || s.n == 0 || s.len == 0) return;
   const int start = s.first > 0 ? s.first : 0;
   const int pg = (start >> plog) + item, base = pg << plog;
@@ -289,7 +247,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvCacheArgs c, const
   __shared__ __attribute__((aligned(16))) uint32_t tile[D * 16 + D / 2];
   const int tid = threadIdx.x, head = blockIdx.y;
   int b, item;
-  const SeqView s = item_seq(c, blockIdx.x, 6, 1, b, item);
+  const SeqView s = item_seq(c, blockIdx.x, [](int row, int q) { return (row >> 6) + q; }, b, item);
   const int base = item << 6;
   if (b < 0 || item < 0 || base >= s.n) return;
   const int rows = s.n - base < 64 ? s.n - base : 64, have = s.len - base < rows ? s.len - base : rows;

@@ -72,6 +72,12 @@ def test_a_workgroup_per_unit():
         table, pages = table_of(lens, 64, 710)
         cache = random_cache(pages, heads, 64, 64, "int8", 711)
         check_attention(randn((seqs, heads * 2, 64), 712, torch.bfloat16), cache, lens, table)
+        new = [min(n, b % 4) if b % 7 else min(n, 40) for b, n in enumerate(lens)]
+        starts = starts_of(new)
+        q = randn((starts[-1], heads * 2, 64), 713, torch.bfloat16)
+        check_attention(q, cache, lens, table, starts, max_q_len=40)
+        check_attention(q, cache, lens, table, starts, max_q_len=1)
+    check_attention(randn((seqs, heads * 20, 64), 714, torch.bfloat16), cache, lens, table)      # two blocks of rows
 
 
 @pytest.mark.parametrize("fmt", ["int8", "fp8"])
