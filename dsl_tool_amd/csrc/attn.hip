@@ -22,13 +22,15 @@
 namespace dsl {
 
 constexpr int kTile = 64;      // tokens per step of a wave
-constexpr int kRowsWgs = 2;    // workgroups of a CU: what its registers hold
+// Workgroups of a CU: what its registers hold.
+constexpr int rows_wgs(int dim, int rb) { return dim * rb <= 128 ? 2 : 1; }
 // Up to kFewRows query rows of a sequence and cache head, or where the line gives a
 // run kFewRounds rounds at most, the kernel of few rows serves, else
 // attn_prompt.hip's: 32 query heads on 8 of dim 128, 16 sequences of up to 4000
 // tokens, rows 64 / 96 / 128: 67 / 90 / 108 against 81 / 85 / 91 us; one of 8000:
 // 29 / 34 / 35 against 32 / 35 / 37, and rows 256, 4 rounds: 48 against 40; one of
 // 1000, rows 256: 18 against 30.
+constexpr int kPartTiles = 4;  // of 64 tokens: the shortest part of a prompt's context
 constexpr int kFewRows = 96, kFewRounds = 2;
 // Whether units are split into runs (and joined, about 5 us), by the rounds R that
 // the table has room for and the units U per run; else a workgroup takes a unit
@@ -115,7 +117,7 @@ constexpr uint32_t kOnes = 0x38383838u;          // 1.0 four times
 
 // RB blocks of 16 query rows share every load.
 template <int SRC, bool FP8, int D, int RB>
-__global__ __launch_bounds__(256, D * RB <= 128 ? 2 : 1) void attn_rows_kernel(const KvCacheArgs c, const AttnArgs p, const int chunk, const bool split) {
+__global__ __launch_bounds__(256, rows_wgs(D, RB)) void attn_rows_kernel(const KvCacheArgs c, const AttnArgs p, const int chunk, const bool split) {
   constexpr bool F16 = SRC == SRC_F16;
   constexpr int NW = 4, DT = D / 16, DC = D / 64, ROWS = 16 * RB;
   constexpr int LD = D + 4;                      // floats per row of the joined tile
@@ -168,7 +170,13 @@ __global__ __launch_bounds__(256, D * RB <= 128 ? 2 : 1) void attn_rows_kernel(c
     if (rb * ROWS >= rows) return;               // (a workgroup for every block there may be)
     const int room = c.width * c.page;           // tokens that the table has pages for
     const int seen = s.len < room ? s.len : room, ntiles = (seen + kTile - 1) / kTile;
-    const int t0 = r0 * chunk, t1 = split && ntiles - t0 > count * chunk ? t0 + count * chunk : ntiles;
+    int nsee = ntiles;                           // tiles that some row of the block sees
+    if (p.causal) {
+      const int high = s.first + ((rb + 1) * ROWS < rows ? (rb + 1) * ROWS - 1 : rows - 1) / p.group + 1;
+      const int nh = high > 0 ? (high + kTile - 1) / kTile : 0;
+      nsee = nh < ntiles ? nh : ntiles;
+    }
+    const int t0 = r0 * chunk, t1 = split && nsee - t0 > count * chunk ? t0 + count * chunk : nsee;
     // the rows' queries, as they stand in the products
     v4i qf[RB][2 * DC];
     int limit[RB];
@@ -428,32 +436,22 @@ __global__ __launch_bounds__(256, D * RB <= 128 ? 2 : 1) void attn_rows_kernel(c
 // Joins the parts of one query row and head in a workgroup: a part per thread for
 // the maximum and the sum, then four columns per thread, the parts dealt to 1024 / D
 // threads of each.  (All parts in one thread's loop, a load's latency each, took 14
-// to 27 us.)  ROWS: the parts of attn_rows_kernel; 0: one per split of a prompt,
-// [split][row][head].  A part that saw no token has no sums.
+// to 27 us.)  A part that saw no token has no sums.
 constexpr int kMaxParts = 1024;
 template <int SRC, int D, int ROWS>
-__global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const int64_t rows, const int runs) {
+__global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const int runs) {
   constexpr int CG = D / 4, SL = 256 / CG;
   __shared__ float s_f[kMaxParts], s_red[8];
   __shared__ v4f s_v[SL][CG];
-  const int64_t at = blockIdx.x, n = rows * p.q_heads;
+  const int64_t at = blockIdx.x;
   const int tid = threadIdx.x;
-  int parts = runs, first = 0, row = 0;
-  const float *ml = p.ws + (int64_t)runs * n * D;
-  if constexpr (ROWS > 0) {
-    const Parts<D, ROWS> part(p.ws, runs);
-    const int2 w = part.where[at];
-    if (w.x < 0 || w.x >= runs) return;          // written already (or a row of no sequence)
-    ml = part.ml;
-    first = w.x;
-    row = w.y & (ROWS - 1);
-    parts = (w.y >> 6) - first + 1;
-    parts = parts < runs - first ? parts : runs - first;
-  }
-  auto index = [&](int s) -> int64_t {
-    if constexpr (ROWS > 0) return (int64_t)(s == 0 ? 2 * first + 1 : 2 * (first + s)) * ROWS + row;
-    else return s * n + at;
-  };
+  const Parts<D, ROWS> part(p.ws, runs);
+  const int2 w = part.where[at];
+  if (w.x < 0 || w.x >= runs) return;            // written already (or a row of no sequence)
+  const float *const ml = part.ml;
+  const int first = w.x, row = w.y & (ROWS - 1), many = (w.y >> 6) - first + 1;
+  const int parts = many < runs - first ? many : runs - first;
+  auto index = [&](int s) { return (int64_t)(s == 0 ? 2 * first + 1 : 2 * (first + s)) * ROWS + row; };
   float top = -INFINITY, l = 0.f;
   for (int s = tid; s < parts; s += 256) {
     const float m = ml[index(s) * 2];
@@ -492,10 +490,37 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const 
   *reinterpret_cast<uint2 *>(op) = make_uint2(narrow2<SRC>(v[0] * inv, v[1] * inv), narrow2<SRC>(v[2] * inv, v[3] * inv));
 }
 
+// Joins the parts [part][row][head] of a prompt's context: D / 4 threads of each row
+// and head, as there are many of them and few parts (a workgroup each: 18 us for 500
+// rows of 32 heads and two parts).
+template <int SRC, int D>
+__global__ __launch_bounds__(256) void attn_join_prompt_kernel(const AttnArgs p, const int64_t rows, const int parts) {
+  constexpr int CG = D / 4;
+  const int64_t n = rows * p.q_heads, at = (int64_t)blockIdx.x * (256 / CG) + threadIdx.x / CG;
+  const int col = threadIdx.x % CG * 4;
+  if (at >= n) return;
+  const float2 *ml = reinterpret_cast<const float2 *>(p.ws + (int64_t)parts * n * D) + at;
+  float top = -INFINITY, l = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) top = fmaxf(top, ml[s * n].x);
+  v4f v = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float2 x = ml[s * n];
+    if (x.x == -INFINITY) continue;
+    const float f = __builtin_amdgcn_exp2f(x.x - top);
+    l += x.y * f;
+    v += *reinterpret_cast<const v4f *>(p.ws + (s * n + at) * D + col) * f;
+  }
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  uint16_t *op = static_cast<uint16_t *>(p.o) + (at / p.q_heads) * p.o_row + (at % p.q_heads) * p.o_head + col;
+  *reinterpret_cast<uint2 *>(op) = make_uint2(narrow2<SRC>(v[0] * inv, v[1] * inv), narrow2<SRC>(v[2] * inv, v[3] * inv));
+}
+
 struct AttnPlan {
   bool prompt;
-  int rb, nblk, nsplit;          // prompts: row blocks, splits
-  int runs, chunk;               // few rows: workgroups, tiles of a round
+  int rb, nblk, nsplit;          // prompts: row blocks, parts of the context
+  int runs, chunk;               // few rows: workgroups, tiles of a round; prompts: tokens of a part
   bool split;                    // they are runs of the line, and parts are joined
 };
 static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
@@ -506,7 +531,7 @@ static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
   const int64_t group = q_heads / c.heads, most = c.rows < c.seqs ? c.rows : c.seqs;
   const int64_t likely = c.heads * most * ((rows + 16 * a.rb - 1) / (16 * a.rb));        // units
   const int64_t tiles = ((int64_t)c.width * c.page + kTile - 1) / kTile;
-  a.runs = kRowsWgs * device_cu_count();
+  a.runs = rows_wgs(c.dim, a.rb) * device_cu_count();
   if (a.runs > kMaxParts) a.runs = kMaxParts;
   const char *few = getenv("DSL_ATTN_FEW_ROWS");       // read per launch (tests switch it)
   if (few) a.prompt = rows > atoi(few);
@@ -516,11 +541,16 @@ static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
     const int64_t pairs = (int64_t)c.heads * c.seqs, blocks = (rows + per - 1) / per;
     const int64_t room = ((int64_t)1 << 30) / pairs;
     a.nblk = (int)(blocks < room ? blocks : room);
-    // one workgroup per CU; a split has four tiles at least
-    int64_t ns = device_cu_count() / (pairs * a.nblk);
-    if (ns > tiles / 4) ns = tiles / 4;
-    if (ns > 64) ns = 64;
-    a.nsplit = ns < 1 ? 1 : (int)ns;
+    // Parts of equal length, as long as one round of workgroups (one per CU) makes
+    // them if each row block sees half of the new tokens; where that is half of the
+    // context or more, none.
+    const int64_t seen = tiles - (tiles < max_q / kTile ? tiles : max_q / kTile) / 2;
+    int64_t len = (pairs * a.nblk * seen + device_cu_count() - 1) / device_cu_count();
+    if (len < kPartTiles) len = kPartTiles;
+    if (len < (tiles + 63) / 64) len = (tiles + 63) / 64;
+    len += len & 1;                              // whole tiles of 128 tokens
+    a.nsplit = 2 * len > tiles ? 1 : (int)((tiles + len - 1) / len);
+    a.chunk = (int)len * kTile;
     return a;
   }
   // rounds of a tile per wave, longer ones where the line's length would pass an int
@@ -549,16 +579,18 @@ static void launch_rows(const KvCacheArgs &c, const AttnArgs &p, const AttnPlan 
   const dim3 grid((unsigned)a.runs, a.split ? 1u : (unsigned)c.heads);
   if (c.fp8) attn_rows_kernel<SRC, true, D, RB><<<grid, 256, 0, st>>>(c, p, a.chunk, a.split);
   else attn_rows_kernel<SRC, false, D, RB><<<grid, 256, 0, st>>>(c, p, a.chunk, a.split);
-  if (a.split) attn_join_kernel<SRC, D, 16 * RB><<<(unsigned)c.rows * (unsigned)p.q_heads, 256, 0, st>>>(p, c.rows, a.runs);
+  if (a.split) attn_join_kernel<SRC, D, 16 * RB><<<(unsigned)c.rows * (unsigned)p.q_heads, 256, 0, st>>>(p, a.runs);
 }
 
 template <int SRC, int D>
 static hipError_t launch_dim(const KvCacheArgs &c, const AttnArgs &p, hipStream_t st) {
   const AttnPlan a = attn_plan(c, p.q_heads, p.max_q);
   if (a.prompt) {
-    const hipError_t e = launch_attn_prompt(SRC, c, p, a.nblk, a.nsplit, st);
+    const hipError_t e = launch_attn_prompt(SRC, c, p, a.nblk, a.nsplit, a.chunk, st);
     if (e != hipSuccess) return e;
-    if (a.nsplit > 1) attn_join_kernel<SRC, D, 0><<<(unsigned)c.rows * (unsigned)p.q_heads, 256, 0, st>>>(p, c.rows, a.nsplit);
+    constexpr int each = 1024 / D;               // rows and heads of a workgroup
+    const int64_t n = (int64_t)c.rows * p.q_heads;
+    if (a.nsplit > 1) attn_join_prompt_kernel<SRC, D><<<(unsigned)((n + each - 1) / each), 256, 0, st>>>(p, c.rows, a.nsplit);
   } else if (a.rb == 1) {
     launch_rows<SRC, D, 1>(c, p, a, st);
   } else if constexpr (D <= 128) {

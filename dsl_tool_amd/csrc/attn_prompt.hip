@@ -87,7 +87,7 @@ struct PromptCfg {
 // blockIdx: x (row block from the last on) * heads * sequences + ..., y split.
 template <int SRC, bool FP8, int D>
 __global__ __launch_bounds__(PromptCfg<D>::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, const int nsplit) {
+void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, const int nsplit, const int part) {
   using Cfg = PromptCfg<D>;
   constexpr bool F16 = SRC == SRC_F16;
   constexpr int T = Cfg::T, G = Cfg::G, TS = Cfg::TS, DT = Cfg::DT, VT = Cfg::VT, VG = VT / 16;
@@ -135,8 +135,9 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
     };
     const int every = sees(rb * Cfg::ROWS), end = sees(rb * Cfg::ROWS + Cfg::ROWS - 1);
     const int ntiles = (end + T - 1) / T;
-    const int t0 = (int)((int64_t)ntiles * split / nsplit), t1 = (int)((int64_t)ntiles * (split + 1) / nsplit);
-
+    int t0 = nsplit > 1 ? split * (part / T) : 0;
+    int t1 = nsplit > 1 && ntiles - t0 > part / T ? t0 + part / T : ntiles;
+    asm volatile("" : "+s"(t0), "+s"(t1));       // (what they are made of would be kept in registers, which spill)
     v4i qf[KK];
     const int qrow = rb * Cfg::ROWS + wrow + r32;
     {
@@ -519,12 +520,14 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
       const int qi = row / p.group, hq = head * p.group + row % p.group;
       if (nsplit > 1) {
         const int64_t n = (int64_t)c.rows * p.q_heads, at = (int64_t)split * n + (int64_t)(s.row0 + qi) * p.q_heads + hq;
+        if (t0 < t1) {                           // (a part of no tile has no sums)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+          for (int d = 0; d < DT; ++d)
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<v4f *>(p.ws + at * D + col + 32 * d + 8 * q) =
-                (v4f){o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<v4f *>(p.ws + at * D + col + 32 * d + 8 * q) =
+                  (v4f){o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
+        }
         if (h == 0 && half == 0) {
           float *ml = p.ws + (int64_t)nsplit * n * D + at * 2;
           ml[0] = m;
@@ -546,21 +549,21 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
 }
 
 template <int SRC, bool FP8, int D>
-static hipError_t launch_prompt_cfg(const KvCacheArgs &c, const AttnArgs &p, int nblk, int nsplit, hipStream_t st) {
+static hipError_t launch_prompt_cfg(const KvCacheArgs &c, const AttnArgs &p, int nblk, int nsplit, int part, hipStream_t st) {
   const dim3 grid((unsigned)(nblk * c.heads * c.seqs), (unsigned)nsplit);
-  attn_prompt_kernel<SRC, FP8, D><<<grid, PromptCfg<D>::NT, 0, st>>>(c, p, nblk, nsplit);
+  attn_prompt_kernel<SRC, FP8, D><<<grid, PromptCfg<D>::NT, 0, st>>>(c, p, nblk, nsplit, part);
   return hipGetLastError();
 }
 
 int attn_prompt_rows(int dim) { return dim > 128 ? PromptCfg<256>::ROWS : PromptCfg<128>::ROWS; }
 
-hipError_t launch_attn_prompt(int src, const KvCacheArgs &c, const AttnArgs &p, int nblk, int nsplit, hipStream_t st) {
+hipError_t launch_attn_prompt(int src, const KvCacheArgs &c, const AttnArgs &p, int nblk, int nsplit, int part, hipStream_t st) {
   auto go = [&](auto src_tag, auto fp8_tag) {
     constexpr int S = decltype(src_tag)::value;
     constexpr bool F = decltype(fp8_tag)::value;
-    if (c.dim == 64) return launch_prompt_cfg<S, F, 64>(c, p, nblk, nsplit, st);
-    if (c.dim == 128) return launch_prompt_cfg<S, F, 128>(c, p, nblk, nsplit, st);
-    return launch_prompt_cfg<S, F, 256>(c, p, nblk, nsplit, st);
+    if (c.dim == 64) return launch_prompt_cfg<S, F, 64>(c, p, nblk, nsplit, part, st);
+    if (c.dim == 128) return launch_prompt_cfg<S, F, 128>(c, p, nblk, nsplit, part, st);
+    return launch_prompt_cfg<S, F, 256>(c, p, nblk, nsplit, part, st);
   };
   using B = std::integral_constant<int, SRC_BF16>;
   using H = std::integral_constant<int, SRC_F16>;

@@ -215,15 +215,17 @@ template <int SRC, int FMT, bool NORM, bool W32 = false>
 static hipError_t launch_rows(const RowQuantArgs &p, hipStream_t st) {
   const int nch = p.cols / 8;
   if (p.rows == 0) return hipSuccess;
+  const int few = 2 * device_cu_count();
   // workgroups that are resident together, each walking its rows
-  const int waves = nch <= 64 ? 1 : nch <= 128 ? 2 : nch <= 256 ? 4 : nch <= 1024 ? 8 : 16;
+  const int waves = nch <= 64 ? 1 : nch <= 128 ? 2 : nch <= 256 ? 4 : nch <= 512 ? 8 : nch <= 1024 && p.rows > few ? 8 : 16;
   const int64_t most = (int64_t)device_cu_count() * (kResident / waves);
   const unsigned grid = (unsigned)(p.rows < most ? p.rows : most);
   if (nch <= 64) row_quant_kernel<SRC, FMT, NORM, W32, 64, 1><<<grid, 64, 0, st>>>(p);
   else if (nch <= 128) row_quant_kernel<SRC, FMT, NORM, W32, 128, 1><<<grid, 128, 0, st>>>(p);
   else if (nch <= 256) row_quant_kernel<SRC, FMT, NORM, W32, 256, 1><<<grid, 256, 0, st>>>(p);
   else if (nch <= 512) row_quant_kernel<SRC, FMT, NORM, W32, 512, 1><<<grid, 512, 0, st>>>(p);
-  else if (nch <= 1024) row_quant_kernel<SRC, FMT, NORM, W32, 512, 2><<<grid, 512, 0, st>>>(p);
+  else if (nch <= 1024 && p.rows > few) row_quant_kernel<SRC, FMT, NORM, W32, 512, 2><<<grid, 512, 0, st>>>(p);
+  else if (nch <= 1024) row_quant_kernel<SRC, FMT, NORM, W32, 1024, 1><<<grid, 1024, 0, st>>>(p);
   else if (nch <= 2048) row_quant_kernel<SRC, FMT, NORM, W32, 1024, 2><<<grid, 1024, 0, st>>>(p);
   else row_quant_kernel<SRC, FMT, NORM, W32, 1024, 4><<<grid, 1024, 0, st>>>(p);
   return hipGetLastError();

@@ -71,9 +71,10 @@ struct AttnArgs {
 };
 size_t attn_workspace_bytes(const KvCacheArgs &c, int q_heads, int max_q);
 // Many query rows (attn_prompt.hip): blocks of attn_prompt_rows(dim) rows, nblk of
-// them per sequence and head (each walks every nblk-th), nsplit parts of the context.
+// them per sequence and head (each walks every nblk-th); the context in nsplit parts
+// of `part` tokens.
 int attn_prompt_rows(int dim);
-hipError_t launch_attn_prompt(int src, const KvCacheArgs &c, const AttnArgs &p, int nblk, int nsplit, hipStream_t st);
+hipError_t launch_attn_prompt(int src, const KvCacheArgs &c, const AttnArgs &p, int nblk, int nsplit, int part, hipStream_t st);
 hipError_t launch_attn(int src, const KvCacheArgs &c, const AttnArgs &p, hipStream_t st);
 
 }  // namespace dsl
