@@ -114,6 +114,8 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
   if (pairs % 8 == 0) {
     const int n = pairs / 8, j = (blockIdx.x >> 3) % n;
     pair = (j + (n == 2 ? blk / 2 : blk)) % n * 8 + (blockIdx.x & 7);
+  } else {                                       // an XCD would get every 2nd, 4th or 8th pair only
+    pair = (pair + blockIdx.x / (pairs * (8 / (pairs & -pairs)))) % pairs;
   }
   blk = nblk - 1 - blk;
   const int head = pair % c.heads, b = pair / c.heads, split = blockIdx.y;
