@@ -30,7 +30,10 @@ constexpr int rows_wgs(int dim, int rb) { return dim * rb <= 128 ? 2 : 1; }
 // tokens, rows 64 / 96 / 128: 67 / 90 / 108 against 81 / 85 / 91 us; one of 8000:
 // 29 / 34 / 35 against 32 / 35 / 37, and rows 256, 4 rounds: 48 against 40; one of
 // 1000, rows 256: 18 against 30.
-constexpr int kPartTiles = 4;  // of 64 tokens: the shortest part of a prompt's context
+// The shortest part of a prompt's context, in tiles of 64 tokens: 893 tokens of 16
+// heads on 8, 500 of 32 on 8, 4 x 400 at dim 256: 4 tiles 32 / 34 / 48 us; 8 tiles (or
+// whole) 36 / 30 / 59; 2 tiles 42 / 32 / 48.
+constexpr int kPartTiles = 4;
 constexpr int kFewRows = 96, kFewRounds = 2;
 // Whether units are split into runs (and joined, about 5 us), by the rounds R that
 // the table has room for and the units U per run; else a workgroup takes a unit
@@ -117,7 +120,8 @@ constexpr uint32_t kOnes = 0x38383838u;          // 1.0 four times
 
 // RB blocks of 16 query rows share every load.
 template <int SRC, bool FP8, int D, int RB>
-__global__ __launch_bounds__(256, rows_wgs(D, RB)) void attn_rows_kernel(const KvCacheArgs c, const AttnArgs p, const int chunk, const bool split) {
+__global__ __launch_bounds__(256, rows_wgs(D, RB)) void attn_rows_kernel(const KvCacheArgs c, const AttnArgs p,
+                                                                           const int chunk, const bool split) {
   constexpr bool F16 = SRC == SRC_F16;
   constexpr int NW = 4, DT = D / 16, DC = D / 64, ROWS = 16 * RB;
   constexpr int LD = D + 4;                      // floats per row of the joined tile
@@ -285,7 +289,8 @@ __global__ __launch_bounds__(256, rows_wgs(D, RB)) void attn_rows_kernel(const K
         // products, and the rows that see it get it by the count of such codes
         bool any = false;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) any |= (nan_bytes(vr[d].x) | nan_bytes(vr[d].y) | nan_bytes(vr[d].z) | nan_bytes(vr[d].w)) != 0;
+        for (int d = 0; d < DT; ++d)
+          any |= (nan_bytes(vr[d].x) | nan_bytes(vr[d].y) | nan_bytes(vr[d].z) | nan_bytes(vr[d].w)) != 0;
         if (__any(any)) {
           v4i vis[RB][2];
 #pragma unroll
@@ -413,9 +418,11 @@ __global__ __launch_bounds__(256, rows_wgs(D, RB)) void attn_rows_kernel(const K
           v += *reinterpret_cast<const v4f *>(&so[w][row * LD + col]);
         }
         const int i = r / p.group, hq = head * p.group + r % p.group;
-        if (split && r0 == 0 && col == 0)
+        if (split && r0 == 0 && col == 0) {
+          const int last = (int)blockIdx.x + (left - count + per - 1) / per;
           part.where[(int64_t)(s.row0 + i) * p.q_heads + hq] =
-              make_int2(parted ? (int)blockIdx.x : -1, parted ? ((int)blockIdx.x + (left - count + per - 1) / per) * 64 + k * 16 + row : 0);
+              parted ? make_int2((int)blockIdx.x, last * 64 + k * 16 + row) : make_int2(-1, 0);
+        }
         if (parted) {
           const int64_t at = ((int64_t)2 * blockIdx.x + (r0 == 0)) * ROWS + k * 16 + row;
           *reinterpret_cast<v4f *>(part.v + at * D + col) = v;

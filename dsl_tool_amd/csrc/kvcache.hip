@@ -177,8 +177,10 @@ __global__ __launch_bounds__(NT) void kv_write_kernel(const KvCacheArgs c, const
       uint32_t w[8];                             // four tokens of each dimension
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t a = __builtin_amdgcn_perm(q[1][h], q[0][h], 0x05010400u), c2 = __builtin_amdgcn_perm(q[3][h], q[2][h], 0x05010400u);
-        const uint32_t e = __builtin_amdgcn_perm(q[1][h], q[0][h], 0x07030602u), g = __builtin_amdgcn_perm(q[3][h], q[2][h], 0x07030602u);
+        const uint32_t a = __builtin_amdgcn_perm(q[1][h], q[0][h], 0x05010400u);
+        const uint32_t c2 = __builtin_amdgcn_perm(q[3][h], q[2][h], 0x05010400u);
+        const uint32_t e = __builtin_amdgcn_perm(q[1][h], q[0][h], 0x07030602u);
+        const uint32_t g = __builtin_amdgcn_perm(q[3][h], q[2][h], 0x07030602u);
         w[4 * h] = __builtin_amdgcn_perm(c2, a, 0x05040100u);
         w[4 * h + 1] = __builtin_amdgcn_perm(c2, a, 0x07060302u);
         w[4 * h + 2] = __builtin_amdgcn_perm(g, e, 0x05040100u);

@@ -76,9 +76,13 @@ def test_cache_entry_points(lib):
         args[at] = value
         refused(lib, "dsl_kv8_write", args, -1, word)
     for at, value, st, word in [(3, 5, -1, "q_heads"), (0, P + 4, -1, "q must"), (1, 10, -1, "strides of q"),
-                                (21, 64, -1, "strides of out"), (24, float("inf"), -1, "scale"), (26, 7, -1, "x_dtype"),
-                                (27, None, -3, "workspace"), (28, 16, -3, "workspace")]:
+                                (21, 64, -1, "strides of out"), (24, float("inf"), -1, "scale"), (26, 7, -1, "x_dtype")]:
         args = list(attn)
+        args[at] = value
+        refused(lib, "dsl_kv8_attention", args, st, word)
+    for at, value, st, word in [(27, None, -3, "workspace"), (28, 16, -3, "workspace")]:
+        args = list(attn)
+        args[14] = args[15] = 64                 # contexts long enough to be split
         args[at] = value
         refused(lib, "dsl_kv8_attention", args, st, word)
     # nothing to do is no error
