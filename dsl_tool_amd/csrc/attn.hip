@@ -548,15 +548,25 @@ static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
     const int64_t pairs = (int64_t)c.heads * c.seqs, blocks = (rows + per - 1) / per;
     const int64_t room = ((int64_t)1 << 30) / pairs;
     a.nblk = (int)(blocks < room ? blocks : room);
-    // Parts of equal length, as long as one round of workgroups (one per CU) makes
-    // them if each row block sees half of the new tokens; where that is half of the
-    // context or more, none.
-    const int64_t seen = tiles - (tiles < max_q / kTile ? tiles : max_q / kTile) / 2;
-    int64_t len = (pairs * a.nblk * seen + device_cu_count() - 1) / device_cu_count();
-    if (len < kPartTiles) len = kPartTiles;
-    if (len < (tiles + 63) / 64) len = (tiles + 63) / 64;
+    // Parts of equal length, the shortest that one round of workgroups (one per CU)
+    // holds if block i of n sees the first i / n of the new tokens; none where that
+    // saves fewer tiles than a part has at least.
+    const int64_t q = tiles < max_q / kTile ? tiles : max_q / kTile, room_for = device_cu_count() / pairs;
+    auto fits = [&](int64_t len) {
+      int64_t parts = 0;
+      for (int64_t i = 1; i <= a.nblk; ++i) parts += (tiles - q + (q * i + a.nblk - 1) / a.nblk + len - 1) / len;
+      return parts <= room_for;
+    };
+    int64_t len = tiles, lo = kPartTiles > (tiles + 63) / 64 ? kPartTiles : (tiles + 63) / 64;
+    if (a.nblk < room_for) {
+      for (int64_t hi = tiles; lo < hi;) {
+        const int64_t mid = (lo + hi) / 2;
+        if (fits(mid)) len = hi = mid;
+        else lo = mid + 1;
+      }
+    }
     len += len & 1;                              // whole tiles of 128 tokens
-    a.nsplit = 2 * len > tiles ? 1 : (int)((tiles + len - 1) / len);
+    a.nsplit = len + kPartTiles > tiles ? 1 : (int)((tiles + len - 1) / len);
     a.chunk = (int)len * kTile;
     return a;
   }

@@ -118,3 +118,9 @@ def test_python_refusals():
         KV.kv8_read(c, lens, table, lens, 3, dtype=torch.float32)
     with pytest.raises(ValueError, match="total"):
         KV.kv8_read(c, lens, table, lens, -1)
+
+
+def test_attention_counts_rows_in_ints(lib):
+    attn = [P, 512, 128, 4] + CACHE + [P, 512, 128, 7, 4, 0.1, 1, 0, P, 1 << 30, None]
+    attn[22] = (1 << 28) + 1
+    refused(lib, "dsl_kv8_attention", attn, -1, "query heads")
