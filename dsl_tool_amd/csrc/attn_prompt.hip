@@ -501,13 +501,16 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
       }
     }
     if constexpr (FP8) {
+      // (of no tile: no barrier since other waves cleared s_row, and nothing in it)
+      if (t0 < t1) {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const uint32_t bad = s_row[wrow + r32][half * DT + d];
-        if (__any(bad)) {
+        for (int d = 0; d < DT; ++d) {
+          const uint32_t bad = s_row[wrow + r32][half * DT + d];
+          if (__any(bad)) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (bad >> (8 * (i >> 2) + 4 * h + (i & 3)) & 1) o[d][i] = __builtin_nanf("");
+            for (int i = 0; i < 16; ++i)
+              if (bad >> (8 * (i >> 2) + 4 * h + (i & 3)) & 1) o[d][i] = __builtin_nanf("");
+          }
         }
       }
     }

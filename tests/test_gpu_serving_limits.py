@@ -1,0 +1,49 @@
+"""The 8-bit layer's operators at their limits on the GPU: rows that see
+nothing, NaN over contexts that are split, launches of very many workgroups,
+lengths and scores at the ends of their types."""
+import math
+
+import pytest
+import torch
+
+from dsl_tool_amd import attention as A
+from dsl_tool_amd import fused as FU
+from dsl_tool_amd import gemm as G
+from dsl_tool_amd import kvcache as KV
+from dsl_tool_amd import quant as Q
+from oracle import serving as O
+from tests.test_gpu_serving import DEV, check_attention, random_cache, randn, table_of, to, within
+from tests.test_gpu_serving_edges import DIM, HIDDEN, HKV, HQ, ints, new_layer, route, starts_of  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------ rows that see nothing --
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_blocks_that_see_nothing_after_nan_ones(dim, src, causal, monkeypatch):
+    """Whole blocks of prompts' rows that see no token are zeros, whatever the
+    workgroups' shared memory held before: a call all of whose rows get NaN
+    columns goes first, with a workgroup or more for every CU."""
+    monkeypatch.setenv("DSL_ATTN_FEW_ROWS", "0")
+    seqs, heads, new = 40, 8, 70
+    table, pages = table_of([new] * seqs, 64, 960)
+    cache = random_cache(pages, heads, dim, 64, "fp8", 961)
+    dirty = cache._replace(v=torch.full(cache.v.shape, 0x7f, dtype=torch.uint8).view(cache.v.dtype))
+    starts = starts_of([new] * seqs)
+    q = randn((starts[-1], heads * 4, dim), 962, src).to(DEV)
+    st, tb = ints(starts).to(DEV), table.to(DEV)
+    dirty, clean = to(dirty, DEV), to(cache, DEV)
+    for lens in ([0] * seqs, [0 if b % 2 else 3 for b in range(seqs)]):
+        full = A.kv8_attention(q, dirty, ints([new] * seqs).to(DEV), tb, q_starts=st, max_q_len=new)
+        got = A.kv8_attention(q, clean, ints(lens).to(DEV), tb, q_starts=st, max_q_len=new, causal=causal)
+        assert full.isnan().all()
+        for b, n in enumerate(lens):
+            none = got[starts[b]:starts[b + 1] - (n if causal else new if n else 0)]
+            assert (none == 0).all(), b
+    # two blocks, the first of which sees nothing and the second the only tokens
+    lens, starts = [5, 0, 40], [0, 300, 600, 900]
+    check_attention(randn((900, 4, dim), 963, src), random_cache(pages, 4, dim, 64, "fp8", 964), lens, table[:3],
+                    starts, max_q_len=300, causal=causal)
