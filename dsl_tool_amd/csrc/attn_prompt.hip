@@ -338,7 +338,8 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
       }
     };
     // True where the scores need no `settle`: no token hidden from a row, no scale
-    // off the common path, no row's maximum grown by more than 2^16.
+    // off the common path, no row's maximum grown by more than 2^16.  (Of a row that has
+    // none yet, all scores minus infinity, the difference is NaN: settle.)
     auto common = [&](int tile) __attribute__((always_inline)) {
       odd = s_odd[tile & 3];
       float top = -INFINITY;
@@ -352,7 +353,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
         top = fmaxf(top, x * kq[g]);
       }
       top = halves_max(top);
-      return !__builtin_amdgcn_readfirstlane((int)(__any(!(top <= m + 16.f)) || odd || tile * T + T > low));
+      return !__builtin_amdgcn_readfirstlane((int)(__any(!(top - m <= 16.f)) || odd || tile * T + T > low));
     };
     // In general: scores to powers of two, -infinity where hidden; sum and output to
     // their maximum.  (Outside the loop of the common tiles: there, the compiler kept

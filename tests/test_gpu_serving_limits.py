@@ -47,3 +47,30 @@ def test_blocks_that_see_nothing_after_nan_ones(dim, src, causal, monkeypatch):
     lens, starts = [5, 0, 40], [0, 300, 600, 900]
     check_attention(randn((900, 4, dim), 963, src), random_cache(pages, 4, dim, 64, "fp8", 964), lens, table[:3],
                     starts, max_q_len=300, causal=causal)
+
+
+# ------------------------------------------------------------------ scores --
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("seqs", [1, 130])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_scores_that_overflow_below(dim, seqs, fmt, route):
+    """Tokens whose products fall below the least fp32 number, several tiles of
+    them before any other: probability 0, as in 64 bits.  One sequence, whose
+    context is split, and enough that none is."""
+    new = 9
+    lens, starts = [720] * seqs, starts_of([new] * seqs)
+    table, pages = table_of([720], 64, 930)
+    table = table.repeat(seqs, 1)
+    cache = random_cache(pages, 2, dim, 64, fmt, 931)
+    early = table[0, :8].long()
+    cache.k.view(torch.uint8)[:, :, :, 0] = 0
+    cache.k[early, :, :, 0] = torch.full((), 100.0).to(cache.k.dtype)
+    q = randn((starts[-1], 4, dim), 932, torch.bfloat16)
+    q[:, :, 0] = -3e38
+    lt, st = ints(lens), ints(starts)
+    got = A.kv8_attention(q.to(DEV), to(cache, DEV), lt.to(DEV), table.to(DEV), q_starts=st.to(DEV), max_q_len=new)
+    q[:, :, 0] = 0                                         # the others' scores do not have it
+    late = table.clone()
+    late[:, :8] = -1
+    within(got, *O.attention(q, cache, lt, late, st))
