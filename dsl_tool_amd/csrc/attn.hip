@@ -414,7 +414,8 @@ __global__ __launch_bounds__(256, rows_wgs(D, RB)) void attn_rows_kernel(const K
         v4f v = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-          lr += mr == -INFINITY ? 0.f : sl[w][row] * __builtin_amdgcn_exp2f(sm[w][row] - mr);
+          // (no maximum: nothing seen, 0, or nothing but NaN, NaN)
+          lr += mr == -INFINITY ? sl[w][row] : sl[w][row] * __builtin_amdgcn_exp2f(sm[w][row] - mr);
           v += *reinterpret_cast<const v4f *>(&so[w][row * LD + col]);
         }
         const int i = r / p.group, hq = head * p.group + r % p.group;
@@ -427,7 +428,7 @@ __global__ __launch_bounds__(256, rows_wgs(D, RB)) void attn_rows_kernel(const K
           const int64_t at = ((int64_t)2 * blockIdx.x + (r0 == 0)) * ROWS + k * 16 + row;
           *reinterpret_cast<v4f *>(part.v + at * D + col) = v;
           if (col == 0) {
-            part.ml[2 * at] = mr;
+            part.ml[2 * at] = lr == lr ? mr : lr;          // a NaN sum without a maximum stays NaN in the join
             part.ml[2 * at + 1] = lr;
           }
         } else {
@@ -443,7 +444,9 @@ __global__ __launch_bounds__(256, rows_wgs(D, RB)) void attn_rows_kernel(const K
 // Joins the parts of one query row and head in a workgroup: a part per thread for
 // the maximum and the sum, then four columns per thread, the parts dealt to 1024 / D
 // threads of each.  (All parts in one thread's loop, a load's latency each, took 14
-// to 27 us.)  A part that saw no token has no sums.
+// to 27 us.)  A part without a maximum saw no token and has sums of 0; one whose
+// sum is NaN comes with a NaN for its maximum, and so has a NaN factor.  Values enter
+// whatever the factor: a NaN in them is one behind a factor of 0 too.
 constexpr int kMaxParts = 1024;
 template <int SRC, int D, int ROWS>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const int runs) {
@@ -473,7 +476,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const 
   for (int s = tid; s < parts; s += 256) {
     const float m = s_f[s], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
     s_f[s] = f;
-    l += f != 0.f ? ml[index(s) * 2 + 1] * f : 0.f;
+    l += ml[index(s) * 2 + 1] * f;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
@@ -483,8 +486,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const 
   v4f v = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = sl; s < parts; s += SL) {
-    const float fs = s_f[s];
-    if (fs != 0.f) v += *reinterpret_cast<const v4f *>(p.ws + index(s) * D + cg * 4) * fs;
+    v += *reinterpret_cast<const v4f *>(p.ws + index(s) * D + cg * 4) * s_f[s];
   }
   s_v[sl][cg] = v;
   __syncthreads();
@@ -499,7 +501,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const 
 
 // Joins the parts [part][row][head] of a prompt's context: D / 4 threads of each row
 // and head, as there are many of them and few parts (a workgroup each: 18 us for 500
-// rows of 32 heads and two parts).
+// rows of 32 heads and two parts).  A part without a maximum may have no sums; NaN ones
+// as above.
 template <int SRC, int D>
 __global__ __launch_bounds__(256) void attn_join_prompt_kernel(const AttnArgs p, const int64_t rows, const int parts) {
   constexpr int CG = D / 4;

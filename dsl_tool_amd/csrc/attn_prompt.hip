@@ -536,7 +536,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
         }
         if (h == 0 && half == 0) {
           float *ml = p.ws + (int64_t)nsplit * n * D + at * 2;
-          ml[0] = m;
+          ml[0] = l == l ? m : l;                // (attn_join_prompt_kernel skips a part without a maximum)
           ml[1] = l;
         }
       } else {

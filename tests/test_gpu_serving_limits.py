@@ -74,3 +74,69 @@ def test_scores_that_overflow_below(dim, seqs, fmt, route):
     late = table.clone()
     late[:, :8] = -1
     within(got, *O.attention(q, cache, lt, late, st))
+
+
+# ------------------------------------------------------ NaN and joined parts --
+
+def nan_where_it_belongs(q, cache, lens, table, starts=None, **kw):
+    """The oracle's NaNs, no others; the rest within the tolerance."""
+    lt, st = ints(lens), None if starts is None else ints(starts)
+    got = A.kv8_attention(q.to(DEV), to(cache, DEV), lt.to(DEV), table.to(DEV),
+                          q_starts=None if st is None else st.to(DEV), **kw).cpu()
+    o, a, reach = O.attention(q, cache, lt, table, st, **kw)
+    assert torch.equal(got.isnan(), o.isnan())
+    rows = o.isnan().any(-1, keepdim=True).expand_as(o)
+    zero = torch.zeros_like(o)
+    within(got.masked_fill(rows, 0), *(torch.where(rows, zero, t.expand_as(o)) for t in (o, a, reach)))
+    return got
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_nan_queries_over_long_contexts(dim, src, fmt, route):
+    """A NaN query is a NaN row, whether its context is split or not."""
+    lens = [5000, 300, 2000]
+    table, pages = table_of(lens, 64, 900)
+    cache = random_cache(pages, 2, dim, 64, fmt, 901)
+    q = randn((3, 8, dim), 902, src)
+    q[0, 3, 5] = q[1, 0, 0] = q[2, 7, dim - 1] = math.nan
+    got = nan_where_it_belongs(q, cache, lens, table)
+    assert got[0, 3].isnan().all() and got[1, 0].isnan().all() and got[2, 7].isnan().all()
+    new = [3, 200, 1]
+    starts = starts_of(new)
+    q = randn((starts[-1], 8, dim), 903, src)
+    q[1, 2, 9] = q[50, 4, 1] = q[203, 0, 2] = math.nan
+    nan_where_it_belongs(q, cache, lens, table, starts)
+
+
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_nan_keys_that_are_all_a_part_sees(dim, src, route):
+    """The part that begins at token 5120 has three tokens; the first new row sees
+    one of them, a NaN key."""
+    lens, starts = [20 * 256 + 3], [0, 3]
+    table, pages = table_of(lens, 64, 910)
+    cache = random_cache(pages, 2, dim, 64, "fp8", 911)
+    cache.k.view(torch.uint8)[table[0, 80], 1, 0, 7] = 0x7f
+    got = nan_where_it_belongs(randn((3, 4, dim), 912, src), cache, lens, table, starts)
+    assert got[:, 2:].isnan().all() and not got[:, :2].isnan().any()
+
+
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_nan_values_of_vanishing_probability(dim, src, route):
+    """A NaN value in a part whose scores lie so far below the others that its
+    factor is 0: 0 times NaN is NaN, as in a context that is not split."""
+    lens = [20 * 256]
+    table, pages = table_of(lens, 64, 920)
+    cache = random_cache(pages, 1, dim, 64, "fp8", 921)
+    first = table[0, :4].long()
+    cache.k.view(torch.uint8)[:, :, :, 0] = 0
+    cache.k[first, :, :, 0] = torch.full((), -64.0).to(torch.float8_e4m3fn)
+    cache.k_scale.fill_(0.02)
+    cache.v.view(torch.uint8)[table[0, 1], 0, 11, 3] = 0xff
+    q = randn((1, 3, dim), 922, src)
+    q[:, :, 0] = 64
+    got = nan_where_it_belongs(q, cache, lens, table, scale=4.0)
+    assert got[:, :, 11].isnan().all()
