@@ -28,7 +28,9 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, seq_lens: torch.Tensor, page
     included.  Query head h reads cache head ``h // (q_heads // heads)``.  With
     ``causal`` a row sees the tokens up to its own, else all of them; a row that
     sees none is zeros.  ``scale`` defaults to ``1/sqrt(dim)``.  ``max_q_len``
-    (the most new tokens of a sequence) sizes the launch and its workspace.
+    (the most new tokens of a sequence) sizes the launch and its workspace; the
+    result does not depend on it, but the default, all rows where there are
+    ``q_starts``, launches many idle workgroups for a batch of prompts.
     """
     if out is None:
         r = N.fast().kv8_attention(q, *cache, seq_lens, page_table, q_starts, max_q_len, scale, causal)

@@ -527,6 +527,11 @@ __global__ __launch_bounds__(256) void attn_join_prompt_kernel(const AttnArgs p,
   *reinterpret_cast<uint2 *>(op) = make_uint2(narrow2<SRC>(v[0] * inv, v[1] * inv), narrow2<SRC>(v[2] * inv, v[3] * inv));
 }
 
+// A launch has fewer than 2^32 threads.  Only calls whose max_q is not that of their
+// sequences come near it (max_q far above it: prompts' row blocks; far below: rows of
+// few, and the joins), and any plan is right for them.
+static bool launchable(int64_t workgroups, int threads) { return workgroups * threads < (int64_t)1 << 32; }
+
 struct AttnPlan {
   bool prompt;
   int rb, nblk, nsplit;          // prompts: row blocks, parts of the context
@@ -546,10 +551,13 @@ static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
   const char *few = getenv("DSL_ATTN_FEW_ROWS");       // read per launch (tests switch it)
   if (few) a.prompt = rows > atoi(few);
   else a.prompt = rows > kFewRows && (double)likely * (double)((tiles + 3) / 4) > (double)(kFewRounds * a.runs);
+  const int64_t pairs = (int64_t)c.heads * c.seqs;
+  if (!launchable((int64_t)c.rows * group / (16 * a.rb) + c.seqs, 256)) a.prompt = true;
+  if (!launchable(pairs, kPromptThreads)) a.prompt = false;     // (65535 sequences: more than 128 heads, and few rows of each)
   if (a.prompt) {
     const int per = attn_prompt_rows(c.dim);
-    const int64_t pairs = (int64_t)c.heads * c.seqs, blocks = (rows + per - 1) / per;
-    const int64_t room = ((int64_t)1 << 30) / pairs;
+    const int64_t blocks = (rows + per - 1) / per;
+    const int64_t room = (((int64_t)1 << 32) - 1) / kPromptThreads / pairs;   // (a workgroup walks every nblk-th block)
     a.nblk = (int)(blocks < room ? blocks : room);
     // Parts of equal length, the shortest that one round of workgroups (one per CU)
     // holds if block i of n sees the first i / n of the new tokens; none where that
@@ -569,7 +577,8 @@ static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
       }
     }
     len += len & 1;                              // whole tiles of 128 tokens
-    a.nsplit = len + kPartTiles > tiles ? 1 : (int)((tiles + len - 1) / len);
+    a.nsplit = len + kPartTiles > tiles || !launchable(((int64_t)c.rows * q_heads * c.dim + 1023) / 1024, 256)
+                   ? 1 : (int)((tiles + len - 1) / len);
     a.chunk = (int)len * kTile;
     return a;
   }
@@ -578,7 +587,7 @@ static AttnPlan attn_plan(const KvCacheArgs &c, int q_heads, int max_q) {
   a.chunk = 4;
   while ((tiles + a.chunk - 1) / a.chunk * units > 1 << 30 && a.chunk < tiles) a.chunk *= 2;
   const int64_t rounds = (tiles + a.chunk - 1) / a.chunk;
-  a.split = likely < kFewUnits * (int64_t)a.runs && c.seqs <= kLineSeqs &&
+  a.split = likely < kFewUnits * (int64_t)a.runs && c.seqs <= kLineSeqs && launchable((int64_t)c.rows * q_heads, 256) &&
             (rounds >= kLongRounds || (rounds - 3) * a.runs >= 8 * likely);
   if (!a.split) {
     const int64_t per = 16 * a.rb;

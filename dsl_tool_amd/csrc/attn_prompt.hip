@@ -70,7 +70,7 @@ DSL_DEV void wait_reads(bool more) {
 
 template <int D>
 struct PromptCfg {
-  static constexpr int NW = 8, NT = NW * 64;                 // two waves per SIMD
+  static constexpr int NT = kPromptThreads, NW = NT / 64;    // two waves per SIMD
   // Dim 256: two waves compute the same scores, each half of the output's columns
   // (all of them would take 128 of its 256 registers).
   static constexpr int HALVES = D > 128 ? 2 : 1;

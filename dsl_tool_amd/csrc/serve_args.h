@@ -74,6 +74,7 @@ size_t attn_workspace_bytes(const KvCacheArgs &c, int q_heads, int max_q);
 // them per sequence and head (each walks every nblk-th); the context in nsplit parts
 // of `part` tokens.
 int attn_prompt_rows(int dim);
+constexpr int kPromptThreads = 512;              // of a workgroup
 hipError_t launch_attn_prompt(int src, const KvCacheArgs &c, const AttnArgs &p, int nblk, int nsplit, int part, hipStream_t st);
 hipError_t launch_attn(int src, const KvCacheArgs &c, const AttnArgs &p, hipStream_t st);
 

@@ -398,7 +398,9 @@ int dsl_add_rmsnorm_quant(const void *x, int64_t rows, int64_t cols, int64_t ldx
  * outside [0, pages), tokens past the table's row and rows outside [0, rows)
  * are skipped, wherever the device tables hold them.  starts
  * ascend.  max_q (most new tokens of a sequence) sizes the attention's launch;
- * a smaller number costs time only. */
+ * a wrong number costs time only: under a smaller one few workgroups walk many
+ * rows, under a larger one (all rows, say, for a batch of prompts) sequences x
+ * heads x max_q / 256 are launched, most of which find no row. */
 
 /* Writes the new tokens' keys and values (k, v [rows][heads][dim], bf16 or
  * fp16, strides in elements, unit stride in dim).  A page's scale becomes

@@ -140,3 +140,57 @@ def test_nan_values_of_vanishing_probability(dim, src, route):
     q[:, :, 0] = 64
     got = nan_where_it_belongs(q, cache, lens, table, scale=4.0)
     assert got[:, :, 11].isnan().all()
+
+
+# ---------------------------------------------------------------- launches --
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_a_workgroup_walks_several_blocks(dim, fmt, monkeypatch):
+    """Prompts under a max_q_len far too small: one block's workgroups take all."""
+    monkeypatch.setenv("DSL_ATTN_FEW_ROWS", "0")
+    lens, starts = [420, 700, 0, 33], [0, 400, 900, 903, 910]
+    table, pages = table_of(lens, 32, 970)
+    cache = random_cache(pages, 2, dim, 32, fmt, 971)
+    q = randn((910, 8, dim), 972, torch.bfloat16)
+    for causal in (True, False):
+        check_attention(q, cache, lens, table, starts, max_q_len=1, causal=causal)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_more_workgroups_than_a_launch_has(fmt):
+    """8192 sequences x 16 heads without max_q_len: by all 16384 rows they would be
+    2^23 workgroups of 512 threads, one more than a launch may have."""
+    seqs, heads = 8192, 16
+    lens = [(b * 7) % 15 + 2 for b in range(seqs)]
+    table = ints([b % 61 for b in range(seqs)])[:, None].contiguous()
+    cache = random_cache(61, heads, 64, 16, fmt, 980)
+    q = randn((2 * seqs, heads, 64), 981, torch.bfloat16)
+    check_attention(q, cache, lens, table, starts_of([2] * seqs))
+
+
+def test_more_rows_than_a_join_takes():
+    """2^24 rows and heads over a context that is long enough to be split, under a
+    max_q_len far too small: a workgroup of 256 threads for each would be 2^32."""
+    rows, hq, dim, n = 1 << 18, 64, 64, 2304
+    table, pages = table_of([n], 256, 990)
+    cache = random_cache(pages, 1, dim, 256, "int8", 991)
+    q = torch.randn((rows, hq, dim), dtype=torch.bfloat16, device=DEV, generator=torch.Generator(DEV).manual_seed(992))
+    got = A.kv8_attention(q, to(cache, DEV), ints([n]).to(DEV), table.to(DEV), q_starts=ints([0, rows]).to(DEV),
+                          max_q_len=1, causal=False)
+    pick = torch.tensor([0, 1, 99999, rows - 2, rows - 1])
+    some = q[pick.to(DEV)].cpu()
+    within(got[pick.to(DEV)], *O.attention(some, cache, ints([n]), table, ints([0, 5]), causal=False))
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("seqs,heads", [(2, 8), (4, 8), (3, 8), (3, 16), (8, 8), (5, 4), (3, 2)])
+def test_blocks_of_pairs_over_the_xcds(seqs, heads):
+    """Every pair of sequence and cache head gets each of its blocks, however many
+    pairs rotate over the XCDs."""
+    new = [700 - 90 * (b % 4) for b in range(seqs)]
+    table, pages = table_of([n + 8 for n in new], 64, 995)
+    cache = random_cache(pages, heads, 64, 64, "int8", 996)
+    starts = starts_of(new)
+    check_attention(randn((starts[-1], 2 * heads, 64), 997, torch.bfloat16), cache, [n + 8 for n in new], table, starts,
+                    max_q_len=700)
