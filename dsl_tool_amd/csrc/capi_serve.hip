@@ -25,15 +25,11 @@ int check_rows(const char *fn, const char *name, int64_t rows, int64_t cols, int
   return DSL_OK;
 }
 
-// The cache and the sequences of a call, checked and packed.
-int check_cache(const char *fn, dsl::KvCacheArgs *c, const void *k, const void *v, const float *ks, const float *vs,
-                int64_t pages, int64_t heads, int64_t page, int64_t dim, int fmt, const int32_t *table,
-                int64_t table_ld, int64_t width, const int32_t *lens, const int32_t *starts, int64_t seqs,
-                int64_t rows, int x_dtype) {
-  if (pages < 0 || heads <= 0 || seqs < 0 || rows < 0 || width < 0)
+// The sizes of a call: what the kernels and their plans hold in ints.
+int check_sizes(const char *fn, int64_t heads, int64_t page, int64_t dim, int64_t width, int64_t seqs, int64_t rows) {
+  if (heads <= 0 || seqs < 0 || rows < 0 || width < 0)
     return fail(DSL_ERR_ARG, "%s: need pages, seqs, rows, width >= 0 and heads > 0", fn);
-  if (pages >= (int64_t)1 << 31 || rows >= (int64_t)1 << 31)
-    return fail(DSL_ERR_ARG, "%s: pages and rows must be < 2^31", fn);
+  if (rows >= (int64_t)1 << 31) return fail(DSL_ERR_ARG, "%s: pages and rows must be < 2^31", fn);
   if (dim != 64 && dim != 128 && dim != 256)
     return fail(DSL_ERR_UNSUPPORTED, "%s: head dim %lld must be 64, 128 or 256", fn, (long long)dim);
   if (page != 16 && page != 32 && page != 64 && page != 128 && page != 256)
@@ -43,6 +39,25 @@ int check_cache(const char *fn, dsl::KvCacheArgs *c, const void *k, const void *
   // tokens are counted in ints, whole tiles beyond a sequence's last one included
   if (width > (((int64_t)1 << 31) - 65536) / page)
     return fail(DSL_ERR_ARG, "%s: page table rows span more than 2^31 - 65536 tokens", fn);
+  return DSL_OK;
+}
+int check_q_heads(const char *fn, int64_t q_heads, int64_t heads, int64_t rows, int64_t max_q) {
+  if (q_heads <= 0 || q_heads % heads != 0 || q_heads > 1 << 20)
+    return fail(DSL_ERR_ARG, "%s: q_heads=%lld must be a multiple of heads=%lld", fn, (long long)q_heads,
+                (long long)heads);
+  if (max_q < 0) return fail(DSL_ERR_ARG, "%s: max_q must be >= 0", fn);
+  if (rows > ((int64_t)1 << 30) / q_heads) return fail(DSL_ERR_ARG, "%s: rows x query heads must be at most 2^30", fn);
+  return DSL_OK;
+}
+
+// The cache and the sequences of a call, checked and packed.
+int check_cache(const char *fn, dsl::KvCacheArgs *c, const void *k, const void *v, const float *ks, const float *vs,
+                int64_t pages, int64_t heads, int64_t page, int64_t dim, int fmt, const int32_t *table,
+                int64_t table_ld, int64_t width, const int32_t *lens, const int32_t *starts, int64_t seqs,
+                int64_t rows, int x_dtype) {
+  if (pages < 0) return fail(DSL_ERR_ARG, "%s: need pages, seqs, rows, width >= 0 and heads > 0", fn);
+  if (pages >= (int64_t)1 << 31) return fail(DSL_ERR_ARG, "%s: pages and rows must be < 2^31", fn);
+  if (const int rc = check_sizes(fn, heads, page, dim, width, seqs, rows)) return rc;
   if (fmt != DSL_KV_INT8 && fmt != DSL_KV_FP8) return fail(DSL_ERR_ARG, "%s: unknown fmt %d", fn, fmt);
   if (x_dtype != DSL_IN_BF16 && x_dtype != DSL_IN_F16)
     return fail(DSL_ERR_ARG, "%s: x_dtype %d must be bf16 or fp16", fn, x_dtype);
@@ -214,9 +229,9 @@ int dsl_kv8_read(const void *k_cache, const void *v_cache, const float *k_scale,
 
 size_t dsl_kv8_attention_workspace_bytes(int64_t heads, int64_t page, int64_t dim, int64_t width, int64_t seqs,
                                          int64_t rows, int64_t q_heads, int64_t max_q) {
-  if (heads <= 0 || q_heads <= 0 || q_heads % heads != 0 || page <= 0 || dim <= 0 || width < 0 || seqs <= 0 ||
-      rows <= 0 || max_q < 0)
-    return 0;
+  const char *fn = "dsl_kv8_attention_workspace_bytes";
+  if (check_sizes(fn, heads, page, dim, width, seqs, rows) || check_q_heads(fn, q_heads, heads, rows, max_q)) return 0;
+  if (rows == 0 || seqs == 0) return 0;
   dsl::KvCacheArgs c{};
   c.heads = (int)heads;
   c.page = (int)page;
@@ -238,13 +253,9 @@ int dsl_kv8_attention(const void *q, int64_t q_row, int64_t q_head, int64_t q_he
   int rc = check_cache(fn, &c, k_cache, v_cache, k_scale, v_scale, pages, heads, page, dim, fmt, table, table_ld,
                        width, seq_lens, starts, seqs, rows, x_dtype);
   if (rc) return rc;
-  if (q_heads <= 0 || q_heads % heads != 0 || q_heads > 1 << 20)
-    return fail(DSL_ERR_ARG, "%s: q_heads=%lld must be a multiple of heads=%lld", fn, (long long)q_heads,
-                (long long)heads);
-  if (max_q < 0) return fail(DSL_ERR_ARG, "%s: max_q must be >= 0", fn);
+  if ((rc = check_q_heads(fn, q_heads, heads, rows, max_q))) return rc;
   if (!(scale - scale == 0.f)) return fail(DSL_ERR_ARG, "%s: scale must be finite", fn);
   if (rows == 0 || seqs == 0) return ok();
-  if (rows > ((int64_t)1 << 30) / q_heads) return fail(DSL_ERR_ARG, "%s: rows x query heads must be at most 2^30", fn);
   if ((rc = check_heads(fn, "q", q, q_row, q_head, q_heads, dim)) ||
       (rc = check_heads(fn, "out", out, o_row, o_head, q_heads, dim)))
     return rc;

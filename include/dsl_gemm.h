@@ -428,7 +428,8 @@ int dsl_kv8_read(const void *k_cache, const void *v_cache, const float *k_scale,
  * them.  q and out [rows][q_heads][dim], bf16 or fp16; query head h reads cache
  * head h / (q_heads / heads).  A row that sees no token is zeros; rows of no
  * sequence are not specified.  Workspace: the partial results of a context
- * that is split over workgroups; it depends on the sizes only. */
+ * that is split over workgroups; it depends on the sizes only (the query is 0 for
+ * sizes that the call refuses). */
 int dsl_kv8_attention(const void *q, int64_t q_row, int64_t q_head, int64_t q_heads,
                       const void *k_cache, const void *v_cache, const float *k_scale,
                       const float *v_scale, int64_t pages, int64_t heads, int64_t page, int64_t dim,
