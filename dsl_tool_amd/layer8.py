@@ -22,6 +22,14 @@ from . import kvcache as KV
 from . import quant as Q
 
 
+def _product(q, w, s, sw, dtype):
+    """The int8 product in the activations' type.  Its results are bf16 or fp32, so
+    fp16 comes from fp32 by a pass of its own: one rounding, and fp16's bits."""
+    if dtype == torch.bfloat16:
+        return G.int8_gemm_packed(q, w, s, sw, out_dtype=dtype)
+    return G.int8_gemm_packed(q, w, s, sw, out_dtype=torch.float32).to(dtype)
+
+
 class Int8AttentionLayer:
     """``w_qkv [(q_heads + 2 kv_heads) * dim, hidden]`` (queries, keys, values in
     this order), ``w_out [hidden, q_heads * dim]`` and ``norm [hidden]``: bf16,
@@ -44,12 +52,12 @@ class Int8AttentionLayer:
 
     def __call__(self, x: torch.Tensor, residual: torch.Tensor | None, cache: KV.KV8Cache, seq_lens: torch.Tensor,
                  page_table: torch.Tensor, *, q_starts: torch.Tensor | None = None, max_q_len: int | None = None):
-        """The layer's output for the new tokens ``x [rows, hidden]`` and the new
-        residual: ``(out, h)``.  Their keys and values go into the cache;
-        ``seq_lens`` counts them, rows and starts are those of
-        :func:`kvcache.kv8_write`."""
+        """The layer's output for the new tokens ``x [rows, hidden]`` (bf16 or fp16)
+        and the new residual: ``(out, h)``, both of x's type, as the next layer
+        takes them.  Their keys and values go into the cache; ``seq_lens`` counts
+        them, rows and starts are those of :func:`kvcache.kv8_write`."""
         codes, scales, h = FU.add_rmsnorm_quant(x, residual, self.norm, self.eps)
-        qkv = G.int8_gemm_packed(codes, self.w_qkv, scales, self.s_qkv, out_dtype=torch.bfloat16)
+        qkv = _product(codes, self.w_qkv, scales, self.s_qkv, x.dtype)
         qkv = qkv.view(x.shape[0], self.q_heads + 2 * self.kv_heads, self.dim)
         q, k, v = qkv.split([self.q_heads, self.kv_heads, self.kv_heads], dim=1)
         if self.rotate is not None:
@@ -57,4 +65,4 @@ class Int8AttentionLayer:
         KV.kv8_write(cache, k, v, seq_lens, page_table, q_starts=q_starts, max_q_len=max_q_len)
         o = A.kv8_attention(q, cache, seq_lens, page_table, q_starts=q_starts, max_q_len=max_q_len)
         codes, scales = Q.quant_int8_rows(o.view(x.shape[0], self.q_heads * self.dim))
-        return G.int8_gemm_packed(codes, self.w_out, scales, self.s_out, out_dtype=torch.bfloat16), h
+        return _product(codes, self.w_out, scales, self.s_out, x.dtype), h

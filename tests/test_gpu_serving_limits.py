@@ -194,3 +194,33 @@ def test_blocks_of_pairs_over_the_xcds(seqs, heads):
     starts = starts_of(new)
     check_attention(randn((starts[-1], 2 * heads, 64), 997, torch.bfloat16), cache, [n + 8 for n in new], table, starts,
                     max_q_len=700)
+
+
+# ------------------------------------------------------------------- layers --
+
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
+def test_layers_chain(src):
+    """Two layers one behind the other, a prompt and a single token: the results
+    of the first enter the second.  A projection is off by the rounding of its
+    type once: fp16's are those of the fp32 product."""
+    layers = [new_layer()[0] for _ in range(2)]
+    lens = [9, 4]
+    table, pages = table_of([n + 1 for n in lens], 16, 950)
+    caches = [KV.new_kv8_cache(pages, HKV, DIM, page=16, device=DEV) for _ in layers]
+    for new, have in ((lens, lens), ([1, 1], [n + 1 for n in lens])):
+        starts = starts_of(new)
+        x, h = randn((starts[-1], HIDDEN), 951, src).to(DEV), randn((starts[-1], HIDDEN), 952, src).to(DEV)
+        args = (ints(have).to(DEV), table.to(DEV))
+        for layer, cache in zip(layers, caches):
+            before = KV.KV8Cache(*(t.clone() for t in cache))
+            codes, s, _ = FU.add_rmsnorm_quant(x, h, layer.norm)
+            qkv = G.int8_gemm_packed(codes, layer.w_qkv, s, layer.s_qkv, out_dtype=torch.float32).to(src).view(len(x), -1, DIM)
+            x, h = layer(x, h, cache, *args, q_starts=ints(starts).to(DEV), max_q_len=max(new))
+            assert x.dtype == h.dtype == src and x.isfinite().all()
+            KV.kv8_write(before, qkv[:, HQ:HQ + HKV], qkv[:, HQ + HKV:], *args, q_starts=ints(starts).to(DEV))
+            for a, b in zip(before, cache):
+                assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+            o = A.kv8_attention(qkv[:, :HQ], before, *args, q_starts=ints(starts).to(DEV), max_q_len=max(new))
+            codes, s = Q.quant_int8_rows(o.view(len(x), -1))
+            want = G.int8_gemm_packed(codes, layer.w_out, s, layer.s_out, out_dtype=torch.float32)
+            assert torch.equal(x, want.to(src))
