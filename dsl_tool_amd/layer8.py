@@ -46,7 +46,7 @@ class Int8AttentionLayer:
             raise ValueError(f"w_qkv must be [{(q_heads + 2 * kv_heads) * dim}, {hidden}] and w_out "
                              f"[{hidden}, {q_heads * dim}] (got {tuple(w_qkv.shape)}, {tuple(w_out.shape)})")
         self.q_heads, self.kv_heads, self.dim, self.eps, self.rotate = q_heads, kv_heads, dim, eps, rotate
-        self.norm = norm
+        self.norm = norm.float() if norm.dtype == torch.float16 else norm      # once: the kernels take bf16 and fp32
         self.w_qkv, self.s_qkv = Q.quant_int8_rows(w_qkv)
         self.w_out, self.s_out = Q.quant_int8_rows(w_out)
 

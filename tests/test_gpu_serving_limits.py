@@ -10,6 +10,7 @@ from dsl_tool_amd import attention as A
 from dsl_tool_amd import fused as FU
 from dsl_tool_amd import gemm as G
 from dsl_tool_amd import kvcache as KV
+from dsl_tool_amd import layer8 as L
 from dsl_tool_amd import quant as Q
 from oracle import serving as O
 from tests.test_gpu_serving import DEV, check_attention, random_cache, randn, table_of, to, within
@@ -224,3 +225,17 @@ def test_layers_chain(src):
             codes, s = Q.quant_int8_rows(o.view(len(x), -1))
             want = G.int8_gemm_packed(codes, layer.w_out, s, layer.s_out, out_dtype=torch.float32)
             assert torch.equal(x, want.to(src))
+
+
+def test_fp16_norm_weights_are_converted_once():
+    """... by the constructor, not by a launch in every call; with the same results."""
+    w = [randn((n, k), 980 + i).to(DEV) / math.sqrt(k) for i, (n, k) in
+         enumerate((((HQ + 2 * HKV) * DIM, HIDDEN), (HIDDEN, HQ * DIM)))]
+    norm = (1 + 0.1 * randn((HIDDEN,), 985)).half().to(DEV)
+    x, table, outs = randn((3, HIDDEN), 986, torch.bfloat16).to(DEV), ints([[0]]).to(DEV), []
+    for weight in (norm, norm.float()):
+        layer = L.Int8AttentionLayer(*w, weight, q_heads=HQ, kv_heads=HKV, dim=DIM)
+        assert layer.norm.dtype == torch.float32
+        cache = KV.new_kv8_cache(1, HKV, DIM, page=16, device=DEV)
+        outs.append(layer(x, None, cache, ints([3]).to(DEV), table, q_starts=ints([0, 3]).to(DEV))[0])
+    assert torch.equal(*outs)
