@@ -239,3 +239,14 @@ def test_fp16_norm_weights_are_converted_once():
         cache = KV.new_kv8_cache(1, HKV, DIM, page=16, device=DEV)
         outs.append(layer(x, None, cache, ints([3]).to(DEV), table, q_starts=ints([0, 3]).to(DEV))[0])
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("width", [3, 160])
+def test_lengths_next_to_the_largest_int(width, causal, route):
+    """A length far past the table's row: the row's tokens are seen."""
+    lens = [2 ** 31 - 1, 2 ** 31 - 40, 150]
+    table, pages = table_of([width * 16, width * 16, 40], 16, 940)
+    cache = random_cache(pages, 2, 64, 16, "int8", 941)
+    check_attention(randn((3, 4, 64), 942, torch.bfloat16), cache, lens, table, causal=causal)
+    check_attention(randn((7, 4, 64), 943, torch.bfloat16), cache, lens, table, [0, 2, 6, 7], max_q_len=4, causal=causal)
