@@ -61,6 +61,9 @@ DSL_DEV int pslot(int row, int c) {
 // memory stay in flight (__syncthreads would wait for them).
 DSL_DEV void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// 16 bits of a 64-bit word in LDS, which a thread writes and another reads whole.
+typedef uint16_t __attribute__((may_alias)) Piece16;
+
 // A wave's LDS reads but the last N (all: more false) have returned.
 template <int N>
 DSL_DEV void wait_reads(bool more) {
@@ -223,7 +226,7 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
           }
           *w = v;
         }
-        reinterpret_cast<uint16_t *>(&s_nan[tile & 1][g / VG][d])[g % VG] = (uint16_t)at;
+        reinterpret_cast<Piece16 *>(&s_nan[tile & 1][g / VG][d])[g % VG] = (Piece16)at;
         if (__any(at) && lane == 0) s_bad[tile & 3] = 1;
       }
     };
