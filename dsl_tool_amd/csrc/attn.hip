@@ -177,7 +177,8 @@ __global__ __launch_bounds__(256, rows_wgs(D, RB)) void attn_rows_kernel(const K
     int nsee = ntiles;                           // tiles that some row of the block sees
     if (p.causal) {
       const int high = s.first + ((rb + 1) * ROWS < rows ? (rb + 1) * ROWS - 1 : rows - 1) / p.group + 1;
-      nsee = high >= seen ? ntiles : high > 0 ? (high + kTile - 1) / kTile : 0;      // (seen leaves room for a tile)
+      const int h = high < seen ? high : seen;
+      nsee = h > 0 ? (h + kTile - 1) / kTile : 0;
     }
     const int t0 = r0 * chunk, t1 = split && nsee - t0 > count * chunk ? t0 + count * chunk : nsee;
     // the rows' queries, as they stand in the products
