@@ -27,10 +27,14 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, seq_lens: torch.Tensor, page
     sequence b (None: one each, row b), ``seq_lens[b]`` its cached tokens, those
     included.  Query head h reads cache head ``h // (q_heads // heads)``.  With
     ``causal`` a row sees the tokens up to its own, else all of them; a row that
-    sees none is zeros.  ``scale`` defaults to ``1/sqrt(dim)``.  ``max_q_len``
+    sees none is zeros, and rows outside every sequence are not specified (``out``'s
+    may be written).  ``scale`` defaults to ``1/sqrt(dim)``.  ``max_q_len``
     (the most new tokens of a sequence) sizes the launch and its workspace; the
     result does not depend on it, but the default, all rows where there are
-    ``q_starts``, launches many idle workgroups for a batch of prompts.
+    ``q_starts``, launches many idle workgroups for a batch of prompts (64 of 512
+    tokens, 32 heads on 8: 1000 us, 416 with it).  Contexts are split by the width
+    of ``page_table``: one much wider than the longest costs time (500 tokens behind
+    7500: 100 us, 250 with a table for 131072), and no more than that.
     """
     if out is None:
         r = N.fast().kv8_attention(q, *cache, seq_lens, page_table, q_starts, max_q_len, scale, causal)

@@ -457,7 +457,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs p, const 
   const int tid = threadIdx.x;
   const Parts<D, ROWS> part(p.ws, runs);
   const int2 w = part.where[at];
-  if (w.x < 0 || w.x >= runs) return;            // written already (or a row of no sequence)
+  // written already.  (A row of no sequence has what the workspace held: in bounds, and
+  // its result is not specified.)
+  if (w.x < 0 || w.x >= runs) return;
   const float *const ml = part.ml;
   const int first = w.x, row = w.y & (ROWS - 1), many = (w.y >> 6) - first + 1;
   const int parts = many < runs - first ? many : runs - first;

@@ -1,17 +1,19 @@
 // Attention of many query rows (prompts) over the paged 8-bit cache;
 // attn_core.h has the mathematics.
 //
-// Bound by the matrix units and the softmax's vector operations side by side:
+// Bound by the matrix units and the softmax's vector operations together:
 // per 64 tokens a wave of 32 rows (dim 128) feeds 32 32x32x16 products, about
-// 1000 cycles, and spends about as many on 2048 exponentials and their sums.  So
-// two waves share a SIMD, one's products behind the other's softmax, and the
-// codes are converted once per workgroup, not once per wave: eight waves (256
+// 1000 cycles, and spends about as many on 2048 exponentials and their sums.  Two
+// waves share a SIMD and are in phase (one barrier per tile), so the two kinds
+// overlap in part: over the prompts below matrix units are busy 31% of the time,
+// vector instructions at work 41%, CUs busy 80% (profiles/serving_counters.txt).
+// The codes are converted once per workgroup, not once per wave: eight waves (256
 // rows; 128 at dim 256) stage a tile of 8192 / D tokens in LDS as 16-bit
 // operands, one 16-byte chunk of K and of V per thread, while the tile after
 // next is on its way from memory into registers.  K and V have two tiles each
 // and a step has one barrier.  Two prompts of up to 3600 tokens, contexts of up to
-// 4600 (32 query heads on 8 of dim 128, 193 GFLOP): 254 us, 760 TFLOP/s
-// from E4M3; int8 225 us; fp16 results, whose second product runs twice, 335.
+// 4600 (32 query heads on 8 of dim 128, 193 GFLOP): 246 to 258 us by card, 750 to 785
+// TFLOP/s from E4M3; int8 233 us; fp16 results, whose second product runs twice, 331.
 // (A wave that converted its own tiles from memory, as attn.hip's do: 951.)
 //
 // S^T = K Q^T on 32x32 tiles gives a lane 16 tokens of its query row: register
@@ -111,8 +113,10 @@ void attn_prompt_kernel(const KvCacheArgs c, const AttnArgs p, const int nblk, c
   // Row blocks from the last, the longest, on.  Workgroups go to the eight XCDs,
   // and there to four shader engines, in turn: the pairs of an XCD (whose rows
   // share its L2) are rotated from row to row, or every other engine could get
-  // one sequence's and run idle where that is the shorter one (two prompts of
-  // 3600 and 2000 tokens: CUs busy 54% of the time).
+  // one sequence's and run idle where that is the shorter one.  n = pairs / 8; the
+  // pairs moved by blk, by blk / 2 and not at all, ragged prompts, us: n 2, two of
+  // 3600 on 8 heads 368 / 258 / 375, four of 2000 on 4 126 / 120 / 126; n 3 158 / 158 /
+  // 156; n 4 168 / 171 / 245; n 8 147 / 155 / 186.
   int blk = blockIdx.x / pairs, pair = blockIdx.x % pairs;
   if (pairs % 8 == 0) {
     const int n = pairs / 8, j = (blockIdx.x >> 3) % n;

@@ -155,7 +155,8 @@ def kv8_read(cache: KV8Cache, seq_lens: torch.Tensor, page_table: torch.Tensor, 
              dtype: torch.dtype = torch.bfloat16):
     """The cached tokens back in 16 bits: ``(k, v)``, each ``[total, heads,
     dim]``; rows ``starts[b] .. starts[b+1]`` (ascending) are sequence b's tokens from its
-    first on (rows past its length are zeros)."""
+    first on (rows past its length are zeros; rows outside every
+    sequence are not written)."""
     if dtype not in _SRC:
         raise TypeError(f"kv8_read: dtype must be bfloat16 or float16 (got {dtype})")
     if not isinstance(total, int) or total < 0:

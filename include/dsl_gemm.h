@@ -400,7 +400,9 @@ int dsl_add_rmsnorm_quant(const void *x, int64_t rows, int64_t cols, int64_t ldx
  * ascend.  max_q (most new tokens of a sequence) sizes the attention's launch;
  * a wrong number costs time only: under a smaller one few workgroups walk many
  * rows, under a larger one (all rows, say, for a batch of prompts) sequences x
- * heads x max_q / 256 are launched, most of which find no row. */
+ * heads x max_q / 256 are launched, most of which find no row.  width * page is
+ * what the attention's plan takes for the longest context: a table much wider
+ * than the contexts splits them too far or not at all, and costs time only. */
 
 /* Writes the new tokens' keys and values (k, v [rows][heads][dim], bf16 or
  * fp16, strides in elements, unit stride in dim).  A page's scale becomes
@@ -416,7 +418,8 @@ int dsl_kv8_write(void *k_cache, void *v_cache, float *k_scale, float *v_scale, 
 
 /* Rows starts[b] .. starts[b+1]-1 of k and v [rows][heads][dim] (out_dtype bf16
  * or fp16) become sequence b's tokens from its first on, code * scale.  Rows
- * past its length, and of pages that are none, are zeros. */
+ * past its length, and of pages that are none, are zeros; rows of no sequence are
+ * not written. */
 int dsl_kv8_read(const void *k_cache, const void *v_cache, const float *k_scale,
                  const float *v_scale, int64_t pages, int64_t heads, int64_t page, int64_t dim,
                  int fmt, const int32_t *table, int64_t table_ld, int64_t width,
@@ -426,8 +429,8 @@ int dsl_kv8_read(const void *k_cache, const void *v_cache, const float *k_scale,
 /* out = softmax(scale q k^T) v over each sequence's cached tokens; causal: new
  * token i of n sees the tokens up to its own position len - n + i, else all of
  * them.  q and out [rows][q_heads][dim], bf16 or fp16; query head h reads cache
- * head h / (q_heads / heads).  A row that sees no token is zeros; rows of no
- * sequence are not specified.  Workspace: the partial results of a context
+ * head h / (q_heads / heads).  A row that sees no token is zeros, and a NaN that it
+ * sees is one in its result; rows of no sequence are not specified (they may be written).  Workspace: the partial results of a context
  * that is split over workgroups; it depends on the sizes only (the query is 0 for
  * sizes that the call refuses). */
 int dsl_kv8_attention(const void *q, int64_t q_row, int64_t q_head, int64_t q_heads,
