@@ -43,7 +43,7 @@ W_BF16, W_F32 = 0, 1
 IN_BF16, IN_F32, IN_F16 = 0, 1, 2
 ROWQ_INT8, ROWQ_FP8, ROWQ_FP8_G128 = 0, 1, 2
 KV_INT8, KV_FP8 = 0, 1
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 
 class DslLibraryError(ImportError):
@@ -109,6 +109,19 @@ SIGNATURES = {
     "dsl_kv8_attention": (_i32, [_vp, _i64, _i64, _i64] + [_vp] * 4 + _CACHE +
                           [_vp, _i64, _i64, _i64, _i64, ctypes.c_float, _i32, _i32, _vp, _sz, _vp]),
     "dsl_kv8_attention_workspace_bytes": (_sz, [_i64] * 8),
+    "dsl_kv8_shared_attention": (_i32, [_vp, _i64, _i64, _i64] + [_vp] * 4 + _CACHE + [_vp, _vp, _i64, _i64] +
+                                 [_vp, _i64, _i64, _i64, _i64, ctypes.c_float, _i32, _i32, _vp, _sz, _vp]),
+    "dsl_kv8_shared_attention_workspace_bytes": (_sz, [_i64] * 10),
+    "dsl_kv8_fork": (_i32, [_vp] * 4 + [_i64] * 4 + [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _i64] + [_vp] * 6 +
+                     [_sz, _vp]),
+    "dsl_kv8_fork_workspace_bytes": (_sz, [_i64] * 4),
+    "dsl_kv8_compact": (_i32, [_vp] * 4 + [_i64] * 4 + [_vp, _i64, _i64, _i64] + [_vp] * 6 + [_sz, _vp]),
+    "dsl_kv8_compact_workspace_bytes": (_sz, [_i64]),
+    "dsl_rotary": (_i32, [_vp, _i64, _i64, _i64] * 2 + [_i64, _i64, _i64, _vp, _i32, _i64, _i64, _vp, _vp,
+                                                        ctypes.c_float, _i32, _i32] + [_vp, _i64, _i64] * 2 + [_vp]),
+    "dsl_token_logprobs": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _i64, _i64, ctypes.c_float, _i64] + [_vp] * 5 +
+                           [_sz, _vp]),
+    "dsl_token_logprobs_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32]),
 }
 
 _lib = None

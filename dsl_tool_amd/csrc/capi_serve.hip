@@ -50,6 +50,16 @@ int check_q_heads(const char *fn, int64_t q_heads, int64_t heads, int64_t rows, 
   return DSL_OK;
 }
 
+// Groups of sequences that share a prefix.
+int check_groups(const char *fn, int64_t q_heads, int64_t rows, int64_t groups, int64_t max_group) {
+  if (groups < 0 || max_group < 0) return fail(DSL_ERR_ARG, "%s: groups and max_group must be >= 0", fn);
+  if (groups > 65535) return fail(DSL_ERR_UNSUPPORTED, "%s: at most 65535 groups in a call", fn);
+  // (each has two parts in the workspace, and a workgroup of the join)
+  if (rows > ((int64_t)1 << 22) / q_heads)
+    return fail(DSL_ERR_UNSUPPORTED, "%s: rows x query heads must be at most 2^22", fn);
+  return DSL_OK;
+}
+
 // The cache and the sequences of a call, checked and packed.
 int check_cache(const char *fn, dsl::KvCacheArgs *c, const void *k, const void *v, const float *ks, const float *vs,
                 int64_t pages, int64_t heads, int64_t page, int64_t dim, int fmt, const int32_t *table,
@@ -277,6 +287,69 @@ int dsl_kv8_attention(const void *q, int64_t q_row, int64_t q_head, int64_t q_he
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(DSL_ERR_WORKSPACE, "%s: workspace of %zu bytes (16-B aligned) required", fn, need);
   return hip_status(dsl::launch_attn(src_of(x_dtype), c, p, static_cast<hipStream_t>(stream)), fn);
+}
+
+size_t dsl_kv8_shared_attention_workspace_bytes(int64_t heads, int64_t page, int64_t dim, int64_t width, int64_t seqs,
+                                                int64_t rows, int64_t q_heads, int64_t max_q, int64_t groups,
+                                                int64_t max_group) {
+  const char *fn = "dsl_kv8_shared_attention_workspace_bytes";
+  if (check_sizes(fn, heads, page, dim, width, seqs, rows) || check_q_heads(fn, q_heads, heads, rows, max_q) ||
+      check_groups(fn, q_heads, rows, groups, max_group))
+    return 0;
+  if (rows == 0 || seqs == 0) return 0;
+  dsl::KvCacheArgs c{};
+  c.heads = (int)heads;
+  c.page = (int)page;
+  c.dim = (int)dim;
+  c.width = (int)width;
+  c.seqs = (int)seqs;
+  c.rows = (int)rows;
+  return dsl::attn_shared_workspace_bytes(c, (int)groups, (int)q_heads, (int)(max_q < rows ? max_q : rows),
+                                          (int)(max_group < seqs ? max_group : seqs));
+}
+
+int dsl_kv8_shared_attention(const void *q, int64_t q_row, int64_t q_head, int64_t q_heads, const void *k_cache,
+                             const void *v_cache, const float *k_scale, const float *v_scale, int64_t pages,
+                             int64_t heads, int64_t page, int64_t dim, int fmt, const int32_t *table, int64_t table_ld,
+                             int64_t width, const int32_t *seq_lens, const int32_t *starts, int64_t seqs,
+                             const int32_t *group_starts, const int32_t *shared_lens, int64_t groups, int64_t max_group,
+                             void *out, int64_t o_row, int64_t o_head, int64_t rows, int64_t max_q, float scale,
+                             int causal, int x_dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  const char *fn = "dsl_kv8_shared_attention";
+  dsl::KvCacheArgs c{};
+  int rc = check_cache(fn, &c, k_cache, v_cache, k_scale, v_scale, pages, heads, page, dim, fmt, table, table_ld,
+                       width, seq_lens, starts, seqs, rows, x_dtype);
+  if (rc) return rc;
+  if ((rc = check_q_heads(fn, q_heads, heads, rows, max_q)) ||
+      (rc = check_groups(fn, q_heads, rows, groups, max_group)))
+    return rc;
+  if (!(scale - scale == 0.f)) return fail(DSL_ERR_ARG, "%s: scale must be finite", fn);
+  if (rows == 0 || seqs == 0) return ok();
+  if ((rc = check_heads(fn, "q", q, q_row, q_head, q_heads, dim)) ||
+      (rc = check_heads(fn, "out", out, o_row, o_head, q_heads, dim)))
+    return rc;
+  if (groups > 0 && (!group_starts || !shared_lens || !aligned(group_starts, 4) || !aligned(shared_lens, 4)))
+    return fail(DSL_ERR_ARG, "%s: group_starts or shared_lens is NULL or misaligned", fn);
+  dsl::AttnArgs p{};
+  p.q = q;
+  p.q_row = q_row;
+  p.q_head = q_head;
+  p.o = out;
+  p.o_row = o_row;
+  p.o_head = o_head;
+  p.q_heads = (int)q_heads;
+  p.group = (int)(q_heads / heads);
+  p.max_q = (int)(max_q < rows ? max_q : rows);
+  p.scale = scale;
+  p.causal = causal != 0;
+  p.ws = static_cast<float *>(workspace);
+  const dsl::SharedArgs h{group_starts, shared_lens, (int)groups, (int)(max_group < seqs ? max_group : seqs)};
+  // (the plan depends on the sizes alone, so the query gives the same one)
+  const size_t need = dsl_kv8_shared_attention_workspace_bytes(heads, page, dim, c.width, seqs, rows, q_heads, max_q,
+                                                               groups, max_group);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+    return fail(DSL_ERR_WORKSPACE, "%s: workspace of %zu bytes (16-B aligned) required", fn, need);
+  return hip_status(dsl::launch_attn_shared(src_of(x_dtype), c, p, h, static_cast<hipStream_t>(stream)), fn);
 }
 
 }  // extern "C"

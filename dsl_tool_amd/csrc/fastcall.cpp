@@ -711,6 +711,165 @@ PyObject *kv8_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// an int32 vector of n values (n < 0: any number) on a device, or nullptr
+const Tensor *int_vector(PyObject *o, const at::Device &d, int64_t n) {
+  const Tensor *t = gpu_tensor(o);
+  return t && t->scalar_type() == ScalarType::Int && t->dim() == 1 && t->is_contiguous() && t->device() == d &&
+                 t->numel() > 0 && (n < 0 || t->size(0) == n)
+             ? t
+             : nullptr;
+}
+
+// kv8_shared_attention(q, k_cache, v_cache, k_scale, v_scale, seq_lens, page_table, starts, max_q, scale, causal,
+//                      group_starts, shared_lens, max_group)
+PyObject *kv8_shared_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  CacheView c;
+  if (n != 14 || !PyBool_Check(a[10]) || (a[9] != Py_None && !PyFloat_CheckExact(a[9])) || !cache_view(a + 1, a + 5, &c))
+    return none();
+  const Tensor *q = gpu_tensor(a[0]);
+  if (!head_rows(q, c) || q->size(1) % c.heads != 0) return none();
+  const Tensor *sl = int_vector(a[12], q->device(), -1);
+  const Tensor *gs = sl ? int_vector(a[11], q->device(), sl->size(0) + 1) : nullptr;
+  if (!gs) return none();
+  const int dt = src_code(q->scalar_type());
+  const int64_t rows = q->size(0), hq = q->size(1), most = most_new(a[8], c, rows), groups = sl->size(0);
+  const int64_t group = a[13] == Py_None ? c.seqs : most_new(a[13], c, rows);
+  if (dt < 0 || most < 0 || group < 0 || (!c.starts && rows != c.seqs)) return none();
+  const double sc = a[9] == Py_None ? 1.0 / std::sqrt((double)c.dim) : PyFloat_AS_DOUBLE(a[9]);
+  const bool causal = a[10] == Py_True;
+  Tensor o;
+  const bool ok = on_device(*q, [&] {
+    o = empty({rows, hq, c.dim}, q->scalar_type(), *q);
+    const size_t nb = dsl_kv8_shared_attention_workspace_bytes(c.heads, c.page, c.dim, c.width, c.seqs, rows, hq, most,
+                                                               groups, group);
+    const Tensor ws = bytes((int64_t)nb, *q);
+    return dsl_kv8_shared_attention(ptr(*q), q->stride(0), q->stride(1), hq, DSL_CACHE(c), ptr<int32_t>(*gs),
+                                    ptr<int32_t>(*sl), groups, group, ptr(o), hq * c.dim, c.dim, rows, most, (float)sc,
+                                    causal, dt, ptr(ws), nb, stream_of(*q)) == DSL_OK;
+  });
+  return ok ? THPVariable_Wrap(o) : none();
+  END_HANDLE_TH_ERRORS
+}
+
+// kv8_fork(k_cache, v_cache, k_scale, v_scale, seq_lens, page_table, parents, refs, new)
+PyObject *kv8_fork(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  CacheView c;
+  PyObject *const seqs[3] = {n == 9 ? a[4] : nullptr, n == 9 ? a[5] : nullptr, Py_None};
+  if (n != 9 || !cache_view(a, seqs, &c)) return none();
+  const at::Device d = c.k->device();
+  const Tensor *parents = int_vector(a[6], d, -1), *refs = int_vector(a[7], d, c.pages);
+  if (!parents || !refs) return none();
+  const int64_t children = parents->size(0);
+  const Tensor *more = nullptr;
+  int64_t all = 0;
+  if (PyLong_CheckExact(a[8])) {
+    int over = 0;
+    all = PyLong_AsLongLongAndOverflow(a[8], &over);
+    if (over || all < 0 || all >= (int64_t)1 << 31) return none();
+  } else if (!(more = int_vector(a[8], d, children))) {
+    return none();
+  }
+  Tensor lens, table, counts, lacking;
+  const bool ok = on_device(*c.k, [&] {
+    lens = empty({children}, ScalarType::Int, *c.k);
+    table = empty({children, c.width}, ScalarType::Int, *c.k);
+    counts = empty({c.pages}, ScalarType::Int, *c.k);
+    lacking = empty({1}, ScalarType::Int, *c.k);
+    const size_t nb = dsl_kv8_fork_workspace_bytes(c.seqs, c.width, children, c.pages);
+    const Tensor ws = bytes((int64_t)nb, *c.k);
+    return dsl_kv8_fork(ptr(*c.k), ptr(*c.v), ptr<float>(*c.ks), ptr<float>(*c.vs), c.pages, c.heads, c.page, c.dim,
+                        ptr<int32_t>(*c.table), c.ld, c.width, ptr<int32_t>(*c.lens), c.seqs, ptr<int32_t>(*parents),
+                        more ? ptr<int32_t>(*more) : nullptr, all, children, ptr<int32_t>(*refs), ptr<int32_t>(lens),
+                        ptr<int32_t>(table), ptr<int32_t>(counts), ptr<int32_t>(lacking), ptr(ws), nb,
+                        stream_of(*c.k)) == DSL_OK;
+  });
+  return ok ? pack({lens, table, counts, lacking}) : none();
+  END_HANDLE_TH_ERRORS
+}
+
+// [rows][heads][dim] that the rotary kernel reads in place
+bool turned_heads(const Tensor *t) {
+  return t && t->dim() == 3 && t->numel() > 0 && t->stride(2) == 1 && t->stride(1) >= t->size(2) && t->stride(0) >= 0;
+}
+
+// rotary(q, k or None, positions, freqs, axis_of or None, adjacent, magnitude)
+PyObject *rotary(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7 || !PyBool_Check(a[5]) || !PyFloat_CheckExact(a[6])) return none();
+  const Tensor *q = gpu_tensor(a[0]), *k = a[1] == Py_None ? nullptr : gpu_tensor(a[1]);
+  const Tensor *pos = gpu_tensor(a[2]), *freqs = gpu_tensor(a[3]);
+  if (!turned_heads(q) || (a[1] != Py_None && !turned_heads(k)) || !pos || !freqs) return none();
+  const at::Device d = q->device();
+  const int64_t rows = q->size(0), dim = q->size(2);
+  const int dt = src_code(q->scalar_type());
+  if (dt < 0 || (k && (k->scalar_type() != q->scalar_type() || k->device() != d || k->size(0) != rows || k->size(2) != dim)))
+    return none();
+  const bool wide = pos->scalar_type() == ScalarType::Long;
+  if ((!wide && pos->scalar_type() != ScalarType::Int) || pos->device() != d || !pos->is_contiguous() ||
+      pos->numel() == 0 || (pos->dim() != 1 && pos->dim() != 2) || pos->size(-1) != rows)
+    return none();
+  const int64_t axes = pos->dim() == 2 ? pos->size(0) : 1;
+  if (freqs->scalar_type() != ScalarType::Double || freqs->dim() != 1 || !freqs->is_contiguous() || freqs->device() != d ||
+      freqs->numel() == 0)
+    return none();
+  const Tensor *axis = a[4] == Py_None ? nullptr : int_vector(a[4], d, freqs->size(0));
+  if (a[4] != Py_None && !axis) return none();
+  Tensor yq, yk;
+  const bool ok = on_device(*q, [&] {
+    yq = empty({rows, q->size(1), dim}, q->scalar_type(), *q);
+    if (k) yk = empty({rows, k->size(1), dim}, q->scalar_type(), *q);
+    return dsl_rotary(ptr(*q), q->stride(0), q->stride(1), q->size(1), k ? ptr(*k) : nullptr, k ? k->stride(0) : 0,
+                      k ? k->stride(1) : 0, k ? k->size(1) : 0, rows, dim, freqs->size(0), ptr(*pos), wide, rows, axes,
+                      axis ? ptr<int32_t>(*axis) : nullptr, ptr<double>(*freqs), (float)PyFloat_AS_DOUBLE(a[6]),
+                      a[5] == Py_True, dt, ptr(yq), q->size(1) * dim, dim, k ? ptr(yk) : nullptr,
+                      k ? k->size(1) * dim : 0, k ? dim : 0, stream_of(*q)) == DSL_OK;
+  });
+  if (!ok) return none();
+  if (k) return pack({yq, yk});
+  PyObject *r = PyTuple_New(2);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(yq));
+  Py_INCREF(Py_None);
+  PyTuple_SET_ITEM(r, 1, Py_None);
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// token_logprobs(logits, ids, top, scale)
+PyObject *token_logprobs(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4 || !PyLong_CheckExact(a[2]) || !PyFloat_CheckExact(a[3])) return none();
+  const Tensor *x = gpu_tensor(a[0]), *ids = gpu_tensor(a[1]);
+  if (!x || !ids || x->dim() != 2 || x->numel() == 0 || x->stride(1) != 1 || x->stride(0) < x->size(1)) return none();
+  const ScalarType t = x->scalar_type();
+  const int dt = t == ScalarType::Float ? DSL_IN_F32 : src_code(t);
+  const int64_t rows = x->size(0), vocab = x->size(1);
+  if (dt < 0 || ids->scalar_type() != ScalarType::Int || !ids->is_contiguous() || ids->numel() == 0 ||
+      (ids->dim() != 1 && ids->dim() != 2) || ids->size(0) != rows || ids->device() != x->device())
+    return none();
+  int over = 0;
+  const long long top = PyLong_AsLongLongAndOverflow(a[2], &over);
+  if (over || top < 0 || top > vocab) return none();
+  const int64_t n_ids = ids->numel() / rows;
+  Tensor logp, entropy, tl, ti;
+  const bool ok = on_device(*x, [&] {
+    logp = empty(ids->sizes(), ScalarType::Float, *x);
+    entropy = empty({rows}, ScalarType::Float, *x);
+    tl = empty({rows, (int64_t)top}, ScalarType::Float, *x);
+    ti = empty({rows, (int64_t)top}, ScalarType::Int, *x);
+    const size_t nb = dsl_token_logprobs_workspace_bytes(rows, vocab, top, dt);
+    Tensor ws;
+    if (nb) ws = bytes((int64_t)nb, *x);
+    return dsl_token_logprobs(ptr(*x), rows, vocab, x->stride(0), dt, ptr<int32_t>(*ids), n_ids, n_ids,
+                              (float)PyFloat_AS_DOUBLE(a[3]), top, ptr<float>(logp), ptr<float>(entropy), ptr<float>(tl),
+                              ptr<int32_t>(ti), nb ? ptr(ws) : nullptr, nb, stream_of(*x)) == DSL_OK;
+  });
+  return ok ? pack({logp, entropy, tl, ti}) : none();
+  END_HANDLE_TH_ERRORS
+}
+
 #define DSL_FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {DSL_FN(quant_fp8_tensor), DSL_FN(quant_fp8_blocks), DSL_FN(quant_mxfp4),
                          DSL_FN(quant_nvfp4),      DSL_FN(fp8_gemm),         DSL_FN(fp4_gemm),
@@ -718,6 +877,7 @@ PyMethodDef methods[] = {DSL_FN(quant_fp8_tensor), DSL_FN(quant_fp8_blocks), DSL
                          DSL_FN(swiglu_quant),     DSL_FN(moe_projection),   DSL_FN(lora_gemm),
                          DSL_FN(quant_fp8_rows_batched), DSL_FN(int8_gemm),        DSL_FN(quant_int8_rows), DSL_FN(add_rmsnorm_quant),
                          DSL_FN(kv8_write),        DSL_FN(kv8_read),         DSL_FN(kv8_attention),
+                         DSL_FN(kv8_shared_attention), DSL_FN(kv8_fork),     DSL_FN(rotary),           DSL_FN(token_logprobs),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "dsl_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

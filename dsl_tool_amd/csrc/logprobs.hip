@@ -1,0 +1,353 @@
+// Log probabilities of given tokens, the entropy and the largest logits of a
+// row, in one pass over its logits.
+//
+// With z = scale x log2(e) in powers of two, m = max z, S = sum 2^(z - m) and
+// T = sum (z - m) 2^(z - m):
+//   logp(t) = ((z_t - m) - log2 S) ln 2,  H = (log2 S - T / S) ln 2.
+// Every thread keeps m, S and T of its elements in fp32 (S and T join in 64 bits);
+// z - m is one fused product, so its error is that of scale log2(e)'s rounding.
+// A masked token, x = -inf, has no part in either sum; a row of nothing else gives
+// entropy 0 and -inf for every token; NaN or +inf give NaN.
+//
+// The largest: by value, then by lowest index, as 64-bit keys (the value's order,
+// then the index turned round) that no two elements share.  In the pass a thread
+// only notes which of its 16-byte words holds its largest value.  Of these, one
+// element per thread, the `top`-th largest is a bound that no element of the
+// result lies below, and only threads whose own largest reaches it can hold any: as many
+// threads as `top`, so their words are read once more and everything else is not.
+// Keys are sorted 64 to a wave, and sorted runs are merged, best 64 kept.
+//
+// Bound by the logits' bytes.  Few rows are split over workgroups, and a second
+// launch joins the parts.
+#include "common.h"
+#include "generate_args.h"
+#include "kv_core.h"
+#include "launch.h"
+
+namespace dsl {
+
+constexpr int kLogThreads = 512, kLogWaves = kLogThreads / 64;
+constexpr float kLog2eF = 1.44269504088896341f;
+constexpr double kLn2 = 0.693147180559945309417;
+
+// ------------------------------------------------------------------- keys --
+DSL_DEV uint64_t key_of(float v, int index) {
+  v = v == v ? v + 0.f : -INFINITY;              // -0 is 0; NaN is no candidate before the others
+  const uint32_t u = f2u(v);
+  return (uint64_t)(u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u)) << 32 | (uint32_t)~(uint32_t)index;
+}
+DSL_DEV int index_of(uint64_t key) { return (int)~(uint32_t)key; }
+DSL_DEV float value_of(uint64_t key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return u2f(u ^ ((u >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
+// One step of a bitonic network over the wave: the larger of a pair to the lane
+// with `up`'s bit.
+DSL_DEV uint64_t exchange(uint64_t k, int j, bool larger) {
+  const uint64_t o = __shfl_xor((unsigned long long)k, j);
+  return (o > k) == larger ? o : k;
+}
+// The wave's keys in falling order.
+DSL_DEV uint64_t sort_wave(uint64_t k) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int n = 2; n <= 64; n <<= 1)
+#pragma unroll
+    for (int j = n >> 1; j > 0; j >>= 1) k = exchange(k, j, ((lane & j) == 0) == ((lane & n) == 0));
+  return k;
+}
+// The best 64 of two runs in falling order, in falling order; b reversed: lane l
+// holds b[63 - l].
+DSL_DEV uint64_t merge_reversed(uint64_t a, uint64_t b) {
+  const int lane = threadIdx.x & 63;
+  uint64_t k = a > b ? a : b;
+#pragma unroll
+  for (int j = 32; j > 0; j >>= 1) k = exchange(k, j, (lane & j) == 0);
+  return k;
+}
+DSL_DEV uint64_t merge_wave(uint64_t a, uint64_t b) {
+  return merge_reversed(a, __shfl((unsigned long long)b, 63 - (int)(threadIdx.x & 63)));
+}
+// The best 64 of all waves' runs, in runs[0 .. 63] and in wave 0's lanes.
+template <int NW>
+DSL_DEV uint64_t merge_waves(uint64_t k, uint64_t *runs) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __syncthreads();                               // the last readers of runs
+  runs[wave * 64 + lane] = k;
+#pragma unroll
+  for (int half = NW / 2; half > 0; half >>= 1) {
+    __syncthreads();
+    if (wave < half) {
+      k = merge_reversed(k, runs[(wave + half) * 64 + 63 - lane]);
+      runs[wave * 64 + lane] = k;
+    }
+  }
+  __syncthreads();
+  return k;
+}
+
+// ------------------------------------------------------------------- sums --
+struct Sums {
+  float m;
+  double s, t;
+};
+DSL_DEV Sums join_sums(const Sums &a, const Sums &b) {
+  Sums r;
+  r.m = fmaxf(a.m, b.m);
+  // of a part without a maximum: no sums, or nothing but NaN
+  const float da = a.m == -INFINITY ? 0.f : a.m - r.m, db = b.m == -INFINITY ? 0.f : b.m - r.m;
+  const double fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+  r.s = a.s * fa + b.s * fb;
+  // (a difference past every exponent leaves nothing, and times a sum of 0 no NaN)
+  r.t = (a.t + (double)fmaxf(da, -1000.f) * a.s) * fa + (b.t + (double)fmaxf(db, -1000.f) * b.s) * fb;
+  return r;
+}
+DSL_DEV Sums sums_of_wave(Sums v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    Sums u;
+    u.m = __shfl_xor(v.m, o);
+    u.s = __shfl_xor(v.s, o);
+    u.t = __shfl_xor(v.t, o);
+    v = join_sums(v, u);
+  }
+  return v;
+}
+template <int NW>
+DSL_DEV Sums sums_of_group(Sums v, Sums *sh) {
+  v = sums_of_wave(v);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = sh[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) v = join_sums(v, sh[w]);
+  return v;
+}
+
+template <int SRC>
+DSL_DEV float logit(const void *x, int64_t at) {
+  if constexpr (SRC == SRC_F32) return static_cast<const float *>(x)[at];
+  else return widen<SRC>(static_cast<const uint16_t *>(x)[at]);
+}
+template <int SRC>
+constexpr int kWord = SRC == SRC_F32 ? 4 : 8;    // logits of 16 bytes
+template <int SRC>
+DSL_DEV void widen_word(const uint4 &v, float *f) {
+  if constexpr (SRC == SRC_F32) {
+    f[0] = u2f(v.x);
+    f[1] = u2f(v.y);
+    f[2] = u2f(v.z);
+    f[3] = u2f(v.w);
+  } else {
+    widen8s<SRC>(v, f);
+  }
+}
+
+// What a row's results are made of.
+template <int SRC>
+DSL_DEV void write_row(const LogprobArgs &p, int row, const Sums &v, uint64_t key, int tid, int threads) {
+  const bool none = v.s == 0.0;                  // no token has a probability
+  const double ls = none ? 0.0 : log(v.s) / kLn2;
+  const float c = p.scale * kLog2eF;
+  auto logp = [&](float x) {
+    if (none || x == -INFINITY) return v.s == v.s ? -INFINITY : __builtin_nanf("");
+    return (float)(((double)__builtin_fmaf(x, c, -v.m) - ls) * kLn2);
+  };
+  for (int i = tid; i < p.n_ids; i += threads) {
+    const int id = p.ids[(int64_t)row * p.ids_ld + i];
+    p.logp[(int64_t)row * p.n_ids + i] =
+        logp(id >= 0 && id < p.vocab ? logit<SRC>(p.x, (int64_t)row * p.ld + id) : -INFINITY);
+  }
+  if (tid == 0) {
+    const double h = none ? 0.0 : (ls - v.t / v.s) * kLn2;
+    p.entropy[row] = (float)(h < 0.0 ? 0.0 : h);
+  }
+  if (tid < p.top) {
+    p.top_logp[(int64_t)row * p.top + tid] = logp(value_of(key));
+    p.top_ids[(int64_t)row * p.top + tid] = index_of(key);
+  }
+}
+
+// Parts of split rows: [part] sums, then [part][top] keys.
+struct LogParts {
+  Sums *sums;
+  uint64_t *keys;
+  DSL_HD LogParts(void *ws, int64_t parts) : sums(static_cast<Sums *>(ws)), keys(reinterpret_cast<uint64_t *>(sums + parts)) {}
+};
+
+template <int SRC, bool TOP>
+__global__ __launch_bounds__(kLogThreads) void logprob_kernel(const LogprobArgs p, const int splits) {
+  constexpr int E = kWord<SRC>, NT = kLogThreads, U = 4;
+  __shared__ Sums s_sums[kLogWaves];
+  __shared__ uint64_t s_runs[TOP ? NT : 1], s_cand[TOP ? NT * E + 64 : 1];
+  __shared__ int s_count;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int row = (int)(blockIdx.x / (unsigned)splits), split = (int)(blockIdx.x % (unsigned)splits);
+  constexpr int B = SRC == SRC_F32 ? 4 : 2;
+  const uint8_t *x = static_cast<const uint8_t *>(p.x) + (int64_t)row * p.ld * B;
+  // the row: elements up to the first whole word, words, elements behind them
+  int head = (int)((-reinterpret_cast<uintptr_t>(x) & 15) / B);
+  head = head < p.vocab ? head : p.vocab;
+  const int words = (p.vocab - head) / E, tail = head + words * E;
+  const int w0 = (int)((int64_t)words * split / splits), w1 = (int)((int64_t)words * (split + 1) / splits);
+  const uint4 *xw = reinterpret_cast<const uint4 *>(x + (int64_t)head * B);
+  const float c = p.scale * kLog2eF;
+
+  float m = -INFINITY, s = 0.f, t = 0.f, best = -INFINITY;
+  int bestw = w0 + tid < w1 ? w0 + tid : -1;
+  auto raise = [&](float top) __attribute__((always_inline)) {
+    if (top > m) {
+      const float d = m - top;                   // -inf at first
+      const float f = __builtin_amdgcn_exp2f(d);
+      t = (t + fmaxf(d, -1000.f) * s) * f;
+      s *= f;
+      m = top;
+    }
+  };
+  auto take = [&](float v, float less) __attribute__((always_inline)) {
+    const float d = __builtin_fmaf(v, c, less);
+    const float e = __builtin_amdgcn_exp2f(d);
+    s += e;
+    t = __builtin_fmaf(e, fmaxf(d, -1000.f), t);
+  };
+  auto word = [&](const uint4 &raw, int w) __attribute__((always_inline)) {
+    float f[E], top;
+    widen_word<SRC>(raw, f);
+    top = f[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) top = fmaxf(top, f[e]);
+    if (TOP && top > best) {
+      best = top;
+      bestw = w;
+    }
+    raise(top * c);
+    const float less = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+    for (int e = 0; e < E; ++e) take(f[e], less);
+  };
+  int w = w0 + tid;
+  for (; w + (U - 1) * NT < w1; w += U * NT) {
+    uint4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = xw[w + u * NT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) word(v[u], w + u * NT);
+  }
+  for (; w < w1; w += NT) word(xw[w], w);
+  // the elements of no whole word: a thread each
+  int edge = -1;
+  if (split == 0 && tid < head) edge = tid;
+  if (split == splits - 1 && tid >= 64 && tail + tid - 64 < p.vocab) edge = tail + tid - 64;
+  float edgev = 0.f;
+  if (edge >= 0) {
+    edgev = logit<SRC>(x, edge);
+    raise(edgev * c);
+    take(edgev, m == -INFINITY ? 0.f : -m);
+  }
+  const Sums all = sums_of_group<kLogWaves>(Sums{m, s, t}, s_sums);
+
+  uint64_t kept = 0;                             // the wave's best, falling
+  if constexpr (TOP) {
+    auto read = [&](int at, float *f) __attribute__((always_inline)) {
+      widen_word<SRC>(xw[at], f);
+    };
+    uint64_t mine = 0;
+    if (bestw >= 0) {
+      float f[E];
+      read(bestw, f);
+#pragma unroll
+      for (int e = E - 1; e >= 0; --e) {
+        const uint64_t k = key_of(f[e], head + bestw * E + e);
+        mine = k > mine ? k : mine;
+      }
+    }
+    merge_waves<kLogWaves>(sort_wave(mine), s_runs);
+    const uint64_t bound = s_runs[p.top - 1];
+    int held = 0;                                // threads that can hold one: s_runs[0 .. held)
+    for (int i = 0; i < p.top; ++i) held += s_runs[i] != 0;
+    const int each = (w1 - w0 + NT - 1) / NT;    // words of a thread
+    const int items = held * each;
+    for (int i0 = 0; i0 < items || i0 == 0; i0 += NT) {
+      if (tid == 0) s_count = 0;
+      __syncthreads();
+      auto offer = [&](uint64_t k) __attribute__((always_inline)) {
+        if (k >= bound) s_cand[atomicAdd(&s_count, 1)] = k;
+      };
+      if (i0 == 0 && edge >= 0) offer(key_of(edgev, edge));
+      const int i = i0 + tid;
+      if (i < items) {
+        const int owner = ((index_of(s_runs[i / each]) - head) / E - w0) % NT, at = w0 + owner + i % each * NT;
+        if (at < w1) {
+          float f[E];
+          read(at, f);
+#pragma unroll
+          for (int e = 0; e < E; ++e) offer(key_of(f[e], head + at * E + e));
+        }
+      }
+      __syncthreads();
+      const int n = s_count;
+      for (int j = wave * 64; j < n; j += NT) kept = merge_wave(kept, sort_wave(j + lane < n ? s_cand[j + lane] : 0));
+      __syncthreads();                           // s_count's readers
+    }
+    kept = merge_waves<kLogWaves>(kept, s_runs);
+  }
+  if (splits > 1) {
+    const LogParts part(p.ws, (int64_t)p.rows * splits);
+    if (tid == 0) part.sums[blockIdx.x] = all;
+    if (TOP && tid < p.top) part.keys[(int64_t)blockIdx.x * p.top + tid] = kept;
+  } else {
+    write_row<SRC>(p, row, all, kept, tid, NT);
+  }
+}
+
+// A workgroup per row: its parts' sums and keys.
+template <int SRC>
+__global__ __launch_bounds__(256) void logprob_join_kernel(const LogprobArgs p, const int splits) {
+  __shared__ Sums s_sums[4];
+  __shared__ uint64_t s_runs[256];
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const LogParts part(p.ws, (int64_t)p.rows * splits);
+  Sums v{-INFINITY, 0.0, 0.0};
+  for (int i = tid; i < splits; i += 256) v = join_sums(v, part.sums[(int64_t)row * splits + i]);
+  v = sums_of_group<4>(v, s_sums);
+  uint64_t kept = 0;
+  if (p.top) {
+    const int n = splits * p.top;
+    const uint64_t *keys = part.keys + (int64_t)row * n;
+    for (int j = wave * 64; j < n; j += 256) kept = merge_wave(kept, sort_wave(j + lane < n ? keys[j + lane] : 0));
+    kept = merge_waves<4>(kept, s_runs);
+  }
+  write_row<SRC>(p, row, v, kept, tid, 256);
+}
+
+// Parts of a row: two workgroups per CU, of 4096 words' worth of threads' loads at least.
+static int logprob_splits(int src, int rows, int vocab) {
+  const int words = vocab / (src == SRC_F32 ? 4 : 8);
+  int64_t s = (2 * (int64_t)device_cu_count() + rows - 1) / (rows > 0 ? rows : 1);
+  const int64_t most = words / (2 * kLogThreads);
+  s = s < most ? s : most;
+  return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
+}
+size_t logprob_workspace_bytes(int src, int rows, int vocab, int top) {
+  const int splits = logprob_splits(src, rows, vocab);
+  return splits > 1 ? (size_t)rows * splits * (sizeof(Sums) + top * sizeof(uint64_t)) : 0;
+}
+
+template <int SRC>
+static hipError_t launch_logprobs_src(const LogprobArgs &p, hipStream_t st) {
+  const int splits = logprob_splits(SRC, p.rows, p.vocab);
+  const unsigned grid = (unsigned)p.rows * (unsigned)splits;
+  if (p.top) logprob_kernel<SRC, true><<<grid, kLogThreads, 0, st>>>(p, splits);
+  else logprob_kernel<SRC, false><<<grid, kLogThreads, 0, st>>>(p, splits);
+  if (splits > 1) logprob_join_kernel<SRC><<<(unsigned)p.rows, 256, 0, st>>>(p, splits);
+  return hipGetLastError();
+}
+hipError_t launch_logprobs(int src, const LogprobArgs &p, hipStream_t st) {
+  if (p.rows == 0) return hipSuccess;
+  if (src == SRC_BF16) return launch_logprobs_src<SRC_BF16>(p, st);
+  if (src == SRC_F16) return launch_logprobs_src<SRC_F16>(p, st);
+  return launch_logprobs_src<SRC_F32>(p, st);
+}
+
+}  // namespace dsl

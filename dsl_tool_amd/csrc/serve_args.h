@@ -78,4 +78,14 @@ constexpr int kPromptThreads = 512;              // of a workgroup
 hipError_t launch_attn_prompt(int src, const KvCacheArgs &c, const AttnArgs &p, int nblk, int nsplit, int part, hipStream_t st);
 hipError_t launch_attn(int src, const KvCacheArgs &c, const AttnArgs &p, hipStream_t st);
 
+// Groups of sequences that share a prefix (attn_shared.hip): sequences groups[g] ..
+// groups[g + 1] - 1 hold the same pages for their first shared[g] tokens.
+struct SharedArgs {
+  const int32_t *groups, *shared;        // [n + 1], [n]
+  int n;
+  int most;              // most sequences of a group (sizes the launch)
+};
+size_t attn_shared_workspace_bytes(const KvCacheArgs &c, int groups, int q_heads, int max_q, int max_group);
+hipError_t launch_attn_shared(int src, const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, hipStream_t st);
+
 }  // namespace dsl

@@ -10,6 +10,14 @@ code stands for ``code * scale[page, head]``:
     o = attention.kv8_attention(q, cache, seq_lens, page_table)
     k, v = kv8_read(cache, seq_lens, page_table, starts, total)
 
+Who holds a page is counted on the device too: ``refs [pages]`` is the number
+of table entries that name it (0: free), and every step's sequences are made
+from the last step's, forked, dropped or grown:
+
+    refs = torch.zeros(pages, dtype=torch.int32, device="cuda")
+    seq_lens, page_table, refs, lacking = kv8_fork(cache, seq_lens, page_table, parents, refs, new=1)
+    page_table, refs, moved, live = kv8_compact(cache, page_table, refs)
+
 ``seq_lens`` counts a sequence's tokens with the new ones, which are its last.
 Lengths, starts and the table are int32 tensors on the device and nothing is
 copied to the host: page numbers outside the cache, tokens past a table row
@@ -173,3 +181,93 @@ def kv8_read(cache: KV8Cache, seq_lens: torch.Tensor, page_table: torch.Tensor, 
         N.call("dsl_kv8_read", *args, N.ptr(k), N.ptr(v), total, _SRC[dtype], N.stream_of(k.device))
     del alive
     return k, v
+
+
+class KV8Fork(NamedTuple):
+    seq_lens: torch.Tensor       # [children] int32, the new tokens counted
+    page_table: torch.Tensor     # [children, width] int32, -1 where there is no page
+    refs: torch.Tensor           # [pages] int32
+    lacking: torch.Tensor        # [1] int32: pages asked for and not there
+
+
+class KV8Compact(NamedTuple):
+    page_table: torch.Tensor     # [seqs, width] int32
+    refs: torch.Tensor           # [pages] int32
+    moved: torch.Tensor          # [pages] int32: a page's new number, -1 where it was free
+    live: torch.Tensor           # [1] int32: pages 0 .. live - 1 are in use
+
+
+def _pool_args(fn: str, cache: KV8Cache, seq_lens, page_table, refs):
+    """The cache's, table's and counts' arguments, checked and converted."""
+    args, (lens, table, _) = cache_args(fn, cache, seq_lens, page_table, None)
+    refs = _ints(refs, "refs", cache.k.device).contiguous()
+    if refs.dim() != 1 or refs.shape[0] != cache.k.shape[0]:
+        raise ValueError(f"{fn}: refs must be [{cache.k.shape[0]}], a count for each page")
+    pages, heads, page, dim, _, tptr, ld, width = args[4:12]
+    return args[:4] + [pages, heads, page, dim, tptr, ld, width], lens, table, refs
+
+
+def kv8_fork(cache: KV8Cache, seq_lens: torch.Tensor, page_table: torch.Tensor, parents: torch.Tensor,
+             refs: torch.Tensor, *, new: int | torch.Tensor = 0) -> KV8Fork:
+    """The next step's sequences: child c continues sequence ``parents[c]``
+    (``[children]`` int32; outside the sequences: an empty one), and sequences
+    that no child continues are dropped, their pages free.
+
+    Children share their parent's full pages; its partly filled page stays with
+    its first child, and every other child gets a copy.  Each gets pages for
+    ``new`` more tokens (a number, or ``[children]`` int32), which the result's
+    ``seq_lens`` count: they go to :func:`kv8_write` and attention as they are.
+    Fresh pages are taken in order of their numbers, by child and position.
+    Lengths, table and counts are new tensors; of what the call is given only free
+    pages of the cache change, so a step with ``lacking > 0`` (their
+    entries are -1 and tokens there are skipped) can be made again with
+    fewer children.  A sequence's partly filled page must be its own; other
+    holders of a page (a kept prefix) count in ``refs`` by their own additions.
+    A sequence starts as a child of none with ``new`` tokens.
+    """
+    r = N.fast().kv8_fork(*cache, seq_lens, page_table, parents, refs, new)
+    if r is not None:
+        return KV8Fork(*r)
+    more = new if isinstance(new, torch.Tensor) else None
+    if more is None and (not isinstance(new, int) or isinstance(new, bool) or not 0 <= new < 1 << 31):
+        raise ValueError(f"kv8_fork: new must be a number >= 0 or a tensor (got {new!r})")
+    args, lens, table, refs = _pool_args("kv8_fork", cache, seq_lens, page_table, refs)
+    dev = cache.k.device
+    parents = _ints(parents, "parents", dev).contiguous()
+    if parents.dim() != 1:
+        raise ValueError("kv8_fork: parents must be [children]")
+    children = parents.shape[0]
+    if more is not None:
+        more = _ints(more, "new", dev).contiguous()
+        if more.shape != parents.shape:
+            raise ValueError("kv8_fork: new must be [children]")
+    width = table.shape[1]
+    out = KV8Fork(*(torch.empty(s, dtype=torch.int32, device=dev)
+                    for s in ((children,), (children, width), refs.shape, (1,))))
+    with torch.cuda.device(dev):
+        nb = N.lib().dsl_kv8_fork_workspace_bytes(lens.shape[0], width, children, refs.shape[0])
+        ws = torch.empty(-(-nb // 4), dtype=torch.int32, device=dev)
+        N.call("dsl_kv8_fork", *args, N.ptr(lens), lens.shape[0], N.ptr(parents), N.ptr(more),
+               0 if more is not None else new, children, N.ptr(refs), *(N.ptr(t) for t in out), N.ptr(ws), nb,
+               N.stream_of(dev))
+    return out
+
+
+def kv8_compact(cache: KV8Cache, page_table: torch.Tensor, refs: torch.Tensor) -> KV8Compact:
+    """The pages that ``refs`` counts move to the cache's front, so that what
+    lies behind them can be given up: live pages past the number of live ones
+    go, in order, to the free pages before it, and the rest stay.  Table and
+    counts come in the new numbers, as new tensors; ``moved`` renumbers whatever
+    else holds pages."""
+    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
+        raise ValueError("kv8_compact: page_table must be [seqs, width]")
+    seqs = page_table.shape[0]
+    # (lengths are not looked at: any of the right number and device)
+    args, _, table, refs = _pool_args("kv8_compact", cache, page_table.new_empty(seqs, dtype=torch.int32), page_table, refs)
+    dev, width = cache.k.device, table.shape[1]
+    out = KV8Compact(*(torch.empty(s, dtype=torch.int32, device=dev) for s in ((seqs, width), refs.shape, refs.shape, (1,))))
+    with torch.cuda.device(dev):
+        nb = N.lib().dsl_kv8_compact_workspace_bytes(refs.shape[0])
+        ws = torch.empty(-(-nb // 4), dtype=torch.int32, device=dev)
+        N.call("dsl_kv8_compact", *args, seqs, N.ptr(refs), *(N.ptr(t) for t in out), N.ptr(ws), nb, N.stream_of(dev))
+    return out

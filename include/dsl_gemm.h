@@ -445,6 +445,95 @@ size_t dsl_kv8_attention_workspace_bytes(int64_t heads, int64_t page, int64_t di
                                          int64_t seqs, int64_t rows, int64_t q_heads,
                                          int64_t max_q);
 
+/* ------------------------------------------- several continuations --
+ * What generates samples, beams or scored candidates of a prompt beside the
+ * operators above.  The reference has none of it.
+ */
+
+/* dsl_kv8_attention where sequences group_starts[g] .. group_starts[g+1]-1
+ * (ascending) hold the same pages for their first shared_lens[g] tokens: that prefix,
+ * cut to whole pages, is read once for the group instead of once for each
+ * sequence, from the table row of its first sequence that is as long (else its
+ * longest).  The result is dsl_kv8_attention's but for the order of the sums.
+ * Sequences outside every group share nothing.  max_group (most sequences of a group)
+ * sizes the launch with max_q; wrong numbers cost time only.  rows x q_heads at most
+ * 2^22; the workspace is never empty. */
+int dsl_kv8_shared_attention(const void *q, int64_t q_row, int64_t q_head, int64_t q_heads,
+                             const void *k_cache, const void *v_cache, const float *k_scale,
+                             const float *v_scale, int64_t pages, int64_t heads, int64_t page,
+                             int64_t dim, int fmt, const int32_t *table, int64_t table_ld,
+                             int64_t width, const int32_t *seq_lens, const int32_t *starts,
+                             int64_t seqs, const int32_t *group_starts, const int32_t *shared_lens,
+                             int64_t groups, int64_t max_group, void *out, int64_t o_row,
+                             int64_t o_head, int64_t rows, int64_t max_q, float scale, int causal,
+                             int x_dtype, void *workspace, size_t workspace_bytes, void *stream);
+size_t dsl_kv8_shared_attention_workspace_bytes(int64_t heads, int64_t page, int64_t dim,
+                                                int64_t width, int64_t seqs, int64_t rows,
+                                                int64_t q_heads, int64_t max_q, int64_t groups,
+                                                int64_t max_group);
+
+/* The sequences of a step from the last step's.  refs [pages] counts the table
+ * entries that hold a page; pages of count 0 are free.  Child c continues
+ * sequence a = parents[c] (outside [0, seqs): an empty sequence); sequences that are
+ * no child's parent are dropped.  With len = seq_lens[a]: out_lens[c] = len + new
+ * tokens (more[c], or more_all with more NULL; negative ones count as 0).  Row c of
+ * out_table [children][width] holds a's pages of whole tokens (entries < len / page),
+ * shared; a's partly filled page, kept by a's first child, for every other one a fresh
+ * page with that page's codes and scales (all of it); fresh pages for the new tokens;
+ * -1 behind them.  Entries of a that are no page of the cache become -1.  The k-th
+ * fresh page asked for (by child, then entry) is the k-th page whose count is 0
+ * without the old table's entries and with the ones held so far.  out_refs
+ * [pages]: the counts of the new table; lacking[0]: fresh pages asked for and not there (their entries
+ * are -1), those past the table's row included.  Nothing that the call reads is changed but the
+ * fresh pages' codes and scales, so a step that lacked pages can be made again with
+ * fewer children.  A partly filled page must belong to one sequence alone. */
+int dsl_kv8_fork(void *k_cache, void *v_cache, float *k_scale, float *v_scale, int64_t pages,
+                 int64_t heads, int64_t page, int64_t dim, const int32_t *table, int64_t table_ld,
+                 int64_t width, const int32_t *seq_lens, int64_t seqs, const int32_t *parents,
+                 const int32_t *more, int64_t more_all, int64_t children, const int32_t *refs,
+                 int32_t *out_lens, int32_t *out_table, int32_t *out_refs, int32_t *lacking,
+                 void *workspace, size_t workspace_bytes, void *stream);
+size_t dsl_kv8_fork_workspace_bytes(int64_t seqs, int64_t width, int64_t children, int64_t pages);
+
+/* The pages of refs > 0, live[0] of them, move to the cache's front: the k-th
+ * live page from number live[0] on goes to the k-th other page before it, codes and
+ * scales; pages from live[0] on keep what they held.  moved [pages]: a page's new
+ * number (-1: it was free); out_table [seqs][width] (may be the table itself if
+ * table_ld is width) and out_refs [pages] in the new numbers. */
+int dsl_kv8_compact(void *k_cache, void *v_cache, float *k_scale, float *v_scale, int64_t pages,
+                    int64_t heads, int64_t page, int64_t dim, const int32_t *table,
+                    int64_t table_ld, int64_t width, int64_t seqs, const int32_t *refs,
+                    int32_t *out_table, int32_t *out_refs, int32_t *moved, int32_t *live,
+                    void *workspace, size_t workspace_bytes, void *stream);
+size_t dsl_kv8_compact_workspace_bytes(int64_t pages);
+
+/* Rotary positions: pair i < pairs of each head of q [rows][q_heads][dim] and k
+ * (k_heads 0: none), bf16 or fp16 with unit stride in dim, is turned by the angle
+ * positions[axis_of[i] * positions_ld + row] * freqs[i] and multiplied by
+ * magnitude; axis_of NULL: one axis; an axis outside [0, axes) turns by nothing.
+ * Pairs are the dimensions (i, i + pairs), or (2 i, 2 i + 1) with `adjacent`;
+ * dimensions from 2 pairs on stay.  Positions are int32, or int64; angles are formed
+ * in 64 bits (positions below 2^53 count exactly).  A result may be its source, in
+ * place; other overlaps are not allowed.  Strides in elements. */
+int dsl_rotary(const void *q, int64_t q_row, int64_t q_head, int64_t q_heads, const void *k,
+               int64_t k_row, int64_t k_head, int64_t k_heads, int64_t rows, int64_t dim,
+               int64_t pairs, const void *positions, int positions_64, int64_t positions_ld,
+               int64_t axes, const int32_t *axis_of, const double *freqs, float magnitude,
+               int adjacent, int x_dtype, void *q_out, int64_t qo_row, int64_t qo_head,
+               void *k_out, int64_t ko_row, int64_t ko_head, void *stream);
+
+/* Of softmax(scale * logits) by rows (bf16, fp16 or fp32, ld apart): logp
+ * [rows][n_ids] of the tokens ids[row * ids_ld + i], entropy [rows], and the `top`
+ * (0 .. 32) largest logits' log probabilities and numbers [rows][top], falling, ties
+ * by lowest number (NaN after the others).  Natural logarithms.  A logit of -inf has
+ * probability 0 (log -inf), as has an id outside [0, vocab); where all are -inf the
+ * entropy is 0.  NaN or +inf in a row make all its entropy and log probabilities NaN. */
+int dsl_token_logprobs(const void *logits, int64_t rows, int64_t vocab, int64_t ld, int x_dtype,
+                       const int32_t *ids, int64_t ids_ld, int64_t n_ids, float scale, int64_t top,
+                       float *logp, float *entropy, float *top_logp, int32_t *top_ids,
+                       void *workspace, size_t workspace_bytes, void *stream);
+size_t dsl_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top, int x_dtype);
+
 #ifdef __cplusplus
 }
 #endif
