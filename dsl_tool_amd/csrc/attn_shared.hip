@@ -10,8 +10,11 @@
 // kernel joins them in their order.  A row sees of the prefix what its length and
 // its position allow, so rows of sequences that are shorter than it, or empty, are
 // right too.
-#include "attn_rows.h"
+#include "attn_tile.h"
 #include "launch.h"
+
+#include <cstdlib>
+#include <type_traits>
 
 namespace dsl {
 
@@ -20,15 +23,16 @@ constexpr int kMaxRuns = 512;
 // The workspace.  The beginning of a unit is kept by its rows, the first of two
 // for each query row and head's prefix and own tokens; what a run holds of a unit
 // that began before it (one at most) by the run.
-template <int D, int ROWS>
 struct SharedParts {
-  float *first, *more;           // [row][query head][2][D], [run][ROWS][D]
-  float2 *first_ml, *more_ml;    // their maxima and sums
-  int2 *where;                   // [row][query head][2]: (run of the beginning, or -1: no part; last run * 64 + row of its block)
-  DSL_DEV SharedParts(float *ws, int64_t n, int runs)
-      : first(ws), more(first + 2 * n * D), first_ml(reinterpret_cast<float2 *>(more + (int64_t)runs * ROWS * D)),
-        more_ml(first_ml + 2 * n), where(reinterpret_cast<int2 *>(more_ml + (int64_t)runs * ROWS)) {}
+  float *first;                  // [row][query head][2][D]
+  float2 *first_ml;              // [row][query head][2]: maxima and sums
+  int2 *where;                   // ...: (run of the beginning, or -1: no part; last run * 64 + row of its block)
+  // of prefixes and of own tokens, the same where one launch has both
+  float *more[2];                // [run][ROWS][D]
+  float2 *more_ml[2];            // [run][ROWS]
+  int runs[2], rows[2];
 };
+enum { UNITS_PREFIX = 1, UNITS_OWN = 2 };        // what a launch walks
 
 // Tokens of group g's prefix: whole pages that the table has room for.
 DSL_DEV int prefix_of(const KvCacheArgs &c, const SharedArgs &h, int g) {
@@ -43,6 +47,26 @@ DSL_DEV int first_row(const KvCacheArgs &c, int b) {
   const int v = c.starts ? c.starts[b] : b;
   return v < 0 ? 0 : v > c.rows ? c.rows : v;
 }
+// The largest of each N lanes (16, 32 or 64).  (No shuffles: what their addresses
+// are made of would be kept through the walk, and spill.)
+template <int N>
+DSL_DEV int lanes_most(int v) {
+  auto most = [](int a, int b) { return a > b ? a : b; };
+  v = most(v, __builtin_amdgcn_update_dpp(v, v, 0xb1, 0xf, 0xf, false));    // lanes ^ 1, ^ 2, then mirrors of 8 and 16
+  v = most(v, __builtin_amdgcn_update_dpp(v, v, 0x4e, 0xf, 0xf, false));
+  v = most(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xf, 0xf, false));
+  v = most(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xf, 0xf, false));
+  if constexpr (N >= 32) {
+    const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+    v = most((int)a[0], (int)a[1]);
+  }
+  if constexpr (N >= 64) {
+    const auto a = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+    v = most((int)a[0], (int)a[1]);
+  }
+  return v;
+}
+DSL_DEV int one(int v) { return __builtin_amdgcn_readfirstlane(v); }
 // The last i of 0 .. n - 1 with at(i) <= x, or -1.
 template <class F>
 DSL_DEV int last_upto(int n, int x, const F &at) {
@@ -84,22 +108,30 @@ DSL_DEV SharedUnit shared_unit(const KvCacheArgs &c, const SharedArgs &h, int u)
   return s;
 }
 
-// The line of all units' rounds: by unit, cache head, row block.
+// The line of all units' rounds: by unit, cache head, row block.  64 units are looked
+// at at a time; what a wave knows of them is in shared memory (the same for all waves),
+// not in registers, which a walk needs.
+struct LineUnits {
+  int rounds[64], blocks[64], upto[64];          // of a unit; the line's length up to and with it, from the first of the 64
+};
 template <int ROWS>
 struct SharedLine {
   const KvCacheArgs &c;
   const SharedArgs &h;
-  const int group, chunk, lane;
-  int at, rounds, blocks;        // of this lane's unit
-  int before, total, upto;       // the line's length before these 64; theirs; theirs up to and with this lane's
-  DSL_DEV SharedLine(const KvCacheArgs &c, const SharedArgs &h, int group, int chunk)
-      : c(c), h(h), group(group), chunk(chunk), lane(threadIdx.x & 63), at(-64), before(0), total(0), upto(0) {}
+  LineUnits &in;
+  const int group, chunk, begin, units;
+  int at, before, total;         // the first of the 64; the line's length before them, theirs
+  DSL_DEV SharedLine(const KvCacheArgs &c, const SharedArgs &h, LineUnits &in, int group, int chunk, int what)
+      : c(c), h(h), in(in), group(group), chunk(chunk), begin(what & UNITS_PREFIX ? 0 : h.n),
+        units(what & UNITS_OWN ? h.n + c.seqs : h.n), at(begin - 64), before(0), total(0) {}
   DSL_DEV void advance() {
     before += total;
     at += 64;
-    rounds = blocks = 0;
-    const int u = at + lane;
-    if (u < c.seqs + h.n) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, u = at + lane;
+    int rounds = 0, blocks = 0;
+    if (u < units) {
       const SharedUnit s = shared_unit(c, h, u);
       const int room = c.width * c.page, len = s.len < room ? s.len : room;
       const int tiles = len > s.off ? (len - s.off + kTile - 1) / kTile : 0;
@@ -107,14 +139,19 @@ struct SharedLine {
       if (u >= h.n && rounds == 0) rounds = 1;   // of no token: one, for its parts
       blocks = rounds ? (int)(((int64_t)s.n * group + ROWS - 1) / ROWS) : 0;
     }
-    upto = lanes_sum(rounds * c.heads * blocks);
+    const int upto = lanes_sum(rounds * c.heads * blocks);
     total = __builtin_amdgcn_readlane(upto, 63);
+    __syncthreads();                             // the last 64's readers
+    in.rounds[lane] = rounds;
+    in.blocks[lane] = blocks;
+    in.upto[lane] = upto;
+    __syncthreads();
   }
   DSL_DEV int length() {                         // of the whole line; back to its beginning
-    while (at + 64 < c.seqs + h.n) advance();
+    while (at + 64 < units) advance();
     const int n = before + total;
-    if (at > 0) {
-      at = -64;
+    if (at > begin) {
+      at = begin - 64;
       before = total = 0;
       advance();
     }
@@ -123,39 +160,96 @@ struct SharedLine {
   // The unit of position x, not before an earlier one; its rounds and row
   // blocks, and x in it.  (-1: none, of groups or starts that do not ascend.)
   DSL_DEV int find(int x, int &ur, int &ub, int &off) {
-    while (x >= before + total && at + 64 < c.seqs + h.n) advance();
+    while (x >= before + total && at + 64 < units) advance();
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int upto = in.upto[tid & 63];
     const uint64_t past = __ballot(before + upto > x);
     if (!past) return -1;
     const int k = __builtin_ctzll(past);
-    ur = __builtin_amdgcn_readlane(rounds, k);
-    ub = __builtin_amdgcn_readlane(blocks, k);
+    ur = __builtin_amdgcn_readfirstlane(in.rounds[k]);
+    ub = __builtin_amdgcn_readfirstlane(in.blocks[k]);
     off = x - before - __builtin_amdgcn_readlane(upto, k) + ur * c.heads * ub;
     return at + k;
   }
 };
 
-template <int SRC, bool FP8, int D, int RB>
-__global__ __launch_bounds__(256, rows_wgs(D, RB)) void attn_shared_kernel(const KvCacheArgs c, const AttnArgs p,
-                                                                             const SharedArgs h, const int chunk) {
-  constexpr bool F16 = SRC == SRC_F16;
-  constexpr int DC = D / 64, ROWS = 16 * RB;
-  __shared__ __align__(16) RowsJoin<D> sh;
-  const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
-  const SharedParts<D, ROWS> part(p.ws, (int64_t)c.rows * p.q_heads, gridDim.x);
-  SharedLine<ROWS> line(c, h, p.group, chunk);
-  const int whole = line.length(), per = (whole + (int)gridDim.x - 1) / (int)gridDim.x;
-  int x = (int)blockIdx.x * per;
+// Up to 16 rows of a unit, by attn.hip's walk.
+template <int SRC_, bool FP8_, int D_>
+struct FewWalk : RowsWalk<SRC_ == SRC_F16, FP8_, D_, 1> {
+  static constexpr int SRC = SRC_, D = D_, NB = 1, BLOCK = 16, ROWS = 16, WGS = rows_wgs(D, 1);
+  static constexpr bool FP8 = FP8_;
+  using Base = RowsWalk<SRC_ == SRC_F16, FP8_, D_, 1>;
+  static constexpr bool SHARED = false;          // (queries in registers)
+  typedef int Queries;
+  DSL_DEV explicit FewWalk(Queries &) {}
+  float qs[NB];
+  DSL_DEV float load(int b, const uint16_t *q) {
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int y = 0; y < D / 64; ++y)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) this->qf[b][2 * y + z] = *reinterpret_cast<const v4i *>(q + 64 * y + 16 * g + 8 * z);
+    return 1.f;
+  }
+  DSL_DEV void walk(const KvCacheArgs &c, const Context &ctx, float scale, int head, int t0, int t1, int lo, Word16 *) {
+    Base::walk(c, ctx, scale, true, head, t0, t1, lo);
+  }
+};
+template <class Walk>
+struct JoinOf {
+  using type = TileJoin<Walk::D, Walk::ROWS>;
+};
+template <int SRC, bool FP8, int D>
+struct JoinOf<FewWalk<SRC, FP8, D>> {
+  using type = RowsJoin<D>;
+};
+template <class Walk, class G, class F>
+DSL_DEV void join_waves(TileJoin<Walk::D, Walk::ROWS> &sh, const Walk &w, int rows, const G &restore, const F &emit) {
+  join_tiles(sh, w, rows, restore, emit);
+}
+template <class Walk, class G, class F>
+DSL_DEV void join_waves(RowsJoin<Walk::D> &sh, const Walk &w, int rows, const G &, const F &emit) {
+  join_rows<Walk::D, 1>(sh, w, rows, [&](int, int row, int col, const v4f &v, float m, float l) { emit(row, col, v, m, l); });
+}
+
+// Workgroups go to the eight XCDs in turn: each XCD takes a piece of the line, so that
+// the row blocks of a head, which read the same tokens, share its L2.
+DSL_DEV int run_of(int block, int runs) { return runs % 8 == 0 ? block % 8 * (runs / 8) + block / 8 : block; }
+
+template <class Walk>
+__global__ __launch_bounds__(256, Walk::WGS) void attn_shared_kernel(const KvCacheArgs c, const AttnArgs p,
+                                                                     const SharedArgs h, const SharedParts part,
+                                                                     const int chunk, const int what) {
+  constexpr int D = Walk::D, ROWS = Walk::ROWS, BLOCK = Walk::BLOCK, NB = Walk::NB;
+  __shared__ __align__(16) typename JoinOf<Walk>::type sh;
+  __shared__ __align__(16) typename Walk::Queries queries;
+  __shared__ int s_limit[ROWS];                  // (every wave writes all)
+  __shared__ float2 s_row[NB][BLOCK];            // what a row's queries were divided by, the tokens it sees
+  __shared__ LineUnits s_units;
+  SharedLine<ROWS> line(c, h, s_units, p.group, chunk, what);
+  const int whole = one(line.length()), per = one((whole + (int)gridDim.x - 1) / (int)gridDim.x);
+  const int run = run_of(blockIdx.x, gridDim.x);
+  int x = run * per;
   const int end = whole - per > x ? x + per : whole;
 
   while (x < end) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));                // (what is made of it is formed in each unit: kept, it spills)
+    const int lane = tid & 63, mine = lane & (BLOCK - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int rounds, blocks, off;
     const int u = line.find(x, rounds, blocks, off);
     if (u < 0) return;
     const bool prefix = u < h.n;
-    const int unit = off / rounds, r0 = off % rounds, head = unit / blocks, rb = unit % blocks;
+    // (one number for the wave, each: in scalar registers)
+    const int unit = one(off / rounds), r0 = off - unit * rounds, head = one(unit / blocks), rb = unit - head * blocks;
     const int left = rounds - r0, count = left < end - x ? left : end - x;
     x += count;
-    const SharedUnit s = shared_unit(c, h, u);
+    SharedUnit s = shared_unit(c, h, u);
+    s.rows0 = one(s.rows0);
+    s.n = one(s.n);
+    s.off = one(s.off);
+    s.len = one(s.len);
     const int rows = s.n * p.group, room = c.width * c.page, seen = s.len < room ? s.len : room;
     // whose table row, from which page on; tokens of it
     int from = u - h.n;
@@ -172,64 +266,85 @@ __global__ __launch_bounds__(256, rows_wgs(D, RB)) void attn_shared_kernel(const
           from = b + __builtin_ctzll(enough);
           break;
         }
-        int most = n;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) most = most > __shfl_xor(most, o) ? most : __shfl_xor(most, o);
+        const int most = lanes_most<64>(n);
         if (most > best) {
           best = most;
           from = b + __builtin_ctzll(__ballot(n == most));
         }
       }
-      from = __builtin_amdgcn_readfirstlane(from);
+      from = one(from);
     }
-    const Context ctx{c.table + (int64_t)from * c.table_ld + s.off / c.page, c.width - s.off / c.page, s.len - s.off};
-    RowsWalk<F16, FP8, D, RB> w;
-    int lo = 0x7fffffff, high = 0;               // tokens that every row sees, that some row sees
-#pragma unroll
-    for (int k = 0; k < RB; ++k) {
-      const int r = rb * ROWS + k * 16 + r16, rr = r < rows ? r : rows - 1;
+    const int skip = one(s.off / c.page);
+    const Context ctx{c.table + (int64_t)from * c.table_ld + skip, c.width - skip, s.len - s.off};
+    Walk w(queries);
+    if constexpr (Walk::SHARED) w.limit = s_limit;
+    // A row of the block: its queries, and the tokens of the unit that it sees; by
+    // one wave for all where they share them.
+    auto row_of = [&](int k) __attribute__((always_inline)) {
+      const int r = rb * ROWS + k * BLOCK + mine, rr = r < rows ? r : rows - 1;
       const int i = rr / p.group, hq = head * p.group + rr % p.group, row = s.rows0 + i;
-      const uint16_t *qp = static_cast<const uint16_t *>(p.q) + (int64_t)row * p.q_row + (int64_t)hq * p.q_head;
-#pragma unroll
-      for (int y = 0; y < DC; ++y)
-#pragma unroll
-        for (int z = 0; z < 2; ++z)
-          w.qf[k][2 * y + z] = *reinterpret_cast<const v4i *>(qp + 64 * y + 16 * g + 8 * z);
-      // tokens of its own sequence that the row sees
+      const float by = w.load(k, static_cast<const uint16_t *>(p.q) + (int64_t)row * p.q_row + (int64_t)hq * p.q_head);
       int b = u - h.n;
       if (prefix) b = c.starts ? last_upto(c.seqs, row, [&](int j) { return first_row(c, j); }) : row;
       const SeqView v = seq_view(c, b);
       int n = p.causal ? v.first + (row - v.row0) + 1 : v.len;
       n = (n < seen ? n : seen) - s.off;
-      w.limit[k] = n > 0 ? n : 0;
-      lo = lo < w.limit[k] ? lo : w.limit[k];
-      high = high > w.limit[k] ? high : w.limit[k];
+      s_row[k][mine] = make_float2(by, __builtin_bit_cast(float, n > 0 ? n : 0));
+    };
+    if (Walk::SHARED) {
+      if (wave < NB) row_of(wave);
+      __syncthreads();
+    } else {
+      row_of(0);
     }
+    int lo = 0x7fffffff, high = 0;               // tokens that every other row sees, that some row sees
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
-      const int a = __shfl_xor(lo, o), z = __shfl_xor(high, o);
-      lo = lo < a ? lo : a;
-      high = high > z ? high : z;
+    for (int k = 0; k < NB; ++k) {
+      const float2 x = s_row[k][mine];
+      const int n = __builtin_bit_cast(int, x.y);
+      w.qs[k] = x.x;
+      // (a row that sees no token of the unit keeps no tile off the common path: it goes
+      // along, and is cleared)
+      const int limit = n == 0 ? 0x7fffffff : n;
+      if constexpr (Walk::SHARED) s_limit[k * BLOCK + mine] = limit;
+      else w.limit[k] = limit;
+      lo = lo < limit ? lo : limit;
+      high = high > n ? high : n;
     }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    const int nsee = (__builtin_amdgcn_readfirstlane(high) + kTile - 1) / kTile;
+    lo = __builtin_amdgcn_readfirstlane(-lanes_most<BLOCK>(-lo));
+    const int nsee = (__builtin_amdgcn_readfirstlane(lanes_most<BLOCK>(high)) + kTile - 1) / kTile;
     const int t0 = r0 * chunk, t1 = nsee - t0 > count * chunk ? t0 + count * chunk : nsee;
-    w.walk(c, ctx, p.scale, true, head, t0, t1, lo);
-    const int last = (int)blockIdx.x + (left - count + per - 1) / per;
-    join_rows<D, RB>(sh, w, rows - rb * ROWS, [&](int k, int row, int col, const v4f &v, float mr, float lr) {
-      const int r = rb * ROWS + k * 16 + row, i = r / p.group, hq = head * p.group + r % p.group;
+    w.walk(c, ctx, p.scale, head, t0, t1, lo, reinterpret_cast<Word16 *>(sh.so[wave]));
+#pragma unroll
+    for (int k = 0; k < NB; ++k)
+      if (__builtin_bit_cast(int, s_row[k][mine].y) == 0) {
+        w.m[k] = -INFINITY;
+        w.l[k] = 0.f;
+#pragma unroll
+        for (int d = 0; d < (int)(sizeof(w.o[k]) / sizeof(w.o[k][0])); ++d)
+#pragma unroll
+          for (int i = 0; i < (int)(sizeof(w.o[k][0]) / sizeof(float)); ++i) w.o[k][d][i] = 0.f;
+      }
+    const int last = one(run + (left - count + per - 1) / per);
+    auto restore = [&](float *so) __attribute__((always_inline)) {
+      if constexpr (Walk::SHARED)
+        w.restore(c, ctx, head, t0, t1, so, [&](int r) { return __builtin_bit_cast(int, s_row[r / BLOCK][r % BLOCK].y); });
+    };
+    join_waves(sh, w, rows - rb * ROWS, restore, [&](int row, int col, const v4f &v, float mr, float lr) {
+      const int r = rb * ROWS + row, i = r / p.group, hq = head * p.group + r % p.group;
       const float2 ml = make_float2(lr == lr ? mr : lr, lr);   // a NaN sum without a maximum stays NaN in the join
       if (r0 == 0) {
         const int64_t rh = (int64_t)(s.rows0 + i) * p.q_heads + hq, at = 2 * rh + (prefix ? 0 : 1);
         *reinterpret_cast<v4f *>(part.first + at * D + col) = v;
         if (col != 0) return;
         part.first_ml[at] = ml;
-        part.where[at] = make_int2((int)blockIdx.x, last * 64 + k * 16 + row);
+        part.where[at] = make_int2(run, last * 64 + row);
         if (!prefix && s.off == 0) part.where[2 * rh] = make_int2(-1, 0);
       } else {
-        const int64_t at = (int64_t)blockIdx.x * ROWS + k * 16 + row;
-        *reinterpret_cast<v4f *>(part.more + at * D + col) = v;
-        if (col == 0) part.more_ml[at] = ml;
+        const int64_t at = (int64_t)run * ROWS + row;
+        const int kind = prefix ? 0 : 1;
+        *reinterpret_cast<v4f *>(part.more[kind] + at * D + col) = v;
+        if (col == 0) part.more_ml[kind][at] = ml;
       }
     });
   }
@@ -238,32 +353,32 @@ __global__ __launch_bounds__(256, rows_wgs(D, RB)) void attn_shared_kernel(const
 // Joins the parts of one query row and head in a workgroup, as attn.hip's does: a
 // part per thread for the maximum and the sum, then four columns per thread, the
 // parts dealt to 1024 / D threads of each.
-template <int SRC, int D, int ROWS>
-__global__ __launch_bounds__(256) void attn_shared_join_kernel(const AttnArgs p, const int64_t n, const int runs) {
+template <int SRC, int D>
+__global__ __launch_bounds__(256) void attn_shared_join_kernel(const AttnArgs p, const SharedParts part) {
   constexpr int CG = D / 4, SL = 256 / CG;
   __shared__ float s_f[2 * kMaxRuns], s_red[8];
   __shared__ v4f s_v[SL][CG];
   const int64_t at = blockIdx.x;
   const int tid = threadIdx.x;
-  const SharedParts<D, ROWS> part(p.ws, n, runs);
   // (A row of no sequence has what the workspace held: in bounds, and its result
   // is not specified.)
-  auto span = [&](const int2 &w) {
+  auto span = [&](const int2 &w, int runs) {
     if (w.x < 0 || w.x >= runs) return 0;
     const int many = (w.y >> 6) - w.x + 1, most = runs - w.x;
     return many < 0 ? 0 : many < most ? many : most;
   };
   const int2 wp = part.where[2 * at], wo = part.where[2 * at + 1];
-  const int np = span(wp), parts = np + span(wo);
+  const int np = span(wp, part.runs[0]), parts = np + span(wo, part.runs[1]);
   // part s: a row's beginning, or the run that holds more of it
   auto beginning = [&](int s) { return s == 0 && np > 0 ? 2 * at : s == np ? 2 * at + 1 : (int64_t)-1; };
   auto run_row = [&](int s) {
-    const int2 w = s < np ? wp : wo;
-    return (int64_t)(w.x + (s < np ? s : s - np)) * ROWS + (w.y & (ROWS - 1));
+    const int kind = s < np ? 0 : 1;
+    const int2 w = kind ? wo : wp;
+    return (int64_t)(w.x + (kind ? s - np : s)) * part.rows[kind] + (w.y & (part.rows[kind] - 1));
   };
   auto max_sum = [&](int s) {
     const int64_t b = beginning(s);
-    return b >= 0 ? part.first_ml[b] : part.more_ml[run_row(s)];
+    return b >= 0 ? part.first_ml[b] : part.more_ml[s < np ? 0 : 1][run_row(s)];
   };
   float top = -INFINITY, l = 0.f;
   for (int s = tid; s < parts; s += 256) {
@@ -290,7 +405,7 @@ __global__ __launch_bounds__(256) void attn_shared_join_kernel(const AttnArgs p,
 #pragma unroll 4
   for (int s = sl; s < parts; s += SL) {
     const int64_t b = beginning(s);
-    v += *reinterpret_cast<const v4f *>((b >= 0 ? part.first + b * D : part.more + run_row(s) * D) + cg * 4) * s_f[s];
+    v += *reinterpret_cast<const v4f *>((b >= 0 ? part.first + b * D : part.more[s < np ? 0 : 1] + run_row(s) * D) + cg * 4) * s_f[s];
   }
   s_v[sl][cg] = v;
   __syncthreads();
@@ -303,52 +418,105 @@ __global__ __launch_bounds__(256) void attn_shared_join_kernel(const AttnArgs p,
   *reinterpret_cast<uint2 *>(op) = make_uint2(narrow2<SRC>(v[0] * inv, v[1] * inv), narrow2<SRC>(v[2] * inv, v[3] * inv));
 }
 
-struct SharedPlan {
-  int rb, runs, chunk;
+// How units of a kind are walked: query rows of a block (16, 32 or 64 a wave),
+// workgroups, tiles of a round.
+struct SharedWalk {
+  int rows, runs, chunk;
 };
-static SharedPlan shared_plan(const KvCacheArgs &c, int groups, int q_heads, int max_q, int max_group) {
-  SharedPlan a{};
-  const int64_t group = q_heads / c.heads, rows = (int64_t)max_q * max_group * group;    // of a prefix
-  a.rb = rows <= 16 || c.dim > 128 ? 1 : 2;
-  a.runs = rows_wgs(c.dim, a.rb) * device_cu_count();
+struct SharedPlan {
+  bool one;                      // launch for both kinds, as prefixes are walked
+  SharedWalk prefix, own;
+  size_t bytes;                  // of the workspace
+  SharedParts parts;             // in a workspace at 0
+};
+static SharedWalk shared_walk(const KvCacheArgs &c, int64_t group, int64_t rows, int64_t kinds, int64_t many) {
+  SharedWalk a{};
+  a.rows = rows <= 16 ? 16 : rows <= 32 || c.dim > 128 ? 32 : 64;
+  const char *set = getenv("DSL_ATTN_SHARED_ROWS");    // read per launch (tests switch it)
+  if (set && (atoi(set) == 16 || atoi(set) == 32 || (atoi(set) == 64 && c.dim <= 128))) a.rows = atoi(set);
+  a.runs = (a.rows == 16 ? rows_wgs(c.dim, 1) : 1) * device_cu_count();
   if (a.runs > kMaxRuns) a.runs = kMaxRuns;
   // rounds of a tile per wave, longer ones where the line's length would pass an int
   const int64_t tiles = ((int64_t)c.width * c.page + kTile - 1) / kTile;
-  const int64_t units = c.heads * (2 * ((int64_t)c.rows * group / (16 * a.rb)) + c.seqs + groups);   // at most
+  const int64_t units = c.heads * (kinds * ((int64_t)c.rows * group / a.rows) + many);          // at most
   a.chunk = 4;
   while ((tiles + a.chunk - 1) / a.chunk * units > 1 << 30 && a.chunk < tiles) a.chunk *= 2;
   return a;
 }
+static SharedPlan shared_plan(const KvCacheArgs &c, int groups, int q_heads, int max_q, int max_group) {
+  SharedPlan a{};
+  const int64_t group = q_heads / c.heads, most = (int64_t)max_q * max_group;
+  const int64_t rows = (most < c.rows ? most : c.rows) * group, own = (max_q < c.rows ? max_q : c.rows) * group;
+  a.one = rows <= 16 || groups == 0;
+  a.prefix = shared_walk(c, group, groups ? rows : own, a.one ? 2 : 1, (a.one ? c.seqs : 0) + (int64_t)groups);
+  a.own = a.one ? a.prefix : shared_walk(c, group, own, 1, c.seqs);
+  const size_t n = (size_t)c.rows * q_heads;
+  size_t at = 0;
+  auto room = [&](size_t bytes) {
+    const size_t p = at;
+    at += (bytes + 15) & ~(size_t)15;
+    return p;
+  };
+  auto put = [&](auto *&p, size_t bytes) { p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(room(bytes)); };
+  put(a.parts.first, 2 * n * c.dim * sizeof(float));
+  put(a.parts.first_ml, 2 * n * sizeof(float2));
+  put(a.parts.where, 2 * n * sizeof(int2));
+  for (int k = 0; k < 2; ++k) {
+    const SharedWalk &w = k ? a.own : a.prefix;
+    a.parts.runs[k] = w.runs;
+    a.parts.rows[k] = w.rows;
+    if (k && a.one) {
+      a.parts.more[k] = a.parts.more[0];
+      a.parts.more_ml[k] = a.parts.more_ml[0];
+    } else {
+      put(a.parts.more[k], (size_t)w.runs * w.rows * c.dim * sizeof(float));
+      put(a.parts.more_ml[k], (size_t)w.runs * w.rows * sizeof(float2));
+    }
+  }
+  a.bytes = at;
+  return a;
+}
 
 size_t attn_shared_workspace_bytes(const KvCacheArgs &c, int groups, int q_heads, int max_q, int max_group) {
-  const SharedPlan a = shared_plan(c, groups, q_heads, max_q, max_group);
-  const size_t n = (size_t)c.rows * q_heads, row = (c.dim + 2) * sizeof(float);
-  return 2 * n * (row + sizeof(int2)) + (size_t)a.runs * 16 * a.rb * row;
+  return shared_plan(c, groups, q_heads, max_q, max_group).bytes;
 }
 
-template <int SRC, int D, int RB>
-static void launch_shared_rows(const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, const SharedPlan &a, hipStream_t st) {
-  if (c.fp8) attn_shared_kernel<SRC, true, D, RB><<<(unsigned)a.runs, 256, 0, st>>>(c, p, h, a.chunk);
-  else attn_shared_kernel<SRC, false, D, RB><<<(unsigned)a.runs, 256, 0, st>>>(c, p, h, a.chunk);
-  attn_shared_join_kernel<SRC, D, 16 * RB><<<(unsigned)c.rows * (unsigned)p.q_heads, 256, 0, st>>>(p, (int64_t)c.rows * p.q_heads, a.runs);
+template <int SRC, bool FP8, int D>
+static void launch_shared_units(const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, const SharedParts &parts,
+                                const SharedWalk &w, int what, hipStream_t st) {
+  const unsigned n = (unsigned)w.runs;
+  if (w.rows == 16) attn_shared_kernel<FewWalk<SRC, FP8, D>><<<n, 256, 0, st>>>(c, p, h, parts, w.chunk, what);
+  else if (w.rows == 32) attn_shared_kernel<TileWalk<SRC, FP8, D, 1>><<<n, 256, 0, st>>>(c, p, h, parts, w.chunk, what);
+  else if constexpr (D <= 128) attn_shared_kernel<TileWalk<SRC, FP8, D, 2>><<<n, 256, 0, st>>>(c, p, h, parts, w.chunk, what);
 }
-template <int SRC, int D>
+template <int SRC, bool FP8, int D>
 static hipError_t launch_shared_dim(const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, hipStream_t st) {
-  const SharedPlan a = shared_plan(c, h.n, p.q_heads, p.max_q, h.most);
-  if (a.rb == 1) launch_shared_rows<SRC, D, 1>(c, p, h, a, st);
-  else if constexpr (D <= 128) launch_shared_rows<SRC, D, 2>(c, p, h, a, st);
+  SharedPlan a = shared_plan(c, h.n, p.q_heads, p.max_q, h.most);
+  const uintptr_t ws = reinterpret_cast<uintptr_t>(p.ws);
+  auto move = [&](auto *&x) { x = reinterpret_cast<std::remove_reference_t<decltype(x)>>(reinterpret_cast<uintptr_t>(x) + ws); };
+  move(a.parts.first);
+  move(a.parts.first_ml);
+  move(a.parts.where);
+  for (int k = 0; k < 2; ++k) {
+    move(a.parts.more[k]);
+    move(a.parts.more_ml[k]);
+  }
+  launch_shared_units<SRC, FP8, D>(c, p, h, a.parts, a.prefix, a.one ? UNITS_PREFIX | UNITS_OWN : UNITS_PREFIX, st);
+  if (!a.one) launch_shared_units<SRC, FP8, D>(c, p, h, a.parts, a.own, UNITS_OWN, st);
+  attn_shared_join_kernel<SRC, D><<<(unsigned)c.rows * (unsigned)p.q_heads, 256, 0, st>>>(p, a.parts);
   return hipGetLastError();
 }
-template <int SRC>
+template <int SRC, bool FP8>
 static hipError_t launch_shared_src(const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, hipStream_t st) {
-  if (c.dim == 64) return launch_shared_dim<SRC, 64>(c, p, h, st);
-  if (c.dim == 128) return launch_shared_dim<SRC, 128>(c, p, h, st);
-  return launch_shared_dim<SRC, 256>(c, p, h, st);
+  if (c.dim == 64) return launch_shared_dim<SRC, FP8, 64>(c, p, h, st);
+  if (c.dim == 128) return launch_shared_dim<SRC, FP8, 128>(c, p, h, st);
+  return launch_shared_dim<SRC, FP8, 256>(c, p, h, st);
 }
 
 hipError_t launch_attn_shared(int src, const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, hipStream_t st) {
   if (c.seqs == 0 || c.rows == 0) return hipSuccess;
-  return src == SRC_BF16 ? launch_shared_src<SRC_BF16>(c, p, h, st) : launch_shared_src<SRC_F16>(c, p, h, st);
+  if (src == SRC_BF16) return c.fp8 ? launch_shared_src<SRC_BF16, true>(c, p, h, st) : launch_shared_src<SRC_BF16, false>(c, p, h, st);
+  return c.fp8 ? launch_shared_src<SRC_F16, true>(c, p, h, st) : launch_shared_src<SRC_F16, false>(c, p, h, st);
 }
 
 }  // namespace dsl
