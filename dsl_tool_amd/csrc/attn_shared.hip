@@ -18,7 +18,7 @@
 
 namespace dsl {
 
-constexpr int kMaxRuns = 512;
+constexpr int kMaxRuns = 512, kPad = 4;
 
 // The workspace.  The beginning of a unit is kept by its rows, the first of two
 // for each query row and head's prefix and own tokens; what a run holds of a unit
@@ -88,6 +88,7 @@ DSL_DEV int prefix_behind(const KvCacheArgs &c, const SharedArgs &h, int b) {
 struct SharedUnit {
   int rows0, n;                  // rows of the token tensors
   int off, len;                  // tokens off .. len - 1 (of a prefix: 0 .. len - 1)
+  int from;                      // the sequence whose table row has them (-1: a longer one than the group's first)
 };
 DSL_DEV SharedUnit shared_unit(const KvCacheArgs &c, const SharedArgs &h, int u) {
   SharedUnit s;
@@ -98,12 +99,14 @@ DSL_DEV SharedUnit shared_unit(const KvCacheArgs &c, const SharedArgs &h, int u)
     s.n = end > s.rows0 ? end - s.rows0 : 0;
     s.off = 0;
     s.len = prefix_of(c, h, u);
+    s.from = b1 > b0 && c.lens[b0] >= s.len ? b0 : -1;
   } else {
     const SeqView v = seq_view(c, u - h.n);
     s.rows0 = v.row0;
     s.n = v.n;
     s.off = prefix_behind(c, h, u - h.n);
     s.len = v.len;
+    s.from = u - h.n;
   }
   return s;
 }
@@ -113,6 +116,7 @@ DSL_DEV SharedUnit shared_unit(const KvCacheArgs &c, const SharedArgs &h, int u)
 // not in registers, which a walk needs.
 struct LineUnits {
   int rounds[64], blocks[64], upto[64];          // of a unit; the line's length up to and with it, from the first of the 64
+  SharedUnit unit[64];
 };
 template <int ROWS>
 struct SharedLine {
@@ -120,10 +124,21 @@ struct SharedLine {
   const SharedArgs &h;
   LineUnits &in;
   const int group, chunk, begin, units;
+  int per;                       // rounds that a unit's are rounded up to
   int at, before, total;         // the first of the 64; the line's length before them, theirs
   DSL_DEV SharedLine(const KvCacheArgs &c, const SharedArgs &h, LineUnits &in, int group, int chunk, int what)
       : c(c), h(h), in(in), group(group), chunk(chunk), begin(what & UNITS_PREFIX ? 0 : h.n),
-        units(what & UNITS_OWN ? h.n + c.seqs : h.n), at(begin - 64), before(0), total(0) {}
+        units(what & UNITS_OWN ? h.n + c.seqs : h.n), per(1), at(begin - 64), before(0), total(0) {}
+  // What the lanes have of the 64, rounds rounded up, into shared memory.
+  DSL_DEV void put(int lane, int rounds, int blocks) {
+    rounds = (rounds + per - 1) / per * per;
+    const int upto = lanes_sum(rounds * c.heads * blocks);
+    total = __builtin_amdgcn_readlane(upto, 63);
+    __syncthreads();                             // the last 64's readers
+    in.rounds[lane] = rounds;
+    in.blocks[lane] = blocks;
+    in.upto[lane] = upto;
+  }
   DSL_DEV void advance() {
     before += total;
     at += 64;
@@ -131,35 +146,65 @@ struct SharedLine {
     asm volatile("" : "+v"(tid));
     const int lane = tid & 63, u = at + lane;
     int rounds = 0, blocks = 0;
+    SharedUnit s{};
     if (u < units) {
-      const SharedUnit s = shared_unit(c, h, u);
+      s = shared_unit(c, h, u);
       const int room = c.width * c.page, len = s.len < room ? s.len : room;
       const int tiles = len > s.off ? (len - s.off + kTile - 1) / kTile : 0;
       rounds = (tiles + chunk - 1) / chunk;
       if (u >= h.n && rounds == 0) rounds = 1;   // of no token: one, for its parts
       blocks = rounds ? (int)(((int64_t)s.n * group + ROWS - 1) / ROWS) : 0;
     }
-    const int upto = lanes_sum(rounds * c.heads * blocks);
-    total = __builtin_amdgcn_readlane(upto, 63);
-    __syncthreads();                             // the last 64's readers
-    in.rounds[lane] = rounds;
-    in.blocks[lane] = blocks;
-    in.upto[lane] = upto;
+    put(lane, rounds, blocks);
+    in.unit[lane] = s;
     __syncthreads();
   }
-  DSL_DEV int length() {                         // of the whole line; back to its beginning
+  DSL_DEV void rewind() {
+    at = begin - 64;
+    before = total = 0;
+    advance();
+  }
+  // The rounds of a run, of `runs` equal ones; back to the line's beginning.  A run that
+  // holds the end of a unit and the beginning of the next takes up two (about 8 us):
+  // units' rounds are rounded up to whole runs where runs no more than kPad rounds longer
+  // hold them so (prefixes of 30000 tokens, 32 samples: 44 us unrounded, ROUND rounded).
+  DSL_DEV int share(int runs) {
     while (at + 64 < units) advance();
-    const int n = before + total;
-    if (at > begin) {
-      at = begin - 64;
-      before = total = 0;
+    const int least = one((before + total + runs - 1) / runs);
+    if (least <= 1) {
+      if (at > begin) rewind();
+      return least;
+    }
+    int need[kPad + 1] = {};
+    if (at > begin) rewind();
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63;
+    int r, n;
+    for (;;) {
+      r = in.rounds[lane];
+      n = in.blocks[lane];
+#pragma unroll
+      for (int k = 0; k <= kPad; ++k)
+        need[k] += __builtin_amdgcn_readlane(lanes_sum(n * c.heads * ((r + least + k - 1) / (least + k))), 63);
+      if (at + 64 >= units) break;
       advance();
     }
-    return n;
+    int share = least;
+#pragma unroll
+    for (int k = kPad; k >= 0; --k)
+      if (need[k] <= runs) share = per = least + k;
+    if (at > begin) {
+      rewind();
+    } else if (per > 1) {
+      put(lane, r, n);
+      __syncthreads();
+    }
+    return share;
   }
   // The unit of position x, not before an earlier one; its rounds and row
   // blocks, and x in it.  (-1: none, of groups or starts that do not ascend.)
-  DSL_DEV int find(int x, int &ur, int &ub, int &off) {
+  DSL_DEV int find(int x, int &ur, int &ub, int &off, SharedUnit &s) {
     while (x >= before + total && at + 64 < units) advance();
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
@@ -170,6 +215,8 @@ struct SharedLine {
     ur = __builtin_amdgcn_readfirstlane(in.rounds[k]);
     ub = __builtin_amdgcn_readfirstlane(in.blocks[k]);
     off = x - before - __builtin_amdgcn_readlane(upto, k) + ur * c.heads * ub;
+    s = in.unit[k];
+    s = SharedUnit{one(s.rows0), one(s.n), one(s.off), one(s.len), one(s.from)};
     return at + k;
   }
 };
@@ -204,13 +251,17 @@ template <int SRC, bool FP8, int D>
 struct JoinOf<FewWalk<SRC, FP8, D>> {
   using type = RowsJoin<D>;
 };
-template <class Walk, class G, class F>
-DSL_DEV void join_waves(TileJoin<Walk::D, Walk::ROWS> &sh, const Walk &w, int rows, const G &restore, const F &emit) {
-  join_tiles(sh, w, rows, restore, emit);
+template <class Walk, class G, class R, class F>
+DSL_DEV void join_waves(TileJoin<Walk::D, Walk::ROWS> &sh, const Walk &w, int rows, const G &restore, const R &row_sums,
+                        const F &emit) {
+  join_tiles(sh, w, rows, restore, row_sums, emit);
 }
-template <class Walk, class G, class F>
-DSL_DEV void join_waves(RowsJoin<Walk::D> &sh, const Walk &w, int rows, const G &, const F &emit) {
-  join_rows<Walk::D, 1>(sh, w, rows, [&](int, int row, int col, const v4f &v, float m, float l) { emit(row, col, v, m, l); });
+template <class Walk, class G, class R, class F>
+DSL_DEV void join_waves(RowsJoin<Walk::D> &sh, const Walk &w, int rows, const G &, const R &row_sums, const F &emit) {
+  join_rows<Walk::D, 1>(sh, w, rows, [&](int, int row, int col, const v4f &v, float m, float l) {
+    if (col == 0) row_sums(row, m, l);
+    emit(row, col, v);
+  });
 }
 
 // Workgroups go to the eight XCDs in turn: each XCD takes a piece of the line, so that
@@ -228,33 +279,29 @@ __global__ __launch_bounds__(256, Walk::WGS) void attn_shared_kernel(const KvCac
   __shared__ float2 s_row[NB][BLOCK];            // what a row's queries were divided by, the tokens it sees
   __shared__ LineUnits s_units;
   SharedLine<ROWS> line(c, h, s_units, p.group, chunk, what);
-  const int whole = one(line.length()), per = one((whole + (int)gridDim.x - 1) / (int)gridDim.x);
+  const int per = line.share((int)gridDim.x);
   const int run = run_of(blockIdx.x, gridDim.x);
   int x = run * per;
-  const int end = whole - per > x ? x + per : whole;
+  const int end = x + per;
 
   while (x < end) {
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));                // (what is made of it is formed in each unit: kept, it spills)
     const int lane = tid & 63, mine = lane & (BLOCK - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int rounds, blocks, off;
-    const int u = line.find(x, rounds, blocks, off);
+    SharedUnit s;
+    const int u = line.find(x, rounds, blocks, off, s);
     if (u < 0) return;
     const bool prefix = u < h.n;
     // (one number for the wave, each: in scalar registers)
     const int unit = one(off / rounds), r0 = off - unit * rounds, head = one(unit / blocks), rb = unit - head * blocks;
     const int left = rounds - r0, count = left < end - x ? left : end - x;
     x += count;
-    SharedUnit s = shared_unit(c, h, u);
-    s.rows0 = one(s.rows0);
-    s.n = one(s.n);
-    s.off = one(s.off);
-    s.len = one(s.len);
     const int rows = s.n * p.group, room = c.width * c.page, seen = s.len < room ? s.len : room;
     // whose table row, from which page on; tokens of it
-    int from = u - h.n;
-    if (prefix) {
-      // the first sequence that is as long as the prefix, else the longest
+    int from = s.from;
+    if (from < 0) {
+      // the group's first sequence that is as long as the prefix, else the longest
       const int b0 = group_start(c, h, u), b1 = group_start(c, h, u + 1);
       int best = -1;
       from = b0;
@@ -325,28 +372,32 @@ __global__ __launch_bounds__(256, Walk::WGS) void attn_shared_kernel(const KvCac
 #pragma unroll
           for (int i = 0; i < (int)(sizeof(w.o[k][0]) / sizeof(float)); ++i) w.o[k][d][i] = 0.f;
       }
-    const int last = one(run + (left - count + per - 1) / per);
+    const int last = one(run + (left - count + per - 1) / per), kind = prefix ? 0 : 1;
     auto restore = [&](float *so) __attribute__((always_inline)) {
       if constexpr (Walk::SHARED)
         w.restore(c, ctx, head, t0, t1, so, [&](int r) { return __builtin_bit_cast(int, s_row[r / BLOCK][r % BLOCK].y); });
     };
-    join_waves(sh, w, rows - rb * ROWS, restore, [&](int row, int col, const v4f &v, float mr, float lr) {
-      const int r = rb * ROWS + row, i = r / p.group, hq = head * p.group + r % p.group;
-      const float2 ml = make_float2(lr == lr ? mr : lr, lr);   // a NaN sum without a maximum stays NaN in the join
-      if (r0 == 0) {
-        const int64_t rh = (int64_t)(s.rows0 + i) * p.q_heads + hq, at = 2 * rh + (prefix ? 0 : 1);
-        *reinterpret_cast<v4f *>(part.first + at * D + col) = v;
-        if (col != 0) return;
-        part.first_ml[at] = ml;
-        part.where[at] = make_int2(run, last * 64 + row);
-        if (!prefix && s.off == 0) part.where[2 * rh] = make_int2(-1, 0);
-      } else {
-        const int64_t at = (int64_t)run * ROWS + row;
-        const int kind = prefix ? 0 : 1;
-        *reinterpret_cast<v4f *>(part.more[kind] + at * D + col) = v;
-        if (col == 0) part.more_ml[kind][at] = ml;
-      }
-    });
+    auto place = [&](int row) __attribute__((always_inline)) {       // of a row's beginning
+      const int r = rb * ROWS + row, i = r / p.group;
+      return 2 * ((s.rows0 + i) * p.q_heads + head * p.group + r - i * p.group) + kind;
+    };
+    join_waves(
+        sh, w, rows - rb * ROWS, restore,
+        [&](int row, float mr, float lr) __attribute__((always_inline)) {
+          const float2 ml = make_float2(lr == lr ? mr : lr, lr);     // a NaN sum without a maximum stays NaN in the join
+          if (r0 == 0) {
+            const int at = place(row);
+            part.first_ml[at] = ml;
+            part.where[at] = make_int2(run, last * 64 + row);
+            if (!prefix && s.off == 0) part.where[at - 1] = make_int2(-1, 0);
+          } else {
+            part.more_ml[kind][(int64_t)run * ROWS + row] = ml;
+          }
+        },
+        [&](int row, int col, const v4f &v) __attribute__((always_inline)) {
+          float *to = r0 == 0 ? part.first + (int64_t)place(row) * D : part.more[kind] + ((int64_t)run * ROWS + row) * D;
+          *reinterpret_cast<v4f *>(to + col) = v;
+        });
   }
 }
 
@@ -481,13 +532,21 @@ size_t attn_shared_workspace_bytes(const KvCacheArgs &c, int groups, int q_heads
   return shared_plan(c, groups, q_heads, max_q, max_group).bytes;
 }
 
+template <int SRC, bool FP8, int D, bool WHOLE>
+static void launch_shared_tiles(const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, const SharedParts &parts,
+                                const SharedWalk &w, int what, hipStream_t st) {
+  const unsigned n = (unsigned)w.runs;
+  if (w.rows == 32) attn_shared_kernel<TileWalk<SRC, FP8, D, 1, WHOLE>><<<n, 256, 0, st>>>(c, p, h, parts, w.chunk, what);
+  else if constexpr (D <= 128)
+    attn_shared_kernel<TileWalk<SRC, FP8, D, 2, WHOLE>><<<n, 256, 0, st>>>(c, p, h, parts, w.chunk, what);
+}
 template <int SRC, bool FP8, int D>
 static void launch_shared_units(const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, const SharedParts &parts,
                                 const SharedWalk &w, int what, hipStream_t st) {
   const unsigned n = (unsigned)w.runs;
   if (w.rows == 16) attn_shared_kernel<FewWalk<SRC, FP8, D>><<<n, 256, 0, st>>>(c, p, h, parts, w.chunk, what);
-  else if (w.rows == 32) attn_shared_kernel<TileWalk<SRC, FP8, D, 1>><<<n, 256, 0, st>>>(c, p, h, parts, w.chunk, what);
-  else if constexpr (D <= 128) attn_shared_kernel<TileWalk<SRC, FP8, D, 2>><<<n, 256, 0, st>>>(c, p, h, parts, w.chunk, what);
+  else if (c.page >= kTile) launch_shared_tiles<SRC, FP8, D, true>(c, p, h, parts, w, what, st);
+  else launch_shared_tiles<SRC, FP8, D, false>(c, p, h, parts, w, what, st);
 }
 template <int SRC, bool FP8, int D>
 static hipError_t launch_shared_dim(const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, hipStream_t st) {

@@ -88,7 +88,9 @@ struct TilePages {
   DSL_DEV bool none() const { return (a | b | c | d) < 0; }
 };
 
-template <int SRC_, bool FP8_, int D_, int NB_>
+// WHOLE: pages of 64 tokens and more, which hold whole tiles: one number, and addresses
+// that are the wave's but for a fixed offset of the lane.
+template <int SRC_, bool FP8_, int D_, int NB_, bool WHOLE>
 struct TileWalk {
   static constexpr int SRC = SRC_, D = D_, NB = NB_, BLOCK = 32, ROWS = 32 * NB, NW = 4;
   static constexpr bool FP8 = FP8_, F16 = SRC == SRC_F16;
@@ -163,6 +165,8 @@ struct TileWalk {
     // Pages by scalar loads: a vector load's wait would be one for the codes on
     // their way too.
     const auto table = (const __attribute__((address_space(4))) int32_t *)uniform(ctx.table);
+    const auto kscale = (const __attribute__((address_space(4))) float *)uniform(c.k_scale);
+    const auto vscale = (const __attribute__((address_space(4))) float *)uniform(c.v_scale);
     const int width = __builtin_amdgcn_readfirstlane(ctx.width), len = __builtin_amdgcn_readfirstlane(ctx.len);
     auto pages = [&](int tile) __attribute__((always_inline)) {
       auto page = [&](int g) __attribute__((always_inline)) {
@@ -171,9 +175,25 @@ struct TileWalk {
         const int p = table[in ? i : 0];         // (width > 0 where there is a tile)
         return in && p >= 0 && p < c.pages ? p : -1;
       };
-      return TilePages{page(0), page(1), page(2), page(3)};
+      TilePages pg;
+      pg.a = pg.b = pg.c = pg.d = page(0);
+      if constexpr (!WHOLE) {
+        pg.b = page(1);
+        pg.c = page(2);
+        pg.d = page(3);
+      }
+      return pg;
     };
+    const uint32_t klane = (16 * kgroup + 4 * (r32 >> 3) + (r32 & 3)) * D + 16 * h, vlane = r32 * P + 16 * h;
     auto load_k = [&](int tile, const TilePages &pg) __attribute__((always_inline)) {
+      if constexpr (WHOLE) {
+        const uint8_t *base = c.k + ((int64_t)(pg.a < 0 ? 0 : pg.a) * c.heads + head) * hstride + (tile * kTile & (P - 1)) * D;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int x = 0; x < KX; ++x) kr[t][x] = *reinterpret_cast<const uint4 *>(base + 32 * t * D + 32 * x + klane);
+        return;
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int p = pg.of(t, kgroup != 0);
@@ -185,6 +205,14 @@ struct TileWalk {
       }
     };
     auto load_v = [&](int tile, const TilePages &pg) __attribute__((always_inline)) {
+      if constexpr (WHOLE) {
+        const uint8_t *base = c.v + ((int64_t)(pg.a < 0 ? 0 : pg.a) * c.heads + head) * hstride + (tile * kTile & (P - 1));
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) vr[t][d] = *reinterpret_cast<const uint4 *>(base + 32 * t + d * 32 * P + vlane);
+        return;
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int p = pg.of(t, h != 0);
@@ -195,6 +223,12 @@ struct TileWalk {
       }
     };
     auto load_scales = [&](const TilePages &pg) __attribute__((always_inline)) {
+      if constexpr (WHOLE) {
+        const int64_t at = (int64_t)(pg.a < 0 ? 0 : pg.a) * c.heads + head;
+        kraw[0] = kraw[1] = kscale[at];
+        vraw[0] = vraw[1] = vscale[at];
+        return;
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int p = pg.of(t, h != 0);
@@ -461,22 +495,23 @@ struct TileWalk {
   }
 };
 
-// The waves' shares of a workgroup's rows, joined: common maximum, then one row-major tile
-// per wave, with `restore` for what a wave took from it.  emit(row, column, sums of 4
-// columns, maximum, sum).
+// The waves' shares of a workgroup's rows, joined: each row's maximum, sum and the waves'
+// factors by a thread of its own, then one row-major tile per wave, with `restore` for
+// what a wave took from it.  row_sums(row, maximum, sum); emit(row, column, sums of 4
+// columns).
 template <int D, int ROWS>
 struct TileJoin {
   static constexpr int NW = 4, LD = D + 4;       // floats per row of the joined tile
   float so[NW][ROWS * LD], sm[NW][ROWS], sl[NW][ROWS];
 };
-template <class Walk, class G, class F>
-DSL_DEV void join_tiles(TileJoin<Walk::D, Walk::ROWS> &sh, const Walk &w, int rows, const G &restore, const F &emit) {
+template <class Walk, class G, class R, class F>
+DSL_DEV void join_tiles(TileJoin<Walk::D, Walk::ROWS> &sh, const Walk &w, int rows, const G &restore, const R &row_sums,
+                        const F &emit) {
   constexpr int NW = 4, D = Walk::D, DT = Walk::DT, LD = D + 4;
   int tid = threadIdx.x;
   asm volatile("" : "+v"(tid));                  // (addresses are formed here: kept through the walk, they spill)
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, h = lane >> 5;
-  __syncthreads();                               // the last unit's readers
 #pragma unroll
   for (int b = 0; b < Walk::NB; ++b) {
     const float lw = halves_total(w.l[b]);
@@ -486,12 +521,24 @@ DSL_DEV void join_tiles(TileJoin<Walk::D, Walk::ROWS> &sh, const Walk &w, int ro
     }
   }
   __syncthreads();
+  if (tid < Walk::ROWS) {
+    float mk[NW], lr = 0.f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) mk[k] = sh.sm[k][tid];
+    const float mr = fmaxf(fmaxf(mk[0], mk[1]), fmaxf(mk[2], mk[3]));
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+      // (no maximum: nothing seen, 0, or nothing but NaN, NaN)
+      const float f = mr == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mk[k] - mr);
+      lr += sh.sl[k][tid] * f;
+      sh.sm[k][tid] = mr == -INFINITY ? 0.f : f;
+    }
+    if (tid < rows) row_sums(tid, mr, lr);
+  }
+  __syncthreads();
 #pragma unroll
   for (int b = 0; b < Walk::NB; ++b) {
-    float top = sh.sm[0][b * 32 + r32];
-#pragma unroll
-    for (int k = 1; k < NW; ++k) top = fmaxf(top, sh.sm[k][b * 32 + r32]);
-    const float f = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m[b] - top);
+    const float f = sh.sm[wave][b * 32 + r32];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -505,21 +552,13 @@ DSL_DEV void join_tiles(TileJoin<Walk::D, Walk::ROWS> &sh, const Walk &w, int ro
   __syncthreads();
   // thread -> row, 4 columns at a time
   const int n = (rows < Walk::ROWS ? rows : Walk::ROWS) * (D / 4);
-#pragma unroll 1
+#pragma unroll 2
   for (int x = tid; x < n; x += 256) {
     const int row = x / (D / 4), col = (x % (D / 4)) * 4;
-    float mr = sh.sm[0][row];
+    v4f v = *reinterpret_cast<const v4f *>(&sh.so[0][row * LD + col]);
 #pragma unroll
-    for (int k = 1; k < NW; ++k) mr = fmaxf(mr, sh.sm[k][row]);
-    float lr = 0.f;
-    v4f v = (v4f){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < NW; ++k) {
-      // (no maximum: nothing seen, 0, or nothing but NaN, NaN)
-      lr += mr == -INFINITY ? sh.sl[k][row] : sh.sl[k][row] * __builtin_amdgcn_exp2f(sh.sm[k][row] - mr);
-      v += *reinterpret_cast<const v4f *>(&sh.so[k][row * LD + col]);
-    }
-    emit(row, col, v, mr, lr);
+    for (int k = 1; k < NW; ++k) v += *reinterpret_cast<const v4f *>(&sh.so[k][row * LD + col]);
+    emit(row, col, v);
   }
 }
 
