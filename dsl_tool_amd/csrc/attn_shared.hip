@@ -3,10 +3,11 @@
 //
 // A group's sequences hold the same pages for its first E tokens (whole pages).
 // Their query rows stand together, so the prefix is the context of one unit with
-// all of the group's rows, read once for 16 RB of them instead of once per
-// sequence; what lies behind it is each sequence's own.  Both kinds of units
-// stand in one line of rounds of 256 tokens, prefixes first, and workgroups take
-// equal runs of it, as in attn.hip.  Every row has parts of both; a second
+// all of the group's rows, read once for 16, 32 or 64 of them instead of once per
+// sequence; what lies behind it is each sequence's own.  Units stand in lines of
+// rounds of 256 tokens, of which workgroups take equal runs, as in attn.hip: up to
+// 16 rows to a group both kinds in one line, else prefixes in one and own tokens in
+// another, at the same time or in a launch of their own.  Every row has parts of both; a second
 // kernel joins them in their order.  A row sees of the prefix what its length and
 // its position allow, so rows of sequences that are shorter than it, or empty, are
 // right too.
@@ -27,12 +28,12 @@ struct SharedParts {
   float *first;                  // [row][query head][2][D]
   float2 *first_ml;              // [row][query head][2]: maxima and sums
   int2 *where;                   // ...: (run of the beginning, or -1: no part; last run * 64 + row of its block)
-  // of prefixes and of own tokens, the same where one launch has both
+  // of prefixes and of own tokens, the same where one line has both
   float *more[2];                // [run][ROWS][D]
   float2 *more_ml[2];            // [run][ROWS]
   int runs[2], rows[2];
 };
-enum { UNITS_PREFIX = 1, UNITS_OWN = 2 };        // what a launch walks
+enum { UNITS_PREFIX = 1, UNITS_OWN = 2 };        // what a line has
 
 // Tokens of group g's prefix: whole pages that the table has room for.
 DSL_DEV int prefix_of(const KvCacheArgs &c, const SharedArgs &h, int g) {
@@ -118,16 +119,15 @@ struct LineUnits {
   int rounds[64], blocks[64], upto[64];          // of a unit; the line's length up to and with it, from the first of the 64
   SharedUnit unit[64];
 };
-template <int ROWS>
 struct SharedLine {
   const KvCacheArgs &c;
   const SharedArgs &h;
   LineUnits &in;
-  const int group, chunk, begin, units;
+  const int group, block, chunk, begin, units;     // rows of a block; tiles of a round
   int per;                       // rounds that a unit's are rounded up to
   int at, before, total;         // the first of the 64; the line's length before them, theirs
-  DSL_DEV SharedLine(const KvCacheArgs &c, const SharedArgs &h, LineUnits &in, int group, int chunk, int what)
-      : c(c), h(h), in(in), group(group), chunk(chunk), begin(what & UNITS_PREFIX ? 0 : h.n),
+  DSL_DEV SharedLine(const KvCacheArgs &c, const SharedArgs &h, LineUnits &in, int group, int block, int chunk, int what)
+      : c(c), h(h), in(in), group(group), block(block), chunk(chunk), begin(what & UNITS_PREFIX ? 0 : h.n),
         units(what & UNITS_OWN ? h.n + c.seqs : h.n), per(1), at(begin - 64), before(0), total(0) {}
   // What the lanes have of the 64, rounds rounded up, into shared memory.
   DSL_DEV void put(int lane, int rounds, int blocks) {
@@ -153,7 +153,7 @@ struct SharedLine {
       const int tiles = len > s.off ? (len - s.off + kTile - 1) / kTile : 0;
       rounds = (tiles + chunk - 1) / chunk;
       if (u >= h.n && rounds == 0) rounds = 1;   // of no token: one, for its parts
-      blocks = rounds ? (int)(((int64_t)s.n * group + ROWS - 1) / ROWS) : 0;
+      blocks = rounds ? (int)(((int64_t)s.n * group + block - 1) / block) : 0;
     }
     put(lane, rounds, blocks);
     in.unit[lane] = s;
@@ -167,10 +167,13 @@ struct SharedLine {
   // The rounds of a run, of `runs` equal ones; back to the line's beginning.  A run that
   // holds the end of a unit and the beginning of the next takes up two (about 8 us):
   // units' rounds are rounded up to whole runs where runs no more than kPad rounds longer
-  // hold them so (prefixes of 30000 tokens, 32 samples: 44 us unrounded, ROUND rounded).
-  DSL_DEV int share(int runs) {
+  // hold them so (prefixes of 30000 tokens, 32 samples: 44 us unrounded, 39 rounded).
+  DSL_DEV int length() {
     while (at + 64 < units) advance();
-    const int least = one((before + total + runs - 1) / runs);
+    return one(before + total);
+  }
+  DSL_DEV int share(int runs) {
+    const int least = one((length() + runs - 1) / runs);
     if (least <= 1) {
       if (at > begin) rewind();
       return least;
@@ -268,19 +271,25 @@ DSL_DEV void join_waves(RowsJoin<Walk::D> &sh, const Walk &w, int rows, const G 
 // the row blocks of a head, which read the same tokens, share its L2.
 DSL_DEV int run_of(int block, int runs) { return runs % 8 == 0 ? block % 8 * (runs / 8) + block / 8 : block; }
 
+// What a workgroup's walk of a line needs of shared memory.
 template <class Walk>
-__global__ __launch_bounds__(256, Walk::WGS) void attn_shared_kernel(const KvCacheArgs c, const AttnArgs p,
-                                                                     const SharedArgs h, const SharedParts part,
-                                                                     const int chunk, const int what) {
+struct WalkRoom {
+  __align__(16) typename JoinOf<Walk>::type sh;
+  __align__(16) typename Walk::Queries queries;
+  int limit[Walk::ROWS];                         // (every wave writes all)
+  float2 row[Walk::NB][Walk::BLOCK];             // what a row's queries were divided by, the tokens it sees
+};
+
+// Run `run` of `runs` equal ones of a line.
+template <class Walk>
+DSL_DEV void walk_run(const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, const SharedParts &part, int chunk,
+                      SharedLine &line, WalkRoom<Walk> &room_, int run, int runs) {
   constexpr int D = Walk::D, ROWS = Walk::ROWS, BLOCK = Walk::BLOCK, NB = Walk::NB;
-  __shared__ __align__(16) typename JoinOf<Walk>::type sh;
-  __shared__ __align__(16) typename Walk::Queries queries;
-  __shared__ int s_limit[ROWS];                  // (every wave writes all)
-  __shared__ float2 s_row[NB][BLOCK];            // what a row's queries were divided by, the tokens it sees
-  __shared__ LineUnits s_units;
-  SharedLine<ROWS> line(c, h, s_units, p.group, chunk, what);
-  const int per = line.share((int)gridDim.x);
-  const int run = run_of(blockIdx.x, gridDim.x);
+  auto &sh = room_.sh;
+  auto &queries = room_.queries;
+  auto &s_limit = room_.limit;
+  auto &s_row = room_.row;
+  const int per = line.share(runs);
   int x = run * per;
   const int end = x + per;
 
@@ -401,6 +410,63 @@ __global__ __launch_bounds__(256, Walk::WGS) void attn_shared_kernel(const KvCac
   }
 }
 
+// Both kinds of units in one line.
+template <class Walk>
+__global__ __launch_bounds__(256, Walk::WGS) void attn_shared_kernel(const KvCacheArgs c, const AttnArgs p,
+                                                                     const SharedArgs h, const SharedParts part,
+                                                                     const int chunk, const int what) {
+  __shared__ WalkRoom<Walk> s_room;
+  __shared__ LineUnits s_units;
+  SharedLine line(c, h, s_units, p.group, Walk::ROWS, chunk, what);
+  walk_run<Walk>(c, p, h, part, chunk, line, s_room, run_of(blockIdx.x, gridDim.x), gridDim.x);
+}
+
+// Prefixes by some of the workgroups, 32 or 64 rows a wave, own tokens by the others, 16
+// rows a wave where no sequence has more.  (own_chunk 0: prefixes only.)  The workgroups
+// are dealt by what the lines take: a round of either as much where a head has at most 128
+// columns, one of own tokens twice that where it has 256; taking up a sequence's own tokens
+// 1.5 rounds, or 1.  (128 columns, 8 heads, 32 sequences of 4 rows and 200 tokens behind a
+// prefix of 10000 or 30000: 34 and 48 us; both kinds in one line of 64 rows 48 and 94, a
+// launch for each kind 40 and 53.  256 columns, 64 sequences behind 30000: 133 us, dealt
+// as for 128 columns 143.)
+template <class Walk, class Own>
+__global__ __launch_bounds__(256, 1) void attn_shared_two_kernel(const KvCacheArgs c, const AttnArgs p, const SharedArgs h,
+                                                                 const SharedParts part, const int chunk,
+                                                                 const int own_chunk) {
+  __shared__ union Room {
+    WalkRoom<Walk> prefix;
+    WalkRoom<Own> own;
+    DSL_DEV Room() {}
+  } s_room;
+  __shared__ LineUnits s_units;
+  const int runs = gridDim.x;
+  int few = 0;
+  if (own_chunk > 0) {
+    SharedLine own(c, h, s_units, p.group, Own::ROWS, own_chunk, UNITS_OWN);
+    few = own.length();
+  }
+  SharedLine prefix(c, h, s_units, p.group, Walk::ROWS, chunk, UNITS_PREFIX);
+  const float much = (float)prefix.length(), take = Walk::D <= 128 ? 1.5f : 1.f;
+  const float rest = (float)few * (Walk::D <= 128 ? 1.f : 2.f) + (float)c.heads * c.seqs * take;
+  const int step = runs % 8 ? 1 : 8;             // (whole pieces of the line for the XCDs)
+  int n = one((int)(much / (much + rest) * runs / step + 0.5f)) * step;
+  n = n < step ? step : n > runs - step ? runs - step : n;
+  if (much == 0.f) n = 0;
+  if (own_chunk == 0) n = runs;
+  const int block = blockIdx.x;
+  if constexpr (std::is_same_v<Walk, Own>) {
+    const bool mine = block < n;
+    SharedLine line(c, h, s_units, p.group, Walk::ROWS, chunk, mine ? UNITS_PREFIX : UNITS_OWN);
+    walk_run<Walk>(c, p, h, part, chunk, line, s_room.prefix, mine ? run_of(block, n) : run_of(block - n, runs - n),
+                   mine ? n : runs - n);
+  } else if (block < n) {
+    walk_run<Walk>(c, p, h, part, chunk, prefix, s_room.prefix, run_of(block, n), n);
+  } else {
+    SharedLine line(c, h, s_units, p.group, Own::ROWS, own_chunk, UNITS_OWN);
+    walk_run<Own>(c, p, h, part, own_chunk, line, s_room.own, run_of(block - n, runs - n), runs - n);
+  }
+}
+
 // Joins the parts of one query row and head in a workgroup, as attn.hip's does: a
 // part per thread for the maximum and the sum, then four columns per thread, the
 // parts dealt to 1024 / D threads of each.
@@ -475,32 +541,43 @@ struct SharedWalk {
   int rows, runs, chunk;
 };
 struct SharedPlan {
-  bool one;                      // launch for both kinds, as prefixes are walked
   SharedWalk prefix, own;
+  bool apart;                    // own tokens in a launch of their own
   size_t bytes;                  // of the workspace
   SharedParts parts;             // in a workspace at 0
 };
-static SharedWalk shared_walk(const KvCacheArgs &c, int64_t group, int64_t rows, int64_t kinds, int64_t many) {
-  SharedWalk a{};
-  a.rows = rows <= 16 ? 16 : rows <= 32 || c.dim > 128 ? 32 : 64;
-  const char *set = getenv("DSL_ATTN_SHARED_ROWS");    // read per launch (tests switch it)
-  if (set && (atoi(set) == 16 || atoi(set) == 32 || (atoi(set) == 64 && c.dim <= 128))) a.rows = atoi(set);
-  a.runs = (a.rows == 16 ? rows_wgs(c.dim, 1) : 1) * device_cu_count();
-  if (a.runs > kMaxRuns) a.runs = kMaxRuns;
+static SharedWalk shared_walk(const KvCacheArgs &c, int64_t group, int rows, int64_t kinds, int64_t many) {
+  SharedWalk a{rows, (rows == 16 ? rows_wgs(c.dim, 1) : 1) * device_cu_count(), 4};
+  a.runs = a.runs < 2 ? 2 : a.runs > kMaxRuns ? kMaxRuns : a.runs;
   // rounds of a tile per wave, longer ones where the line's length would pass an int
   const int64_t tiles = ((int64_t)c.width * c.page + kTile - 1) / kTile;
   const int64_t units = c.heads * (kinds * ((int64_t)c.rows * group / a.rows) + many);          // at most
-  a.chunk = 4;
   while ((tiles + a.chunk - 1) / a.chunk * units > 1 << 30 && a.chunk < tiles) a.chunk *= 2;
   return a;
+}
+static int shared_rows(const KvCacheArgs &c, int64_t rows) {
+  const char *set = getenv("DSL_ATTN_SHARED_ROWS");    // read per launch (tests switch it)
+  if (set && (atoi(set) == 16 || atoi(set) == 32 || (atoi(set) == 64 && c.dim <= 128))) return atoi(set);
+  // As many as a group has, but 64 above 64 only.  128 columns, 8 heads, behind 3000, 10000
+  // and 30000 tokens, with 64 rows: 16 a wave 17.5, 33 and 57 us, 32 a wave 19, 25 and 37,
+  // 64 a wave 24, 28 and 36; with 128 rows: 26, 54 and 116, 24, 34 and 61, 29, 33 and 47.
+  // 256 columns have no registers for 64.
+  return rows <= 16 ? 16 : rows <= 64 || c.dim > 128 ? 32 : 64;
 }
 static SharedPlan shared_plan(const KvCacheArgs &c, int groups, int q_heads, int max_q, int max_group) {
   SharedPlan a{};
   const int64_t group = q_heads / c.heads, most = (int64_t)max_q * max_group;
-  const int64_t rows = (most < c.rows ? most : c.rows) * group, own = (max_q < c.rows ? max_q : c.rows) * group;
-  a.one = rows <= 16 || groups == 0;
-  a.prefix = shared_walk(c, group, groups ? rows : own, a.one ? 2 : 1, (a.one ? c.seqs : 0) + (int64_t)groups);
-  a.own = a.one ? a.prefix : shared_walk(c, group, own, 1, c.seqs);
+  const int64_t own = (max_q < c.rows ? max_q : c.rows) * group;
+  const int rows = shared_rows(c, groups ? (most < c.rows ? most : c.rows) * group : own);
+  const bool same = rows == 16 || groups == 0;    // no prefixes, or both kinds of units in one line
+  a.prefix = shared_walk(c, group, rows, same ? 2 : 1, (same ? c.seqs : 0) + (int64_t)groups);
+  a.own = same ? a.prefix : shared_walk(c, group, own <= 16 ? 16 : rows, 1, c.seqs);
+  // Own tokens at the same time as the prefixes cost no launch of their own (6 to 10 us),
+  // but have a workgroup on a CU where two or more go: a launch of their own from more of
+  // them than CUs.  128 columns, 8 heads, behind 30000 tokens, 200 and 4000 own ones, at the
+  // same time and apart: 6 sequences 29 and 37 us, 33 and 39; 32: 47 and 55, 79 and 79;
+  // 64: 77 and 77, 153 and 137.
+  a.apart = !same && a.own.rows == 16 && (int64_t)c.heads * c.seqs > device_cu_count();
   const size_t n = (size_t)c.rows * q_heads;
   size_t at = 0;
   auto room = [&](size_t bytes) {
@@ -516,7 +593,7 @@ static SharedPlan shared_plan(const KvCacheArgs &c, int groups, int q_heads, int
     const SharedWalk &w = k ? a.own : a.prefix;
     a.parts.runs[k] = w.runs;
     a.parts.rows[k] = w.rows;
-    if (k && a.one) {
+    if (k && same) {
       a.parts.more[k] = a.parts.more[0];
       a.parts.more_ml[k] = a.parts.more_ml[0];
     } else {
@@ -532,21 +609,29 @@ size_t attn_shared_workspace_bytes(const KvCacheArgs &c, int groups, int q_heads
   return shared_plan(c, groups, q_heads, max_q, max_group).bytes;
 }
 
-template <int SRC, bool FP8, int D, bool WHOLE>
-static void launch_shared_tiles(const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, const SharedParts &parts,
-                                const SharedWalk &w, int what, hipStream_t st) {
-  const unsigned n = (unsigned)w.runs;
-  if (w.rows == 32) attn_shared_kernel<TileWalk<SRC, FP8, D, 1, WHOLE>><<<n, 256, 0, st>>>(c, p, h, parts, w.chunk, what);
-  else if constexpr (D <= 128)
-    attn_shared_kernel<TileWalk<SRC, FP8, D, 2, WHOLE>><<<n, 256, 0, st>>>(c, p, h, parts, w.chunk, what);
+template <class Walk, class Few>
+static void launch_shared_tiles(const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, const SharedPlan &a,
+                                hipStream_t st) {
+  const unsigned n = (unsigned)a.prefix.runs;
+  if (a.own.rows == 16) {
+    attn_shared_two_kernel<Walk, Few><<<n, 256, 0, st>>>(c, p, h, a.parts, a.prefix.chunk, a.apart ? 0 : a.own.chunk);
+    if (a.apart) attn_shared_kernel<Few><<<(unsigned)a.own.runs, 256, 0, st>>>(c, p, h, a.parts, a.own.chunk, UNITS_OWN);
+  } else attn_shared_two_kernel<Walk, Walk><<<n, 256, 0, st>>>(c, p, h, a.parts, a.prefix.chunk, a.own.chunk);
 }
 template <int SRC, bool FP8, int D>
-static void launch_shared_units(const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, const SharedParts &parts,
-                                const SharedWalk &w, int what, hipStream_t st) {
-  const unsigned n = (unsigned)w.runs;
-  if (w.rows == 16) attn_shared_kernel<FewWalk<SRC, FP8, D>><<<n, 256, 0, st>>>(c, p, h, parts, w.chunk, what);
-  else if (c.page >= kTile) launch_shared_tiles<SRC, FP8, D, true>(c, p, h, parts, w, what, st);
-  else launch_shared_tiles<SRC, FP8, D, false>(c, p, h, parts, w, what, st);
+static void launch_shared_units(const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, const SharedPlan &a,
+                                hipStream_t st) {
+  using Few = FewWalk<SRC, FP8, D>;
+  const bool whole = c.page >= kTile;
+  if (a.prefix.rows == 16) 
+    attn_shared_kernel<Few><<<(unsigned)a.prefix.runs, 256, 0, st>>>(c, p, h, a.parts, a.prefix.chunk, UNITS_PREFIX | UNITS_OWN);
+  else if (a.prefix.rows == 32) {
+    if (whole) launch_shared_tiles<TileWalk<SRC, FP8, D, 1, true>, Few>(c, p, h, a, st);
+    else launch_shared_tiles<TileWalk<SRC, FP8, D, 1, false>, Few>(c, p, h, a, st);
+  } else if constexpr (D <= 128) {
+    if (whole) launch_shared_tiles<TileWalk<SRC, FP8, D, 2, true>, Few>(c, p, h, a, st);
+    else launch_shared_tiles<TileWalk<SRC, FP8, D, 2, false>, Few>(c, p, h, a, st);
+  }
 }
 template <int SRC, bool FP8, int D>
 static hipError_t launch_shared_dim(const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, hipStream_t st) {
@@ -560,8 +645,7 @@ static hipError_t launch_shared_dim(const KvCacheArgs &c, const AttnArgs &p, con
     move(a.parts.more[k]);
     move(a.parts.more_ml[k]);
   }
-  launch_shared_units<SRC, FP8, D>(c, p, h, a.parts, a.prefix, a.one ? UNITS_PREFIX | UNITS_OWN : UNITS_PREFIX, st);
-  if (!a.one) launch_shared_units<SRC, FP8, D>(c, p, h, a.parts, a.own, UNITS_OWN, st);
+  launch_shared_units<SRC, FP8, D>(c, p, h, a, st);
   attn_shared_join_kernel<SRC, D><<<(unsigned)c.rows * (unsigned)p.q_heads, 256, 0, st>>>(p, a.parts);
   return hipGetLastError();
 }
