@@ -17,8 +17,10 @@
 // threads as `top`, so their words are read once more and everything else is not.
 // Keys are sorted 64 to a wave, and sorted runs are merged, best 64 kept.
 //
-// Bound by the logits' bytes.  Few rows are split over workgroups, and a second
-// launch joins the parts.
+// Bound by the logits' bytes: 3001 rows of 100003 in bf16 take 131 us, 4.6 TB/s (512
+// threads to a workgroup 150: more of it waits for the sorts; 128: 140).  Few rows are
+// split over workgroups, and a second launch joins the parts: 16 rows of 131071 in fp32
+// take 9.6 and 4.8 us, latency of launches, sums and sorts; the bytes would take 1.6.
 #include "common.h"
 #include "generate_args.h"
 #include "kv_core.h"
@@ -26,7 +28,7 @@
 
 namespace dsl {
 
-constexpr int kLogThreads = 512, kLogWaves = kLogThreads / 64;
+constexpr int kLogThreads = 256, kLogWaves = kLogThreads / 64;
 constexpr float kLog2eF = 1.44269504088896341f;
 constexpr double kLn2 = 0.693147180559945309417;
 
@@ -42,30 +44,60 @@ DSL_DEV float value_of(uint64_t key) {
   return u2f(u ^ ((u >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-// One step of a bitonic network over the wave: the larger of a pair to the lane
-// with `up`'s bit.
-DSL_DEV uint64_t exchange(uint64_t k, int j, bool larger) {
-  const uint64_t o = __shfl_xor((unsigned long long)k, j);
-  return (o > k) == larger ? o : k;
+// One step of a bitonic network over the wave: lane l and l ^ J, `larger` to keep the
+// larger key.  In registers: data-parallel moves up to 16 lanes, swaps of rows beyond (by
+// shuffles 16 rows' 20 best of 131071 took 24 us, so 19).
+template <int J>
+DSL_DEV uint64_t exchange(uint64_t k, bool larger) {
+  const uint32_t lo = (uint32_t)k, hi = (uint32_t)(k >> 32);
+  if constexpr (J >= 16) {
+    uint64_t a, b;                               // the pair's, in both lanes
+    if constexpr (J == 16) {
+      const auto l = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+      const auto h = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+      a = (uint64_t)h[0] << 32 | l[0];
+      b = (uint64_t)h[1] << 32 | l[1];
+    } else {
+      const auto l = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+      const auto h = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+      a = (uint64_t)h[0] << 32 | l[0];
+      b = (uint64_t)h[1] << 32 | l[1];
+    }
+    return (a > b) == larger ? a : b;
+  } else {
+    auto other = [](uint32_t v) {
+      if constexpr (J == 1) return __builtin_amdgcn_update_dpp(v, v, 0xb1, 0xf, 0xf, false);
+      if constexpr (J == 2) return __builtin_amdgcn_update_dpp(v, v, 0x4e, 0xf, 0xf, false);
+      if constexpr (J == 4) {                    // ^ 7, ^ 3
+        v = __builtin_amdgcn_update_dpp(v, v, 0x141, 0xf, 0xf, false);
+        return __builtin_amdgcn_update_dpp(v, v, 0x1b, 0xf, 0xf, false);
+      }
+      if constexpr (J == 8) return __builtin_amdgcn_update_dpp(v, v, 0x128, 0xf, 0xf, false);
+    };
+    const uint64_t o = (uint64_t)(uint32_t)other(hi) << 32 | (uint32_t)other(lo);
+    return (o > k) == larger ? o : k;
+  }
+}
+// Steps J, J / 2 .. 1 of runs of N lanes, falling and rising in turn (N 64: falling).
+template <int N, int J>
+DSL_DEV uint64_t exchanges(uint64_t k) {
+  const int lane = threadIdx.x & 63;
+  k = exchange<J>(k, ((lane & J) == 0) == ((lane & N) == 0));
+  if constexpr (J > 1) k = exchanges<N, J / 2>(k);
+  return k;
 }
 // The wave's keys in falling order.
 DSL_DEV uint64_t sort_wave(uint64_t k) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int n = 2; n <= 64; n <<= 1)
-#pragma unroll
-    for (int j = n >> 1; j > 0; j >>= 1) k = exchange(k, j, ((lane & j) == 0) == ((lane & n) == 0));
-  return k;
+  k = exchanges<2, 1>(k);
+  k = exchanges<4, 2>(k);
+  k = exchanges<8, 4>(k);
+  k = exchanges<16, 8>(k);
+  k = exchanges<32, 16>(k);
+  return exchanges<64, 32>(k);
 }
 // The best 64 of two runs in falling order, in falling order; b reversed: lane l
 // holds b[63 - l].
-DSL_DEV uint64_t merge_reversed(uint64_t a, uint64_t b) {
-  const int lane = threadIdx.x & 63;
-  uint64_t k = a > b ? a : b;
-#pragma unroll
-  for (int j = 32; j > 0; j >>= 1) k = exchange(k, j, (lane & j) == 0);
-  return k;
-}
+DSL_DEV uint64_t merge_reversed(uint64_t a, uint64_t b) { return exchanges<64, 32>(a > b ? a : b); }
 DSL_DEV uint64_t merge_wave(uint64_t a, uint64_t b) {
   return merge_reversed(a, __shfl((unsigned long long)b, 63 - (int)(threadIdx.x & 63)));
 }
@@ -234,7 +266,14 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(const LogprobArgs 
 #pragma unroll
     for (int u = 0; u < U; ++u) word(v[u], w + u * NT);
   }
-  for (; w < w1; w += NT) word(xw[w], w);
+  if (w < w1) {                                  // the rest, its loads together too
+    uint4 v[U - 1];
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u) v[u] = xw[w + u * NT < w1 ? w + u * NT : w];
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+      if (w + u * NT < w1) word(v[u], w + u * NT);
+  }
   // the elements of no whole word: a thread each
   int edge = -1;
   if (split == 0 && tid < head) edge = tid;
@@ -301,30 +340,36 @@ __global__ __launch_bounds__(kLogThreads) void logprob_kernel(const LogprobArgs 
   }
 }
 
-// A workgroup per row: its parts' sums and keys.
+// A workgroup per row: its parts' sums and keys, each part's already in falling order.
 template <int SRC>
-__global__ __launch_bounds__(256) void logprob_join_kernel(const LogprobArgs p, const int splits) {
-  __shared__ Sums s_sums[4];
-  __shared__ uint64_t s_runs[256];
+__global__ __launch_bounds__(kLogThreads) void logprob_join_kernel(const LogprobArgs p, const int splits) {
+  __shared__ Sums s_sums[kLogWaves];
+  __shared__ uint64_t s_runs[kLogThreads];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const LogParts part(p.ws, (int64_t)p.rows * splits);
+  const uint64_t *keys = part.keys + (int64_t)row * splits * p.top;
+  const int back = 63 - lane;
+  uint64_t kept = p.top && wave < splits && lane < p.top ? keys[wave * p.top + lane] : 0;
+  uint64_t next = p.top && wave + kLogWaves < splits && back < p.top ? keys[(wave + kLogWaves) * p.top + back] : 0;
   Sums v{-INFINITY, 0.0, 0.0};
-  for (int i = tid; i < splits; i += 256) v = join_sums(v, part.sums[(int64_t)row * splits + i]);
-  v = sums_of_group<4>(v, s_sums);
-  uint64_t kept = 0;
+  for (int i = tid; i < splits; i += kLogThreads) v = join_sums(v, part.sums[(int64_t)row * splits + i]);
+  v = sums_of_group<kLogWaves>(v, s_sums);
   if (p.top) {
-    const int n = splits * p.top;
-    const uint64_t *keys = part.keys + (int64_t)row * n;
-    for (int j = wave * 64; j < n; j += 256) kept = merge_wave(kept, sort_wave(j + lane < n ? keys[j + lane] : 0));
-    kept = merge_waves<4>(kept, s_runs);
+    for (int k = wave + kLogWaves; k < splits; k += kLogWaves) {
+      const uint64_t now = next;
+      if (k + kLogWaves < splits && back < p.top) next = keys[(k + kLogWaves) * p.top + back];
+      kept = merge_reversed(kept, now);
+    }
+    kept = merge_waves<kLogWaves>(kept, s_runs);
   }
-  write_row<SRC>(p, row, v, kept, tid, 256);
+  write_row<SRC>(p, row, v, kept, tid, kLogThreads);
 }
 
-// Parts of a row: two workgroups per CU, of 4096 words' worth of threads' loads at least.
+// Parts of a row: a workgroup per CU, of two words for each thread at least.  (16 rows of
+// 131071 in fp32: 14.4 us; two workgroups per CU 16.4.)
 static int logprob_splits(int src, int rows, int vocab) {
   const int words = vocab / (src == SRC_F32 ? 4 : 8);
-  int64_t s = (2 * (int64_t)device_cu_count() + rows - 1) / (rows > 0 ? rows : 1);
+  int64_t s = ((int64_t)device_cu_count() + rows - 1) / (rows > 0 ? rows : 1);
   const int64_t most = words / (2 * kLogThreads);
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
@@ -340,7 +385,7 @@ static hipError_t launch_logprobs_src(const LogprobArgs &p, hipStream_t st) {
   const unsigned grid = (unsigned)p.rows * (unsigned)splits;
   if (p.top) logprob_kernel<SRC, true><<<grid, kLogThreads, 0, st>>>(p, splits);
   else logprob_kernel<SRC, false><<<grid, kLogThreads, 0, st>>>(p, splits);
-  if (splits > 1) logprob_join_kernel<SRC><<<(unsigned)p.rows, 256, 0, st>>>(p, splits);
+  if (splits > 1) logprob_join_kernel<SRC><<<(unsigned)p.rows, kLogThreads, 0, st>>>(p, splits);
   return hipGetLastError();
 }
 hipError_t launch_logprobs(int src, const LogprobArgs &p, hipStream_t st) {
