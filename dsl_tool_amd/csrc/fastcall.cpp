@@ -590,18 +590,18 @@ struct CacheView {
   int fmt;
   int64_t pages, heads, page, dim, ld, width, seqs;
 };
-// a: k, v, k_scale, v_scale; then b: seq_lens, page_table, starts or None
+// a: k, v, k_scale, v_scale; then b: seq_lens (nullptr: a call without), page_table, starts or None
 bool cache_view(PyObject *const *a, PyObject *const *b, CacheView *c) {
   c->k = gpu_tensor(a[0]);
   c->v = gpu_tensor(a[1]);
   c->ks = gpu_tensor(a[2]);
   c->vs = gpu_tensor(a[3]);
-  c->lens = gpu_tensor(b[0]);
+  c->lens = b[0] ? gpu_tensor(b[0]) : nullptr;
   c->table = gpu_tensor(b[1]);
   c->starts = b[2] == Py_None ? nullptr : gpu_tensor(b[2]);
-  if (!c->k || !c->v || !c->ks || !c->vs || !c->lens || !c->table || (b[2] != Py_None && !c->starts)) return false;
+  if (!c->k || !c->v || !c->ks || !c->vs || (b[0] && !c->lens) || !c->table || (b[2] != Py_None && !c->starts)) return false;
   if (!plain(*c->k, 4) || !plain(*c->v, 4) || !is_scales(*c->ks, ScalarType::Float) ||
-      !is_scales(*c->vs, ScalarType::Float) || !is_scales(*c->lens, ScalarType::Int) || c->lens->dim() != 1 ||
+      !is_scales(*c->vs, ScalarType::Float) || (c->lens && (!is_scales(*c->lens, ScalarType::Int) || c->lens->dim() != 1)) ||
       c->table->scalar_type() != ScalarType::Int || c->table->dim() != 2 || c->table->numel() == 0 ||
       c->table->stride(1) != 1)
     return false;
@@ -612,14 +612,14 @@ bool cache_view(PyObject *const *a, PyObject *const *b, CacheView *c) {
   c->heads = c->k->size(1);
   c->page = c->k->size(2);
   c->dim = c->k->size(3);
-  c->seqs = c->lens->size(0);
+  c->seqs = c->lens ? c->lens->size(0) : c->table->size(0);
   c->width = c->table->size(1);
   c->ld = c->seqs > 1 ? c->table->stride(0) : c->width;
   const at::Device d = c->k->device();
   if (c->v->size(0) != c->pages || c->v->size(1) != c->heads || c->v->size(2) != c->dim || c->v->size(3) != c->page ||
       c->ks->dim() != 2 || c->ks->size(0) != c->pages || c->ks->size(1) != c->heads || c->vs->sizes() != c->ks->sizes() ||
       c->table->size(0) != c->seqs || c->ld < c->width || c->v->device() != d || c->ks->device() != d ||
-      c->vs->device() != d || c->lens->device() != d || c->table->device() != d)
+      c->vs->device() != d || (c->lens && c->lens->device() != d) || c->table->device() != d)
     return false;
   return !c->starts || (is_scales(*c->starts, ScalarType::Int) && c->starts->dim() == 1 &&
                         c->starts->size(0) == c->seqs + 1 && c->starts->device() == d);
@@ -789,6 +789,31 @@ PyObject *kv8_fork(PyObject *, PyObject *const *a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// kv8_compact(k_cache, v_cache, k_scale, v_scale, page_table, refs)
+PyObject *kv8_compact(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  CacheView c;
+  PyObject *const seqs[3] = {nullptr, n == 6 ? a[4] : nullptr, Py_None};
+  if (n != 6 || !cache_view(a, seqs, &c)) return none();
+  const Tensor *refs = int_vector(a[5], c.k->device(), c.pages);
+  if (!refs) return none();
+  Tensor table, counts, moved, live;
+  const bool ok = on_device(*c.k, [&] {
+    table = empty({c.seqs, c.width}, ScalarType::Int, *c.k);
+    counts = empty({c.pages}, ScalarType::Int, *c.k);
+    moved = empty({c.pages}, ScalarType::Int, *c.k);
+    live = empty({1}, ScalarType::Int, *c.k);
+    const size_t nb = dsl_kv8_compact_workspace_bytes(c.pages);
+    const Tensor ws = bytes((int64_t)nb, *c.k);
+    return dsl_kv8_compact(ptr(*c.k), ptr(*c.v), ptr<float>(*c.ks), ptr<float>(*c.vs), c.pages, c.heads, c.page, c.dim,
+                           ptr<int32_t>(*c.table), c.ld, c.width, c.seqs, ptr<int32_t>(*refs), ptr<int32_t>(table),
+                           ptr<int32_t>(counts), ptr<int32_t>(moved), ptr<int32_t>(live), ptr(ws), nb,
+                           stream_of(*c.k)) == DSL_OK;
+  });
+  return ok ? pack({table, counts, moved, live}) : none();
+  END_HANDLE_TH_ERRORS
+}
+
 // [rows][heads][dim] that the rotary kernel reads in place
 bool turned_heads(const Tensor *t) {
   return t && t->dim() == 3 && t->numel() > 0 && t->stride(2) == 1 && t->stride(1) >= t->size(2) && t->stride(0) >= 0;
@@ -877,7 +902,8 @@ PyMethodDef methods[] = {DSL_FN(quant_fp8_tensor), DSL_FN(quant_fp8_blocks), DSL
                          DSL_FN(swiglu_quant),     DSL_FN(moe_projection),   DSL_FN(lora_gemm),
                          DSL_FN(quant_fp8_rows_batched), DSL_FN(int8_gemm),        DSL_FN(quant_int8_rows), DSL_FN(add_rmsnorm_quant),
                          DSL_FN(kv8_write),        DSL_FN(kv8_read),         DSL_FN(kv8_attention),
-                         DSL_FN(kv8_shared_attention), DSL_FN(kv8_fork),     DSL_FN(rotary),           DSL_FN(token_logprobs),
+                         DSL_FN(kv8_shared_attention), DSL_FN(kv8_fork),     DSL_FN(kv8_compact),
+                         DSL_FN(rotary),           DSL_FN(token_logprobs),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "dsl_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

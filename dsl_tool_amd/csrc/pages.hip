@@ -78,9 +78,8 @@ DSL_DEV int valid_page(const ForkArgs &p, int a, int i) {
   const int v = p.table[(int64_t)a * p.table_ld + i];
   return v >= 0 && v < p.pages ? v : -1;
 }
-DSL_DEV Child child_of(const ForkArgs &p, int c) {
+DSL_DEV Child child_of(const ForkArgs &p, int a, int c) {
   Child k;
-  const int a = p.parents[c];
   k.parent = a >= 0 && a < p.seqs ? a : -1;
   const int n = k.parent < 0 ? 0 : p.lens[k.parent];
   k.len = n > 0 ? n : 0;
@@ -126,7 +125,7 @@ DSL_DEV void fork_rows(const ForkArgs &p, int64_t wave, int64_t waves) {
     }
   }
   for (int64_t c = wave; c < p.children; c += waves) {
-    const Child k = child_of(p, (int)c);
+    const Child k = child_of(p, p.parents[c], (int)c);
     const bool keeps = k.part >= 0 && ld_shared(s.first + k.parent) == (int)c;
     for (int i = lane; i < p.width; i += 64) {
       int v = -1;
@@ -142,40 +141,46 @@ DSL_DEV void fork_rows(const ForkArgs &p, int64_t wave, int64_t waves) {
 }
 // The k-th fresh entry that is asked for (by child, a copy before the new tokens')
 // gets the k-th free page.
-DSL_DEV void fork_give(const ForkArgs &p) {
+// (`kids` has the children, `keeper(a)` the first child of a sequence, `off` room for
+// children + 1 ranks.)
+template <class Kids, class Keeper>
+DSL_DEV void fork_give(const ForkArgs &p, const Kids &kids, const Keeper &keeper, int32_t *off) {
   __shared__ int64_t sh[kBook / 64];
   const ForkSpace s(p);
   const int tid = threadIdx.x;
   int64_t asked = 0, beyond = 0, copies = 0;
   for (int64_t c0 = 0; c0 < p.children; c0 += kBook) {
     const int64_t c = c0 + tid;
-    int64_t mine = 0, past = 0;
+    int64_t mine = 0;
     bool copied = false;
     int part = -1;
     if (c < p.children) {
-      const Child k = child_of(p, (int)c);
+      const Child k = kids((int)c);
       const int64_t e = k.end < p.width ? k.end : p.width;
       part = k.part;
-      copied = part >= 0 && ld_shared(s.first + k.parent) != (int)c;
+      copied = part >= 0 && keeper(k.parent) != (int)c;
       const int64_t fresh = e > k.begin ? e - k.begin : 0;
       mine = fresh + copied;
-      past = (k.end > k.begin ? k.end - k.begin : 0) - fresh;
+      beyond += (k.end > k.begin ? k.end - k.begin : 0) - fresh;
     }
-    int64_t all, out;
-    const int64_t rank = asked + scan_book(mine, all, sh);
-    scan_book(past, out, sh);
-    if (c < p.children) s.off[c] = (int)(rank < p.pages ? rank : p.pages);
-    asked += all;
-    beyond += out;
-    const int64_t cr = copies + scan_book((int64_t)copied, all, sh);
+    int64_t all;                                 // both ranks in one sum: copies of 1024 children below
+    const int64_t both = scan_book(mine * (2 * kBook) + copied, all, sh);
+    const int64_t rank = asked + both / (2 * kBook), cr = copies + both % (2 * kBook);
+    if (c < p.children) off[c] = (int)(rank < p.pages ? rank : p.pages);
+    asked += all / (2 * kBook);
     if (copied) {
       s.from[cr] = part;
       s.to[cr] = (int)(rank < p.pages ? rank : p.pages);   // its fresh page's rank, for now
     }
-    copies += all;
+    copies += all % (2 * kBook);
+  }
+  {
+    int64_t all;
+    scan_book(beyond, all, sh);
+    beyond = all;
   }
   const int need = (int)(asked < p.pages ? asked : p.pages);
-  if (tid == 0) s.off[p.children] = need;
+  if (tid == 0) off[p.children] = need;
   int found = 0;
   for (int64_t p0 = 0; p0 < p.pages && found < need; p0 += 4 * kBook) {
     int at[4], zeros = 0;
@@ -201,12 +206,12 @@ DSL_DEV void fork_give(const ForkArgs &p) {
     int lo = 0, hi = p.children;                 // off[lo] <= k < off[hi]
     while (hi - lo > 1) {
       const int mid = lo + (hi - lo) / 2;
-      if (s.off[mid] <= k) lo = mid;
+      if (off[mid] <= k) lo = mid;
       else hi = mid;
     }
-    const Child c = child_of(p, lo);
-    const bool copied = c.part >= 0 && ld_shared(s.first + c.parent) != lo;
-    const int j = k - s.off[lo], page = s.list[k];
+    const Child c = kids(lo);
+    const bool copied = c.part >= 0 && keeper(c.parent) != lo;
+    const int j = k - off[lo], page = s.list[k];
     p.out_table[(int64_t)lo * p.width + (copied && j == 0 ? c.full : c.begin + j - copied)] = page;
     st_shared(p.out_refs + page, 1);
   }
@@ -218,14 +223,64 @@ DSL_DEV void fork_give(const ForkArgs &p) {
   }
 }
 
+// All of it by one workgroup, for kBook sequences and children at most: what a child and a
+// sequence are in shared memory, a thread per table entry, four entries' loads at a time.
 __global__ __launch_bounds__(kBook) void fork_book_kernel(const ForkArgs p) {
-  fork_clear(p, threadIdx.x, kBook);
+  __shared__ int s_count[kBook], s_first[kBook], s_len[kBook], s_off[kBook + 1];
+  __shared__ Child s_child[kBook];
+  const int tid = threadIdx.x;
+  for (int i = tid; i < p.pages; i += kBook) st_shared(p.out_refs + i, p.refs[i]);
+  s_count[tid] = 0;
+  s_first[tid] = 0x7fffffff;
+  const int n = tid < p.seqs ? p.lens[tid] : 0;
+  s_len[tid] = n > 0 ? n : 0;
+  __syncthreads();
+  if (tid < p.children) {
+    const Child k = child_of(p, p.parents[tid], tid);
+    s_child[tid] = k;
+    if (k.parent >= 0) {
+      atomicAdd(&s_count[k.parent], 1);
+      atomicMin(&s_first[k.parent], tid);
+    }
+    const int64_t len = (int64_t)k.len + k.more;
+    p.out_lens[tid] = (int)(len < 0x7fffffff ? len : 0x7fffffff);
+  }
   phase_end();
-  fork_count(p, threadIdx.x, kBook);
+  constexpr int U = 4;
+  const int old = p.seqs * p.width, held = p.children * p.width;
+  for (int e0 = tid; e0 < old; e0 += U * kBook) {
+    int v[U], row[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * kBook;
+      row[u] = e / p.width;
+      v[u] = e < old ? valid_page(p, row[u], e - row[u] * p.width) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (v[u] < 0) continue;
+      const int i = e0 + u * kBook - row[u] * p.width, len = s_len[row[u]], whole = len / p.page, kids = s_count[row[u]];
+      const int now = i < whole ? kids : (i == whole && len % p.page != 0 && kids > 0 ? 1 : 0);
+      if (now != 1) add_shared(p.out_refs + v[u], now - 1);
+    }
+  }
+  for (int e0 = tid; e0 < held; e0 += U * kBook) {
+    int v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * kBook, c = e < held ? e / p.width : 0, i = e - c * p.width;
+      const Child &k = s_child[c];
+      v[u] = -1;
+      if (e >= held) continue;
+      if (i < k.full) v[u] = valid_page(p, k.parent, i);
+      else if (i == k.full && k.part >= 0 && s_first[k.parent] == c) v[u] = k.part;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (e0 + u * kBook < held) p.out_table[e0 + u * kBook] = v[u];
+  }
   phase_end();
-  fork_rows(p, threadIdx.x >> 6, kBook / 64);
-  phase_end();
-  fork_give(p);
+  fork_give(p, [&](int c) { return s_child[c]; }, [&](int a) { return s_first[a]; }, s_off);
 }
 __global__ __launch_bounds__(256) void fork_clear_kernel(const ForkArgs p) {
   fork_clear(p, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)gridDim.x * 256);
@@ -236,7 +291,10 @@ __global__ __launch_bounds__(256) void fork_count_kernel(const ForkArgs p) {
 __global__ __launch_bounds__(256) void fork_rows_kernel(const ForkArgs p) {
   fork_rows(p, (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), (int64_t)gridDim.x * 4);
 }
-__global__ __launch_bounds__(kBook) void fork_give_kernel(const ForkArgs p) { fork_give(p); }
+__global__ __launch_bounds__(kBook) void fork_give_kernel(const ForkArgs p) {
+  const ForkSpace s(p);
+  fork_give(p, [&](int c) { return child_of(p, p.parents[c], c); }, [&](int a) { return ld_shared(s.first + a); }, s.off);
+}
 
 // ----------------------------------------------------------------- copies --
 // Piece `at` of a page: keys, then values; scales with the first.
@@ -246,20 +304,19 @@ DSL_DEV void copy_piece(const PageArgs &c, int from, int to, int64_t at) {
   const int64_t begin = (vals ? at - half : at) * kPiece;
   const int64_t n = c.bytes - begin < kPiece ? c.bytes - begin : kPiece;
   uint8_t *base = (vals ? c.v : c.k) + begin;
-  const uint4 *x = reinterpret_cast<const uint4 *>(base + (int64_t)from * c.bytes);
-  uint4 *y = reinterpret_cast<uint4 *>(base + (int64_t)to * c.bytes);
+  const v4i *x = reinterpret_cast<const v4i *>(base + (int64_t)from * c.bytes);
+  v4i *y = reinterpret_cast<v4i *>(base + (int64_t)to * c.bytes);
   const int words = (int)(n >> 4);
   constexpr int U = kPiece / 16 / 256;
-  uint4 v[U];
+  const int tid = threadIdx.x;
+  if (words == U * 256) {
+    v4i v[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = threadIdx.x + 256 * u;
-    v[u] = x[i < words ? i : 0];
-  }
+    for (int u = 0; u < U; ++u) v[u] = x[tid + 256 * u];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = threadIdx.x + 256 * u;
-    if (i < words) y[i] = v[u];
+    for (int u = 0; u < U; ++u) y[tid + 256 * u] = v[u];
+  } else {
+    for (int i = tid; i < words; i += 256) y[i] = x[i];
   }
   if (at == 0)
     for (int i = threadIdx.x; i < c.heads; i += 256) {
@@ -285,7 +342,7 @@ static unsigned blocks_for(int64_t items, int64_t each, int64_t most) {
 
 hipError_t launch_fork(const PageArgs &c, const ForkArgs &p, hipStream_t st) {
   const int64_t entries = (int64_t)(p.seqs + p.children) * p.width, most = 8 * (int64_t)device_cu_count();
-  if (entries + p.pages <= kSmallWork) {
+  if (entries + p.pages <= kSmallWork && p.seqs <= kBook && p.children <= kBook) {
     fork_book_kernel<<<1, kBook, 0, st>>>(p);
   } else {
     const int64_t flat = p.pages > p.seqs ? p.pages : p.seqs;
@@ -314,6 +371,7 @@ __global__ __launch_bounds__(kBook) void compact_book_kernel(const CompactArgs p
   const CompactSpace s(p);
   const int tid = threadIdx.x;
   int mine = 0;
+#pragma unroll 4
   for (int64_t i = tid; i < p.pages; i += kBook) mine += p.refs[i] > 0;
   int64_t n;
   scan_book((int64_t)mine, n, sh);

@@ -259,6 +259,9 @@ def kv8_compact(cache: KV8Cache, page_table: torch.Tensor, refs: torch.Tensor) -
     go, in order, to the free pages before it, and the rest stay.  Table and
     counts come in the new numbers, as new tensors; ``moved`` renumbers whatever
     else holds pages."""
+    r = N.fast().kv8_compact(*cache, page_table, refs)
+    if r is not None:
+        return KV8Compact(*r)
     if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
         raise ValueError("kv8_compact: page_table must be [seqs, width]")
     seqs = page_table.shape[0]
