@@ -431,7 +431,8 @@ struct TileWalk {
   static DSL_DEV void times(v4i &p, float by) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const v2h x = __builtin_bit_cast(v2h, p[w]);
+      const int both = p[w];                     // (a bit cast of the element itself takes element 0's bits)
+      const v2h x = __builtin_bit_cast(v2h, both);
       p[w] = (int)pack_f16x2((float)x[0] == 0.f ? 0.f : (float)x[0] * by, (float)x[1] == 0.f ? 0.f : (float)x[1] * by);
     }
   }
