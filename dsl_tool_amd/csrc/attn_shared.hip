@@ -448,7 +448,7 @@ __global__ __launch_bounds__(256, 1) void attn_shared_two_kernel(const KvCacheAr
   SharedLine prefix(c, h, s_units, p.group, Walk::ROWS, chunk, UNITS_PREFIX);
   const float much = (float)prefix.length(), take = Walk::D <= 128 ? 1.5f : 1.f;
   const float rest = (float)few * (Walk::D <= 128 ? 1.f : 2.f) + (float)c.heads * c.seqs * take;
-  const int step = runs % 8 ? 1 : 8;             // (whole pieces of the line for the XCDs)
+  const int step = runs % 8 || runs < 16 ? 1 : 8;          // (whole pieces of the line for the XCDs)
   int n = one((int)(much / (much + rest) * runs / step + 0.5f)) * step;
   n = n < step ? step : n > runs - step ? runs - step : n;
   if (much == 0.f) n = 0;
@@ -468,7 +468,7 @@ __global__ __launch_bounds__(256, 1) void attn_shared_two_kernel(const KvCacheAr
 }
 
 // Joins the parts of one query row and head in a workgroup, as attn.hip's does: a
-// part per thread for the maximum and the sum, then four columns per thread, the
+// part per lane for the maximum and the sum, then four columns per thread, the
 // parts dealt to 1024 / D threads of each.
 template <int SRC, int D>
 __global__ __launch_bounds__(256) void attn_shared_join_kernel(const AttnArgs p, const SharedParts part) {
@@ -498,38 +498,58 @@ __global__ __launch_bounds__(256) void attn_shared_join_kernel(const AttnArgs p,
     return b >= 0 ? part.first_ml[b] : part.more_ml[s < np ? 0 : 1][run_row(s)];
   };
   float top = -INFINITY, l = 0.f;
-  for (int s = tid; s < parts; s += 256) {
-    const float m = max_sum(s).x;
-    s_f[s] = m;
-    top = fmaxf(top, m);
-  }
+  auto weight = [&](const float2 &ml) {
+    const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+    l += ml.y * f;
+    return f;
+  };
+  const float *weights = s_f;
+  // Up to 64 parts each wave looks through all, without barriers (3808 rows and heads of 64
+  // columns: 7.6 us, with them 9.0).
+  const bool few = parts <= 64;
+  if (few) {
+    const int lane = tid & 63, wave = tid >> 6;
+    const float2 ml = lane < parts ? max_sum(lane) : make_float2(-INFINITY, 0.f);
+    top = ml.x;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if ((tid & 63) == 0) s_red[tid >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-  for (int s = tid; s < parts; s += 256) {
-    const float m = s_f[s], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-    s_f[s] = f;
-    l += max_sum(s).y * f;
-  }
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    s_f[wave * 64 + lane] = weight(ml);
+    weights = s_f + wave * 64;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
-  if ((tid & 63) == 0) s_red[4 + (tid >> 6)] = l;
-  __syncthreads();
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+  } else {
+    constexpr int U = 2 * kMaxRuns / 256;
+    float2 ml[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      ml[u] = tid + 256 * u < parts ? max_sum(tid + 256 * u) : make_float2(-INFINITY, 0.f);
+      top = fmaxf(top, ml[u].x);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if ((tid & 63) == 0) s_red[tid >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+#pragma unroll
+    for (int u = 0; u < U; ++u) s_f[tid + 256 * u] = weight(ml[u]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+    if ((tid & 63) == 0) s_red[4 + (tid >> 6)] = l;
+    __syncthreads();
+    l = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
+  }
   const int cg = tid % CG, sl = tid / CG;
   v4f v = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = sl; s < parts; s += SL) {
     const int64_t b = beginning(s);
-    v += *reinterpret_cast<const v4f *>((b >= 0 ? part.first + b * D : part.more[s < np ? 0 : 1] + run_row(s) * D) + cg * 4) * s_f[s];
+    v += *reinterpret_cast<const v4f *>((b >= 0 ? part.first + b * D : part.more[s < np ? 0 : 1] + run_row(s) * D) + cg * 4) * weights[s];
   }
   s_v[sl][cg] = v;
   __syncthreads();
   if (tid >= CG) return;
 #pragma unroll
   for (int k = 1; k < SL; ++k) v += s_v[k][cg];
-  l = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
   const float inv = l > 0.f ? 1.0f / l : 0.f;    // a row that sees nothing is 0
   uint16_t *op = static_cast<uint16_t *>(p.o) + (at / p.q_heads) * p.o_row + (at % p.q_heads) * p.o_head + cg * 4;
   *reinterpret_cast<uint2 *>(op) = make_uint2(narrow2<SRC>(v[0] * inv, v[1] * inv), narrow2<SRC>(v[2] * inv, v[3] * inv));

@@ -115,6 +115,8 @@ int dsl_kv8_fork(void *k_cache, void *v_cache, float *k_scale, float *v_scale, i
     return fail(DSL_ERR_ARG, "%s: the new table and counts must not be the old ones", fn);
   if ((rc = check_workspace(fn, workspace, workspace_bytes, dsl_kv8_fork_workspace_bytes(seqs, width, children, pages))))
     return rc;
+  if (seqs > 0 && children > 0 && seq_lens == out_lens)
+    return fail(DSL_ERR_ARG, "%s: the new lengths must not be the old ones", fn);
   dsl::ForkArgs p{};
   p.lens = seq_lens;
   p.table = table;

@@ -67,6 +67,11 @@ def test_fork(lib):
     assert lib.dsl_kv8_fork_workspace_bytes(3, 5, 4, 10) > 0
 
 
+def test_fork_in_place(lib):
+    args = list(FORK)
+    refused(lib, "dsl_kv8_fork", args, -1, "new lengths")      # seq_lens are out_lens
+
+
 def test_compact(lib):
     good = [P, P, P, P, 10, 2, 64, 128, P, 5, 5, 3, P, Q, Q, P, P, P, 1 << 20, None]
     refuse_each(lib, "dsl_kv8_compact", good, [
