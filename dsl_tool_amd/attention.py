@@ -87,9 +87,14 @@ def kv8_shared_attention(q: torch.Tensor, cache: KV8Cache, seq_lens: torch.Tenso
     that is as long, and what lies behind it by each sequence's own.  Sequences
     outside every group share nothing.  ``max_group``, the most sequences of a
     group (default: all of them), sizes the launch with ``max_q_len``; a wrong one costs
-    speed and changes no more than roundings.  Few sequences behind a short prefix (six of
-    four heads to a cache head behind 1000 tokens) are faster by :func:`kv8_attention`.
-    Everything else, ``out`` and the rows that see nothing included, is as there.
+    speed and changes no more than roundings.  Everything else, ``out`` and the rows that
+    see nothing included, is as in :func:`kv8_attention`.
+
+    Sequences of many new tokens (more than 96 query rows to a cache head, or 64 of 64
+    columns, by ``max_q_len``, so give it) fill the matrix units by themselves and are
+    computed as by :func:`kv8_attention`, which is also faster for few sequences behind
+    a short prefix (six of four heads to a cache head behind 1000 tokens).  The workspace
+    is eight bytes for each element of q, up to 32 MB more.
     """
     if out is None:
         r = N.fast().kv8_shared_attention(q, *cache, seq_lens, page_table, q_starts, max_q_len, scale, causal,

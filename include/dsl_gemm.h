@@ -454,10 +454,11 @@ size_t dsl_kv8_attention_workspace_bytes(int64_t heads, int64_t page, int64_t di
  * (ascending) hold the same pages for their first shared_lens[g] tokens: that prefix,
  * cut to whole pages, is read once for the group instead of once for each
  * sequence, from the table row of its first sequence that is as long (else its
- * longest).  The result is dsl_kv8_attention's but for the order of the sums.
+ * longest).  The result is dsl_kv8_attention's but for roundings.
  * Sequences outside every group share nothing.  max_group (most sequences of a group)
- * sizes the launch with max_q; wrong numbers cost time only.  rows x q_heads at most
- * 2^22; the workspace is never empty. */
+ * sizes the launch with max_q; wrong numbers cost time and change roundings only.
+ * With more than 96 rows of max_q x q_heads / heads (64 of dim 64) nothing is shared.
+ * rows x q_heads at most 2^22; the workspace is never empty. */
 int dsl_kv8_shared_attention(const void *q, int64_t q_row, int64_t q_head, int64_t q_heads,
                              const void *k_cache, const void *v_cache, const float *k_scale,
                              const float *v_scale, int64_t pages, int64_t heads, int64_t page,
