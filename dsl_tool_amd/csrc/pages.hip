@@ -224,16 +224,23 @@ DSL_DEV void fork_give(const ForkArgs &p, const Kids &kids, const Keeper &keeper
 }
 
 // All of it by one workgroup, for kBook sequences and children at most: what a child and a
-// sequence are in shared memory, a thread per table entry, four entries' loads at a time.
+// sequence are in shared memory, a thread per table entry, four or eight loads at a time.
 __global__ __launch_bounds__(kBook) void fork_book_kernel(const ForkArgs p) {
-  __shared__ int s_count[kBook], s_first[kBook], s_len[kBook], s_off[kBook + 1];
+  __shared__ int s_count[kBook], s_first[kBook], s_whole[kBook], s_off[kBook + 1];
   __shared__ Child s_child[kBook];
   const int tid = threadIdx.x;
-  for (int i = tid; i < p.pages; i += kBook) st_shared(p.out_refs + i, p.refs[i]);
+  for (int i0 = tid; i0 < p.pages; i0 += 8 * kBook) {
+    int v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = i0 + u * kBook < p.pages ? p.refs[i0 + u * kBook] : 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i0 + u * kBook < p.pages) st_shared(p.out_refs + i0 + u * kBook, v[u]);
+  }
   s_count[tid] = 0;
   s_first[tid] = 0x7fffffff;
-  const int n = tid < p.seqs ? p.lens[tid] : 0;
-  s_len[tid] = n > 0 ? n : 0;
+  const int n = tid < p.seqs && p.lens[tid] > 0 ? p.lens[tid] : 0;
+  s_whole[tid] = n / p.page * 2 + (n % p.page != 0);           // whole pages, and whether there is a part of one
   __syncthreads();
   if (tid < p.children) {
     const Child k = child_of(p, p.parents[tid], tid);
@@ -246,21 +253,22 @@ __global__ __launch_bounds__(kBook) void fork_book_kernel(const ForkArgs p) {
     p.out_lens[tid] = (int)(len < 0x7fffffff ? len : 0x7fffffff);
   }
   phase_end();
-  constexpr int U = 4;
+  constexpr int U = 8;
   const int old = p.seqs * p.width, held = p.children * p.width;
+  const float inv = 1.0f / (float)p.width;       // (e + 0.5) inv is within e 2^-22 / width of its value, so right below 2^21
   for (int e0 = tid; e0 < old; e0 += U * kBook) {
     int v[U], row[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int e = e0 + u * kBook;
-      row[u] = e / p.width;
+      row[u] = (int)(((float)e + 0.5f) * inv);
       v[u] = e < old ? valid_page(p, row[u], e - row[u] * p.width) : -1;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (v[u] < 0) continue;
-      const int i = e0 + u * kBook - row[u] * p.width, len = s_len[row[u]], whole = len / p.page, kids = s_count[row[u]];
-      const int now = i < whole ? kids : (i == whole && len % p.page != 0 && kids > 0 ? 1 : 0);
+      const int i = e0 + u * kBook - row[u] * p.width, has = s_whole[row[u]], whole = has >> 1, kids = s_count[row[u]];
+      const int now = i < whole ? kids : (i == whole && (has & 1) && kids > 0 ? 1 : 0);
       if (now != 1) add_shared(p.out_refs + v[u], now - 1);
     }
   }
@@ -268,7 +276,7 @@ __global__ __launch_bounds__(kBook) void fork_book_kernel(const ForkArgs p) {
     int v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int e = e0 + u * kBook, c = e < held ? e / p.width : 0, i = e - c * p.width;
+      const int e = e0 + u * kBook, c = e < held ? (int)(((float)e + 0.5f) * inv) : 0, i = e - c * p.width;
       const Child &k = s_child[c];
       v[u] = -1;
       if (e >= held) continue;

@@ -320,3 +320,24 @@ def test_long_cache():
     first = O.attention(q, small, ints(lens), table)[0]
     for child, parent in enumerate((1, 0, 1, 2)):
         assert torch.allclose(o[child], first[parent], rtol=1e-10, atol=1e-12)
+
+
+def test_long_groups_of_short_sequences(wide):
+    """100 sequences that all are shorter than their group's prefix, the longest among the last:
+    it is the one whose row has the prefix."""
+    lens, table, groups, shared, pages = forked([(640, [-640 + 3 * b for b in range(90)] + [-70, -1, -300] + [-640] * 7)],
+                                                16, 470)
+    cache = random_cache(pages, 1, 64, 16, "int8", 471)
+    check_shared(randn((100, 2, 64), 472, torch.bfloat16), cache, lens, table, groups, shared)
+
+
+def test_wide_table(wide):
+    """A table far wider than any sequence, whose rounds would pass an int in steps of four tiles."""
+    lens, table, groups, shared, pages = forked([(900, [1 + 5 * b for b in range(64)])], 256, 480)
+    cache = random_cache(pages, 8, 64, 256, "int8", 481)
+    q = randn((64, 8, 64), 482, torch.float16)
+    far = torch.full((64, 1 << 22), -1, dtype=torch.int32, device=DEV)
+    far[:, :table.shape[1]] = table.to(DEV)
+    got = A.kv8_shared_attention(q.to(DEV), to(cache, DEV), ints(lens).to(DEV), far, ints(groups).to(DEV),
+                                 ints(shared).to(DEV), max_group=64)
+    within(got, *O.attention(q, cache, ints(lens), table))
