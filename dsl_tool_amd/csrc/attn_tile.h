@@ -315,11 +315,13 @@ struct TileWalk {
     };
     v4i pf[NB][2][2], pl[F16 ? NB : 1][2][2];    // P, tokens 8 z .. + 7 of the lane's 16 (pl: their low parts)
     float sum[NB][2];
-    // True where a sum has grown past what fp16 holds.
+    // True where a sum has grown past what fp16 holds, or a row has no maximum: all that it
+    // has seen were missing pages or scores of -infinity.
     auto exponentials = [&]() __attribute__((always_inline)) {
       bool grown = false;
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+      for (int b = 0; b < NB; ++b) {
+        grown |= m[b] == -INFINITY;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const float off = kLift + lv[t] - (m[b] == -INFINITY ? 0.f : m[b]);
@@ -342,6 +344,7 @@ struct TileWalk {
               }
             }
         }
+      }
       return __any(grown) != 0;
     };
     auto output = [&]() __attribute__((always_inline)) {
