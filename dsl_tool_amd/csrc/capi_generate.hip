@@ -235,7 +235,7 @@ int dsl_token_logprobs(const void *logits, int64_t rows, int64_t vocab, int64_t 
   if (ld < vocab && rows > 1) return fail(DSL_ERR_ARG, "%s: ld=%lld < vocab", fn, (long long)ld);
   if (n_ids < 0 || n_ids > 1 << 20 || (ids_ld < n_ids && rows > 1))
     return fail(DSL_ERR_ARG, "%s: need 0 .. 2^20 ids of a row, rows at least as far apart", fn);
-  if (!(scale > 0.f) || !(scale - scale == 0.f)) return fail(DSL_ERR_ARG, "%s: scale must be finite and > 0", fn);
+  if (!(scale > 0.f && scale < 0x1p126f)) return fail(DSL_ERR_ARG, "%s: scale must be > 0 and below 2^126", fn);
   if (rows == 0) return ok();
   if (!logits || !aligned(logits, x_dtype == DSL_IN_F32 ? 4 : 2))
     return fail(DSL_ERR_ARG, "%s: logits are NULL or misaligned", fn);

@@ -24,12 +24,14 @@ class TokenLogprobs(NamedTuple):
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None = None, *, top: int = 0,
                    scale: float = 1.0) -> TokenLogprobs:
     """Of ``softmax(scale * logits)``, ``logits [rows, vocab]`` bf16, fp16 or
-    fp32 (``scale``: 1 / temperature): natural log probabilities of the tokens ``ids``
+    fp32 (``scale``: 1 / temperature, below 2^126): natural log probabilities of the tokens ``ids``
     (int32, ``[rows]`` or ``[rows, n]``; None: none, ``logp [rows, 0]``), the entropy, and the
     ``top`` (up to 32) likeliest tokens, ties by the lowest number.
 
     Logits of -inf (tokens that are not allowed) have probability 0, log -inf;
-    so have ids outside the vocabulary.  A row of nothing else has entropy 0.  NaN or
+    so have ids outside the vocabulary.  A row of nothing else has entropy 0.  Finite logits of any
+    size are what they are: tokens masked by the type's lowest value have about that for their
+    log probability, and a row of nothing else is uniform.  NaN or
     +inf make all of a row's results NaN but ``top_ids``.
     """
     r = N.fast().token_logprobs(logits, ids, top, scale)
@@ -47,8 +49,8 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor | None = None, *, top
     if not isinstance(top, int) or isinstance(top, bool) or not 0 <= top <= min(TOP, vocab):
         raise ValueError(f"token_logprobs: top must be 0 .. {min(TOP, vocab)} (got {top!r})")
     scale = float(scale)
-    if not 0 < scale < float("inf"):
-        raise ValueError(f"token_logprobs: scale must be finite and > 0 (got {scale!r})")
+    if not 0 < scale < 2.0 ** 126:
+        raise ValueError(f"token_logprobs: scale must be > 0 and below 2^126 (got {scale!r})")
     dev = logits.device
     if ids is None:
         ids = torch.empty((rows, 0), dtype=torch.int32, device=dev)

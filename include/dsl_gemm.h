@@ -527,7 +527,7 @@ int dsl_rotary(const void *q, int64_t q_row, int64_t q_head, int64_t q_heads, co
 /* Of softmax(scale * logits) by rows (bf16, fp16 or fp32, ld apart): logp
  * [rows][n_ids] of the tokens ids[row * ids_ld + i], entropy [rows], and the `top`
  * (0 .. 32) largest logits' log probabilities and numbers [rows][top], falling, ties
- * by lowest number (NaN after the others).  Natural logarithms.  A logit of -inf has
+ * by lowest number (NaN after the others).  Natural logarithms; 0 < scale < 2^126.  A logit of -inf has
  * probability 0 (log -inf), as has an id outside [0, vocab); where all are -inf the
  * entropy is 0.  NaN or +inf in a row make all its entropy and log probabilities NaN. */
 int dsl_token_logprobs(const void *logits, int64_t rows, int64_t vocab, int64_t ld, int x_dtype,

@@ -102,11 +102,12 @@ def logprobs(logits, ids, top, scale=1.0):
     entropy = torch.zeros(rows, dtype=torch.float64)
     best, at = torch.full((rows, top), -math.inf, dtype=torch.float64), torch.zeros((rows, top), dtype=torch.int32)
     for r in range(rows):
-        z = logits[r].double() * scale
         order = sorted(range(vocab), key=lambda i: (-logits[r, i].item(), i))[:top]
         at[r] = torch.tensor(order, dtype=torch.int32)
-        if z.max() == -math.inf:
+        most = logits[r].double().max()
+        if most == -math.inf:
             continue
+        z = (logits[r].double() - most) * scale         # (differences first: those of logits next to 1e38 matter)
         z = z - z.logsumexp(0)
         p = z.exp()
         entropy[r] = -(p * z)[p > 0].sum()

@@ -1,11 +1,14 @@
 """Several continuations of a prompt at their edges on the GPU: pages that are missing before
-others and scores that overflow, with every number of query rows a wave."""
+others and scores that overflow, with every number of query rows a wave; logits of any size."""
+import math
 import random
 
 import pytest
 import torch
 
 from dsl_tool_amd import attention as A
+from dsl_tool_amd import logprobs as LP
+from oracle import generating as GO
 from oracle import serving as O
 from tests.test_gpu_generate import check_shared, forked, ints, spoil
 from tests.test_gpu_generate_steps import wide  # noqa: F401
@@ -93,3 +96,29 @@ def test_shared_scores_that_overflow_below(dim, fmt, wide):
     args = [ints(lens).to(DEV), table.to(DEV), ints(groups).to(DEV), ints(shared).to(DEV)]
     got = A.kv8_shared_attention(q.to(DEV), to(cache, DEV), *args)
     within(got, *O.attention(q, cache, ints(lens), others))
+
+
+# -------------------------------------------------------------- logits of any size --
+
+@pytest.mark.parametrize("scale", [1.0, 0.5, 1.25, 2.0 ** -120, 2.0 ** -140, 2.0 ** 100])
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("vocab", [9, 1003, 40000])
+def test_logprobs_of_logits_of_any_size(vocab, src, scale):
+    """Rows that are masked by the type's lowest value, in part or all of them, of very low and
+    very high ones, and from one end of the type to the other.  The tolerance: the result's rounding
+    and that of its terms, 2^-22; 2^-19 for the sums."""
+    least, most = torch.finfo(src).min, torch.finfo(src).max
+    i = torch.arange(vocab, dtype=torch.float64)
+    rows = [torch.full((vocab,), v, dtype=torch.float64) for v in (least, most, least / 2, -1e10, 1e10, -1e30, 1e30, -2e4)]
+    rows += [torch.where(i % 5 == 2, i % 3, least), torch.where(i == vocab - 2, most, least), torch.where(i % 2 == 0, least, -math.inf),
+             least + (most / vocab * 2) * i, least * (1 - (i % 7) / 64), most * (1 - (i % 7) / 64)]
+    x = torch.stack(rows).clamp(least, most).where(torch.stack(rows) != -math.inf, -math.inf).to(src)
+    ids = torch.tensor([[0, 1, vocab // 2, vocab - 2, vocab - 1]] * len(rows), dtype=torch.int32)
+    top = min(7, vocab)
+    got = LP.token_logprobs(x.to(DEV), ids.to(DEV), top=top, scale=scale)
+    want = GO.logprobs(x, ids, top, scale)
+    assert torch.equal(got.top_ids.cpu(), want[3])
+    for g, w in ((got.logp, want[0]), (got.entropy, want[1]), (got.top_logp, want[2])):
+        g, none = g.cpu(), w.float().isneginf()
+        assert torch.equal(g.isneginf(), none)
+        assert ((g.double() - w)[~none].abs() <= w[~none].abs() * 2.0 ** -22 + 2.0 ** -19).all()
