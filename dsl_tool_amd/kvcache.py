@@ -218,10 +218,13 @@ def kv8_fork(cache: KV8Cache, seq_lens: torch.Tensor, page_table: torch.Tensor, 
     ``new`` more tokens (a number, or ``[children]`` int32), which the result's
     ``seq_lens`` count: they go to :func:`kv8_write` and attention as they are.
     Fresh pages are taken in order of their numbers, by child and position.
-    Lengths, table and counts are new tensors; of what the call is given only free
-    pages of the cache change, so a step with ``lacking > 0`` (their
-    entries are -1 and tokens there are skipped) can be made again with
-    fewer children.  A sequence's partly filled page must be its own; other
+    Lengths, table and counts are new tensors; of what the call is given only pages
+    change that no sequence with a child holds: free ones, and those of sequences that
+    this step drops, whose codes the copies overwrite.  So a step with ``lacking > 0``
+    (their entries are -1 and tokens there are skipped) can be made again from the same
+    lengths, table and counts with fewer children of the same parents; one that continues a
+    sequence which the lacking step dropped reads overwritten pages, unless the
+    caller kept them (``refs``, below).  A sequence's partly filled page must be its own; other
     holders of a page (a kept prefix) count in ``refs`` by their own additions.
     A sequence starts as a child of none with ``new`` tokens.
     """

@@ -487,7 +487,8 @@ size_t dsl_kv8_shared_attention_workspace_bytes(int64_t heads, int64_t page, int
  * [pages]: the counts of the new table; lacking[0]: fresh pages asked for and not there (their entries
  * are -1), those past the table's row included.  Nothing that the call reads is changed but the
  * fresh pages' codes and scales, so a step that lacked pages can be made again with
- * fewer children.  A partly filled page must belong to one sequence alone; no result may
+ * fewer children of the same parents; the pages of sequences that it dropped were free and
+ * may be overwritten (unless refs counts another holder).  A partly filled page must belong to one sequence alone; no result may
  * be an input. */
 int dsl_kv8_fork(void *k_cache, void *v_cache, float *k_scale, float *v_scale, int64_t pages,
                  int64_t heads, int64_t page, int64_t dim, const int32_t *table, int64_t table_ld,

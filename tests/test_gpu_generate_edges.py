@@ -1,5 +1,6 @@
 """Several continuations of a prompt at their edges on the GPU: pages that are missing before
-others and scores that overflow, with every number of query rows a wave; logits of any size."""
+others and scores that overflow, with every number of query rows a wave; logits of any size;
+steps that lacked pages and are made again."""
 import math
 import random
 
@@ -7,12 +8,13 @@ import pytest
 import torch
 
 from dsl_tool_amd import attention as A
+from dsl_tool_amd import kvcache as KV
 from dsl_tool_amd import logprobs as LP
 from oracle import generating as GO
 from oracle import serving as O
-from tests.test_gpu_generate import check_shared, forked, ints, spoil
+from tests.test_gpu_generate import check_shared, equal, forked, ints, pool, spoil
 from tests.test_gpu_generate_steps import wide  # noqa: F401
-from tests.test_gpu_serving import DEV, randn, random_cache, to, within
+from tests.test_gpu_serving import DEV, randn, random_cache, same_cache, to, within
 
 pytestmark = pytest.mark.gpu
 
@@ -122,3 +124,41 @@ def test_logprobs_of_logits_of_any_size(vocab, src, scale):
         g, none = g.cpu(), w.float().isneginf()
         assert torch.equal(g.isneginf(), none)
         assert ((g.double() - w)[~none].abs() <= w[~none].abs() * 2.0 ** -22 + 2.0 ** -19).all()
+
+
+# ------------------------------------------------------ steps that are made again --
+
+def test_fork_made_again():
+    """A step that lacked pages changes no page of a sequence that it continued, nor one that
+    the caller keeps; fewer children of the same parents then come out as if it had not been
+    made, tokens included.  What it dropped is free: its copies may lie there."""
+    page, lens = 16, [40, 20, 25, 55]
+    table, refs = pool(lens, page, 1, 600, width=5)
+    mine = [table[b, :-(-n // page)].tolist() for b, n in enumerate(lens)]
+    for kept in (False, True):
+        counts = refs.clone()
+        if kept:
+            counts[mine[1]] += 1                 # the sequence that the step drops
+        clean = random_cache(len(refs), 2, 64, page, "int8", 601)
+        cache = to(clean, DEV)
+        given = [t.to(DEV) for t in (ints(lens), table)]
+        first = KV.kv8_fork(cache, *given, ints([0, 0, 2, 3, 3, 0, 2]).to(DEV), counts.to(DEV), new=30)
+        assert first.lacking.item() > 0
+        whole = mine[0] + mine[2] + mine[3] + (mine[1] if kept else [])
+        now = to(cache, "cpu")
+        for a, b in zip(now, clean):
+            assert torch.equal(a.view(torch.uint8)[whole], b.view(torch.uint8)[whole])
+        changed = [p for p in mine[1] if not torch.equal(now.k[p], clean.k[p])]
+        assert bool(changed) != kept
+        again = ints([3, 0, 0])
+        want_cache = KV.KV8Cache(*(t.clone() for t in now))
+        want = GO.fork(want_cache, ints(lens), table, again, counts, 1)
+        got = KV.kv8_fork(cache, *given, again.to(DEV), counts.to(DEV), new=1)
+        equal(got, want)
+        same_cache(cache, want_cache)
+        assert want[3].item() == 0
+        other = KV.KV8Cache(*(t.clone() for t in clean))
+        GO.fork(other, ints(lens), table, again, counts, 1)
+        for row, n in zip(want[1], (55, 40, 40)):
+            a, b = (O.tokens(c, n, row.tolist()) for c in (want_cache, other))
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
