@@ -48,6 +48,8 @@ class Int8AttentionLayer:
             raise ValueError(f"q_heads must be a multiple of kv_heads (got {q_heads}, {kv_heads})")
         if rotate is not None and freqs is not None:
             raise ValueError("positions are encoded by rotate or by freqs, not by both")
+        if freqs is None and (axis_of is not None or adjacent):
+            raise ValueError("axis_of and adjacent say how freqs turn the heads: give freqs too")
         hidden = norm.shape[0]
         if w_qkv.shape != ((q_heads + 2 * kv_heads) * dim, hidden) or w_out.shape != (hidden, q_heads * dim):
             raise ValueError(f"w_qkv must be [{(q_heads + 2 * kv_heads) * dim}, {hidden}] and w_out "

@@ -2,8 +2,10 @@
 import os
 
 import pytest
+import torch
 
 from dsl_tool_amd import _native as N
+from dsl_tool_amd import layer8 as L
 from tests.test_generate_host import refuse_each
 from tests.test_serving_host import P
 
@@ -19,3 +21,12 @@ def test_logprobs_scale(lib):
     good = [P, 7, 1000, 1000, 0, P, 2, 2, 1.0, 5, P, P, P, P, P, 1 << 30, None]
     refuse_each(lib, "dsl_token_logprobs", good, [(8, 2.0 ** 126, -1, "scale"), (8, 3e38, -1, "scale"), (8, -1.0, -1, "scale"),
                                                   (8, 1e-60, -1, "scale")])
+
+
+def test_layer_axes_without_freqs():
+    """What says how freqs turn the heads does not go by without a word where there are none."""
+    w = torch.zeros(512, 128), torch.zeros(128, 256), torch.ones(128)
+    for kw in ({"adjacent": True}, {"axis_of": torch.zeros(32, dtype=torch.int32)},
+               {"adjacent": True, "rotate": lambda q, k: (q, k)}):
+        with pytest.raises(ValueError, match="freqs"):
+            L.Int8AttentionLayer(*w, q_heads=4, kv_heads=2, dim=64, **kw)
