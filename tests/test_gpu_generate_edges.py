@@ -1,6 +1,7 @@
 """Several continuations of a prompt at their edges on the GPU: pages that are missing before
 others and scores that overflow, with every number of query rows a wave; logits of any size;
-steps that lacked pages and are made again."""
+steps that lacked pages and are made again; several new tokens by the kernels that the sizes
+choose, and NaN among tokens that only some rows see."""
 import math
 import random
 
@@ -12,7 +13,7 @@ from dsl_tool_amd import kvcache as KV
 from dsl_tool_amd import logprobs as LP
 from oracle import generating as GO
 from oracle import serving as O
-from tests.test_gpu_generate import check_shared, equal, forked, ints, pool, spoil
+from tests.test_gpu_generate import PLAN, SHARED, check_shared, equal, forked, ints, pool, spoil
 from tests.test_gpu_generate_steps import wide  # noqa: F401
 from tests.test_gpu_serving import DEV, randn, random_cache, same_cache, to, within
 
@@ -162,3 +163,74 @@ def test_fork_made_again():
         for row, n in zip(want[1], (55, 40, 40)):
             a, b = (O.tokens(c, n, row.tolist()) for c in (want_cache, other))
             assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# ---------------------------------------------------------- several new tokens --
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page,dim,heads,group", SHARED)
+@pytest.mark.parametrize("causal", [True, False])
+def test_several_tokens_that_share(page, dim, heads, group, src, fmt, causal):
+    """As many new tokens as share a prefix still (96 rows of a cache head, 64 of 64 columns)
+    and fewer, by the kernels that the sizes choose: none at all, more rows than tokens, new
+    ones that reach into the prefix."""
+    most = (64 if dim == 64 else 96) // group
+    lens, table, groups, shared, pages = forked(PLAN, page, 610)
+    assert lens[4] == 5 and lens[11] == 0
+    cache = random_cache(pages, heads, dim, page, fmt, 611)
+    spoil(cache, lens, table)
+    for bound in sorted({most, min(most, 7), min(most, 2)}):
+        new = [min(n, 1 + 11 * b % bound) for b, n in enumerate(lens)]
+        new[3], new[4], new[5], new[7], new[11] = 0, bound, min(lens[5], bound), bound, min(3, bound)
+        q = randn((sum(new), heads * group, dim), 612, src)
+        for kw in ({"max_group": 7}, {}):
+            check_shared(q, cache, lens, table, groups, shared, new, causal=causal, max_q_len=bound, **kw)
+
+
+@pytest.mark.parametrize("key", [True, False])
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("page,dim", [(16, 64), (64, 64), (64, 128), (128, 256), (32, 128)])
+def test_nan_that_some_rows_see(page, dim, src, key, wide):
+    """A NaN code among new tokens is one in the rows that see it, by whole rows (a key's) or in
+    its column (a value's), and in no other: in a sequence's own tokens, in a prefix that a short
+    sequence sees in part, at a tile's first and last token."""
+    lens, table, groups, shared, pages = forked([(384, [70, 200, -230, 40, 1])], page, 620)
+    clean = random_cache(pages, 2, dim, page, "fp8", 621)
+    spoil(clean, lens, table)
+    new = [6, 7, 5, 9, 1]
+    starts = [sum(new[:b]) for b in range(6)]
+    q = randn((starts[5], 8, dim), 622, src)
+    o, a, reach = O.attention(q, clean, ints(lens), table, ints(starts))
+    for owner, pos in ((0, 450), (1, 577), (1, 583), (1, 400), (3, 419), (2, 150), (2, 153), (0, 383), (0, 448)):
+        p, slot = table[owner, pos // page].item(), pos % page
+        cache = KV.KV8Cache(*(t.clone() for t in clean))
+        if key:
+            cache.k.view(torch.uint8)[p, 1, slot, 5] = 0x7f
+        else:
+            cache.v.view(torch.uint8)[p, 1, 5, slot] = 0xff
+        sees = torch.zeros(o.shape, dtype=torch.bool)
+        for b, n in enumerate(lens):
+            for i in range(new[b]):
+                if pos <= n - new[b] + i and table[b, pos // page] == p:
+                    sees[starts[b] + i, 4:, slice(None) if key else slice(5, 6)] = True
+        assert sees.any()
+        got = check_shared(q, cache, lens, table, groups, shared, new, got_only=True, max_q_len=9).cpu()
+        assert torch.equal(got.isnan(), sees), (owner, pos)
+        within(got.masked_fill(sees, 0), o.masked_fill(sees, 0), a, reach)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
+def test_infinite_queries(dim, src, wide):
+    """Rows of infinities, and of one, whose scores have +infinity among them: NaN; the others'
+    rows are their own."""
+    lens, table, groups, shared, pages = forked([(700, [1, 70, 200, 9, 5, 3])], 64, 630)
+    cache = random_cache(pages, 1, dim, 64, "int8", 631)
+    q = randn((6, 4, dim), 632, src)
+    o, a, reach = O.attention(q, cache, ints(lens), table)
+    q[3], q[5, :, 0] = math.inf, -math.inf
+    got = check_shared(q, cache, lens, table, groups, shared, got_only=True)
+    assert got[3].isnan().all() and got[5].isnan().all()
+    others = [0, 1, 2, 4]
+    within(got[others], o[others], a[others], reach[others])
