@@ -93,8 +93,9 @@ def kv8_shared_attention(q: torch.Tensor, cache: KV8Cache, seq_lens: torch.Tenso
     Sequences of many new tokens (more than 96 query rows to a cache head, or 64 of 64
     columns, by ``max_q_len``, so give it) fill the matrix units by themselves and are
     computed as by :func:`kv8_attention`, which is also faster for few sequences behind
-    a short prefix (six of four heads to a cache head behind 1000 tokens).  The workspace
-    is eight bytes for each element of q, up to 32 MB more.
+    a short prefix (six of four heads to a cache head behind 1000 tokens).  All others' rows
+    times query heads are 2^22 at most; their workspace is eight bytes for each element of q, up
+    to 32 MB more.
     """
     if out is None:
         r = N.fast().kv8_shared_attention(q, *cache, seq_lens, page_table, q_starts, max_q_len, scale, causal,

@@ -575,21 +575,21 @@ static SharedWalk shared_walk(const KvCacheArgs &c, int64_t group, int rows, int
   while ((tiles + a.chunk - 1) / a.chunk * units > 1 << 30 && a.chunk < tiles) a.chunk *= 2;
   return a;
 }
-static int rows_set(const KvCacheArgs &c) {
+static int rows_set(int dim) {
   const char *set = getenv("DSL_ATTN_SHARED_ROWS");    // read per launch (tests switch it)
   const int n = set ? atoi(set) : 0;
-  return n == 16 || n == 32 || (n == 64 && c.dim <= 128) ? n : 0;
+  return n == 16 || n == 32 || (n == 64 && dim <= 128) ? n : 0;
 }
 // A sequence whose own rows fill a workgroup of attn_prompt.hip gains nothing from the
 // others': above 96 of them to a cache head (64 of 64 columns), attention as if nothing were shared.
 // (128 columns behind 20000 tokens, shared and not: 96 rows of 4 sequences 108 and 120 us, of 32
 // 635 and 698; 128 rows 112 and 101, 722 and 646; 256 rows 189 and 106, 1394 and 696.
 // 64 columns: 64 rows 44 and 45, 281 and 259; 96 rows 75 and 64, 400 and 340.)
-static bool shared_not(const KvCacheArgs &c, int q_heads, int max_q) {
-  return (int64_t)max_q * (q_heads / c.heads) > (c.dim == 64 ? 64 : 96) && !rows_set(c);
+bool attn_shared_runs(int heads, int dim, int q_heads, int max_q) {
+  return (int64_t)max_q * (q_heads / heads) <= (dim == 64 ? 64 : 96) || rows_set(dim);
 }
 static int shared_rows(const KvCacheArgs &c, int64_t rows) {
-  if (const int n = rows_set(c)) return n;
+  if (const int n = rows_set(c.dim)) return n;
   // As many as a group has, but 64 above 64 only.  128 columns, 8 heads, behind 3000, 10000
   // and 30000 tokens, with 64 rows: 16 a wave 17.5, 33 and 57 us, 32 a wave 19, 25 and 37,
   // 64 a wave 24, 28 and 36; with 128 rows: 26, 54 and 116, 24, 34 and 61, 29, 33 and 47.
@@ -638,7 +638,7 @@ static SharedPlan shared_plan(const KvCacheArgs &c, int groups, int q_heads, int
 }
 
 size_t attn_shared_workspace_bytes(const KvCacheArgs &c, int groups, int q_heads, int max_q, int max_group) {
-  if (shared_not(c, q_heads, max_q)) return attn_workspace_bytes(c, q_heads, max_q) + 16;      // (never empty)
+  if (!attn_shared_runs(c.heads, c.dim, q_heads, max_q)) return attn_workspace_bytes(c, q_heads, max_q) + 16;      // (never empty)
   return shared_plan(c, groups, q_heads, max_q, max_group).bytes;
 }
 
@@ -691,7 +691,7 @@ static hipError_t launch_shared_src(const KvCacheArgs &c, const AttnArgs &p, con
 
 hipError_t launch_attn_shared(int src, const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, hipStream_t st) {
   if (c.seqs == 0 || c.rows == 0) return hipSuccess;
-  if (shared_not(c, p.q_heads, p.max_q)) return launch_attn(src, c, p, st);
+  if (!attn_shared_runs(c.heads, c.dim, p.q_heads, p.max_q)) return launch_attn(src, c, p, st);
   if (src == SRC_BF16) return c.fp8 ? launch_shared_src<SRC_BF16, true>(c, p, h, st) : launch_shared_src<SRC_BF16, false>(c, p, h, st);
   return c.fp8 ? launch_shared_src<SRC_F16, true>(c, p, h, st) : launch_shared_src<SRC_F16, false>(c, p, h, st);
 }

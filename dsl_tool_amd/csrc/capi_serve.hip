@@ -51,11 +51,13 @@ int check_q_heads(const char *fn, int64_t q_heads, int64_t heads, int64_t rows, 
 }
 
 // Groups of sequences that share a prefix.
-int check_groups(const char *fn, int64_t q_heads, int64_t rows, int64_t groups, int64_t max_group) {
+int check_groups(const char *fn, int64_t heads, int64_t dim, int64_t q_heads, int64_t rows, int64_t max_q, int64_t groups,
+                 int64_t max_group) {
   if (groups < 0 || max_group < 0) return fail(DSL_ERR_ARG, "%s: groups and max_group must be >= 0", fn);
   if (groups > 65535) return fail(DSL_ERR_UNSUPPORTED, "%s: at most 65535 groups in a call", fn);
-  // (each has two parts in the workspace, and a workgroup of the join)
-  if (rows > ((int64_t)1 << 22) / q_heads)
+  // (each has two parts in the workspace, and a workgroup of the join, where anything is shared)
+  if (rows > ((int64_t)1 << 22) / q_heads &&
+      dsl::attn_shared_runs((int)heads, (int)dim, (int)q_heads, (int)(max_q < rows ? max_q : rows)))
     return fail(DSL_ERR_UNSUPPORTED, "%s: rows x query heads must be at most 2^22", fn);
   return DSL_OK;
 }
@@ -294,7 +296,7 @@ size_t dsl_kv8_shared_attention_workspace_bytes(int64_t heads, int64_t page, int
                                                 int64_t max_group) {
   const char *fn = "dsl_kv8_shared_attention_workspace_bytes";
   if (check_sizes(fn, heads, page, dim, width, seqs, rows) || check_q_heads(fn, q_heads, heads, rows, max_q) ||
-      check_groups(fn, q_heads, rows, groups, max_group))
+      check_groups(fn, heads, dim, q_heads, rows, max_q, groups, max_group))
     return 0;
   if (rows == 0 || seqs == 0) return 0;
   dsl::KvCacheArgs c{};
@@ -321,7 +323,7 @@ int dsl_kv8_shared_attention(const void *q, int64_t q_row, int64_t q_head, int64
                        width, seq_lens, starts, seqs, rows, x_dtype);
   if (rc) return rc;
   if ((rc = check_q_heads(fn, q_heads, heads, rows, max_q)) ||
-      (rc = check_groups(fn, q_heads, rows, groups, max_group)))
+      (rc = check_groups(fn, heads, dim, q_heads, rows, max_q, groups, max_group)))
     return rc;
   if (!(scale - scale == 0.f)) return fail(DSL_ERR_ARG, "%s: scale must be finite", fn);
   if (rows == 0 || seqs == 0) return ok();

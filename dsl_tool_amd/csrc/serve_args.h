@@ -85,6 +85,7 @@ struct SharedArgs {
   int n;
   int most;              // most sequences of a group (sizes the launch)
 };
+bool attn_shared_runs(int heads, int dim, int q_heads, int max_q);      // or the call goes to launch_attn
 size_t attn_shared_workspace_bytes(const KvCacheArgs &c, int groups, int q_heads, int max_q, int max_group);
 hipError_t launch_attn_shared(int src, const KvCacheArgs &c, const AttnArgs &p, const SharedArgs &h, hipStream_t st);
 

@@ -458,7 +458,7 @@ size_t dsl_kv8_attention_workspace_bytes(int64_t heads, int64_t page, int64_t di
  * Sequences outside every group share nothing.  max_group (most sequences of a group)
  * sizes the launch with max_q; wrong numbers cost time and change roundings only.
  * With more than 96 rows of max_q x q_heads / heads (64 of dim 64) nothing is shared.
- * rows x q_heads at most 2^22; the workspace is never empty. */
+ * Where it is, rows x q_heads at most 2^22; the workspace is never empty. */
 int dsl_kv8_shared_attention(const void *q, int64_t q_row, int64_t q_head, int64_t q_heads,
                              const void *k_cache, const void *v_cache, const float *k_scale,
                              const float *v_scale, int64_t pages, int64_t heads, int64_t page,

@@ -7,7 +7,7 @@ import torch
 from dsl_tool_amd import _native as N
 from dsl_tool_amd import layer8 as L
 from tests.test_generate_host import refuse_each
-from tests.test_serving_host import P
+from tests.test_serving_host import CACHE, P, refused
 
 
 @pytest.fixture(scope="module")
@@ -30,3 +30,16 @@ def test_layer_axes_without_freqs():
                {"adjacent": True, "rotate": lambda q, k: (q, k)}):
         with pytest.raises(ValueError, match="freqs"):
             L.Int8AttentionLayer(*w, q_heads=4, kv_heads=2, dim=64, **kw)
+
+
+def test_shared_attention_of_many_rows(lib):
+    """More rows than prefixes are read once for: refused by their number where they are, and
+    not where each sequence is computed by itself."""
+    rows = (1 << 20) + 1
+    args = [P, 512, 128, 4] + CACHE + [P, P, 2, 2, P, 512, 128, rows, 48, 0.1, 1, 0, None, 0, None]
+    refused(lib, "dsl_kv8_shared_attention", args, -2, "at most 2^22")
+    args[27] = 500                               # max_q: 1000 rows to a cache head
+    refused(lib, "dsl_kv8_shared_attention", args, -3, "workspace")
+    sizes = [2, 64, 128, 5, 3, rows, 4]
+    assert lib.dsl_kv8_shared_attention_workspace_bytes(*sizes, 48, 2, 2) == 0
+    assert lib.dsl_kv8_shared_attention_workspace_bytes(*sizes, 49, 2, 2) > 0

@@ -8,6 +8,7 @@ import random
 import pytest
 import torch
 
+from dsl_tool_amd import _native as N
 from dsl_tool_amd import attention as A
 from dsl_tool_amd import kvcache as KV
 from dsl_tool_amd import logprobs as LP
@@ -234,3 +235,20 @@ def test_infinite_queries(dim, src, wide):
     assert got[3].isnan().all() and got[5].isnan().all()
     others = [0, 1, 2, 4]
     within(got[others], o[others], a[others], reach[others])
+
+
+def test_prompts_of_very_many_rows():
+    """Prompts together past the rows that share a prefix: kv8_attention's result."""
+    seqs, new, hq, dim, page = 140, 500, 64, 64, 64
+    assert seqs * new * hq > 1 << 22
+    table = torch.arange(seqs * 8, dtype=torch.int32).view(seqs, 8)
+    table[:, 0] = 0                              # a shared first page
+    cache = to(random_cache(seqs * 8, 1, dim, page, "int8", 640), DEV)
+    q = torch.randn((seqs * new, hq, dim), device=DEV, generator=torch.Generator(DEV).manual_seed(641)).to(torch.bfloat16)
+    lens, starts = torch.full((seqs,), new, dtype=torch.int32, device=DEV), torch.arange(seqs + 1, device=DEV).int() * new
+    kw = dict(q_starts=starts, max_q_len=new)
+    got = A.kv8_shared_attention(q, cache, lens, table.to(DEV), ints([0, seqs]).to(DEV), ints([64]).to(DEV), **kw)
+    assert torch.equal(got, A.kv8_attention(q, cache, lens, table.to(DEV), **kw))
+    with pytest.raises(N.DslError, match="at most 2"):
+        A.kv8_shared_attention(q, cache, lens, table.to(DEV), ints([0, seqs]).to(DEV), ints([64]).to(DEV), q_starts=starts,
+                               max_q_len=1)
