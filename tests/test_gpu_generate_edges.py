@@ -14,7 +14,7 @@ from dsl_tool_amd import kvcache as KV
 from dsl_tool_amd import logprobs as LP
 from oracle import generating as GO
 from oracle import serving as O
-from tests.test_gpu_generate import PLAN, SHARED, check_shared, equal, forked, ints, pool, spoil
+from tests.test_gpu_generate import PLAN, SHARED, check_fork, check_shared, equal, forked, ints, pool, spoil
 from tests.test_gpu_generate_steps import wide  # noqa: F401
 from tests.test_gpu_serving import DEV, randn, random_cache, same_cache, to, within
 
@@ -252,3 +252,14 @@ def test_prompts_of_very_many_rows():
     with pytest.raises(N.DslError, match="at most 2"):
         A.kv8_shared_attention(q, cache, lens, table.to(DEV), ints([0, seqs]).to(DEV), ints([64]).to(DEV), q_starts=starts,
                                max_q_len=1)
+
+
+@pytest.mark.parametrize("more", [0, 1])
+def test_fork_next_to_the_bound(more):
+    """The largest table and counts that one workgroup keeps the books of, and one page more."""
+    lens, width = [700, 33, 0, 1601], 120
+    table, refs = pool(lens, 16, 0, 650, width=width)
+    spare = 32768 + more - (4 + 7) * width - len(refs)
+    refs = torch.cat([refs, torch.zeros(spare, dtype=torch.int32)])
+    cache = random_cache(len(refs), 1, 64, 16, "int8", 651)
+    check_fork(cache, ints(lens), table, ints([0, 0, 3, 1, 3, 0, -1]), refs, 40)
