@@ -6,7 +6,10 @@ tokens, grouped query heads included.  Scores, the softmax and the sums are
 fp32; the codes enter the products exactly, and the probabilities are rounded
 to bf16 for the second one (to two bf16 numbers for fp16 results).
 ``kv8_shared_attention`` is the same where groups of sequences share a
-prefix.  The reference's attention (triton/qwen3next/qwen3next_kernels.py) has no cache.
+prefix, up to 16 query rows of a group and cache head.  Above, the probabilities are
+rounded to fp16 (to two fp16 numbers for fp16 results), bf16 queries are brought to fp16 by a
+power of two for each row, within 2^-32 of the row's largest, value scales below 2^-90 count as 0,
+and those of one context are to lie within 2^100 of each other.  The reference's attention (triton/qwen3next/qwen3next_kernels.py) has no cache.
 """
 from __future__ import annotations
 

@@ -18,7 +18,8 @@
 // step, 2^-12, or 2^-33 of the largest where they are below 2^-22 of it (a step of fp16's
 // smallest numbers: without the 2^8, 131072 small ones could lose 2^-8 together).  For
 // fp16 results they enter as two numbers, hi + lo.  Page scales of no logarithm (negative, infinite, NaN) and below 2^-90
-// (which count as 0) act on the probabilities.
+// (which count as 0) act on the probabilities.  Sums stand relative to m too, the scales in it: the factors that join
+// waves and parts are fp32, so of scales 2^126 and more apart the smaller ones' tokens would be lost to the sum.
 //
 // S^T = K Q^T on 32x32 tiles gives a lane 16 tokens of its query row.  Tokens are dealt
 // to the rows of the K tiles so that they are consecutive: row r of tile t is token
@@ -95,7 +96,7 @@ struct TileWalk {
   static constexpr int SRC = SRC_, D = D_, NB = NB_, BLOCK = 32, ROWS = 32 * NB, NW = 4;
   static constexpr bool FP8 = FP8_, F16 = SRC == SRC_F16;
   static constexpr int KX = D / 32, DT = D / 32;
-  static constexpr int WGS = 1;  // of a CU: a wave takes all of a SIMD's registers
+  static constexpr int WGS = 1;  // of a CU: 128 columns take all of a SIMD's registers (64 about half: two are untried)
   // The queries as they stand in the products, the same for all waves, in LDS: in
   // registers they spill.
   static constexpr bool SHARED = true;

@@ -18,10 +18,10 @@
 // threads as `top`, so their words are read once more and everything else is not.
 // Keys are sorted 64 to a wave, and sorted runs are merged, best 64 kept.
 //
-// Bound by the logits' bytes: 3001 rows of 100003 in bf16 take 131 us, 4.6 TB/s (512
-// threads to a workgroup 150: more of it waits for the sorts; 128: 140).  Few rows are
-// split over workgroups, and a second launch joins the parts: 16 rows of 131071 in fp32
-// take 9.6 and 4.8 us, latency of launches, sums and sorts; the bytes would take 1.6.
+// Bound by the logits' bytes: 3001 rows of 100003 in bf16 take 127 us, 4.7 TB/s (with 512
+// threads to a workgroup, which wait for the sorts longer, 150 where 256 took 131; 128: 140).
+// Few rows are split over workgroups, and a second launch joins the parts: 16 rows of 131071 in
+// fp32 take 9.7 and 4.5 us, latency of launches, sums and sorts; the bytes would take 1.6.
 #include "common.h"
 #include "generate_args.h"
 #include "kv_core.h"
@@ -370,7 +370,8 @@ __global__ __launch_bounds__(kLogThreads) void logprob_join_kernel(const Logprob
 }
 
 // Parts of a row: a workgroup per CU, of two words for each thread at least.  (16 rows of
-// 131071 in fp32: 14.4 us; two workgroups per CU 16.4.)
+// 131071 in fp32: 13.2 us, two workgroups per CU 15.1; 64: 16.9 and 16.4, 128: 25.7 and 21.4, 256:
+// 34.3 and 33, 400: 41.6 and 51.5; of 100003 in bf16 16: 13.6 and 15, 128: 16.5 and 17.3, 400: 27.7 and 30.9.)
 static int logprob_splits(int src, int rows, int vocab) {
   const int words = vocab / (src == SRC_F32 ? 4 : 8);
   int64_t s = ((int64_t)device_cu_count() + rows - 1) / (rows > 0 ? rows : 1);

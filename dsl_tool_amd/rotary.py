@@ -7,7 +7,8 @@ Pair i of a head is turned by the angle ``positions[axis_of[i]] * freqs[i]``:
     axis_of = rotary_axes([16, 24, 24])             # which axis turns which pair
     q, k = rotary(q, k, positions, freqs, axis_of=axis_of)
 
-Angles are formed in 64 bits, so far positions keep their digits.  Everything
+Angles are formed in 64 bits, so far positions keep their digits: an angle of a
+radians is off by ``|a| * 2 ** -51`` and the 2^-22 of its turn in 32 bits.  Everything
 runs in ``libdsl_gemm.so``.  The reference's RoPE
 (triton/rope/rope_kernel.py:11-145) has one axis.
 """

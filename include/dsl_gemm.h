@@ -454,7 +454,9 @@ size_t dsl_kv8_attention_workspace_bytes(int64_t heads, int64_t page, int64_t di
  * (ascending) hold the same pages for their first shared_lens[g] tokens: that prefix,
  * cut to whole pages, is read once for the group instead of once for each
  * sequence, from the table row of its first sequence that is as long (else its
- * longest).  The result is dsl_kv8_attention's but for roundings.
+ * longest).  The result is dsl_kv8_attention's but for roundings.  (Above 16 query rows of a
+ * group and cache head: probabilities in fp16, value scales below 2^-90 count as 0, those of one
+ * context are to lie within 2^100 of each other.)
  * Sequences outside every group share nothing.  max_group (most sequences of a group)
  * sizes the launch with max_q; wrong numbers cost time and change roundings only.
  * With more than 96 rows of max_q x q_heads / heads (64 of dim 64) nothing is shared.
@@ -516,7 +518,8 @@ size_t dsl_kv8_compact_workspace_bytes(int64_t pages);
  * magnitude; axis_of NULL: one axis; an axis outside [0, axes) turns by nothing.
  * Pairs are the dimensions (i, i + pairs), or (2 i, 2 i + 1) with `adjacent`;
  * dimensions from 2 pairs on stay.  Positions are int32, or int64; angles are formed
- * in 64 bits (positions below 2^53 count exactly).  A result may be its source, in
+ * in 64 bits, so an angle of a radians is off by |a| 2^-51 and the 2^-22 of its turn in 32
+ * bits (10^9 radians: 7e-7, 10^12: 4e-4).  A result may be its source, in
  * place; other overlaps are not allowed.  Strides in elements. */
 int dsl_rotary(const void *q, int64_t q_row, int64_t q_head, int64_t q_heads, const void *k,
                int64_t k_row, int64_t k_head, int64_t k_heads, int64_t rows, int64_t dim,
